@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 7
+#define GDN_ABI_VERSION 8
 
 #if defined(__GNUC__) || defined(__clang__)
 #define GDN_API __attribute__((visibility("default")))
@@ -348,6 +348,86 @@ GDN_API int gdn_attn_qk_norm_rope_fwd(const void* q_in, int64_t q_row_stride, co
 GDN_API int gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t v_row_stride, const void* gate,
                  int64_t gate_row_stride, void* o, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ,
                  int64_t HKV, int64_t D, int64_t N, float scale, unsigned flags, void* stream);
+
+/*
+ * Linear attention with a decay for each head, chunked (64 tokens): S_t = exp(g_t) S_{t-1} + k_t v_t^T,
+ * o_t = scale S_t^T q_t. bf16 q, k, v, o; initial_state (or NULL: zeros) and final_state (or NULL: not written)
+ * fp32. g: log decays in g_dtype, element strides for the batch row, the token and the value head (0 where it does
+ * not vary: one decay a head is 0, 0, 1), or NULL: no decay. With cu_seqlens the batch stride is not used. Values
+ * below -100 are taken as -100. K and V each 64 or 128; tensors 16-byte aligned. flags: GDN_FLAG_CU_INT32.
+ * states: gdn_decay_attn_states_size(B, T, HV, K, V, N, cu_seqlens != NULL) bytes (0: may be NULL), contents on
+ * entry irrelevant: the states entering the segments that the call cuts its sequences into. gdn_decay_attn_bwd
+ * reads them. Calls that share them must not overlap.
+ */
+GDN_API int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
+                               void* o, float* final_state, const void* cu_seqlens, int64_t B, int64_t T, int64_t H,
+                               int64_t HV, int64_t K, int64_t V, int64_t N, int g_dtype, int64_t g_batch_stride,
+                               int64_t g_token_stride, int64_t g_head_stride, float scale, unsigned flags, void* states,
+                               size_t states_bytes, void* stream);
+
+/* Bytes of states for gdn_decay_attn_fwd / gdn_decay_attn_bwd (0 for invalid sizes, or where a sequence is one segment). */
+GDN_API size_t gdn_decay_attn_states_size(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int64_t N, int varlen);
+
+/*
+ * Backward of gdn_decay_attn_fwd: its inputs and the states it left, d_o [B,T,HV,V] bf16, d_final_state or NULL (zero).
+ * dq, dk [B,T,H,K] and dv [B,T,HV,V] bf16; dg [B,T,HV] contiguous in g_dtype or NULL (not wanted); d_initial_state or
+ * NULL. final_state (the forward's) is read for dg where d_final_state is given. workspace:
+ * gdn_decay_attn_bwd_workspace_size bytes.
+ */
+GDN_API int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
+                               const float* final_state, const void* d_o, const float* d_final_state,
+                               const void* states, const void* cu_seqlens, int64_t B, int64_t T, int64_t H, int64_t HV,
+                               int64_t K, int64_t V, int64_t N, int g_dtype, int64_t g_batch_stride,
+                               int64_t g_token_stride, int64_t g_head_stride, float scale, unsigned flags, void* dq,
+                               void* dk, void* dv, void* dg, float* d_initial_state, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Workspace bytes gdn_decay_attn_bwd needs (0 for invalid sizes). */
+GDN_API size_t gdn_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                                 int64_t N, int varlen);
+
+/*
+ * The recurrence of gdn_decay_attn_fwd token by token in fp32, q, k, v, o in qkv_dtype: the step of single tokens.
+ * final_state may equal initial_state (in-place update). g and its strides as there, without the bound of -100.
+ */
+GDN_API int gdn_decay_attn_recurrent_fwd(const void* q, const void* k, const void* v, const void* g,
+                                         const float* initial_state, void* o, float* final_state,
+                                         const void* cu_seqlens, int64_t B, int64_t T, int64_t H, int64_t HV,
+                                         int64_t K, int64_t V, int64_t N, int qkv_dtype, int g_dtype,
+                                         int64_t g_batch_stride, int64_t g_token_stride, int64_t g_head_stride,
+                                         float scale, unsigned flags, void* stream);
+
+/*
+ * RMSNorm of every head row of q [B, T, HQ, D] and k [B, T, HK, D] (dtype; by element strides, the last axis contiguous,
+ * rows 16-byte aligned) with weights [D] fp32 or NULL (ones), then the rotary embedding of the first rot_dim entries
+ * (element f with f + rot_dim / 2, angle position * theta^(-2f / rot_dim)), in fp32 with one rounding into q_out, k_out
+ * (contiguous). positions: [B, T] int64 (int32 with pos_i32) by strides, or NULL: the token index, restarting at 0 in
+ * every document with cu_seqlens. D 64, 128 or 256; rot_dim a multiple of 16 up to D (0: no rotation).
+ * Unlike gdn_attn_qk_norm_rope_fwd it has a backward, takes positions and all three dtypes, and rounds once.
+ */
+GDN_API int gdn_qk_norm_rope_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                 const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                 const float* q_weight, const float* k_weight, const void* positions,
+                                 int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, void* q_out,
+                                 void* k_out, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HK,
+                                 int64_t D, int64_t N, int dtype, int rot_dim, double theta, float eps, unsigned flags,
+                                 void* stream);
+
+/*
+ * Backward of gdn_qk_norm_rope_fwd: dq_out, dk_out (dtype, contiguous) into dq, dk (dtype, contiguous) and dq_weight,
+ * dk_weight [D] fp32 (either may be NULL). workspace (read only with one of them): gdn_qk_norm_rope_bwd_workspace_size bytes.
+ */
+GDN_API int gdn_qk_norm_rope_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                 const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                 const float* q_weight, const float* k_weight, const void* positions,
+                                 int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, const void* dq_out,
+                                 const void* dk_out, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                                 const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D,
+                                 int64_t N, int dtype, int rot_dim, double theta, float eps, unsigned flags,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes gdn_qk_norm_rope_bwd needs (0 for invalid sizes). */
+GDN_API size_t gdn_qk_norm_rope_bwd_workspace_size(int64_t B, int64_t T, int64_t D);
 
 #ifdef __cplusplus
 }

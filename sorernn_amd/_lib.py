@@ -21,12 +21,13 @@ FLAG_BETA_SIGMOID = 0x2
 FLAG_GATE_IN_KERNEL = 0x4
 FLAG_CU_INT32 = 0x8
 ACT_NONE, ACT_SILU, ACT_SILU_ROUNDED = 0, 1, 2
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _U = ctypes.c_uint
 _SZ = ctypes.c_size_t
 
@@ -60,6 +61,16 @@ SIGNATURES = {
     "gdn_qkv_conv_fwd": [_P, _I64, _P, _P, _P, _P, _P, _P] + [_I64] * 6 + [_INT, _INT, _U, _P],
     "gdn_attn_qk_norm_rope_fwd": [_P, _I64, _P, _I64, _P, _P, _INT, _P, _P, _P] + [_I64] * 6 + [_INT, _F, _F, _U, _P],
     "gdn_attn_fwd": [_P, _P, _P, _I64, _P, _I64, _P, _P] + [_I64] * 6 + [_F, _U, _P],
+    "gdn_decay_attn_fwd": [_P] * 8 + [_I64] * 7 + [_INT] + [_I64] * 3 + [_F, _U, _P, _SZ, _P],
+    "gdn_decay_attn_states_size": [_I64] * 6 + [_INT],
+    "gdn_decay_attn_bwd": [_P] * 10 + [_I64] * 7 + [_INT] + [_I64] * 3 + [_F, _U] + [_P] * 6 + [_SZ, _P],
+    "gdn_decay_attn_bwd_workspace_size": [_I64] * 7 + [_INT],
+    "gdn_decay_attn_recurrent_fwd": [_P] * 8 + [_I64] * 7 + [_INT] * 2 + [_I64] * 3 + [_F, _U, _P],
+    "gdn_qk_norm_rope_fwd": ([_P] + [_I64] * 3) * 2 + [_P] * 3 + [_I64] * 2 + [_INT] + [_P] * 3 + [_I64] * 6
+    + [_INT, _INT, _D, _F, _U, _P],
+    "gdn_qk_norm_rope_bwd": ([_P] + [_I64] * 3) * 2 + [_P] * 3 + [_I64] * 2 + [_INT] + [_P] * 7 + [_I64] * 6
+    + [_INT, _INT, _D, _F, _U, _P, _SZ, _P],
+    "gdn_qk_norm_rope_bwd_workspace_size": [_I64] * 3,
 }
 
 RESTYPES = {
@@ -71,6 +82,9 @@ RESTYPES = {
     "gdn_chunk_bwd_workspace_size": ctypes.c_size_t,
     "gdn_causal_conv1d_bwd_workspace_size": ctypes.c_size_t,
     "gdn_rms_norm_gated_bwd_workspace_size": ctypes.c_size_t,
+    "gdn_decay_attn_states_size": ctypes.c_size_t,
+    "gdn_decay_attn_bwd_workspace_size": ctypes.c_size_t,
+    "gdn_qk_norm_rope_bwd_workspace_size": ctypes.c_size_t,
 }
 
 _lib = None

@@ -1,0 +1,906 @@
+// Linear attention with a decay for each head (the gated delta rule's recurrence without its correction term):
+// chunked forward and backward for gfx950.
+//
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t
+//
+// Over a chunk of 64 tokens, with b_i the sum of g up to token i and b_C that of the whole chunk:
+//   o_i   = scale (exp(b_i) S_in^T q_i + sum_{j <= i} exp(b_i - b_j) (q_i . k_j) v_j)
+//   S_out = exp(b_C) S_in + sum_j exp(b_C - b_j) k_j v_j^T
+//
+// One walker kernel computes the forward and the three gradients, as all of them are this recurrence:
+//   dq_i = scale S_i do_i              the walk itself with (q, k, v) = (do, v, k): its state is S^T
+//   dv_j = R_j^T k_j, dk_j = R_j v_j   R_j = exp(g_{j+1}) R_{j+1} + scale q_j do_j^T: the walk from the end with
+//                                      (k, q, do) and (v, do, q)
+//   dg_t = exp(g_t) <S_{t-1}, R_t> = sum over i >= t of (q_i . dq_i - k_i . dk_i), plus <S_T, dS_T>
+//
+// A workgroup of 4 waves walks one segment of a sequence for one value head. The state stays in fp32 MFMA
+// accumulators, wave w holding all K rows of its V / 4 columns; it is the A operand of S^T Q^T as it stands, split into
+// bf16 parts in registers. Sequences are cut into segments so that few heads fill the chip: a first kernel walks
+// the segments for their own contribution to the state (k and v only), a scan over the segments turns these into the
+// states that enter them, and the walkers then run side by side.
+//
+// Rounding: q, k, v and do are bf16 operands as they come. What is computed is split into bf16 parts that are multiplied
+// one by one: three (24 bits, as fp32 holds) where the result is an fp32 output (the state, and what dg sums), two
+// where the outputs are rounded to bf16 (scores, and the state under o): a single part's 2^-9 would be as large as the
+// rounding of the output itself. The decays are summed in 64 bits: a difference of two sums in 32 would carry the
+// rounding of the sums into every weight.
+
+#include "gdn_mfma.h"
+
+namespace gdn {
+
+constexpr int kLinNT = 256;
+constexpr int kPP = kC + 8;  // pitch of the score tiles
+
+struct LinParams {
+  const bf16 *q, *k, *v, *e;    // [tokens][HV / r*][K or V]: the walk's q, k, v and the rows of the gate's dot products
+  int rq, rk, rv, re;           // value heads that share a head of each
+  const void* g;                // log decays, or null: no decay
+  int dg;
+  int64_t gb, gt, gh;           // element strides of batch row, token and value head
+  const float* init;            // [N][HV][K][V] state before the walk, or null: zeros
+  float* entry;                 // [slots][HV][K][V] states entering the segments, or null: one segment a sequence
+  float* decay;                 // [slots][HV] decay of a whole segment
+  int transposed;               // init and entry are read as [V][K]
+  float* fin;                   // [N][HV][K][V] state after the walk, or null
+  void* o;                      // [tokens][HV][V]
+  float* dot;                   // [HV][tokens] with DOT
+  const void* cu;
+  int cu_i32, shift;            // segments of 1 << shift tokens
+  int64_t T, N, HV, spq;        // spq: segments of a sequence without cu
+  float scale;
+};
+
+// Where a workgroup works: sequence n, the segment's first token (flat) and length, and its place in the sequence.
+struct Segment {
+  int64_t n, slot, tok, row, col;  // row, col: batch row and first token in it (the gate's strides)
+  int len;
+  bool first, last, some;
+};
+
+// Slots of a sequence: with cu, sequence n has the slots from (cu[n] >> shift) + n on, which leaves room for its
+// segments whatever the lengths are, so that the grid depends on T and N alone. All lanes of a wave search together.
+__device__ __forceinline__ Segment find_segment(const LinParams& p, int64_t slot) {
+  Segment s;
+  int64_t bos, len, local;
+  const int64_t L = (int64_t)1 << p.shift;
+  if (p.cu) {
+    const int lane = threadIdx.x % kWave;
+    int64_t lo = 0, hi = p.N;  // first slot of sequence lo <= slot < that of sequence hi
+    while (hi - lo > 1) {
+      const int64_t step = (hi - lo + kWave - 1) / kWave, i = lo + lane * step;
+      const bool in = i < hi && (load_index(p.cu, p.cu_i32, i < hi ? i : lo) >> p.shift) + i <= slot;
+      const int cnt = __popcll(__ballot(in));  // one at least: lane 0's
+      lo += (cnt > 1 ? cnt - 1 : 0) * step;
+      hi = lo + step < hi ? lo + step : hi;
+    }
+    s.n = lo;
+    bos = load_index(p.cu, p.cu_i32, lo);
+    len = load_index(p.cu, p.cu_i32, lo + 1) - bos;
+    local = slot - ((bos >> p.shift) + lo);
+    s.row = 0;
+    s.col = bos + local * L;
+  } else {
+    s.n = slot / p.spq;
+    local = slot % p.spq;
+    bos = s.n * p.T;
+    len = p.T;
+    s.row = s.n;
+    s.col = local * L;
+  }
+  s.slot = slot;
+  s.tok = bos + local * L;
+  const int64_t left = len - local * L;
+  s.some = left > 0;
+  s.len = (int)(left < L ? left : L);
+  s.first = local == 0;
+  s.last = left <= L;
+  return s;
+}
+
+// Decay terms of a chunk, base-2 logarithms: b = h + l in two floats, the weight of a token in the state's update and
+// that of the state in a token's output (each with the factor it carries), and the decay of the whole chunk.
+struct Decays {
+  float h[kC], l[kC], wst[kC], win[kC];
+  float all;
+};
+
+__device__ __forceinline__ double dpp_add64(double v, int lo, int hi) { return v + __hiloint2double(hi, lo); }
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double dpp_scan_step(double v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROW_MASK, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROW_MASK, 0xf, false);
+  return dpp_add64(v, lo, hi);
+}
+
+// Log decays below -100 (exp of it is 0 beside any weight that counts) are taken as -100: a reset of -inf leaves the
+// differences of sums behind it finite.
+__device__ __forceinline__ double log2_decay(uint32_t raw, int dtype) {
+  const float x = raw32_to_f32(raw, dtype);
+  return (double)(x < -100.f ? -100.f : x) * 1.4426950408889634;
+}
+
+template <bool REV>
+__device__ __forceinline__ void chunk_decays(Decays& d, double x, float scale, int lane) {
+  x = dpp_scan_step<0x111, 0xf>(x);
+  x = dpp_scan_step<0x112, 0xf>(x);
+  x = dpp_scan_step<0x114, 0xf>(x);
+  x = dpp_scan_step<0x118, 0xf>(x);
+  x = dpp_scan_step<0x142, 0xa>(x);
+  x = dpp_scan_step<0x143, 0xc>(x);
+  const double all = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), kWave - 1),
+                                      __builtin_amdgcn_readlane(__double2loint(x), kWave - 1));
+  const float head = __builtin_amdgcn_exp2f((float)x), tail = __builtin_amdgcn_exp2f((float)(all - x));
+  d.h[lane] = (float)x;
+  d.l[lane] = (float)(x - (double)(float)x);
+  d.wst[lane] = REV ? scale * head : tail;
+  d.win[lane] = REV ? tail : scale * head;
+  if (lane == 0) d.all = __builtin_amdgcn_exp2f((float)all);
+}
+
+// The next bf16 part of 8 fp32 values: rounds them, and leaves in x what the rounding left out.
+__device__ __forceinline__ bf16x8 next_part(float (&x)[8]) {
+  bf16x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    r[e] = (bf16)x[e];
+    x[e] -= (float)r[e];
+  }
+  return r;
+}
+
+// Columns of wave w's tile ct, lane i of 16: 16 NCT w + 4 NCT (i / 4) + 4 ct + i % 4, so that an accumulator lane's
+// tiles hold 4 NCT neighbouring columns. The transposed read of 8 tokens of a column in the accumulators' token order.
+template <int NCT>
+__device__ __forceinline__ bf16x8 ld8_tr_cols(const bf16* tile, int pitch, int r0, int c0, int lane) {
+  const int g = lane >> 4, li = lane & 15;
+  const bf16* p0 = tile + (r0 + 4 * g + (li >> 2)) * pitch + c0 + 4 * NCT * (li & 3);
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p0));
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p0 + 16 * pitch));
+  return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// A chunk's rows on their way to LDS: thread t holds the 16-byte pieces t, t + 256, ... of the 64 x D tile. Rows past
+// the chunk's end re-read its first row and are written as zeros.
+template <int D>
+struct Tile {
+  bf16x8 r[D / 32];
+  __device__ __forceinline__ void fetch(const bf16* base, int64_t stride, int len) {
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      const int c = threadIdx.x + n * kLinNT, row = c / (D / 8);
+      r[n] = *reinterpret_cast<const bf16x8*>(base + (row < len ? row : 0) * stride + (c % (D / 8)) * 8);
+    }
+  }
+  __device__ __forceinline__ void put(bf16* tile, int len) const {
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      const int c = threadIdx.x + n * kLinNT, row = c / (D / 8);
+      *reinterpret_cast<bf16x8*>(tile + row * (D + 8) + (c % (D / 8)) * 8) = row < len ? r[n] : bf16x8{};
+    }
+  }
+  // any infinity or NaN among the valid rows
+  __device__ __forceinline__ bool unbounded(int len) const {
+    uint32_t any = 0;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      const u32x4 w = __builtin_bit_cast(u32x4, r[n]);
+      const bool in = (int)(threadIdx.x + n * kLinNT) / (D / 8) < len;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= in && ((w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u);
+    }
+    return any;
+  }
+};
+
+// The state of wave w's columns: accumulator tiles s[2u + c][ct], rows 32u + 8g + 4c + r, column as above.
+template <int KD, int VD>
+struct State {
+  static constexpr int NCT = VD / 64;
+  f32x4 s[KD / 16][NCT];
+
+  __device__ __forceinline__ static int row0(int a, int g) { return 32 * (a >> 1) + 8 * g + 4 * (a & 1); }
+  __device__ __forceinline__ static int col(int w, int ct, int i) {
+    return 16 * NCT * w + 4 * NCT * (i >> 2) + 4 * ct + (i & 3);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int a = 0; a < KD / 16; ++a)
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) s[a][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void load(const float* src, bool transposed, int w, int lane) {
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int a = 0; a < KD / 16; ++a)
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        if (transposed) {
+          s[a][ct] = *reinterpret_cast<const f32x4*>(src + (int64_t)col(w, ct, i) * KD + row0(a, g));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][ct][r] = src[(row0(a, g) + r) * VD + col(w, ct, i)];
+        }
+      }
+  }
+  __device__ __forceinline__ void store(float* dst, int w, int lane) const {
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int a = 0; a < KD / 16; ++a)
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dst[(row0(a, g) + r) * VD + col(w, ct, i)] = s[a][ct][r];
+  }
+  // S = all S + K^T (wst V): V weighted in fp32 and split into three bf16 parts (K is exact)
+  __device__ __forceinline__ void update(const Decays& d, const bf16* Ks, const bf16* Vs, int w, int lane) {
+    const int g = lane >> 4;
+    const float all = d.all;
+#pragma unroll
+    for (int a = 0; a < KD / 16; ++a)
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) s[a][ct] *= all;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 4 * g);
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 16 + 4 * g);
+      bf16x8 part[NCT][3];
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        const bf16x8 vf = ld8_tr_cols<NCT>(Vs, VD + 8, 32 * ks, 16 * NCT * w + 4 * ct, lane);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)vf[e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) part[ct][n] = next_part(x);
+      }
+#pragma unroll
+      for (int a = 0; a < KD / 16; ++a) {
+        const bf16x8 kf = ld8_tr_pair(Ks, KD + 8, 32 * ks, 32 * (a >> 1) + 4 * (a & 1), lane);
+#pragma unroll
+        for (int n = 2; n >= 0; --n)
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) s[a][ct] = mma(kf, part[ct][n], s[a][ct]);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t gate_raw(const LinParams& p, const Segment& sg, int64_t hv, int t) {
+  return load_raw32(p.g, p.dg, sg.row * p.gb + (sg.col + t) * p.gt + hv * p.gh);
+}
+
+// ------------------------------------------------------------------------------------------------
+// A segment's own contribution to the state: the walk without outputs, from a zero state. Forward walks leave it in
+// the next segment's slot, walks from the end in the one before; the sequence's last segment (first) has none to give.
+template <int KD, int VD, bool REV>
+__global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_segment_kernel(LinParams p) {
+  __shared__ __align__(16) bf16 Ks[kC * (KD + 8)], Vs[kC * (VD + 8)];
+  __shared__ __align__(16) Decays d;
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  const int64_t hv = blockIdx.x % p.HV;
+  const Segment sg = find_segment(p, blockIdx.x / p.HV);
+  if (!sg.some || (REV ? sg.first : sg.last)) return;
+  const int64_t ks = p.HV / p.rk * KD, vs = p.HV / p.rv * VD;  // token strides
+  const bf16* k0 = p.k + sg.tok * ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + sg.tok * vs + hv / p.rv * VD;
+  const int nc = (sg.len + kC - 1) / kC;
+  Tile<KD> kt;
+  Tile<VD> vt;
+  uint32_t graw = 0;
+  auto fetch = [&](int ci) {
+    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    kt.fetch(k0 + t0 * ks, ks, len);
+    vt.fetch(v0 + t0 * vs, vs, len);
+    if (w == 0 && p.g) graw = lane < len ? gate_raw(p, sg, hv, t0 + lane) : 0u;
+  };
+  State<KD, VD> st;
+  st.zero();
+  double total = 0.;
+  fetch(0);
+  for (int ci = 0; ci < nc; ++ci) {
+    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    kt.put(Ks, len);
+    vt.put(Vs, len);
+    if (w == 0) {
+      const double x = p.g ? log2_decay(graw, p.dg) : 0.;
+      total += x;
+      chunk_decays<REV>(d, x, p.scale, lane);
+    }
+    __syncthreads();
+    if (ci + 1 < nc) fetch(ci + 1);
+    st.update(d, Ks, Vs, w, lane);
+    __syncthreads();
+  }
+  const int64_t to = (sg.slot + (REV ? -1 : 1)) * p.HV + hv;
+  st.store(p.entry + to * (KD * VD), w, lane);
+  if (w == 0) {
+    for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
+    if (lane == 0) p.decay[sg.slot * p.HV + hv] = __builtin_amdgcn_exp2f((float)total);
+  }
+}
+
+// The segments' contributions into the states entering them, in place: entry[s] += decay[s - 1] entry[s - 1] (from the
+// end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread.
+template <bool REV>
+__global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, int64_t elems) {
+  const int64_t per = elems / 1024, chain = blockIdx.x / per;
+  const int64_t hv = chain % p.HV, n = chain / p.HV;
+  const int64_t at = (blockIdx.x % per) * 1024 + threadIdx.x * 4;
+  int64_t slot0, cnt;
+  if (p.cu) {
+    const int64_t bos = load_index(p.cu, p.cu_i32, n), eos = load_index(p.cu, p.cu_i32, n + 1);
+    slot0 = (bos >> p.shift) + n;
+    cnt = (eos - bos + ((int64_t)1 << p.shift) - 1) >> p.shift;
+  } else {
+    slot0 = n * p.spq;
+    cnt = p.spq;
+  }
+  if (cnt < 2) return;
+  const int64_t step = p.HV * elems;
+  float* e = p.entry + (slot0 * p.HV + hv) * elems + at;
+  const float* dc = p.decay + slot0 * p.HV + hv;
+  f32x4 run = {0.f, 0.f, 0.f, 0.f};
+  if (p.init) run = *reinterpret_cast<const f32x4*>(p.init + chain * elems + at);
+  constexpr int U = 4;  // loads in flight
+  for (int64_t s0 = 0; s0 < cnt - 1; s0 += U) {
+    f32x4 x[U];
+    float c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t s = s0 + u < cnt - 1 ? s0 + u : cnt - 2;
+      x[u] = *reinterpret_cast<const f32x4*>(e + (REV ? cnt - 2 - s : s + 1) * step);
+      c[u] = dc[(REV ? cnt - 1 - s : s) * p.HV];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= cnt - 1) break;
+      run = run * c[u] + x[u];
+      *reinterpret_cast<f32x4*>(e + (REV ? cnt - 2 - s0 - u : s0 + u + 1) * step) = run;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// The walk. DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums
+// less the column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.
+template <int KD, int VD, bool REV, int DOT, typename OT>
+__global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinParams p) {
+  constexpr int NCT = VD / 64, KP = KD + 8, VP = VD + 8, NU = KD / 32;
+  constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
+  __shared__ __align__(16) bf16 Qs[kC * KP], Ks[kC * KP], Vs[kC * VP];
+  __shared__ __align__(16) bf16 Ps[2][kC * kPP];  // the two parts of the scores, tok_col columns
+  __shared__ __align__(16) Decays d;
+  __shared__ float dots[DOT ? 4 : 1][kC], rows[kC], cols[DOT == 2 ? 4 : 1][kC];
+  __shared__ int bad[2];
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane >> 4, i = lane & 15;
+  const int64_t hv = blockIdx.x % p.HV;
+  const Segment sg = find_segment(p, blockIdx.x / p.HV);
+  if (!sg.some) return;
+  const int64_t qs = p.HV / p.rq * KD, ks = p.HV / p.rk * KD, vs = p.HV / p.rv * VD, es = DOT ? p.HV / p.re * VD : 0;
+  const bf16* q0 = p.q + sg.tok * qs + hv / p.rq * KD;
+  const bf16* k0 = p.k + sg.tok * ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + sg.tok * vs + hv / p.rv * VD;
+  const bf16* e0 = DOT ? p.e + sg.tok * es + hv / p.re * VD : nullptr;
+  OT* o0 = static_cast<OT*>(p.o) + (sg.tok * p.HV + hv) * VD;
+  const int nc = (sg.len + kC - 1) / kC;
+  Tile<KD> qt, kt;
+  Tile<VD> vt;
+  uint32_t graw = 0;
+  auto fetch = [&](int ci) {
+    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    qt.fetch(q0 + t0 * qs, qs, len);
+    kt.fetch(k0 + t0 * ks, ks, len);
+    vt.fetch(v0 + t0 * vs, vs, len);
+    if (w == 0 && p.g) graw = lane < len ? gate_raw(p, sg, hv, t0 + lane) : 0u;
+  };
+  fetch(0);
+  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+  State<KD, VD> st;
+  const bool inner = REV ? !sg.last : !sg.first;  // a segment of this sequence comes before
+  const float* src = inner ? p.entry + (sg.slot * p.HV + hv) * (KD * VD)
+                           : (p.init ? p.init + (sg.n * p.HV + hv) * (KD * VD) : nullptr);
+  bool held = src != nullptr;  // the state is not known to be zero
+  if (held) st.load(src, p.transposed, w, lane);
+  else st.zero();
+  const bool wants_fin = p.fin && (REV ? sg.first : sg.last);
+  __syncthreads();  // bad[] is set
+  for (int ci = 0; ci < nc; ++ci) {
+    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    qt.put(Qs, len);
+    kt.put(Ks, len);
+    vt.put(Vs, len);
+    if (vt.unbounded(len)) bad[ci & 1] = 1;
+    if (w == 0) chunk_decays<REV>(d, p.g ? log2_decay(graw, p.dg) : 0., p.scale, lane);
+    __syncthreads();
+    if (ci + 1 < nc) fetch(ci + 1);
+    if (threadIdx.x == 0) bad[(ci + 1) & 1] = 0;
+    // ---- the scores of queries 16 w ..: P^T tiles, rows = keys j, column = query
+    {
+      const int iq = 16 * w + i;
+      bf16x8 qf[NU], ef[DOT == 2 ? VD / 32 : 1];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) qf[u] = ld8(Qs + iq * KP + 32 * u + 8 * g);
+      if (DOT == 2) {
+#pragma unroll
+        for (int u = 0; u < VD / 32; ++u) ef[u] = ld8(e0 + (t0 + (iq < len ? iq : 0)) * es + 32 * u + 8 * g);
+      }
+      const float bh = d.h[iq], bl = d.l[iq];
+      float rsum = 0.f;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) {
+        const bool on = REV ? jt >= w : jt <= w;
+        f32x4 pv = {0.f, 0.f, 0.f, 0.f}, cs = pv;
+        if (on) {
+          f32x4 a = pv, a2 = pv;
+#pragma unroll
+          for (int u = 0; u < NU; ++u) a = mma(ld8(Ks + (16 * jt + i) * KP + 32 * u + 8 * g), qf[u], a);
+          if (DOT == 2) {
+#pragma unroll
+            for (int u = 0; u < VD / 32; ++u) a2 = mma(ld8(Vs + (16 * jt + i) * VP + 32 * u + 8 * g), ef[u], a2);
+          }
+          const f32x4 jh = *reinterpret_cast<const f32x4*>(d.h + 16 * jt + 4 * g);
+          const f32x4 jl = *reinterpret_cast<const f32x4*>(d.l + 16 * jt + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * jt + 4 * g + r;
+            const float diff = REV ? (jh[r] - bh) + (jl[r] - bl) : (bh - jh[r]) + (bl - jl[r]);
+            const float x = a[r] * (p.scale * __builtin_amdgcn_exp2f(diff));
+            pv[r] = (REV ? j >= iq : j <= iq) ? x : 0.f;
+            if (DOT == 2) {
+              const float ww = (REV ? j >= iq : j <= iq) && iq < len && j < len ? x * a2[r] : 0.f;
+              rsum += ww;
+              cs[r] = group_sum<16>(ww);
+            }
+          }
+        }
+        if (DOT == 2 && i == 0) *reinterpret_cast<f32x4*>(cols[w] + 16 * jt + 4 * g) = cs;
+        const bf16x4 hi = to_bf16x4(pv[0], pv[1], pv[2], pv[3]);
+        const bf16x4 lo = to_bf16x4(pv[0] - (float)hi[0], pv[1] - (float)hi[1], pv[2] - (float)hi[2], pv[3] - (float)hi[3]);
+        const int at = iq * kPP + 32 * (jt >> 1) + 8 * g + 4 * (jt & 1);
+        *reinterpret_cast<bf16x4*>(Ps[0] + at) = hi;
+        *reinterpret_cast<bf16x4*>(Ps[1] + at) = lo;
+      }
+      if (DOT == 2) {
+        rsum = xor32_sum(xor16_sum(rsum));
+        if (g == 0) rows[iq] = rsum;
+      }
+    }
+    // ---- the state's share: O^T = S^T Q^T, columns = tokens
+    f32x4 acc[4][NCT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (held) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        bf16x8 part[NCT][NS];
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = st.s[2 * u + (e >> 2)][ct][e & 3];
+#pragma unroll
+          for (int n = 0; n < NS; ++n) part[ct][n] = next_part(x);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const bf16x8 qf = ld8(Qs + (16 * t + i) * KP + 32 * u + 8 * g);
+#pragma unroll
+          for (int n = NS - 1; n >= 0; --n)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(part[ct][n], qf, acc[t][ct]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float wi = d.win[16 * t + i];
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) acc[t][ct] *= wi;
+      }
+    }
+    if (DOT) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int row = 16 * t + i;
+        const bf16* er = e0 + (t0 + (row < len ? row : 0)) * es + 16 * NCT * w + 4 * NCT * g;
+        float x = 0.f;
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          const bf16x4 ev = *reinterpret_cast<const bf16x4*>(er + 4 * ct);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x += acc[t][ct][r] * (float)ev[r];
+        }
+        x = xor32_sum(xor16_sum(x));
+        if (g == 0) dots[w][row] = x;
+      }
+    }
+    __syncthreads();  // scores and dots are written
+    // ---- the scores' share: O^T += V^T P^T
+    if (!bad[ci & 1]) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        bf16x8 vf[NCT];
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) vf[ct] = ld8_tr_cols<NCT>(Vs, VP, 32 * k2, 16 * NCT * w + 4 * ct, lane);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (REV ? t >= 2 && k2 == 0 : t < 2 && k2 == 1) continue;  // all masked
+#pragma unroll
+          for (int n = 1; n >= 0; --n) {
+            const bf16x8 pf = ld8(Ps[n] + (16 * t + i) * kPP + 32 * k2 + 8 * g);
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(vf[ct], pf, acc[t][ct]);
+          }
+        }
+      }
+    } else {  // an infinity or NaN in v reaches the tokens that see it, not those whose score is masked
+      for (int j = 0; j < len; ++j) {
+        const bf16* vr = Vs + j * VP + 16 * NCT * w + 4 * NCT * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int row = 16 * t + i;
+          if (REV ? j < row : j > row) continue;
+          const float x = (float)Ps[0][row * kPP + tok_col(j)] + (float)Ps[1][row * kPP + tok_col(j)];
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][ct][r] += x * (float)vr[4 * ct + r];
+        }
+      }
+    }
+    if (ci + 1 < nc || wants_fin) {
+      st.update(d, Ks, Vs, w, lane);
+      held = true;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = 16 * t + i;
+      if (row >= len) continue;
+      OT* dst = o0 + (int64_t)(t0 + row) * p.HV * VD + 16 * NCT * w + 4 * NCT * g;
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) {
+        if constexpr (sizeof(OT) == 4) {
+          *reinterpret_cast<f32x4*>(dst + 4 * ct) = acc[t][ct];
+        } else if constexpr (NCT == 2) {
+          if (ct == 0) *reinterpret_cast<bf16x8*>(dst) = pack8(acc[t][0], acc[t][NCT - 1]);
+        } else {
+          *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
+        }
+      }
+    }
+    if (DOT && w == 0 && lane < len) {
+      float x = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < 4; ++ww) x += dots[DOT ? ww : 0][lane];
+      if (DOT == 2) {
+        x += rows[lane];
+#pragma unroll
+        for (int ww = 0; ww < 4; ++ww) x -= cols[DOT == 2 ? ww : 0][lane];
+      }
+      const int64_t tokens = p.cu ? p.T : p.N * p.T;
+      p.dot[hv * tokens + sg.tok + t0 + lane] = x;
+    }
+    __syncthreads();  // the tiles are read
+  }
+  if (wants_fin) st.store(p.fin + (sg.n * p.HV + hv) * (KD * VD), w, lane);
+}
+
+// ------------------------------------------------------------------------------------------------
+// dg of a segment: what lies behind it is <S, R> at its end (the state entering the next segment with what the walk from
+// the end brings there; <S_T, dS_T> at the sequence's end), then the sum from the end of q . dq - k . dk.
+struct LinGateGrad {
+  const float *x, *y;              // [HV][tokens] q . dq and k . dk
+  const float *entry, *rentry;     // the states at the segments' borders, or null
+  const float *fin, *dfin;         // at the sequences' ends; either may be null (dfin: a zero gradient)
+  void* out;                       // [tokens][HV]
+  int dtype;
+  int64_t elems;                   // K V
+};
+
+__global__ __launch_bounds__(256) void gated_deltaless_gate_grad_kernel(LinParams p, LinGateGrad a) {
+  __shared__ double part[4];
+  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
+  const int64_t hv = blockIdx.x % p.HV;
+  const Segment sg = find_segment(p, blockIdx.x / p.HV);
+  if (!sg.some) return;
+  const float *s = nullptr, *r = nullptr;
+  if (!sg.last) {
+    s = a.entry + ((sg.slot + 1) * p.HV + hv) * a.elems;
+    r = a.rentry + (sg.slot * p.HV + hv) * a.elems;
+  } else if (a.fin && a.dfin) {
+    s = a.fin + (sg.n * p.HV + hv) * a.elems;
+    r = a.dfin + (sg.n * p.HV + hv) * a.elems;
+  }
+  double sum = 0.;
+  if (s) {
+    for (int64_t at = threadIdx.x * 4; at < a.elems; at += 1024) {
+      const f32x4 u = *reinterpret_cast<const f32x4*>(s + at), v = *reinterpret_cast<const f32x4*>(r + at);
+      sum += (double)(u[0] * v[0] + u[1] * v[1]) + (double)(u[2] * v[2] + u[3] * v[3]);
+    }
+    for (int m = 1; m < kWave; m <<= 1) sum += __shfl_xor(sum, m, kWave);
+    if (lane == 0) part[w] = sum;
+    __syncthreads();
+    sum = part[0] + part[1] + part[2] + part[3];
+    __syncthreads();
+  }
+  const int64_t tokens = p.cu ? p.T : p.N * p.T, base = hv * tokens + sg.tok;
+  for (int hi = sg.len; hi > 0; hi -= 256) {  // 256 tokens a step: wave w those from hi - 64 (w + 1) on
+    const int t = hi - kWave * (w + 1) + lane;
+    const double x = t >= 0 ? (double)a.x[base + t] - (double)a.y[base + t] : 0.;
+    double run = x;
+    for (int m = 1; m < kWave; m <<= 1) {
+      const double other = __shfl_down(run, m, kWave);
+      if (lane + m < kWave) run += other;
+    }
+    if (lane == 0) part[w] = run;
+    __syncthreads();
+    for (int ww = 0; ww < 4; ++ww) {
+      if (ww < w) run += part[ww];
+    }
+    if (t >= 0) store_from_f32(a.out, a.dtype, (sg.tok + t) * p.HV + hv, (float)(sum + run));
+    sum += part[0] + part[1] + part[2] + part[3];
+    __syncthreads();
+  }
+}
+
+// Sums the gradients of the value heads that share a q/k head: [rows][rep][D] fp32 -> [rows][D] bf16.
+__global__ __launch_bounds__(256) void gated_deltaless_head_sum_kernel(const float* x, bf16* y, int64_t rows, int rep, int D) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= rows * D) return;
+  const float* src = x + at / D * rep * D + at % D;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(src);
+  for (int r = 1; r < rep; ++r) sum += *reinterpret_cast<const f32x4*>(src + (int64_t)r * D);
+  *reinterpret_cast<bf16x4*>(y + at) = to_bf16x4(sum[0], sum[1], sum[2], sum[3]);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+struct LinPlan {
+  int shift;
+  int64_t spq, slots;  // segments of a sequence without cu, slots in all
+  bool split;
+};
+
+// Segments of a power of two of tokens, as short as gives kLinGroups workgroups and no shorter than kLinMinSegment.
+constexpr int64_t kLinGroups = 512, kLinMinSegment = 256;
+
+static LinPlan lin_plan(int64_t B, int64_t T, int64_t HV, int64_t N, bool varlen) {
+  LinPlan pl{};
+  int64_t L = kLinMinSegment;
+  pl.shift = 8;
+  while (L < T && (B * T / L) * HV > kLinGroups) {
+    L <<= 1;
+    ++pl.shift;
+  }
+  pl.spq = T > L ? (T + L - 1) / L : 1;
+  pl.slots = varlen ? (T >> pl.shift) + N : N * pl.spq;
+  pl.split = T > L;
+  return pl;
+}
+
+static int64_t align256l(int64_t b) { return (b + 255) / 256 * 256; }
+static int64_t lin_states_bytes(const LinPlan& pl, int64_t HV, int64_t K, int64_t V) {
+  return pl.split ? align256l(pl.slots * HV * K * V * 4) + align256l(pl.slots * HV * 4) : 0;
+}
+
+template <bool REV>
+static void launch_segments(LinParams p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
+  const dim3 grid((unsigned)(pl.slots * p.HV)), nt(kLinNT);
+  if (K == 128 && V == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, 128, REV>), grid, nt, 0, s, p);
+  else if (K == 64 && V == 64) hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, 64, REV>), grid, nt, 0, s, p);
+  else if (K == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, 64, REV>), grid, nt, 0, s, p);
+  else hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, 128, REV>), grid, nt, 0, s, p);
+  hipLaunchKernelGGL((gated_deltaless_scan_kernel<REV>), dim3((unsigned)(p.N * p.HV * (K * V / 1024))), dim3(256), 0, s, p,
+                     K * V);
+}
+
+template <bool REV, int DOT, typename OT>
+static void launch_walk(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
+  const dim3 grid((unsigned)(pl.slots * p.HV)), nt(kLinNT);
+  if (K == 128 && V == 128) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<128, 128, REV, DOT, OT>), grid, nt, 0, s, p);
+  else if (K == 64 && V == 64) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<64, 64, REV, DOT, OT>), grid, nt, 0, s, p);
+  else if (K == 128) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<128, 64, REV, DOT, OT>), grid, nt, 0, s, p);
+  else hipLaunchKernelGGL((gated_deltaless_chunk_kernel<64, 128, REV, DOT, OT>), grid, nt, 0, s, p);
+}
+
+static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int64_t N,
+                     bool varlen, int g_dtype, const void* const* ptrs, int nptrs) {
+  if (B <= 0 || T < 0 || H <= 0 || HV <= 0 || HV % H || N <= 0 || (varlen ? B != 1 : N != B)) {
+    gdn_internal_set_error("%s: bad sizes B=%lld T=%lld H=%lld HV=%lld N=%lld (cu_seqlens requires B == 1, N == B without "
+                           "it)", name, (long long)B, (long long)T, (long long)H, (long long)HV, (long long)N);
+    return GDN_ERR_INVALID;
+  }
+  if ((K != 64 && K != 128) || (V != 64 && V != 128)) {
+    gdn_internal_set_error("%s: head dims K=%lld V=%lld unsupported (each must be 64 or 128)", name, (long long)K,
+                           (long long)V);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (g_dtype < GDN_DTYPE_F32 || g_dtype > GDN_DTYPE_F16) {
+    gdn_internal_set_error("%s: unknown gate dtype %d", name, g_dtype);
+    return GDN_ERR_INVALID;
+  }
+  for (int n = 0; n < nptrs; ++n)
+    if (reinterpret_cast<uintptr_t>(ptrs[n]) & 15) {
+      gdn_internal_set_error("%s: tensors must be 16-byte aligned", name);
+      return GDN_ERR_INVALID;
+    }
+  const LinPlan pl = lin_plan(B, T, HV, N, varlen);
+  if (pl.slots * HV > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
+    gdn_internal_set_error("%s: too many sequences, heads or tokens for one launch", name);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  return GDN_OK;
+}
+
+static LinParams lin_params(const LinPlan& pl, const void* g, int g_dtype, int64_t gb, int64_t gt, int64_t gh, const void* cu,
+                            unsigned flags, int64_t T, int64_t N, int64_t HV, float scale) {
+  LinParams p{};
+  p.g = g;
+  p.dg = g_dtype;
+  p.gb = gb;
+  p.gt = gt;
+  p.gh = gh;
+  p.cu = cu;
+  p.cu_i32 = (flags & GDN_FLAG_CU_INT32) ? 1 : 0;
+  p.shift = pl.shift;
+  p.T = T;
+  p.N = N;
+  p.HV = HV;
+  p.spq = pl.spq;
+  p.scale = scale;
+  return p;
+}
+
+// The walk's q, k, v and e with the number of value heads that share a head of each.
+static void lin_roles(LinParams& p, const void* q, int rq, const void* k, int rk, const void* v, int rv, const void* e,
+                      int re) {
+  p.q = static_cast<const bf16*>(q);
+  p.k = static_cast<const bf16*>(k);
+  p.v = static_cast<const bf16*>(v);
+  p.e = static_cast<const bf16*>(e);
+  p.rq = rq;
+  p.rk = rk;
+  p.rv = rv;
+  p.re = re;
+}
+
+static void lin_states(LinParams& p, const LinPlan& pl, char* states, int64_t K, int64_t V) {
+  p.entry = pl.split ? reinterpret_cast<float*>(states) : nullptr;
+  p.decay = pl.split ? reinterpret_cast<float*>(states + align256l(pl.slots * p.HV * K * V * 4)) : nullptr;
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" size_t gdn_decay_attn_states_size(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int64_t N, int varlen) {
+  if (B <= 0 || T < 0 || HV <= 0 || K <= 0 || V <= 0 || N <= 0) return 0;
+  return (size_t)lin_states_bytes(lin_plan(B, T, HV, N, varlen != 0), HV, K, V);
+}
+
+extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
+                                  void* o, float* final_state, const void* cu_seqlens, int64_t B, int64_t T, int64_t H,
+                                  int64_t HV, int64_t K, int64_t V, int64_t N, int g_dtype, int64_t g_batch_stride,
+                                  int64_t g_token_stride, int64_t g_head_stride, float scale, unsigned flags, void* states,
+                                  size_t states_bytes, void* stream) {
+  if (!q || !k || !v || !o) {
+    gdn_internal_set_error("gdn_decay_attn_fwd: null tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  const void* ptrs[] = {q, k, v, o, initial_state, final_state, states};
+  if (int rc = lin_check("gdn_decay_attn_fwd", B, T, H, HV, K, V, N, cu_seqlens != nullptr, g_dtype, ptrs, 7)) return rc;
+  const LinPlan pl = lin_plan(B, T, HV, N, cu_seqlens != nullptr);
+  const size_t need = (size_t)lin_states_bytes(pl, HV, K, V);
+  if (need && (!states || states_bytes < need)) {
+    gdn_internal_set_error("gdn_decay_attn_fwd: states of %zu bytes needed", need);
+    return GDN_ERR_INVALID;
+  }
+  if (T == 0) return GDN_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rep = (int)(HV / H);
+  LinParams p = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N, HV, scale);
+  lin_roles(p, q, rep, k, rep, v, 1, nullptr, 1);
+  lin_states(p, pl, static_cast<char*>(states), K, V);
+  p.init = initial_state;
+  if (pl.split) launch_segments<false>(p, pl, K, V, s);
+  p.fin = final_state;
+  p.o = o;
+  launch_walk<false, 0, bf16>(p, pl, K, V, s);
+  return gdn_internal_check_launch("gated_deltaless_chunk_kernel");
+}
+
+// Workspace of the backward: the states of the walk from the end, the gate's two dot products, and with shared q/k heads
+// dq and dk of every value head in fp32.
+namespace {
+struct LinBwdSpace {
+  int64_t states, dots, heads;
+  int64_t bytes(bool shared) const { return states + 2 * dots + (shared ? 2 * heads : 0); }
+};
+LinBwdSpace lin_bwd_space(const LinPlan& pl, int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V) {
+  return {lin_states_bytes(pl, HV, K, V), align256l(B * T * HV * 4), align256l(B * T * HV * K * 4)};
+}
+}  // namespace
+
+extern "C" size_t gdn_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                                    int64_t N, int varlen) {
+  if (B <= 0 || T < 0 || H <= 0 || HV <= 0 || HV % H || K <= 0 || V <= 0 || N <= 0) return 0;
+  return (size_t)lin_bwd_space(lin_plan(B, T, HV, N, varlen != 0), B, T, HV, K, V).bytes(HV != H);
+}
+
+extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
+                                  const float* final_state, const void* d_o, const float* d_final_state, const void* states,
+                                  const void* cu_seqlens, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                  int64_t N, int g_dtype, int64_t g_batch_stride, int64_t g_token_stride,
+                                  int64_t g_head_stride, float scale, unsigned flags, void* dq, void* dk, void* dv, void* dg,
+                                  float* d_initial_state, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k || !v || !d_o || !dq || !dk || !dv || (dg && !g)) {
+    gdn_internal_set_error("gdn_decay_attn_bwd: null tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  if (dg && d_final_state && !final_state) {
+    gdn_internal_set_error("gdn_decay_attn_bwd: dg with d_final_state needs final_state");
+    return GDN_ERR_INVALID;
+  }
+  const void* ptrs[] = {q, k, v, d_o, dq, dk, dv, initial_state, final_state, d_final_state, d_initial_state, states,
+                        workspace};
+  if (int rc = lin_check("gdn_decay_attn_bwd", B, T, H, HV, K, V, N, cu_seqlens != nullptr, g_dtype, ptrs, 13)) return rc;
+  const LinPlan pl = lin_plan(B, T, HV, N, cu_seqlens != nullptr);
+  const bool shared = H != HV;
+  const LinBwdSpace sp = lin_bwd_space(pl, B, T, HV, K, V);
+  if ((pl.split && !states) || (sp.bytes(shared) && (!workspace || workspace_bytes < (size_t)sp.bytes(shared)))) {
+    gdn_internal_set_error("gdn_decay_attn_bwd: the forward's states and a workspace of %lld bytes are needed",
+                           (long long)sp.bytes(shared));
+    return GDN_ERR_INVALID;
+  }
+  if (T == 0) return GDN_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rep = (int)(HV / H);
+  char* ws = static_cast<char*>(workspace);
+  float* dot_q = reinterpret_cast<float*>(ws + sp.states);
+  float* dot_k = reinterpret_cast<float*>(ws + sp.states + sp.dots);
+  float* dq_heads = reinterpret_cast<float*>(ws + sp.states + 2 * sp.dots);
+  float* dk_heads = reinterpret_cast<float*>(ws + sp.states + 2 * sp.dots + sp.heads);
+  const LinParams base = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N,
+                                    HV, scale);
+  // from the end: R's segments, then dv and dk
+  LinParams r = base;
+  lin_roles(r, k, rep, q, rep, d_o, 1, nullptr, 1);
+  lin_states(r, pl, ws, K, V);
+  r.init = d_final_state;
+  if (pl.split) launch_segments<true>(r, pl, K, V, s);
+  LinParams a = r;
+  a.o = dv;
+  a.fin = d_initial_state;
+  launch_walk<true, 0, bf16>(a, pl, K, V, s);
+  a = r;
+  lin_roles(a, v, 1, d_o, 1, q, rep, k, rep);
+  a.transposed = 1;
+  a.dot = dot_k;
+  a.o = shared ? static_cast<void*>(dk_heads) : dk;
+  if (shared) dg ? launch_walk<true, 1, float>(a, pl, V, K, s) : launch_walk<true, 0, float>(a, pl, V, K, s);
+  else dg ? launch_walk<true, 1, bf16>(a, pl, V, K, s) : launch_walk<true, 0, bf16>(a, pl, V, K, s);
+  // from the start: dq
+  LinParams f = base;
+  lin_roles(f, d_o, 1, v, 1, k, rep, q, rep);
+  lin_states(f, pl, static_cast<char*>(const_cast<void*>(states)), K, V);
+  f.init = initial_state;
+  f.transposed = 1;
+  f.dot = dot_q;
+  f.o = shared ? static_cast<void*>(dq_heads) : dq;
+  if (shared) dg ? launch_walk<false, 2, float>(f, pl, V, K, s) : launch_walk<false, 0, float>(f, pl, V, K, s);
+  else dg ? launch_walk<false, 2, bf16>(f, pl, V, K, s) : launch_walk<false, 0, bf16>(f, pl, V, K, s);
+  if (dg) {
+    const LinGateGrad gg{dot_q, dot_k, f.entry, r.entry, final_state, d_final_state, dg, g_dtype, K * V};
+    hipLaunchKernelGGL(gated_deltaless_gate_grad_kernel, dim3((unsigned)(pl.slots * HV)), dim3(256), 0, s, base, gg);
+  }
+  if (shared) {
+    const int64_t rows = B * T * H, blocks = (rows * K / 4 + 255) / 256;
+    hipLaunchKernelGGL(gated_deltaless_head_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dq_heads,
+                       static_cast<bf16*>(dq), rows, rep, (int)K);
+    hipLaunchKernelGGL(gated_deltaless_head_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dk_heads,
+                       static_cast<bf16*>(dk), rows, rep, (int)K);
+  }
+  return gdn_internal_check_launch("gated_deltaless_chunk_kernel(bwd)");
+}

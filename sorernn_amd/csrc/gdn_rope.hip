@@ -1,0 +1,299 @@
+// RMSNorm of every query and key head with the rotary position embedding in the same pass, and its backward.
+//
+//   y = x rsqrt(mean(x^2) + eps) w;  out = y with its first rot entries rotated: (lo c - hi s, hi c + lo s),
+//   lo = y[0 : rot / 2], hi = y[rot / 2 : rot], c, s = cos, sin(position theta^(-2f / rot)), f = 0 .. rot / 2 - 1
+//
+// fp32 throughout, one rounding at the end. Bound by the bytes of the rows: D / 8 lanes take a row, 16 bytes (fp32: 32)
+// each. Angles are taken in turns in 64 bits, position * (theta^(-2f / rot) / 2 pi) less its whole part: at position
+// 1,000,000 a 32-bit angle is off by 0.06 rad. A token's rot / 2 pairs of cos and sin are computed once, into LDS, for
+// all its heads.
+
+#include <math.h>
+
+#include <type_traits>
+
+#include "gdn_common.h"
+
+namespace gdn {
+
+constexpr int kRopeTok = 4;          // tokens of a workgroup's step, at most
+constexpr int kRopeBwdBlocks = 1024; // workgroups of the backward, at most: each leaves one row of weight gradient sums
+
+struct QkRopeParams {
+  const void* x[2];              // q, k [B, T, heads, D] by strides (elements), last axis contiguous
+  int64_t sb[2], st[2], sh[2];
+  const void* dy[2];             // backward: [B, T, heads, D] contiguous
+  const float* w[2];             // [D] or null
+  void* y[2];                    // forward: out, backward: dx; contiguous
+  float* partial;                // backward: [blocks][2][D]
+  const void* pos;               // [B, T] by strides, or null: the token index, from each document's start with cu
+  int64_t pb, pt;
+  const void* cu;
+  int pos_i32, cu_i32;
+  int64_t T, N, tokens;
+  int heads[2], rot, step;       // step: tokens of a workgroup's step
+  float eps;
+  double turns[128];             // theta^(-2f / rot) / 2 pi
+};
+
+__device__ __forceinline__ int64_t rope_position(const QkRopeParams& p, int64_t bt) {
+  if (p.pos) return load_index(p.pos, p.pos_i32, bt / p.T * p.pb + bt % p.T * p.pt);
+  if (!p.cu) return bt % p.T;
+  int64_t lo = 0, hi = p.N;  // cu[lo] <= bt < cu[hi]
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (load_index(p.cu, p.cu_i32, mid) <= bt) lo = mid;
+    else hi = mid;
+  }
+  return bt - load_index(p.cu, p.cu_i32, lo);
+}
+
+template <int D, typename E, bool BWD>
+__global__ __launch_bounds__(256) void gated_delta_qk_norm_rope_kernel(QkRopeParams p) {
+  constexpr int LPR = D / 8, RPP = 256 / LPR, U = sizeof(E) == 2 ? 4 : 2;  // lanes a row, rows a pass, passes in flight
+  using V8 __attribute__((aligned(16))) = E __attribute__((ext_vector_type(8)));
+  __shared__ float cs[kRopeTok][2][D / 2];
+  __shared__ float sums[BWD ? 2 * RPP * D : 1];
+  const int li = threadIdx.x % LPR, d0 = 8 * li, lane = threadIdx.x % kWave, half = p.rot >> 1;
+  const int hs = p.heads[0] + p.heads[1];
+  const bool lo = d0 < half, in_rot = d0 < p.rot;
+  const int other = in_rot ? (lo ? lane + half / 8 : lane - half / 8) : lane;
+  float wt[2][8], dw[2][8];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      wt[m][e] = p.w[m] ? p.w[m][d0 + e] : 1.f;
+      dw[m][e] = 0.f;
+    }
+  for (int64_t bt0 = (int64_t)blockIdx.x * p.step; bt0 < p.tokens; bt0 += (int64_t)gridDim.x * p.step) {
+    const int nt = p.tokens - bt0 < p.step ? (int)(p.tokens - bt0) : p.step, nrows = nt * hs;
+    __syncthreads();  // the table of the step before is read
+    for (int c = threadIdx.x; c < nt * half; c += 256) {
+      const int tk = c / half, f = c % half;
+      const double turn = (double)rope_position(p, bt0 + tk) * p.turns[f];
+      float sv, cv;
+      sincospif(2.f * (float)(turn - rint(turn)), &sv, &cv);
+      cs[tk][0][f] = cv;
+      cs[tk][1][f] = sv;
+    }
+    __syncthreads();
+    for (int r0 = threadIdx.x / LPR; r0 < nrows; r0 += U * RPP) {  // uniform inside a row's lanes
+      V8 xv[U], dv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * RPP < nrows ? r0 + u * RPP : r0, tk = r / hs, m = r % hs >= p.heads[0];
+        const int hh = r % hs - (m ? p.heads[0] : 0);
+        const int64_t bt = bt0 + tk;
+        xv[u] = *reinterpret_cast<const V8*>(static_cast<const E*>(p.x[m]) + bt / p.T * p.sb[m] + bt % p.T * p.st[m] +
+                                             hh * p.sh[m] + d0);
+        if (BWD) dv[u] = *reinterpret_cast<const V8*>(static_cast<const E*>(p.dy[m]) + (bt * p.heads[m] + hh) * D + d0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * RPP;
+        if (r >= nrows) break;
+        const int tk = r / hs, m = r % hs >= p.heads[0], hh = r % hs - (m ? p.heads[0] : 0);
+        float x[8], ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = (float)xv[u][e];
+          ss += x[e] * x[e];
+        }
+        const float rr = 1.f / sqrtf(group_sum<LPR>(ss) / (float)D + p.eps);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = BWD ? (float)dv[u][e] : x[e] * rr * (m ? wt[1][e] : wt[0][e]);
+        float py[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) py[e] = __shfl(y[e], other, kWave);
+        if (in_rot) {
+          const int f = lo ? d0 : d0 - half;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float c = cs[tk][0][f + e], s = cs[tk][1][f + e];
+            y[e] = y[e] * c + ((lo != BWD) ? -py[e] : py[e]) * s;  // the backward turns by the negative angle
+          }
+        }
+        V8 out;
+        if (BWD) {
+          float dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float add = y[e] * (x[e] * rr);
+            dw[0][e] += m ? 0.f : add;
+            dw[1][e] += m ? add : 0.f;
+            y[e] *= m ? wt[1][e] : wt[0][e];
+            dot += y[e] * x[e];
+          }
+          const float c = rr * (rr * (group_sum<LPR>(dot) / (float)D));  // of the order of y: r^3 alone may be subnormal
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = rr * y[e] - x[e] * rr * c;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = (E)y[e];
+        *reinterpret_cast<V8*>(static_cast<E*>(p.y[m]) + ((bt0 + tk) * p.heads[m] + hh) * D + d0) = out;
+      }
+    }
+  }
+  if (BWD && p.partial) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[((int)(threadIdx.x / LPR) * 2 + m) * D + d0 + e] = dw[m][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * D; c += 256) {
+      float x = 0.f;
+      for (int r = 0; r < RPP; ++r) x += sums[r * 2 * D + c];
+      p.partial[(int64_t)blockIdx.x * 2 * D + c] = x;
+    }
+  }
+}
+
+// The weights' gradients from the workgroups' sums: 16 columns a workgroup, 16 threads a column, in a fixed order.
+__global__ __launch_bounds__(256) void gated_delta_qk_norm_rope_param_grad_kernel(const float* partial, int rows, int D,
+                                                                                 float* dqw, float* dkw) {
+  __shared__ float part[16][17];
+  const int col = threadIdx.x % 16, at = blockIdx.x * 16 + col;
+  float x = 0.f;
+  for (int r = threadIdx.x / 16; r < rows; r += 16) x += partial[(int64_t)r * 2 * D + at];
+  part[threadIdx.x / 16][col] = x;
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  x = 0.f;
+  for (int r = 0; r < 16; ++r) x += part[r][col];
+  float* out = at < D ? dqw : dkw;
+  if (out) out[at % D] = x;
+}
+
+static int rope_check(const char* name, QkRopeParams& p, int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t N,
+                      int dtype, int rot_dim, double theta, float eps) {
+  if (B <= 0 || T < 0 || HQ <= 0 || HK <= 0 || HQ + HK > 65536 || N <= 0 || (p.cu && (B != 1 || p.pos)) ||
+      !(theta > 0.) || !(theta < 1e300) || !(eps >= 0.f)) {
+    gdn_internal_set_error("%s: bad arguments B=%lld T=%lld HQ=%lld HK=%lld N=%lld theta=%g eps=%g (cu_seqlens requires "
+                           "B == 1 and no positions)", name, (long long)B, (long long)T, (long long)HQ, (long long)HK,
+                           (long long)N, theta, (double)eps);
+    return GDN_ERR_INVALID;
+  }
+  if ((D != 64 && D != 128 && D != 256) || rot_dim < 0 || rot_dim > D || rot_dim % 16) {
+    gdn_internal_set_error("%s: D=%lld rot_dim=%d unsupported (D = 64, 128 or 256, rot_dim a multiple of 16 up to D)", name,
+                           (long long)D, rot_dim);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (dtype < GDN_DTYPE_F32 || dtype > GDN_DTYPE_F16) {
+    gdn_internal_set_error("%s: unknown dtype %d", name, dtype);
+    return GDN_ERR_INVALID;
+  }
+  if (B * T > (1LL << 40)) {
+    gdn_internal_set_error("%s: too many tokens (%lld)", name, (long long)(B * T));
+    return GDN_ERR_UNSUPPORTED;
+  }
+  const int64_t unit = dtype == GDN_DTYPE_F32 ? 4 : 8;  // elements in 16 bytes
+  uintptr_t all = 0;
+  for (int m = 0; m < 2; ++m) {
+    all |= reinterpret_cast<uintptr_t>(p.x[m]) | reinterpret_cast<uintptr_t>(p.dy[m]) | reinterpret_cast<uintptr_t>(p.y[m]);
+    if (p.sb[m] % unit || p.st[m] % unit || p.sh[m] % unit) all |= 1;
+  }
+  if (all & 15) {
+    gdn_internal_set_error("%s: rows must be 16-byte aligned", name);
+    return GDN_ERR_INVALID;
+  }
+  p.T = T;
+  p.N = N;
+  p.tokens = B * T;
+  p.heads[0] = (int)HQ;
+  p.heads[1] = (int)HK;
+  p.rot = rot_dim;
+  p.eps = eps;
+  // 4 tokens share a workgroup once 1,024 workgroups have work without that
+  p.step = p.tokens >= 1024 * kRopeTok ? kRopeTok : 1;
+  for (int f = 0; f < rot_dim / 2; ++f) p.turns[f] = pow(theta, -2. * f / rot_dim) / 6.283185307179586;
+  return GDN_OK;
+}
+
+template <bool BWD>
+static void launch_rope(const QkRopeParams& p, int64_t D, int dtype, int64_t blocks, hipStream_t s) {
+  auto go = [&](auto e, auto d) {
+    hipLaunchKernelGGL((gated_delta_qk_norm_rope_kernel<decltype(d)::value, decltype(e), BWD>), dim3((unsigned)blocks),
+                       dim3(256), 0, s, p);
+  };
+  auto by_dim = [&](auto e) {
+    if (D == 64) go(e, std::integral_constant<int, 64>{});
+    else if (D == 128) go(e, std::integral_constant<int, 128>{});
+    else go(e, std::integral_constant<int, 256>{});
+  };
+  if (dtype == GDN_DTYPE_BF16) by_dim(bf16{});
+  else if (dtype == GDN_DTYPE_F16) by_dim(f16{});
+  else by_dim(float{});
+}
+
+static int64_t rope_bwd_blocks(int64_t tokens) {
+  const int64_t b = tokens >= 1024 * kRopeTok ? (tokens + kRopeTok - 1) / kRopeTok : tokens;
+  return b < kRopeBwdBlocks ? b : kRopeBwdBlocks;
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_qk_norm_rope_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                    const float* q_weight, const float* k_weight, const void* positions,
+                                    int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, void* q_out, void* k_out,
+                                    const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D,
+                                    int64_t N, int dtype, int rot_dim, double theta, float eps, unsigned flags,
+                                    void* stream) {
+  if (T > 0 && (!q || !k || !q_out || !k_out)) {
+    gdn_internal_set_error("gdn_qk_norm_rope_fwd: null tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  QkRopeParams p{{q, k}, {q_batch_stride, k_batch_stride}, {q_token_stride, k_token_stride}, {q_head_stride, k_head_stride},
+                 {nullptr, nullptr}, {q_weight, k_weight}, {q_out, k_out}, nullptr, positions, pos_batch_stride,
+                 pos_token_stride, cu_seqlens, pos_i32, (flags & GDN_FLAG_CU_INT32) ? 1 : 0};
+  if (int rc = rope_check("gdn_qk_norm_rope_fwd", p, B, T, HQ, HK, D, N, dtype, rot_dim, theta, eps)) return rc;
+  if (T == 0) return GDN_OK;
+  const int64_t steps = (p.tokens + p.step - 1) / p.step;
+  launch_rope<false>(p, D, dtype, steps < 0x7fffffffLL ? steps : 0x7fffffffLL, static_cast<hipStream_t>(stream));
+  return gdn_internal_check_launch("gated_delta_qk_norm_rope_kernel");
+}
+
+extern "C" size_t gdn_qk_norm_rope_bwd_workspace_size(int64_t B, int64_t T, int64_t D) {
+  if (B <= 0 || T < 0 || D <= 0) return 0;
+  return (size_t)(rope_bwd_blocks(B * T) * 2 * D * 4);
+}
+
+extern "C" int gdn_qk_norm_rope_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                    const float* q_weight, const float* k_weight, const void* positions,
+                                    int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, const void* dq_out,
+                                    const void* dk_out, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                                    const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D,
+                                    int64_t N, int dtype, int rot_dim, double theta, float eps, unsigned flags,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (T > 0 && (!q || !k || !dq_out || !dk_out || !dq || !dk)) {
+    gdn_internal_set_error("gdn_qk_norm_rope_bwd: null tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  const bool params = dq_weight || dk_weight;
+  QkRopeParams p{{q, k}, {q_batch_stride, k_batch_stride}, {q_token_stride, k_token_stride}, {q_head_stride, k_head_stride},
+                 {dq_out, dk_out}, {q_weight, k_weight}, {dq, dk}, params ? static_cast<float*>(workspace) : nullptr,
+                 positions, pos_batch_stride, pos_token_stride, cu_seqlens, pos_i32, (flags & GDN_FLAG_CU_INT32) ? 1 : 0};
+  if (int rc = rope_check("gdn_qk_norm_rope_bwd", p, B, T, HQ, HK, D, N, dtype, rot_dim, theta, eps)) return rc;
+  const size_t need = gdn_qk_norm_rope_bwd_workspace_size(B, T, D);
+  if (params && need && (!workspace || workspace_bytes < need)) {
+    gdn_internal_set_error("gdn_qk_norm_rope_bwd: workspace of %zu bytes needed", need);
+    return GDN_ERR_INVALID;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t blocks = rope_bwd_blocks(p.tokens);
+  if (T > 0) {
+    launch_rope<true>(p, D, dtype, blocks, s);
+    if (int rc = gdn_internal_check_launch("gated_delta_qk_norm_rope_kernel(bwd)")) return rc;
+  }
+  if (params) {  // without tokens: zeros
+    hipLaunchKernelGGL(gated_delta_qk_norm_rope_param_grad_kernel, dim3((unsigned)(2 * D / 16)), dim3(256), 0, s, p.partial,
+                       (int)blocks, (int)D, dq_weight, dk_weight);
+    return gdn_internal_check_launch("gated_delta_qk_norm_rope_param_grad_kernel");
+  }
+  return GDN_OK;
+}
