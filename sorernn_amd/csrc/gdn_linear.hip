@@ -13,8 +13,8 @@
 //                                      (k, q, do) and (v, do, q)
 //   dg_t = exp(g_t) <S_{t-1}, R_t> = sum over i >= t of (q_i . dq_i - k_i . dk_i), plus <S_T, dS_T>
 //
-// A workgroup of 4 waves walks one segment of a sequence for one value head. The state stays in fp32 MFMA
-// accumulators, wave w holding all K rows of its V / 4 columns; it is the A operand of S^T Q^T as it stands, split into
+// A workgroup of V / 16 waves walks one segment of a sequence for one value head. The state stays in fp32 MFMA
+// accumulators, wave w holding all K rows of 16 columns; it is the A operand of S^T Q^T as it stands, split into
 // bf16 parts in registers. Sequences are cut into segments so that few heads fill the chip: a first kernel walks
 // the segments for their own contribution to the state (k and v only), a scan over the segments turns these into the
 // states that enter them, and the walkers then run side by side.
@@ -25,16 +25,16 @@
 // rounding of the output itself. The decays are summed in 64 bits: a difference of two sums in 32 would carry the
 // rounding of the sums into every weight.
 
+#include <type_traits>
+
 #include "gdn_mfma.h"
 
 namespace gdn {
 
-constexpr int kLinNT = 256;
-constexpr int kPP = kC + 8;  // pitch of the score tiles
-
 struct LinParams {
-  const bf16 *q, *k, *v, *e;    // [tokens][HV / r*][K or V]: the walk's q, k, v and the rows of the gate's dot products
-  int rq, rk, rv, re;           // value heads that share a head of each
+  const bf16 *q, *k, *v, *e;    // [tokens][heads][K or V]: the walk's q, k, v and the rows of the gate's dot products
+  int64_t qs, ks, vs, es;       // elements between tokens
+  unsigned rq, rk, rv, re;      // value heads that share a head of each
   const void* g;                // log decays, or null: no decay
   int dg;
   int64_t gb, gt, gh;           // element strides of batch row, token and value head
@@ -47,7 +47,8 @@ struct LinParams {
   float* dot;                   // [HV][tokens] with DOT
   const void* cu;
   int cu_i32, shift;            // segments of 1 << shift tokens
-  int64_t T, N, HV, spq;        // spq: segments of a sequence without cu
+  int64_t T, N;
+  unsigned HV, spq;             // spq: segments of a sequence without cu
   float scale;
 };
 
@@ -60,7 +61,7 @@ struct Segment {
 
 // Slots of a sequence: with cu, sequence n has the slots from (cu[n] >> shift) + n on, which leaves room for its
 // segments whatever the lengths are, so that the grid depends on T and N alone. All lanes of a wave search together.
-__device__ __forceinline__ Segment find_segment(const LinParams& p, int64_t slot) {
+__device__ __forceinline__ Segment find_segment(const LinParams& p, unsigned slot) {
   Segment s;
   int64_t bos, len, local;
   const int64_t L = (int64_t)1 << p.shift;
@@ -105,12 +106,11 @@ struct Decays {
   float all;
 };
 
-__device__ __forceinline__ double dpp_add64(double v, int lo, int hi) { return v + __hiloint2double(hi, lo); }
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ double dpp_scan_step(double v) {
   const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROW_MASK, 0xf, false);
   const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROW_MASK, 0xf, false);
-  return dpp_add64(v, lo, hi);
+  return v + __hiloint2double(hi, lo);
 }
 
 // Log decays below -100 (exp of it is 0 beside any weight that counts) are taken as -100: a reset of -inf leaves the
@@ -120,6 +120,7 @@ __device__ __forceinline__ double log2_decay(uint32_t raw, int dtype) {
   return (double)(x < -100.f ? -100.f : x) * 1.4426950408889634;
 }
 
+// One wave, lane = token.
 template <bool REV>
 __device__ __forceinline__ void chunk_decays(Decays& d, double x, float scale, int lane) {
   x = dpp_scan_step<0x111, 0xf>(x);
@@ -138,66 +139,84 @@ __device__ __forceinline__ void chunk_decays(Decays& d, double x, float scale, i
   if (lane == 0) d.all = __builtin_amdgcn_exp2f((float)all);
 }
 
-// The next bf16 part of 8 fp32 values: rounds them, and leaves in x what the rounding left out.
-__device__ __forceinline__ bf16x8 next_part(float (&x)[8]) {
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// A pair of bf16 as bits, kept in a scalar register: as a literal -1 the pair (-1, 0) is encoded as an inline constant,
+// which the dot product takes for (0, -1).
+__device__ __forceinline__ bf16x2 scalar_pair(uint32_t bits) {
+  asm("" : "+s"(bits));
+  return __builtin_bit_cast(bf16x2, bits);
+}
+
+// The next bf16 part of 8 fp32 values: rounds them, and leaves in x what the rounding left out. x - part is exact; as a
+// product with (-1, 0) or (0, -1) it needs no unpacking of the pair.
+__device__ __forceinline__ bf16x8 next_part(float (&x)[8], bool more) {
+  const bf16x2 lo = scalar_pair(0x0000bf80u), hi = scalar_pair(0xbf800000u);
   bf16x8 r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    r[e] = (bf16)x[e];
-    x[e] -= (float)r[e];
+  for (int e = 0; e < 8; e += 2) {
+    const bf16x2 h = {(bf16)x[e], (bf16)x[e + 1]};
+    r[e] = h[0];
+    r[e + 1] = h[1];
+    if (more) {
+      x[e] = __builtin_amdgcn_fdot2_f32_bf16(h, lo, x[e], false);
+      x[e + 1] = __builtin_amdgcn_fdot2_f32_bf16(h, hi, x[e + 1], false);
+    }
   }
   return r;
 }
 
-// Columns of wave w's tile ct, lane i of 16: 16 NCT w + 4 NCT (i / 4) + 4 ct + i % 4, so that an accumulator lane's
-// tiles hold 4 NCT neighbouring columns. The transposed read of 8 tokens of a column in the accumulators' token order.
-template <int NCT>
-__device__ __forceinline__ bf16x8 ld8_tr_cols(const bf16* tile, int pitch, int r0, int c0, int lane) {
-  const int g = lane >> 4, li = lane & 15;
-  const bf16* p0 = tile + (r0 + 4 * g + (li >> 2)) * pitch + c0 + 4 * NCT * (li & 3);
-  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p0));
-  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p0 + 16 * pitch));
+// Tiles in LDS: rows of D elements without padding, the 16-byte piece c of row r at piece c ^ swz(r). A row fragment
+// (16 rows, one piece) then falls on all 64 banks, and so do 8 rows of two neighbouring pieces (the transposed reads of
+// 16 columns); the transposed reads of 32 columns, half a piece each, take two turns.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D == 128 ? ((r & 3) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1))
+                  : (((r >> 2) & 1) << 2 | ((r >> 1) & 1) << 1 | ((r >> 3) & 1));
+}
+template <int D>
+__device__ __forceinline__ bf16x8 ld_row(const bf16* tile, int row, int piece) {
+  return ld8(tile + row * D + ((piece ^ swz<D>(row)) << 3));
+}
+// Rows r0 + 4g + m and r0 + 16 + 4g + m, m = 0..3, of one column: c0 + STEP (i / 4) + i % 4.
+template <int D, int STEP>
+__device__ __forceinline__ bf16x8 ld_cols(const bf16* tile, int r0, int c0, int lane) {
+  const int g = lane >> 4, li = lane & 15, row = r0 + 4 * g + (li >> 2), col = c0 + STEP * (li & 3);
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds_bf16x4*)(tile + row * D + (((col >> 3) ^ swz<D>(row)) << 3) + (col & 7)));
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds_bf16x4*)(tile + (row + 16) * D + (((col >> 3) ^ swz<D>(row + 16)) << 3) + (col & 7)));
   return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A chunk's rows on their way to LDS: thread t holds the 16-byte pieces t, t + 256, ... of the 64 x D tile. Rows past
-// the chunk's end re-read its first row and are written as zeros.
-template <int D>
+// A chunk's rows on their way to LDS: thread t of NT holds the 16-byte pieces t, t + NT, ... of the 64 x D tile. Rows
+// past the chunk's end re-read its first row and are written as zeros.
+template <int D, int NT>
 struct Tile {
-  bf16x8 r[D / 32];
+  static constexpr int NP = kC * D / 8 / NT;
+  bf16x8 r[NP];
   __device__ __forceinline__ void fetch(const bf16* base, int64_t stride, int len) {
 #pragma unroll
-    for (int n = 0; n < D / 32; ++n) {
-      const int c = threadIdx.x + n * kLinNT, row = c / (D / 8);
+    for (int n = 0; n < NP; ++n) {
+      const int c = threadIdx.x + n * NT, row = c / (D / 8);
       r[n] = *reinterpret_cast<const bf16x8*>(base + (row < len ? row : 0) * stride + (c % (D / 8)) * 8);
     }
   }
   __device__ __forceinline__ void put(bf16* tile, int len) const {
 #pragma unroll
-    for (int n = 0; n < D / 32; ++n) {
-      const int c = threadIdx.x + n * kLinNT, row = c / (D / 8);
-      *reinterpret_cast<bf16x8*>(tile + row * (D + 8) + (c % (D / 8)) * 8) = row < len ? r[n] : bf16x8{};
+    for (int n = 0; n < NP; ++n) {
+      const int c = threadIdx.x + n * NT, row = c / (D / 8);
+      *reinterpret_cast<bf16x8*>(tile + row * D + (((c % (D / 8)) ^ swz<D>(row)) << 3)) = row < len ? r[n] : bf16x8{};
     }
-  }
-  // any infinity or NaN among the valid rows
-  __device__ __forceinline__ bool unbounded(int len) const {
-    uint32_t any = 0;
-#pragma unroll
-    for (int n = 0; n < D / 32; ++n) {
-      const u32x4 w = __builtin_bit_cast(u32x4, r[n]);
-      const bool in = (int)(threadIdx.x + n * kLinNT) / (D / 8) < len;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) any |= in && ((w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u);
-    }
-    return any;
   }
 };
 
-// The state of wave w's columns: accumulator tiles s[2u + c][ct], rows 32u + 8g + 4c + r, column as above.
-template <int KD, int VD>
+// The state's columns of wave w of NW: accumulator tiles s[2u + c][ct], rows 32u + 8g + 4c + r, columns
+// 16 NCT w + 4 NCT (i / 4) + 4 ct + i % 4, so that 4 NCT neighbouring columns of O^T fall on a lane.
+template <int KD, int VD, int NW>
 struct State {
-  static constexpr int NCT = VD / 64;
-  f32x4 s[KD / 16][NCT];
+  static constexpr int NA = KD / 16, NCT = VD / 16 / NW;
+  f32x4 s[NA][NCT];
 
   __device__ __forceinline__ static int row0(int a, int g) { return 32 * (a >> 1) + 8 * g + 4 * (a & 1); }
   __device__ __forceinline__ static int col(int w, int ct, int i) {
@@ -205,18 +224,18 @@ struct State {
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int a = 0; a < KD / 16; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) s[a][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   __device__ __forceinline__ void load(const float* src, bool transposed, int w, int lane) {
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-    for (int a = 0; a < KD / 16; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
         if (transposed) {
-          s[a][ct] = *reinterpret_cast<const f32x4*>(src + (int64_t)col(w, ct, i) * KD + row0(a, g));
+          s[a][ct] = *reinterpret_cast<const f32x4*>(src + col(w, ct, i) * KD + row0(a, g));
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[a][ct][r] = src[(row0(a, g) + r) * VD + col(w, ct, i)];
@@ -226,94 +245,121 @@ struct State {
   __device__ __forceinline__ void store(float* dst, int w, int lane) const {
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
-    for (int a = 0; a < KD / 16; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) dst[(row0(a, g) + r) * VD + col(w, ct, i)] = s[a][ct][r];
+  }
+  // The wave's columns of 32 rows of V from r0 on, as the accumulators' token order has them.
+  __device__ __forceinline__ static void columns(const bf16* Vs, int r0, int w, int lane, bf16x8 (&vf)[NCT]) {
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) vf[ct] = ld_cols<VD, 4 * NCT>(Vs, r0, 16 * NCT * w + 4 * ct, lane);
   }
   // S = all S + K^T (wst V): V weighted in fp32 and split into three bf16 parts (K is exact)
   __device__ __forceinline__ void update(const Decays& d, const bf16* Ks, const bf16* Vs, int w, int lane) {
     const int g = lane >> 4;
     const float all = d.all;
 #pragma unroll
-    for (int a = 0; a < KD / 16; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) s[a][ct] *= all;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const f32x4 w0 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 4 * g);
       const f32x4 w1 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 16 + 4 * g);
-      bf16x8 part[NCT][3];
+      bf16x8 vf[NCT], part[NCT][3];
+      columns(Vs, 32 * ks, w, lane, vf);
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
-        const bf16x8 vf = ld8_tr_cols<NCT>(Vs, VD + 8, 32 * ks, 16 * NCT * w + 4 * ct, lane);
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)vf[e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+        for (int e = 0; e < 8; ++e) x[e] = (float)vf[ct][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) part[ct][n] = next_part(x);
+        for (int n = 0; n < 3; ++n) part[ct][n] = next_part(x, n < 2);
       }
+      constexpr int AB = 4 / NCT;  // rows of tiles whose products run side by side
 #pragma unroll
-      for (int a = 0; a < KD / 16; ++a) {
-        const bf16x8 kf = ld8_tr_pair(Ks, KD + 8, 32 * ks, 32 * (a >> 1) + 4 * (a & 1), lane);
+      for (int a0 = 0; a0 < NA; a0 += AB) {
+        bf16x8 kf[AB];
+#pragma unroll
+        for (int a = 0; a < AB; ++a)
+          kf[a] = ld_cols<KD, 8>(Ks, 32 * ks, 32 * ((a0 + a) >> 1) + 4 * ((a0 + a) & 1), lane);
 #pragma unroll
         for (int n = 2; n >= 0; --n)
 #pragma unroll
-          for (int ct = 0; ct < NCT; ++ct) s[a][ct] = mma(kf, part[ct][n], s[a][ct]);
+          for (int a = 0; a < AB; ++a)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) s[a0 + a][ct] = mma(kf[a], part[ct][n], s[a0 + a][ct]);
       }
     }
   }
 };
 
-__device__ __forceinline__ uint32_t gate_raw(const LinParams& p, const Segment& sg, int64_t hv, int t) {
+__device__ __forceinline__ uint32_t gate_raw(const LinParams& p, const Segment& sg, unsigned hv, int t) {
   return load_raw32(p.g, p.dg, sg.row * p.gb + (sg.col + t) * p.gt + hv * p.gh);
 }
+
+// The gate of a segment's chunks in walking order, read by one wave: the raw values of the chunk after the next in flight.
+template <bool REV>
+struct GateWalk {
+  uint32_t raw = 0;
+  __device__ __forceinline__ void fetch(const LinParams& p, const Segment& sg, unsigned hv, int ci, int nc, int lane) {
+    const int t = (REV ? nc - 1 - ci : ci) * kC + lane;
+    raw = p.g && ci < nc && t < sg.len ? gate_raw(p, sg, hv, t) : 0u;
+  }
+  __device__ __forceinline__ double value(const LinParams& p) const { return p.g ? log2_decay(raw, p.dg) : 0.; }
+};
 
 // ------------------------------------------------------------------------------------------------
 // A segment's own contribution to the state: the walk without outputs, from a zero state. Forward walks leave it in
 // the next segment's slot, walks from the end in the one before; the sequence's last segment (first) has none to give.
-template <int KD, int VD, bool REV>
-__global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_segment_kernel(LinParams p) {
-  __shared__ __align__(16) bf16 Ks[kC * (KD + 8)], Vs[kC * (VD + 8)];
-  __shared__ __align__(16) Decays d;
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  const int64_t hv = blockIdx.x % p.HV;
+template <int KD, int VD, int NW, bool REV>
+__global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_segment_kernel(LinParams p) {
+  constexpr int NT = NW * kWave;
+  __shared__ __align__(16) bf16 Ks[kC * KD], Vs[kC * VD];
+  __shared__ __align__(16) Decays d[2];
+  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const unsigned hv = blockIdx.x % p.HV;
   const Segment sg = find_segment(p, blockIdx.x / p.HV);
   if (!sg.some || (REV ? sg.first : sg.last)) return;
-  const int64_t ks = p.HV / p.rk * KD, vs = p.HV / p.rv * VD;  // token strides
-  const bf16* k0 = p.k + sg.tok * ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * vs + hv / p.rv * VD;
+  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
   const int nc = (sg.len + kC - 1) / kC;
-  Tile<KD> kt;
-  Tile<VD> vt;
-  uint32_t graw = 0;
+  Tile<KD, NT> kt;
+  Tile<VD, NT> vt;
+  GateWalk<REV> gate;
   auto fetch = [&](int ci) {
     const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    kt.fetch(k0 + t0 * ks, ks, len);
-    vt.fetch(v0 + t0 * vs, vs, len);
-    if (w == 0 && p.g) graw = lane < len ? gate_raw(p, sg, hv, t0 + lane) : 0u;
+    kt.fetch(k0 + t0 * p.ks, p.ks, len);
+    vt.fetch(v0 + t0 * p.vs, p.vs, len);
   };
-  State<KD, VD> st;
+  State<KD, VD, NW> st;
   st.zero();
   double total = 0.;
+  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
   fetch(0);
+  if (w == 0) {
+    total = gate.value(p);
+    chunk_decays<REV>(d[0], total, p.scale, lane);
+    gate.fetch(p, sg, hv, 1, nc, lane);
+  }
   for (int ci = 0; ci < nc; ++ci) {
     const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
     kt.put(Ks, len);
     vt.put(Vs, len);
-    if (w == 0) {
-      const double x = p.g ? log2_decay(graw, p.dg) : 0.;
-      total += x;
-      chunk_decays<REV>(d, x, p.scale, lane);
-    }
     __syncthreads();
     if (ci + 1 < nc) fetch(ci + 1);
-    st.update(d, Ks, Vs, w, lane);
+    if (w == 0 && ci + 1 < nc) {
+      const double x = gate.value(p);
+      total += x;
+      chunk_decays<REV>(d[(ci + 1) & 1], x, p.scale, lane);
+      gate.fetch(p, sg, hv, ci + 2, nc, lane);
+    }
+    st.update(d[ci & 1], Ks, Vs, w, lane);
     __syncthreads();
   }
-  const int64_t to = (sg.slot + (REV ? -1 : 1)) * p.HV + hv;
-  st.store(p.entry + to * (KD * VD), w, lane);
+  st.store(p.entry + ((sg.slot + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD), w, lane);
   if (w == 0) {
     for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
     if (lane == 0) p.decay[sg.slot * p.HV + hv] = __builtin_amdgcn_exp2f((float)total);
@@ -324,20 +370,19 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_segment_kernel(LinP
 // end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread.
 template <bool REV>
 __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, int64_t elems) {
-  const int64_t per = elems / 1024, chain = blockIdx.x / per;
-  const int64_t hv = chain % p.HV, n = chain / p.HV;
+  const unsigned per = (unsigned)elems / 1024, chain = blockIdx.x / per, hv = chain % p.HV, n = chain / p.HV;
   const int64_t at = (blockIdx.x % per) * 1024 + threadIdx.x * 4;
   int64_t slot0, cnt;
   if (p.cu) {
-    const int64_t bos = load_index(p.cu, p.cu_i32, n), eos = load_index(p.cu, p.cu_i32, n + 1);
+    const int64_t bos = load_index(p.cu, p.cu_i32, n), eos = load_index(p.cu, p.cu_i32, (int64_t)n + 1);
     slot0 = (bos >> p.shift) + n;
     cnt = (eos - bos + ((int64_t)1 << p.shift) - 1) >> p.shift;
   } else {
-    slot0 = n * p.spq;
+    slot0 = (int64_t)n * p.spq;
     cnt = p.spq;
   }
   if (cnt < 2) return;
-  const int64_t step = p.HV * elems;
+  const int64_t step = (int64_t)p.HV * elems;
   float* e = p.entry + (slot0 * p.HV + hv) * elems + at;
   const float* dc = p.decay + slot0 * p.HV + hv;
   f32x4 run = {0.f, 0.f, 0.f, 0.f};
@@ -364,39 +409,38 @@ __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, 
 // ------------------------------------------------------------------------------------------------
 // The walk. DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums
 // less the column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.
-template <int KD, int VD, bool REV, int DOT, typename OT>
-__global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinParams p) {
-  constexpr int NCT = VD / 64, KP = KD + 8, VP = VD + 8, NU = KD / 32;
+template <int KD, int VD, int NW, bool REV, int DOT, typename OT>
+__global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_chunk_kernel(LinParams p) {
+  constexpr int NT = NW * kWave, NCT = VD / 16 / NW, NU = KD / 32;
   constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
-  __shared__ __align__(16) bf16 Qs[kC * KP], Ks[kC * KP], Vs[kC * VP];
-  __shared__ __align__(16) bf16 Ps[2][kC * kPP];  // the two parts of the scores, tok_col columns
-  __shared__ __align__(16) Decays d;
-  __shared__ float dots[DOT ? 4 : 1][kC], rows[kC], cols[DOT == 2 ? 4 : 1][kC];
-  __shared__ int bad[2];
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave, g = lane >> 4, i = lane & 15;
-  const int64_t hv = blockIdx.x % p.HV;
+  constexpr int HALVES = NW / 4;   // waves that share the scores of 16 queries
+  __shared__ __align__(16) bf16 Qs[kC * KD], Ks[kC * KD], Vs[kC * VD];
+  __shared__ __align__(16) bf16 Ps[2][kC * kC];  // the two parts of the scores, tok_col columns, swizzled as the tiles
+  __shared__ __align__(16) Decays d[2];
+  __shared__ __align__(16) float dots[DOT ? NW : 1][kC], rows[HALVES][kC], cols[DOT == 2 ? 4 : 1][kC];
+  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int g = lane >> 4, i = lane & 15;
+  const unsigned hv = blockIdx.x % p.HV;
   const Segment sg = find_segment(p, blockIdx.x / p.HV);
   if (!sg.some) return;
-  const int64_t qs = p.HV / p.rq * KD, ks = p.HV / p.rk * KD, vs = p.HV / p.rv * VD, es = DOT ? p.HV / p.re * VD : 0;
-  const bf16* q0 = p.q + sg.tok * qs + hv / p.rq * KD;
-  const bf16* k0 = p.k + sg.tok * ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * vs + hv / p.rv * VD;
-  const bf16* e0 = DOT ? p.e + sg.tok * es + hv / p.re * VD : nullptr;
+  const bf16* q0 = p.q + sg.tok * p.qs + hv / p.rq * KD;
+  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
+  const bf16* e0 = DOT ? p.e + sg.tok * p.es + hv / p.re * VD : nullptr;
   OT* o0 = static_cast<OT*>(p.o) + (sg.tok * p.HV + hv) * VD;
   const int nc = (sg.len + kC - 1) / kC;
-  Tile<KD> qt, kt;
-  Tile<VD> vt;
-  uint32_t graw = 0;
+  Tile<KD, NT> qt, kt;
+  Tile<VD, NT> vt;
+  GateWalk<REV> gate;
   auto fetch = [&](int ci) {
     const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    qt.fetch(q0 + t0 * qs, qs, len);
-    kt.fetch(k0 + t0 * ks, ks, len);
-    vt.fetch(v0 + t0 * vs, vs, len);
-    if (w == 0 && p.g) graw = lane < len ? gate_raw(p, sg, hv, t0 + lane) : 0u;
+    qt.fetch(q0 + t0 * p.qs, p.qs, len);
+    kt.fetch(k0 + t0 * p.ks, p.ks, len);
+    vt.fetch(v0 + t0 * p.vs, p.vs, len);
   };
+  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
   fetch(0);
-  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-  State<KD, VD> st;
+  State<KD, VD, NW> st;
   const bool inner = REV ? !sg.last : !sg.first;  // a segment of this sequence comes before
   const float* src = inner ? p.entry + (sg.slot * p.HV + hv) * (KD * VD)
                            : (p.init ? p.init + (sg.n * p.HV + hv) * (KD * VD) : nullptr);
@@ -404,43 +448,49 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
   if (held) st.load(src, p.transposed, w, lane);
   else st.zero();
   const bool wants_fin = p.fin && (REV ? sg.first : sg.last);
-  __syncthreads();  // bad[] is set
+  if (w == 0) {
+    chunk_decays<REV>(d[0], gate.value(p), p.scale, lane);
+    gate.fetch(p, sg, hv, 1, nc, lane);
+  }
   for (int ci = 0; ci < nc; ++ci) {
     const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    const Decays& dc = d[ci & 1];
     qt.put(Qs, len);
     kt.put(Ks, len);
     vt.put(Vs, len);
-    if (vt.unbounded(len)) bad[ci & 1] = 1;
-    if (w == 0) chunk_decays<REV>(d, p.g ? log2_decay(graw, p.dg) : 0., p.scale, lane);
     __syncthreads();
     if (ci + 1 < nc) fetch(ci + 1);
-    if (threadIdx.x == 0) bad[(ci + 1) & 1] = 0;
-    // ---- the scores of queries 16 w ..: P^T tiles, rows = keys j, column = query
+    if (w == 0 && ci + 1 < nc) {
+      chunk_decays<REV>(d[(ci + 1) & 1], gate.value(p), p.scale, lane);
+      gate.fetch(p, sg, hv, ci + 2, nc, lane);
+    }
+    // ---- the scores of 16 queries: P^T tiles, rows = keys j, column = query; with 8 waves two take every other tile
     {
-      const int iq = 16 * w + i;
+      const int t = w / HALVES, iq = 16 * t + i;
       bf16x8 qf[NU], ef[DOT == 2 ? VD / 32 : 1];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) qf[u] = ld8(Qs + iq * KP + 32 * u + 8 * g);
+      for (int u = 0; u < NU; ++u) qf[u] = ld_row<KD>(Qs, iq, 4 * u + g);
       if (DOT == 2) {
 #pragma unroll
-        for (int u = 0; u < VD / 32; ++u) ef[u] = ld8(e0 + (t0 + (iq < len ? iq : 0)) * es + 32 * u + 8 * g);
+        for (int u = 0; u < VD / 32; ++u) ef[u] = ld8(e0 + (t0 + (iq < len ? iq : 0)) * p.es + 32 * u + 8 * g);
       }
-      const float bh = d.h[iq], bl = d.l[iq];
+      const float bh = dc.h[iq], bl = dc.l[iq];
       float rsum = 0.f;
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt) {
-        const bool on = REV ? jt >= w : jt <= w;
+      for (int jj = 0; jj < 4 / HALVES; ++jj) {
+        const int jt = HALVES == 1 ? jj : 2 * jj + (w & 1);
+        const bool on = REV ? jt >= t : jt <= t;
         f32x4 pv = {0.f, 0.f, 0.f, 0.f}, cs = pv;
         if (on) {
           f32x4 a = pv, a2 = pv;
 #pragma unroll
-          for (int u = 0; u < NU; ++u) a = mma(ld8(Ks + (16 * jt + i) * KP + 32 * u + 8 * g), qf[u], a);
+          for (int u = 0; u < NU; ++u) a = mma(ld_row<KD>(Ks, 16 * jt + i, 4 * u + g), qf[u], a);
           if (DOT == 2) {
 #pragma unroll
-            for (int u = 0; u < VD / 32; ++u) a2 = mma(ld8(Vs + (16 * jt + i) * VP + 32 * u + 8 * g), ef[u], a2);
+            for (int u = 0; u < VD / 32; ++u) a2 = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), ef[u], a2);
           }
-          const f32x4 jh = *reinterpret_cast<const f32x4*>(d.h + 16 * jt + 4 * g);
-          const f32x4 jl = *reinterpret_cast<const f32x4*>(d.l + 16 * jt + 4 * g);
+          const f32x4 jh = *reinterpret_cast<const f32x4*>(dc.h + 16 * jt + 4 * g);
+          const f32x4 jl = *reinterpret_cast<const f32x4*>(dc.l + 16 * jt + 4 * g);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = 16 * jt + 4 * g + r;
@@ -454,16 +504,16 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
             }
           }
         }
-        if (DOT == 2 && i == 0) *reinterpret_cast<f32x4*>(cols[w] + 16 * jt + 4 * g) = cs;
+        if (DOT == 2 && i == 0) *reinterpret_cast<f32x4*>(cols[t] + 16 * jt + 4 * g) = cs;
         const bf16x4 hi = to_bf16x4(pv[0], pv[1], pv[2], pv[3]);
         const bf16x4 lo = to_bf16x4(pv[0] - (float)hi[0], pv[1] - (float)hi[1], pv[2] - (float)hi[2], pv[3] - (float)hi[3]);
-        const int at = iq * kPP + 32 * (jt >> 1) + 8 * g + 4 * (jt & 1);
+        const int at = iq * kC + (((4 * (jt >> 1) + g) ^ (iq & 7)) << 3) + 4 * (jt & 1);
         *reinterpret_cast<bf16x4*>(Ps[0] + at) = hi;
         *reinterpret_cast<bf16x4*>(Ps[1] + at) = lo;
       }
       if (DOT == 2) {
         rsum = xor32_sum(xor16_sum(rsum));
-        if (g == 0) rows[iq] = rsum;
+        if (g == 0) rows[HALVES == 1 ? 0 : w & 1][iq] = rsum;
       }
     }
     // ---- the state's share: O^T = S^T Q^T, columns = tokens
@@ -475,27 +525,27 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
     if (held) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        bf16x8 part[NCT][NS];
+        bf16x8 part[NCT][NS], qf[4];
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = st.s[2 * u + (e >> 2)][ct][e & 3];
 #pragma unroll
-          for (int n = 0; n < NS; ++n) part[ct][n] = next_part(x);
+          for (int n = 0; n < NS; ++n) part[ct][n] = next_part(x, n + 1 < NS);
         }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const bf16x8 qf = ld8(Qs + (16 * t + i) * KP + 32 * u + 8 * g);
+        for (int t = 0; t < 4; ++t) qf[t] = ld_row<KD>(Qs, 16 * t + i, 4 * u + g);
 #pragma unroll
-          for (int n = NS - 1; n >= 0; --n)
+        for (int n = NS - 1; n >= 0; --n)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(part[ct][n], qf, acc[t][ct]);
-        }
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(part[ct][n], qf[t], acc[t][ct]);
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const float wi = d.win[16 * t + i];
+        const float wi = dc.win[16 * t + i];
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) acc[t][ct] *= wi;
       }
@@ -504,7 +554,7 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int row = 16 * t + i;
-        const bf16* er = e0 + (t0 + (row < len ? row : 0)) * es + 16 * NCT * w + 4 * NCT * g;
+        const bf16* er = e0 + (t0 + (row < len ? row : 0)) * p.es + 16 * NCT * w + 4 * NCT * g;
         float x = 0.f;
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) {
@@ -518,40 +568,48 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
     }
     __syncthreads();  // scores and dots are written
     // ---- the scores' share: O^T += V^T P^T
-    if (!bad[ci & 1]) {
+    bf16x8 vf[2][NCT];
+    float bad = 0.f;  // NaN where the wave's columns of v hold an infinity or NaN: a sum of products with zero
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        bf16x8 vf[NCT];
+    for (int k2 = 0; k2 < 2; ++k2) {
+      State<KD, VD, NW>::columns(Vs, 32 * k2, w, lane, vf[k2]);
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) vf[ct] = ld8_tr_cols<NCT>(Vs, VP, 32 * k2, 16 * NCT * w + 4 * ct, lane);
+      for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (REV ? t >= 2 && k2 == 0 : t < 2 && k2 == 1) continue;  // all masked
+        for (int e = 0; e < 8; e += 2)
+          bad = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{vf[k2][ct][e], vf[k2][ct][e + 1]}, scalar_pair(0u), bad, false);
+    }
+    if (__ballot(!(bad == 0.f)) == 0) {
 #pragma unroll
-          for (int n = 1; n >= 0; --n) {
-            const bf16x8 pf = ld8(Ps[n] + (16 * t + i) * kPP + 32 * k2 + 8 * g);
+      for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(vf[ct], pf, acc[t][ct]);
+        for (int n = 1; n >= 0; --n)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (REV ? t >= 2 && k2 == 0 : t < 2 && k2 == 1) continue;  // all masked
+            const bf16x8 pf = ld8(Ps[n] + (16 * t + i) * kC + (((4 * k2 + g) ^ (i & 7)) << 3));
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(vf[k2][ct], pf, acc[t][ct]);
           }
-        }
-      }
-    } else {  // an infinity or NaN in v reaches the tokens that see it, not those whose score is masked
+    } else {  // they reach the tokens that see them, not those whose score is masked
       for (int j = 0; j < len; ++j) {
-        const bf16* vr = Vs + j * VP + 16 * NCT * w + 4 * NCT * g;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int row = 16 * t + i;
+          const int row = 16 * t + i, at = row * kC + (((tok_col(j) >> 3) ^ (row & 7)) << 3) + (tok_col(j) & 7);
           if (REV ? j < row : j > row) continue;
-          const float x = (float)Ps[0][row * kPP + tok_col(j)] + (float)Ps[1][row * kPP + tok_col(j)];
+          const float x = (float)Ps[0][at] + (float)Ps[1][at];
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][ct][r] += x * (float)vr[4 * ct + r];
+            for (int r = 0; r < 4; ++r) {
+              const int col = 16 * NCT * w + 4 * NCT * g + 4 * ct + r;
+              acc[t][ct][r] += x * (float)Vs[j * VD + (((col >> 3) ^ swz<VD>(j)) << 3) + (col & 7)];
+            }
         }
       }
     }
     if (ci + 1 < nc || wants_fin) {
-      st.update(d, Ks, Vs, w, lane);
+      st.update(dc, Ks, Vs, w, lane);
       held = true;
     }
 #pragma unroll
@@ -559,25 +617,24 @@ __global__ __launch_bounds__(kLinNT, 2) void gated_deltaless_chunk_kernel(LinPar
       const int row = 16 * t + i;
       if (row >= len) continue;
       OT* dst = o0 + (int64_t)(t0 + row) * p.HV * VD + 16 * NCT * w + 4 * NCT * g;
+      if constexpr (sizeof(OT) == 4) {
 #pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) {
-        if constexpr (sizeof(OT) == 4) {
-          *reinterpret_cast<f32x4*>(dst + 4 * ct) = acc[t][ct];
-        } else if constexpr (NCT == 2) {
-          if (ct == 0) *reinterpret_cast<bf16x8*>(dst) = pack8(acc[t][0], acc[t][NCT - 1]);
-        } else {
-          *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
-        }
+        for (int ct = 0; ct < NCT; ++ct) *reinterpret_cast<f32x4*>(dst + 4 * ct) = acc[t][ct];
+      } else if constexpr (NCT == 2) {
+        *reinterpret_cast<bf16x8*>(dst) = pack8(acc[t][0], acc[t][NCT - 1]);
+      } else {
+        *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
       }
     }
     if (DOT && w == 0 && lane < len) {
       float x = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < 4; ++ww) x += dots[DOT ? ww : 0][lane];
+      for (int ww = 0; ww < NW; ++ww) x += dots[DOT ? ww : 0][lane];
       if (DOT == 2) {
-        x += rows[lane];
 #pragma unroll
-        for (int ww = 0; ww < 4; ++ww) x -= cols[DOT == 2 ? ww : 0][lane];
+        for (int ww = 0; ww < HALVES; ++ww) x += rows[ww][lane];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x -= cols[DOT == 2 ? t : 0][lane];
       }
       const int64_t tokens = p.cu ? p.T : p.N * p.T;
       p.dot[hv * tokens + sg.tok + t0 + lane] = x;
@@ -602,7 +659,7 @@ struct LinGateGrad {
 __global__ __launch_bounds__(256) void gated_deltaless_gate_grad_kernel(LinParams p, LinGateGrad a) {
   __shared__ double part[4];
   const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  const int64_t hv = blockIdx.x % p.HV;
+  const unsigned hv = blockIdx.x % p.HV;
   const Segment sg = find_segment(p, blockIdx.x / p.HV);
   if (!sg.some) return;
   const float *s = nullptr, *r = nullptr;
@@ -685,24 +742,35 @@ static int64_t lin_states_bytes(const LinPlan& pl, int64_t HV, int64_t K, int64_
   return pl.split ? align256l(pl.slots * HV * K * V * 4) + align256l(pl.slots * HV * 4) : 0;
 }
 
+// Waves of a workgroup for V columns.
+constexpr int kLinWaves64 = 4, kLinWaves128 = 4;
+
+template <typename F>
+static void lin_by_dims(int64_t K, int64_t V, F go) {
+  using C64 = std::integral_constant<int, 64>;
+  using C128 = std::integral_constant<int, 128>;
+  if (K == 128 && V == 128) go(C128{}, C128{}, std::integral_constant<int, kLinWaves128>{});
+  else if (K == 64 && V == 64) go(C64{}, C64{}, std::integral_constant<int, kLinWaves64>{});
+  else if (K == 128) go(C128{}, C64{}, std::integral_constant<int, kLinWaves64>{});
+  else go(C64{}, C128{}, std::integral_constant<int, kLinWaves128>{});
+}
+
 template <bool REV>
-static void launch_segments(LinParams p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  const dim3 grid((unsigned)(pl.slots * p.HV)), nt(kLinNT);
-  if (K == 128 && V == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, 128, REV>), grid, nt, 0, s, p);
-  else if (K == 64 && V == 64) hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, 64, REV>), grid, nt, 0, s, p);
-  else if (K == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, 64, REV>), grid, nt, 0, s, p);
-  else hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, 128, REV>), grid, nt, 0, s, p);
+static void launch_segments(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
+  lin_by_dims(K, V, [&](auto k, auto v, auto w) {
+    hipLaunchKernelGGL((gated_deltaless_segment_kernel<decltype(k)::value, decltype(v)::value, decltype(w)::value, REV>),
+                       dim3((unsigned)(pl.slots * p.HV)), dim3(decltype(w)::value * kWave), 0, s, p);
+  });
   hipLaunchKernelGGL((gated_deltaless_scan_kernel<REV>), dim3((unsigned)(p.N * p.HV * (K * V / 1024))), dim3(256), 0, s, p,
                      K * V);
 }
 
 template <bool REV, int DOT, typename OT>
 static void launch_walk(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  const dim3 grid((unsigned)(pl.slots * p.HV)), nt(kLinNT);
-  if (K == 128 && V == 128) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<128, 128, REV, DOT, OT>), grid, nt, 0, s, p);
-  else if (K == 64 && V == 64) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<64, 64, REV, DOT, OT>), grid, nt, 0, s, p);
-  else if (K == 128) hipLaunchKernelGGL((gated_deltaless_chunk_kernel<128, 64, REV, DOT, OT>), grid, nt, 0, s, p);
-  else hipLaunchKernelGGL((gated_deltaless_chunk_kernel<64, 128, REV, DOT, OT>), grid, nt, 0, s, p);
+  lin_by_dims(K, V, [&](auto k, auto v, auto w) {
+    hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k)::value, decltype(v)::value, decltype(w)::value, REV, DOT, OT>),
+                       dim3((unsigned)(pl.slots * p.HV)), dim3(decltype(w)::value * kWave), 0, s, p);
+  });
 }
 
 static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int64_t N,
@@ -727,7 +795,7 @@ static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t 
       return GDN_ERR_INVALID;
     }
   const LinPlan pl = lin_plan(B, T, HV, N, varlen);
-  if (pl.slots * HV > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
+  if (pl.slots * HV > 0x7fffffffLL || pl.spq > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
     gdn_internal_set_error("%s: too many sequences, heads or tokens for one launch", name);
     return GDN_ERR_UNSUPPORTED;
   }
@@ -747,15 +815,15 @@ static LinParams lin_params(const LinPlan& pl, const void* g, int g_dtype, int64
   p.shift = pl.shift;
   p.T = T;
   p.N = N;
-  p.HV = HV;
-  p.spq = pl.spq;
+  p.HV = (unsigned)HV;
+  p.spq = (unsigned)pl.spq;
   p.scale = scale;
   return p;
 }
 
 // The walk's q, k, v and e with the number of value heads that share a head of each.
 static void lin_roles(LinParams& p, const void* q, int rq, const void* k, int rk, const void* v, int rv, const void* e,
-                      int re) {
+                      int re, int64_t K, int64_t V) {
   p.q = static_cast<const bf16*>(q);
   p.k = static_cast<const bf16*>(k);
   p.v = static_cast<const bf16*>(v);
@@ -764,6 +832,10 @@ static void lin_roles(LinParams& p, const void* q, int rq, const void* k, int rk
   p.rk = rk;
   p.rv = rv;
   p.re = re;
+  p.qs = p.HV / rq * K;
+  p.ks = p.HV / rk * K;
+  p.vs = p.HV / rv * V;
+  p.es = p.HV / re * V;
 }
 
 static void lin_states(LinParams& p, const LinPlan& pl, char* states, int64_t K, int64_t V) {
@@ -801,7 +873,7 @@ extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, c
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rep = (int)(HV / H);
   LinParams p = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N, HV, scale);
-  lin_roles(p, q, rep, k, rep, v, 1, nullptr, 1);
+  lin_roles(p, q, rep, k, rep, v, 1, nullptr, 1, K, V);
   lin_states(p, pl, static_cast<char*>(states), K, V);
   p.init = initial_state;
   if (pl.split) launch_segments<false>(p, pl, K, V, s);
@@ -866,7 +938,7 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
                                     HV, scale);
   // from the end: R's segments, then dv and dk
   LinParams r = base;
-  lin_roles(r, k, rep, q, rep, d_o, 1, nullptr, 1);
+  lin_roles(r, k, rep, q, rep, d_o, 1, nullptr, 1, K, V);
   lin_states(r, pl, ws, K, V);
   r.init = d_final_state;
   if (pl.split) launch_segments<true>(r, pl, K, V, s);
@@ -875,7 +947,7 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   a.fin = d_initial_state;
   launch_walk<true, 0, bf16>(a, pl, K, V, s);
   a = r;
-  lin_roles(a, v, 1, d_o, 1, q, rep, k, rep);
+  lin_roles(a, v, 1, d_o, 1, q, rep, k, rep, V, K);
   a.transposed = 1;
   a.dot = dot_k;
   a.o = shared ? static_cast<void*>(dk_heads) : dk;
@@ -883,7 +955,7 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   else dg ? launch_walk<true, 1, bf16>(a, pl, V, K, s) : launch_walk<true, 0, bf16>(a, pl, V, K, s);
   // from the start: dq
   LinParams f = base;
-  lin_roles(f, d_o, 1, v, 1, k, rep, q, rep);
+  lin_roles(f, d_o, 1, v, 1, k, rep, q, rep, V, K);
   lin_states(f, pl, static_cast<char*>(const_cast<void*>(states)), K, V);
   f.init = initial_state;
   f.transposed = 1;
