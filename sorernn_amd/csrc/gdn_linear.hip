@@ -189,25 +189,41 @@ __device__ __forceinline__ bf16x8 ld_cols(const bf16* tile, int r0, int c0, int 
   return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A chunk's rows on their way to LDS: thread t of NT holds the 16-byte pieces t, t + NT, ... of the 64 x D tile. Rows
-// past the chunk's end re-read its first row and are written as zeros.
-template <int D, int NT>
+// A chunk's rows on their way to LDS: thread t of 256 holds the 16-byte pieces t, t + 256, ... of the 64 x D tile, RP rows
+// apart. Whole chunks are read at a scalar address plus the thread's offset; in a sequence's last chunk the rows past its
+// end re-read its first row and are written as zeros.
+template <int D>
 struct Tile {
-  static constexpr int NP = kC * D / 8 / NT;
+  static constexpr int NP = kC * D / 8 / 256, RP = 256 / (D / 8);
+  static_assert(RP % 16 == 0, "the swizzle has a period of 16 rows");
   bf16x8 r[NP];
-  __device__ __forceinline__ void fetch(const bf16* base, int64_t stride, int len) {
+  __device__ __forceinline__ static int row0() { return threadIdx.x % 256 / (D / 8); }
+  __device__ __forceinline__ static int piece() { return threadIdx.x % (D / 8); }
+  __device__ __forceinline__ static uint32_t offset(int64_t stride) {
+    return (uint32_t)(row0() * (int)stride + piece() * 8) * 2u;
+  }
+  __device__ __forceinline__ void fetch(const bf16* base, int64_t stride, uint32_t off, int len) {
+    if (len == kC) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      const int c = threadIdx.x + n * NT, row = c / (D / 8);
-      r[n] = *reinterpret_cast<const bf16x8*>(base + (row < len ? row : 0) * stride + (c % (D / 8)) * 8);
+      for (int n = 0; n < NP; ++n)
+        r[n] = *reinterpret_cast<const bf16x8*>(reinterpret_cast<const char*>(base + n * RP * stride) + off);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const int row = row0() + n * RP;
+        r[n] = *reinterpret_cast<const bf16x8*>(base + (row < len ? row : 0) * stride + piece() * 8);
+      }
     }
   }
-  __device__ __forceinline__ void put(bf16* tile, int len) const {
+  __device__ __forceinline__ void put(bf16* tile, int len) {
+    if (len < kC) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-      const int c = threadIdx.x + n * NT, row = c / (D / 8);
-      *reinterpret_cast<bf16x8*>(tile + row * D + (((c % (D / 8)) ^ swz<D>(row)) << 3)) = row < len ? r[n] : bf16x8{};
+      for (int n = 0; n < NP; ++n)
+        if (row0() + n * RP >= len) r[n] = bf16x8{};
     }
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+      *reinterpret_cast<bf16x8*>(tile + (row0() + n * RP) * D + ((piece() ^ swz<D>(row0())) << 3)) = r[n];
   }
 };
 
@@ -242,14 +258,14 @@ struct State {
         }
       }
   }
-  __device__ __forceinline__ void store(float* dst, int w, int lane) const {
+  __device__ __forceinline__ void store(float* dst, int pitch, int w, int lane) const {
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
     for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dst[(row0(a, g) + r) * VD + col(w, ct, i)] = s[a][ct][r];
+        for (int r = 0; r < 4; ++r) dst[(row0(a, g) + r) * pitch + col(w, ct, i)] = s[a][ct][r];
   }
   // The wave's columns of 32 rows of V from r0 on, as the accumulators' token order has them.
   __device__ __forceinline__ static void columns(const bf16* Vs, int r0, int w, int lane, bf16x8 (&vf)[NCT]) {
@@ -257,7 +273,7 @@ struct State {
     for (int ct = 0; ct < NCT; ++ct) vf[ct] = ld_cols<VD, 4 * NCT>(Vs, r0, 16 * NCT * w + 4 * ct, lane);
   }
   // S = all S + K^T (wst V): V weighted in fp32 and split into three bf16 parts (K is exact)
-  __device__ __forceinline__ void update(const Decays& d, const bf16* Ks, const bf16* Vs, int w, int lane) {
+  __device__ __forceinline__ void update(const Decays& d, const bf16* Ks, const bf16x8 (&vf)[2][NCT], int lane) {
     const int g = lane >> 4;
     const float all = d.all;
 #pragma unroll
@@ -268,13 +284,12 @@ struct State {
     for (int ks = 0; ks < 2; ++ks) {
       const f32x4 w0 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 4 * g);
       const f32x4 w1 = *reinterpret_cast<const f32x4*>(d.wst + 32 * ks + 16 + 4 * g);
-      bf16x8 vf[NCT], part[NCT][3];
-      columns(Vs, 32 * ks, w, lane, vf);
+      bf16x8 part[NCT][3];
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)vf[ct][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
+        for (int e = 0; e < 8; ++e) x[e] = (float)vf[ks][ct][e] * (e < 4 ? w0[e & 3] : w1[e & 3]);
 #pragma unroll
         for (int n = 0; n < 3; ++n) part[ct][n] = next_part(x, n < 2);
       }
@@ -314,27 +329,28 @@ struct GateWalk {
 // ------------------------------------------------------------------------------------------------
 // A segment's own contribution to the state: the walk without outputs, from a zero state. Forward walks leave it in
 // the next segment's slot, walks from the end in the one before; the sequence's last segment (first) has none to give.
-template <int KD, int VD, int NW, bool REV>
-__global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_segment_kernel(LinParams p) {
-  constexpr int NT = NW * kWave;
-  __shared__ __align__(16) bf16 Ks[kC * KD], Vs[kC * VD];
+// Two workgroups share 128 columns, which doubles the waves in flight.
+template <int KD, bool REV>
+__global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinParams p, int VD) {
+  __shared__ __align__(16) bf16 Ks[kC * KD], Vs[kC * 64];
   __shared__ __align__(16) Decays d[2];
   const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const unsigned hv = blockIdx.x % p.HV;
   const Segment sg = find_segment(p, blockIdx.x / p.HV);
   if (!sg.some || (REV ? sg.first : sg.last)) return;
   const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
+  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD + blockIdx.y * 64;
   const int nc = (sg.len + kC - 1) / kC;
-  Tile<KD, NT> kt;
-  Tile<VD, NT> vt;
+  Tile<KD> kt;
+  Tile<64> vt;
   GateWalk<REV> gate;
+  const uint32_t koff = kt.offset(p.ks), voff = vt.offset(p.vs);
   auto fetch = [&](int ci) {
     const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    kt.fetch(k0 + t0 * p.ks, p.ks, len);
-    vt.fetch(v0 + t0 * p.vs, p.vs, len);
+    kt.fetch(k0 + t0 * p.ks, p.ks, koff, len);
+    vt.fetch(v0 + t0 * p.vs, p.vs, voff, len);
   };
-  State<KD, VD, NW> st;
+  State<KD, 64, 4> st;
   st.zero();
   double total = 0.;
   if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
@@ -356,11 +372,14 @@ __global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_segment_ke
       chunk_decays<REV>(d[(ci + 1) & 1], x, p.scale, lane);
       gate.fetch(p, sg, hv, ci + 2, nc, lane);
     }
-    st.update(d[ci & 1], Ks, Vs, w, lane);
+    bf16x8 vf[2][1];
+    st.columns(Vs, 0, w, lane, vf[0]);
+    st.columns(Vs, 32, w, lane, vf[1]);
+    st.update(d[ci & 1], Ks, vf, lane);
     __syncthreads();
   }
-  st.store(p.entry + ((sg.slot + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD), w, lane);
-  if (w == 0) {
+  st.store(p.entry + ((sg.slot + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, w, lane);
+  if (w == 0 && blockIdx.y == 0) {
     for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
     if (lane == 0) p.decay[sg.slot * p.HV + hv] = __builtin_amdgcn_exp2f((float)total);
   }
@@ -407,122 +426,70 @@ __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, 
 }
 
 // ------------------------------------------------------------------------------------------------
-// The walk. DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums
-// less the column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.
-template <int KD, int VD, int NW, bool REV, int DOT, typename OT>
-__global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_chunk_kernel(LinParams p) {
-  constexpr int NT = NW * kWave, NCT = VD / 16 / NW, NU = KD / 32;
+// The walk. One workgroup a CU: waves 0-3 hold the state and make the outputs of chunk c, waves 4-7 meanwhile bring the
+// tiles of chunks c + 1 and c + 2 into LDS and make the scores of chunk c + 1; one barrier a chunk. At 4 x 4,096 tokens, 16 heads of 128, 82 us;
+// its loads and stores alone 59 us, the state's waves alone 64 us.
+// DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums less the
+// column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.
+//
+// Scores are kept for the tiles that are not masked, in blocks of 16 queries x 32 keys (tok_col order): queries 0-15 and
+// 16-31 have one block, the others two (walks from the end: mirrored).
+template <int KD, int VD, int DOT>
+struct WalkLds {
+  bf16 q[3][kC * KD], k[3][kC * KD], v[2][kC * VD];
+  bf16 ps[2][2][6 * 512];  // [slot][part]
+  Decays d[3];
+  float dots[DOT ? 2 : 1][4][DOT ? kC : 1];
+  float rows[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1], cols[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1];
+};
+
+template <int KD, int VD, bool REV, int DOT, typename OT>
+__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams p) {
+  constexpr int SW = 4, NCT = VD / 16 / SW, NU = KD / 32;
   constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
-  constexpr int HALVES = NW / 4;   // waves that share the scores of 16 queries
-  __shared__ __align__(16) bf16 Qs[kC * KD], Ks[kC * KD], Vs[kC * VD];
-  __shared__ __align__(16) bf16 Ps[2][kC * kC];  // the two parts of the scores, tok_col columns, swizzled as the tiles
-  __shared__ __align__(16) Decays d[2];
-  __shared__ __align__(16) float dots[DOT ? NW : 1][kC], rows[HALVES][kC], cols[DOT == 2 ? 4 : 1][kC];
-  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  __shared__ __align__(16) WalkLds<KD, VD, DOT> lds;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, i = lane & 15;
   const unsigned hv = blockIdx.x % p.HV;
   const Segment sg = find_segment(p, blockIdx.x / p.HV);
   if (!sg.some) return;
-  const bf16* q0 = p.q + sg.tok * p.qs + hv / p.rq * KD;
-  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
-  const bf16* e0 = DOT ? p.e + sg.tok * p.es + hv / p.re * VD : nullptr;
-  OT* o0 = static_cast<OT*>(p.o) + (sg.tok * p.HV + hv) * VD;
   const int nc = (sg.len + kC - 1) / kC;
-  Tile<KD, NT> qt, kt;
-  Tile<VD, NT> vt;
-  GateWalk<REV> gate;
-  auto fetch = [&](int ci) {
-    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    qt.fetch(q0 + t0 * p.qs, p.qs, len);
-    kt.fetch(k0 + t0 * p.ks, p.ks, len);
-    vt.fetch(v0 + t0 * p.vs, p.vs, len);
-  };
-  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
-  fetch(0);
-  State<KD, VD, NW> st;
-  const bool inner = REV ? !sg.last : !sg.first;  // a segment of this sequence comes before
-  const float* src = inner ? p.entry + (sg.slot * p.HV + hv) * (KD * VD)
-                           : (p.init ? p.init + (sg.n * p.HV + hv) * (KD * VD) : nullptr);
-  bool held = src != nullptr;  // the state is not known to be zero
-  if (held) st.load(src, p.transposed, w, lane);
-  else st.zero();
-  const bool wants_fin = p.fin && (REV ? sg.first : sg.last);
-  if (w == 0) {
-    chunk_decays<REV>(d[0], gate.value(p), p.scale, lane);
-    gate.fetch(p, sg, hv, 1, nc, lane);
-  }
-  for (int ci = 0; ci < nc; ++ci) {
-    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    const Decays& dc = d[ci & 1];
-    qt.put(Qs, len);
-    kt.put(Ks, len);
-    vt.put(Vs, len);
+  auto first_of = [&](int c) { return (REV ? nc - 1 - c : c) * kC; };  // first token of the walk's chunk c
+  auto len_of = [&](int c) { return sg.len - first_of(c) < kC ? sg.len - first_of(c) : kC; };
+  const bf16* e0 = DOT ? p.e + sg.tok * p.es + hv / p.re * VD : nullptr;
+
+  if (wave < SW) {  // ------------------------------------------------------------------ the state's waves
+    const int w = wave;
+    OT* o0 = static_cast<OT*>(p.o) + (sg.tok * p.HV + hv) * VD;
+    State<KD, VD, SW> st;
+    const bool inner = REV ? !sg.last : !sg.first;  // a segment of this sequence comes before
+    const float* src = inner ? p.entry + (sg.slot * p.HV + hv) * (KD * VD)
+                             : (p.init ? p.init + (sg.n * p.HV + hv) * (KD * VD) : nullptr);
+    if (src) st.load(src, p.transposed, w, lane);
+    else st.zero();
+    const bool wants_fin = p.fin && (REV ? sg.first : sg.last);
     __syncthreads();
-    if (ci + 1 < nc) fetch(ci + 1);
-    if (w == 0 && ci + 1 < nc) {
-      chunk_decays<REV>(d[(ci + 1) & 1], gate.value(p), p.scale, lane);
-      gate.fetch(p, sg, hv, ci + 2, nc, lane);
-    }
-    // ---- the scores of 16 queries: P^T tiles, rows = keys j, column = query; with 8 waves two take every other tile
-    {
-      const int t = w / HALVES, iq = 16 * t + i;
-      bf16x8 qf[NU], ef[DOT == 2 ? VD / 32 : 1];
+    __syncthreads();
+    for (int c = 0; c < nc; ++c) {
+      const int t0 = first_of(c), len = len_of(c);
+      const Decays& d = lds.d[c % 3];
+      const bf16 *Qs = lds.q[c % 3], *Ks = lds.k[c % 3], *Vs = lds.v[c & 1];
+      bf16x4 ev[4][NCT];
+      if (DOT) {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) qf[u] = ld_row<KD>(Qs, iq, 4 * u + g);
-      if (DOT == 2) {
+        for (int t = 0; t < 4; ++t) {
+          const int row = 16 * t + i;
+          const bf16* er = e0 + (t0 + (row < len ? row : 0)) * p.es + 16 * NCT * w + 4 * NCT * g;
 #pragma unroll
-        for (int u = 0; u < VD / 32; ++u) ef[u] = ld8(e0 + (t0 + (iq < len ? iq : 0)) * p.es + 32 * u + 8 * g);
-      }
-      const float bh = dc.h[iq], bl = dc.l[iq];
-      float rsum = 0.f;
-#pragma unroll
-      for (int jj = 0; jj < 4 / HALVES; ++jj) {
-        const int jt = HALVES == 1 ? jj : 2 * jj + (w & 1);
-        const bool on = REV ? jt >= t : jt <= t;
-        f32x4 pv = {0.f, 0.f, 0.f, 0.f}, cs = pv;
-        if (on) {
-          f32x4 a = pv, a2 = pv;
-#pragma unroll
-          for (int u = 0; u < NU; ++u) a = mma(ld_row<KD>(Ks, 16 * jt + i, 4 * u + g), qf[u], a);
-          if (DOT == 2) {
-#pragma unroll
-            for (int u = 0; u < VD / 32; ++u) a2 = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), ef[u], a2);
-          }
-          const f32x4 jh = *reinterpret_cast<const f32x4*>(dc.h + 16 * jt + 4 * g);
-          const f32x4 jl = *reinterpret_cast<const f32x4*>(dc.l + 16 * jt + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * jt + 4 * g + r;
-            const float diff = REV ? (jh[r] - bh) + (jl[r] - bl) : (bh - jh[r]) + (bl - jl[r]);
-            const float x = a[r] * (p.scale * __builtin_amdgcn_exp2f(diff));
-            pv[r] = (REV ? j >= iq : j <= iq) ? x : 0.f;
-            if (DOT == 2) {
-              const float ww = (REV ? j >= iq : j <= iq) && iq < len && j < len ? x * a2[r] : 0.f;
-              rsum += ww;
-              cs[r] = group_sum<16>(ww);
-            }
-          }
+          for (int ct = 0; ct < NCT; ++ct) ev[t][ct] = *reinterpret_cast<const bf16x4*>(er + 4 * ct);
         }
-        if (DOT == 2 && i == 0) *reinterpret_cast<f32x4*>(cols[t] + 16 * jt + 4 * g) = cs;
-        const bf16x4 hi = to_bf16x4(pv[0], pv[1], pv[2], pv[3]);
-        const bf16x4 lo = to_bf16x4(pv[0] - (float)hi[0], pv[1] - (float)hi[1], pv[2] - (float)hi[2], pv[3] - (float)hi[3]);
-        const int at = iq * kC + (((4 * (jt >> 1) + g) ^ (iq & 7)) << 3) + 4 * (jt & 1);
-        *reinterpret_cast<bf16x4*>(Ps[0] + at) = hi;
-        *reinterpret_cast<bf16x4*>(Ps[1] + at) = lo;
       }
-      if (DOT == 2) {
-        rsum = xor32_sum(xor16_sum(rsum));
-        if (g == 0) rows[HALVES == 1 ? 0 : w & 1][iq] = rsum;
-      }
-    }
-    // ---- the state's share: O^T = S^T Q^T, columns = tokens
-    f32x4 acc[4][NCT];
+      // the state's share: O^T = S^T Q^T, columns = tokens
+      f32x4 acc[4][NCT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (held) {
+        for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         bf16x8 part[NCT][NS], qf[4];
@@ -545,103 +512,257 @@ __global__ __launch_bounds__(NW * kWave, NW / 2) void gated_deltaless_chunk_kern
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const float wi = dc.win[16 * t + i];
+        const float wi = d.win[16 * t + i];
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct) acc[t][ct] *= wi;
       }
-    }
-    if (DOT) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int row = 16 * t + i;
-        const bf16* er = e0 + (t0 + (row < len ? row : 0)) * p.es + 16 * NCT * w + 4 * NCT * g;
-        float x = 0.f;
-#pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) {
-          const bf16x4 ev = *reinterpret_cast<const bf16x4*>(er + 4 * ct);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x += acc[t][ct][r] * (float)ev[r];
-        }
-        x = xor32_sum(xor16_sum(x));
-        if (g == 0) dots[w][row] = x;
-      }
-    }
-    __syncthreads();  // scores and dots are written
-    // ---- the scores' share: O^T += V^T P^T
-    bf16x8 vf[2][NCT];
-    float bad = 0.f;  // NaN where the wave's columns of v hold an infinity or NaN: a sum of products with zero
-#pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) {
-      State<KD, VD, NW>::columns(Vs, 32 * k2, w, lane, vf[k2]);
-#pragma unroll
-      for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          bad = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{vf[k2][ct][e], vf[k2][ct][e + 1]}, scalar_pair(0u), bad, false);
-    }
-    if (__ballot(!(bad == 0.f)) == 0) {
-#pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-        for (int n = 1; n >= 0; --n)
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            if (REV ? t >= 2 && k2 == 0 : t < 2 && k2 == 1) continue;  // all masked
-            const bf16x8 pf = ld8(Ps[n] + (16 * t + i) * kC + (((4 * k2 + g) ^ (i & 7)) << 3));
-#pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(vf[k2][ct], pf, acc[t][ct]);
-          }
-    } else {  // they reach the tokens that see them, not those whose score is masked
-      for (int j = 0; j < len; ++j) {
+      if (DOT) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int row = 16 * t + i, at = row * kC + (((tok_col(j) >> 3) ^ (row & 7)) << 3) + (tok_col(j) & 7);
-          if (REV ? j < row : j > row) continue;
-          const float x = (float)Ps[0][at] + (float)Ps[1][at];
+          float x = 0.f;
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int col = 16 * NCT * w + 4 * NCT * g + 4 * ct + r;
-              acc[t][ct][r] += x * (float)Vs[j * VD + (((col >> 3) ^ swz<VD>(j)) << 3) + (col & 7)];
-            }
+            for (int r = 0; r < 4; ++r) x += acc[t][ct][r] * (float)ev[t][ct][r];
+          x = xor32_sum(xor16_sum(x));
+          if (g == 0) lds.dots[DOT ? c & 1 : 0][w][DOT ? 16 * t + i : 0] = x;
         }
       }
-    }
-    if (ci + 1 < nc || wants_fin) {
-      st.update(dc, Ks, Vs, w, lane);
-      held = true;
-    }
+      // the scores' share: O^T += V^T P^T
+      bf16x8 vf[2][NCT];
+      float bad = 0.f;  // NaN where the wave's columns of v hold an infinity or NaN: a sum of products with zero
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int row = 16 * t + i;
-      if (row >= len) continue;
-      OT* dst = o0 + (int64_t)(t0 + row) * p.HV * VD + 16 * NCT * w + 4 * NCT * g;
-      if constexpr (sizeof(OT) == 4) {
+      for (int k2 = 0; k2 < 2; ++k2) {
+        State<KD, VD, SW>::columns(Vs, 32 * k2, w, lane, vf[k2]);
 #pragma unroll
-        for (int ct = 0; ct < NCT; ++ct) *reinterpret_cast<f32x4*>(dst + 4 * ct) = acc[t][ct];
-      } else if constexpr (NCT == 2) {
-        *reinterpret_cast<bf16x8*>(dst) = pack8(acc[t][0], acc[t][NCT - 1]);
-      } else {
-        *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
+        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2)
+            bad = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{vf[k2][ct][e], vf[k2][ct][e + 1]}, scalar_pair(0u), bad, false);
       }
-    }
-    if (DOT && w == 0 && lane < len) {
-      float x = 0.f;
+      const auto* ps = lds.ps[c & 1];
+      if (__ballot(!(bad == 0.f)) == 0) {
 #pragma unroll
-      for (int ww = 0; ww < NW; ++ww) x += dots[DOT ? ww : 0][lane];
-      if (DOT == 2) {
+        for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-        for (int ww = 0; ww < HALVES; ++ww) x += rows[ww][lane];
+          for (int n = 1; n >= 0; --n)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x -= cols[DOT == 2 ? t : 0][lane];
+            for (int t = 0; t < 4; ++t) {
+              const int ta = REV ? 3 - t : t, ka = REV ? 1 - k2 : k2;
+              if (ta < 2 && ka == 1) continue;  // all masked
+              const int block = ta < 2 ? ta : 2 * ta - 2 + ka;
+              const bf16x8 pf = ld8(ps[n] + block * 512 + i * 32 + ((g ^ (i >> 2)) << 3));
+#pragma unroll
+              for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(vf[k2][ct], pf, acc[t][ct]);
+            }
+      } else {  // they reach the tokens that see them, not those whose score is masked
+        for (int j = 0; j < len; ++j) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (REV ? j < 16 * t + i : j > 16 * t + i) continue;
+            const int ta = REV ? 3 - t : t, ka = REV ? 1 - (j >> 5) : j >> 5, col = tok_col(j & 31);
+            const int at = (ta < 2 ? ta : 2 * ta - 2 + ka) * 512 + i * 32 + (((col >> 3) ^ (i >> 2)) << 3) + (col & 7);
+            const float x = (float)ps[0][at] + (float)ps[1][at];
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int vc = 16 * NCT * w + 4 * NCT * g + 4 * ct + r;
+                acc[t][ct][r] += x * (float)Vs[j * VD + (((vc >> 3) ^ swz<VD>(j)) << 3) + (vc & 7)];
+              }
+          }
+        }
       }
-      const int64_t tokens = p.cu ? p.T : p.N * p.T;
-      p.dot[hv * tokens + sg.tok + t0 + lane] = x;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int row = 16 * t + i;
+        if (row >= len) continue;
+        OT* dst = o0 + (int64_t)(t0 + row) * p.HV * VD + 16 * NCT * w + 4 * NCT * g;
+        if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) *reinterpret_cast<f32x4*>(dst + 4 * ct) = acc[t][ct];
+        } else if constexpr (NCT == 2) {
+          *reinterpret_cast<bf16x8*>(dst) = pack8(acc[t][0], acc[t][NCT - 1]);
+        } else {
+          *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
+        }
+      }
+      if (c + 1 < nc || wants_fin) st.update(d, Ks, vf, lane);
+      __syncthreads();
     }
-    __syncthreads();  // the tiles are read
+    if (wants_fin) st.store(p.fin + (sg.n * p.HV + hv) * (KD * VD), VD, w, lane);
+    return;
   }
-  if (wants_fin) st.store(p.fin + (sg.n * p.HV + hv) * (KD * VD), w, lane);
+
+  // ------------------------------------------------------------------------------------ the scores' waves
+  const int w = wave - SW;
+  const bf16* q0 = p.q + sg.tok * p.qs + hv / p.rq * KD;
+  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
+  // Two sets of tiles in flight: a chunk's loads are issued two steps before their rows go to LDS. With one step between
+  // the two, a step lasted as long as the loads of all CUs took, and the memory had nothing to do meanwhile.
+  Tile<KD> qt[2], kt[2];
+  Tile<VD> vt[2];
+  const uint32_t qoff = qt[0].offset(p.qs), koff = kt[0].offset(p.ks), voff = vt[0].offset(p.vs);
+  auto fetch_qk = [&](int c, int set) {
+    if (c >= nc) return;
+    const int t0 = first_of(c), len = len_of(c);
+    qt[set].fetch(q0 + t0 * p.qs, p.qs, qoff, len);
+    kt[set].fetch(k0 + t0 * p.ks, p.ks, koff, len);
+  };
+  auto fetch_v = [&](int c, int set) {
+    if (c < nc) vt[set].fetch(v0 + first_of(c) * p.vs, p.vs, voff, len_of(c));
+  };
+  auto put_qk = [&](int c, int set) {
+    if (c >= nc) return;
+    qt[set].put(lds.q[c % 3], len_of(c));
+    kt[set].put(lds.k[c % 3], len_of(c));
+  };
+  auto put_v = [&](int c, int set) {
+    if (c < nc) vt[set].put(lds.v[c & 1], len_of(c));
+  };
+  GateWalk<REV> gate;
+  auto decays = [&](int c) {  // of chunk c, whose raw gate has been fetched; then the next chunk's
+    if (w != 0 || c >= nc) return;
+    chunk_decays<REV>(lds.d[c % 3], gate.value(p), p.scale, lane);
+    gate.fetch(p, sg, hv, c + 1, nc, lane);
+  };
+  // 12 tiles of 16 keys x 16 queries are written (2 of zeros), 3 a wave: P^T, rows = keys j, column = query
+  f32x4 pv[3];
+  auto tile_of = [&](int n, int& ta, int& ja) {
+    const int sl = w + 4 * n;
+    ta = n == 0 ? sl >> 1 : 1 + n;
+    ja = n == 0 ? sl & 1 : w;
+  };
+  auto scores = [&](int c) {
+    if (c >= nc) return;
+    const bf16 *Qs = lds.q[c % 3], *Ks = lds.k[c % 3];
+    const Decays& d = lds.d[c % 3];
+    auto* ps = lds.ps[c & 1];
+    // the three tiles side by side, also where all of one is masked; tiles 1 and 2 have the same keys
+    bf16x8 kf[2][NU], qf[3][NU];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      int ta, ja;
+      tile_of(n, ta, ja);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        qf[n][u] = ld_row<KD>(Qs, 16 * (REV ? 3 - ta : ta) + i, 4 * u + g);
+        if (n < 2) kf[n][u] = ld_row<KD>(Ks, 16 * (REV ? 3 - ja : ja) + i, 4 * u + g);
+      }
+      pv[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int n = 0; n < 3; ++n) pv[n] = mma(kf[n > 0][u], qf[n][u], pv[n]);
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      int ta, ja;
+      tile_of(n, ta, ja);
+      const int t = REV ? 3 - ta : ta, jt = REV ? 3 - ja : ja, iq = 16 * t + i;
+      const float bh = d.h[iq], bl = d.l[iq];
+      const f32x4 jh = *reinterpret_cast<const f32x4*>(d.h + 16 * jt + 4 * g);
+      const f32x4 jl = *reinterpret_cast<const f32x4*>(d.l + 16 * jt + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + 4 * g + r;
+        const float diff = REV ? (jh[r] - bh) + (jl[r] - bl) : (bh - jh[r]) + (bl - jl[r]);
+        const float x = pv[n][r] * (p.scale * __builtin_amdgcn_exp2f(diff));
+        pv[n][r] = (REV ? j >= iq : j <= iq) ? x : 0.f;
+      }
+      const f32x4 x = pv[n];
+      const bf16x4 hi = to_bf16x4(x[0], x[1], x[2], x[3]);
+      const bf16x4 lo = to_bf16x4(x[0] - (float)hi[0], x[1] - (float)hi[1], x[2] - (float)hi[2], x[3] - (float)hi[3]);
+      const int block = ta < 2 ? ta : 2 * ta - 2 + (ja >> 1);
+      const int at = block * 512 + i * 32 + ((g ^ (i >> 2)) << 3) + 4 * (jt & 1);
+      *reinterpret_cast<bf16x4*>(ps[0] + at) = hi;
+      *reinterpret_cast<bf16x4*>(ps[1] + at) = lo;
+    }
+  };
+  // DOT 2: the sums of W over the tiles whose scores this wave holds (pv, of the chunk before the one just scored)
+  auto score_dots = [&](int c, const f32x4 (&x)[3]) {
+    const int t0 = first_of(c), len = len_of(c);
+    const bf16* Vs = lds.v[c & 1];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      int ta, ja;
+      tile_of(n, ta, ja);
+      if (ja > ta) continue;
+      const int t = REV ? 3 - ta : ta, jt = REV ? 3 - ja : ja, iq = 16 * t + i;
+      const bf16* er = e0 + (t0 + (iq < len ? iq : 0)) * p.es + 8 * g;
+      f32x4 a = {0.f, 0.f, 0.f, 0.f}, cs;
+#pragma unroll
+      for (int u = 0; u < VD / 32; ++u) a = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), ld8(er + 32 * u), a);
+      float rs = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + 4 * g + r;
+        const float ww = (REV ? j >= iq : j <= iq) && iq < len && j < len ? x[n][r] * a[r] : 0.f;
+        rs += ww;
+        cs[r] = group_sum<16>(ww);
+      }
+      rs = xor32_sum(xor16_sum(rs));
+      const int idx = ta * (ta + 1) / 2 + ja, sl = DOT == 2 ? c & 1 : 0;
+      if (g == 0) lds.rows[sl][idx][DOT == 2 ? i : 0] = rs;
+      if (i == 0) *reinterpret_cast<f32x4*>(&lds.cols[sl][idx][DOT == 2 ? 4 * g : 0]) = cs;
+    }
+  };
+  // the gate's dot products of chunk c, all of whose shares are in LDS
+  auto finish_dots = [&](int c) {
+    if (!DOT || c < 0 || w != 1 || lane >= len_of(c)) return;
+    const int sl = DOT ? c & 1 : 0;
+    float x = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < SW; ++ww) x += lds.dots[sl][ww][DOT ? lane : 0];
+    if (DOT == 2) {
+      const int ta = REV ? 3 - g : g;  // the token's tile, as query and as key
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        if (o <= ta) x += lds.rows[DOT == 2 ? sl : 0][ta * (ta + 1) / 2 + o][DOT == 2 ? i : 0];
+        if (o >= ta) x -= lds.cols[DOT == 2 ? sl : 0][o * (o + 1) / 2 + ta][DOT == 2 ? i : 0];
+      }
+    }
+    const int64_t tokens = p.cu ? p.T : p.N * p.T;
+    p.dot[hv * tokens + sg.tok + first_of(c) + lane] = x;
+  };
+  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
+  fetch_qk(0, 0);
+  fetch_v(0, 0);
+  fetch_qk(1, 1);
+  fetch_v(1, 1);
+  decays(0);
+  decays(1);
+  put_qk(0, 0);
+  fetch_qk(2, 0);
+  put_v(0, 0);
+  fetch_v(2, 0);
+  put_qk(1, 1);
+  fetch_qk(3, 1);
+  __syncthreads();
+  scores(0);
+  __syncthreads();
+  auto step = [&](int c, int set) {  // set: c & 1
+    put_v(c + 1, 1 - set);
+    fetch_v(c + 3, 1 - set);
+    put_qk(c + 2, set);
+    fetch_qk(c + 4, set);
+    decays(c + 2);
+    f32x4 held[3];
+    if (DOT == 2) {
+#pragma unroll
+      for (int n = 0; n < 3; ++n) held[n] = pv[n];
+    }
+    scores(c + 1);
+    if (DOT == 2) score_dots(c, held);
+    finish_dots(c - 1);
+    __syncthreads();
+  };
+  for (int c = 0; c < nc; c += 2) {
+    step(c, 0);
+    if (c + 1 < nc) step(c + 1, 1);
+  }
+  finish_dots(nc - 1);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -721,7 +842,7 @@ struct LinPlan {
 };
 
 // Segments of a power of two of tokens, as short as gives kLinGroups workgroups and no shorter than kLinMinSegment.
-constexpr int64_t kLinGroups = 512, kLinMinSegment = 256;
+constexpr int64_t kLinGroups = 256, kLinMinSegment = 256;
 
 static LinPlan lin_plan(int64_t B, int64_t T, int64_t HV, int64_t N, bool varlen) {
   LinPlan pl{};
@@ -742,34 +863,30 @@ static int64_t lin_states_bytes(const LinPlan& pl, int64_t HV, int64_t K, int64_
   return pl.split ? align256l(pl.slots * HV * K * V * 4) + align256l(pl.slots * HV * 4) : 0;
 }
 
-// Waves of a workgroup for V columns.
-constexpr int kLinWaves64 = 4, kLinWaves128 = 4;
-
 template <typename F>
 static void lin_by_dims(int64_t K, int64_t V, F go) {
   using C64 = std::integral_constant<int, 64>;
   using C128 = std::integral_constant<int, 128>;
-  if (K == 128 && V == 128) go(C128{}, C128{}, std::integral_constant<int, kLinWaves128>{});
-  else if (K == 64 && V == 64) go(C64{}, C64{}, std::integral_constant<int, kLinWaves64>{});
-  else if (K == 128) go(C128{}, C64{}, std::integral_constant<int, kLinWaves64>{});
-  else go(C64{}, C128{}, std::integral_constant<int, kLinWaves128>{});
+  if (K == 128 && V == 128) go(C128{}, C128{});
+  else if (K == 64 && V == 64) go(C64{}, C64{});
+  else if (K == 128) go(C128{}, C64{});
+  else go(C64{}, C128{});
 }
 
 template <bool REV>
 static void launch_segments(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  lin_by_dims(K, V, [&](auto k, auto v, auto w) {
-    hipLaunchKernelGGL((gated_deltaless_segment_kernel<decltype(k)::value, decltype(v)::value, decltype(w)::value, REV>),
-                       dim3((unsigned)(pl.slots * p.HV)), dim3(decltype(w)::value * kWave), 0, s, p);
-  });
+  const dim3 grid((unsigned)(pl.slots * p.HV), (unsigned)(V / 64));
+  if (K == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, REV>), grid, dim3(256), 0, s, p, (int)V);
+  else hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, REV>), grid, dim3(256), 0, s, p, (int)V);
   hipLaunchKernelGGL((gated_deltaless_scan_kernel<REV>), dim3((unsigned)(p.N * p.HV * (K * V / 1024))), dim3(256), 0, s, p,
                      K * V);
 }
 
 template <bool REV, int DOT, typename OT>
 static void launch_walk(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  lin_by_dims(K, V, [&](auto k, auto v, auto w) {
-    hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k)::value, decltype(v)::value, decltype(w)::value, REV, DOT, OT>),
-                       dim3((unsigned)(pl.slots * p.HV)), dim3(decltype(w)::value * kWave), 0, s, p);
+  lin_by_dims(K, V, [&](auto k, auto v) {
+    hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k)::value, decltype(v)::value, REV, DOT, OT>),
+                       dim3((unsigned)(pl.slots * p.HV)), dim3(512), 0, s, p);
   });
 }
 
@@ -795,7 +912,7 @@ static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t 
       return GDN_ERR_INVALID;
     }
   const LinPlan pl = lin_plan(B, T, HV, N, varlen);
-  if (pl.slots * HV > 0x7fffffffLL || pl.spq > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
+  if (HV > 65536 || pl.slots * HV > 0x7fffffffLL || pl.spq > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
     gdn_internal_set_error("%s: too many sequences, heads or tokens for one launch", name);
     return GDN_ERR_UNSUPPORTED;
   }

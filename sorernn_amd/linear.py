@@ -49,7 +49,7 @@ def _state(x: Optional[Tensor]) -> Optional[Tensor]:
 # ---------------------------------------------------------------------------------------------------
 # sorernn::chunk_decay_linear_attention_fwd / _bwd
 # ---------------------------------------------------------------------------------------------------
-_MIN_SEGMENT, _GROUPS = 256, 512
+_MIN_SEGMENT, _GROUPS = 256, 256
 
 
 def _align256(x):
@@ -58,7 +58,7 @@ def _align256(x):
 
 def states_bytes(b, t, hv, kd, vd, n, varlen: bool):
     """``gdn_decay_attn_states_size`` in Python: the fp32 states entering the segments (a power of two of tokens, 256 at
-    least and as short as gives 512 workgroups) and the segments' decays."""
+    least and as short as gives 256 workgroups) and the segments' decays."""
     seg = _MIN_SEGMENT
     while seg < t and (b * t // seg) * hv > _GROUPS:
         seg *= 2
