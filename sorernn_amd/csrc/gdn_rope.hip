@@ -3,10 +3,11 @@
 //   y = x rsqrt(mean(x^2) + eps) w;  out = y with its first rot entries rotated: (lo c - hi s, hi c + lo s),
 //   lo = y[0 : rot / 2], hi = y[rot / 2 : rot], c, s = cos, sin(position theta^(-2f / rot)), f = 0 .. rot / 2 - 1
 //
-// fp32 throughout, one rounding at the end. Bound by the bytes of the rows: D / 8 lanes take a row, 16 bytes (fp32: 32)
-// each. Angles are taken in turns in 64 bits, position * (theta^(-2f / rot) / 2 pi) less its whole part: at position
-// 1,000,000 a 32-bit angle is off by 0.06 rad. A token's rot / 2 pairs of cos and sin are computed once, into LDS, for
-// all its heads.
+// fp32 throughout, one rounding at the end. Bound by the bytes of the rows. A wave takes a token (with few tokens a
+// workgroup's 4 waves share one) and its heads D / 8 lanes each; a lane holds two pieces of 4 elements that turn with one
+// another, so that nothing is exchanged between lanes but the sum of squares. Angles are taken in turns in 64 bits,
+// position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.
+// A token's rot / 2 pairs of cos and sin are computed once for all its heads and pass through LDS.
 
 #include <math.h>
 
@@ -16,8 +17,8 @@
 
 namespace gdn {
 
-constexpr int kRopeTok = 4;          // tokens of a workgroup's step, at most
-constexpr int kRopeBwdBlocks = 1024; // workgroups of the backward, at most: each leaves one row of weight gradient sums
+constexpr int64_t kRopeBwdBlocks = 512;   // workgroups of the backward, at most: each leaves one row of weight gradient sums
+constexpr int64_t kRopeShared = 1024;     // up to this many tokens the 4 waves of a workgroup share one
 
 struct QkRopeParams {
   const void* x[2];              // q, k [B, T, heads, D] by strides (elements), last axis contiguous
@@ -31,14 +32,14 @@ struct QkRopeParams {
   const void* cu;
   int pos_i32, cu_i32;
   int64_t T, N, tokens;
-  int heads[2], rot, step;       // step: tokens of a workgroup's step
+  int heads[2], rot, wpt;        // wpt: waves that share a token
   float eps;
   double turns[128];             // theta^(-2f / rot) / 2 pi
 };
 
-__device__ __forceinline__ int64_t rope_position(const QkRopeParams& p, int64_t bt) {
-  if (p.pos) return load_index(p.pos, p.pos_i32, bt / p.T * p.pb + bt % p.T * p.pt);
-  if (!p.cu) return bt % p.T;
+__device__ __forceinline__ int64_t rope_position(const QkRopeParams& p, int64_t bt, int64_t bi, int64_t ti) {
+  if (p.pos) return load_index(p.pos, p.pos_i32, bi * p.pb + ti * p.pt);
+  if (!p.cu) return ti;
   int64_t lo = 0, hi = p.N;  // cu[lo] <= bt < cu[hi]
   while (hi - lo > 1) {
     const int64_t mid = (lo + hi) >> 1;
@@ -50,72 +51,90 @@ __device__ __forceinline__ int64_t rope_position(const QkRopeParams& p, int64_t 
 
 template <int D, typename E, bool BWD>
 __global__ __launch_bounds__(256) void gated_delta_qk_norm_rope_kernel(QkRopeParams p) {
-  constexpr int LPR = D / 8, RPP = 256 / LPR, U = sizeof(E) == 2 ? 4 : 2;  // lanes a row, rows a pass, passes in flight
-  using V8 __attribute__((aligned(16))) = E __attribute__((ext_vector_type(8)));
-  __shared__ float cs[kRopeTok][2][D / 2];
-  __shared__ float sums[BWD ? 2 * RPP * D : 1];
-  const int li = threadIdx.x % LPR, d0 = 8 * li, lane = threadIdx.x % kWave, half = p.rot >> 1;
-  const int hs = p.heads[0] + p.heads[1];
-  const bool lo = d0 < half, in_rot = d0 < p.rot;
-  const int other = in_rot ? (lo ? lane + half / 8 : lane - half / 8) : lane;
+  constexpr int LPR = D / 8, RPW = kWave / LPR, U = sizeof(E) == 2 ? 4 : 2;  // lanes a row, rows a pass, passes in flight
+  using V4 __attribute__((aligned(4 * sizeof(E)))) = E __attribute__((ext_vector_type(4)));
+  __shared__ __align__(16) float tab[4][2][D / 2];
+  __shared__ float sums[BWD ? 4 * RPW * 2 * D : 1];
+  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int li = lane % LPR, sub = lane / LPR, half = p.rot >> 1, np = half >> 2;
+  const bool in_rot = li < np;
+  const int d0 = in_rot ? 4 * li : p.rot + 8 * (li - np), d1 = in_rot ? d0 + half : d0 + 4;  // the lane's two pieces
+  const int hs = p.heads[0] + p.heads[1], r_first = (w % p.wpt) * RPW + sub, r_step = p.wpt * RPW;
   float wt[2][8], dw[2][8];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      wt[m][e] = p.w[m] ? p.w[m][d0 + e] : 1.f;
+      wt[m][e] = p.w[m] ? p.w[m][(e < 4 ? d0 : d1) + (e & 3)] : 1.f;
       dw[m][e] = 0.f;
     }
-  for (int64_t bt0 = (int64_t)blockIdx.x * p.step; bt0 < p.tokens; bt0 += (int64_t)gridDim.x * p.step) {
-    const int nt = p.tokens - bt0 < p.step ? (int)(p.tokens - bt0) : p.step, nrows = nt * hs;
-    __syncthreads();  // the table of the step before is read
-    for (int c = threadIdx.x; c < nt * half; c += 256) {
-      const int tk = c / half, f = c % half;
-      const double turn = (double)rope_position(p, bt0 + tk) * p.turns[f];
+  const int64_t stride = (int64_t)gridDim.x * 4 / p.wpt;
+  for (int64_t bt = ((int64_t)blockIdx.x * 4 + w) / p.wpt; bt < p.tokens; bt += stride) {
+    const int64_t bi = bt / p.T, ti = bt - bi * p.T;
+    const E* x0[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) x0[m] = static_cast<const E*>(p.x[m]) + bi * p.sb[m] + ti * p.st[m];
+    const E *dy0 = static_cast<const E*>(p.dy[0]) + bt * p.heads[0] * D, *dy1 = static_cast<const E*>(p.dy[1]) + bt * p.heads[1] * D;
+    E *y0 = static_cast<E*>(p.y[0]) + bt * p.heads[0] * D, *y1 = static_cast<E*>(p.y[1]) + bt * p.heads[1] * D;
+    V4 xv[U][2], dv[U][2];
+    auto load = [&](int r0) {  // U passes' rows; past the last head the last again
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * r_step < hs ? r0 + u * r_step : hs - 1;
+        const bool m = r >= p.heads[0];
+        const int hh = r - (m ? p.heads[0] : 0);
+        const E* src = (m ? x0[1] : x0[0]) + hh * (m ? p.sh[1] : p.sh[0]);
+        xv[u][0] = *reinterpret_cast<const V4*>(src + d0);
+        xv[u][1] = *reinterpret_cast<const V4*>(src + d1);
+        if (BWD) {
+          const E* up = (m ? dy1 : dy0) + hh * D;
+          dv[u][0] = *reinterpret_cast<const V4*>(up + d0);
+          dv[u][1] = *reinterpret_cast<const V4*>(up + d1);
+        }
+      }
+    };
+    int r0 = r_first;
+    load(r0);
+    const int64_t pos = rope_position(p, bt, bi, ti);
+    for (int f = lane; f < half; f += kWave) {
+      const double turn = (double)pos * p.turns[f];
       float sv, cv;
       sincospif(2.f * (float)(turn - rint(turn)), &sv, &cv);
-      cs[tk][0][f] = cv;
-      cs[tk][1][f] = sv;
+      tab[w][0][f] = cv;
+      tab[w][1][f] = sv;
     }
-    __syncthreads();
-    for (int r0 = threadIdx.x / LPR; r0 < nrows; r0 += U * RPP) {  // uniform inside a row's lanes
-      V8 xv[U], dv[U];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the table is the wave's own
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    float c[4], s[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = in_rot ? tab[w][0][d0 + e] : 1.f;
+      s[e] = in_rot ? tab[w][1][d0 + e] : 0.f;
+    }
+    for (; r0 < hs; r0 += U * r_step) {  // uniform inside a row's lanes
+      if (r0 != r_first) load(r0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * RPP < nrows ? r0 + u * RPP : r0, tk = r / hs, m = r % hs >= p.heads[0];
-        const int hh = r % hs - (m ? p.heads[0] : 0);
-        const int64_t bt = bt0 + tk;
-        xv[u] = *reinterpret_cast<const V8*>(static_cast<const E*>(p.x[m]) + bt / p.T * p.sb[m] + bt % p.T * p.st[m] +
-                                             hh * p.sh[m] + d0);
-        if (BWD) dv[u] = *reinterpret_cast<const V8*>(static_cast<const E*>(p.dy[m]) + (bt * p.heads[m] + hh) * D + d0);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * RPP;
-        if (r >= nrows) break;
-        const int tk = r / hs, m = r % hs >= p.heads[0], hh = r % hs - (m ? p.heads[0] : 0);
+        const int r = r0 + u * r_step;
+        if (r >= hs) break;
+        const bool m = r >= p.heads[0];
         float x[8], ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = (float)xv[u][e];
+          x[e] = (float)xv[u][e >> 2][e & 3];
           ss += x[e] * x[e];
         }
         const float rr = 1.f / sqrtf(group_sum<LPR>(ss) / (float)D + p.eps);
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = BWD ? (float)dv[u][e] : x[e] * rr * (m ? wt[1][e] : wt[0][e]);
-        float py[8];
+        for (int e = 0; e < 8; ++e) y[e] = BWD ? (float)dv[u][e >> 2][e & 3] : x[e] * rr * (m ? wt[1][e] : wt[0][e]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) py[e] = __shfl(y[e], other, kWave);
-        if (in_rot) {
-          const int f = lo ? d0 : d0 - half;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float c = cs[tk][0][f + e], s = cs[tk][1][f + e];
-            y[e] = y[e] * c + ((lo != BWD) ? -py[e] : py[e]) * s;  // the backward turns by the negative angle
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float a = y[e], b = y[4 + e], sn = BWD ? -s[e] : s[e];  // the backward turns by the negative angle
+          y[e] = a * c[e] - b * sn;
+          y[4 + e] = b * c[e] + a * sn;
         }
-        V8 out;
         if (BWD) {
           float dot = 0.f;
 #pragma unroll
@@ -126,42 +145,50 @@ __global__ __launch_bounds__(256) void gated_delta_qk_norm_rope_kernel(QkRopePar
             y[e] *= m ? wt[1][e] : wt[0][e];
             dot += y[e] * x[e];
           }
-          const float c = rr * (rr * (group_sum<LPR>(dot) / (float)D));  // of the order of y: r^3 alone may be subnormal
+          const float k = rr * (rr * (group_sum<LPR>(dot) / (float)D));  // of the order of y: r^3 alone may be subnormal
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = rr * y[e] - x[e] * rr * c;
+          for (int e = 0; e < 8; ++e) y[e] = rr * y[e] - x[e] * rr * k;
         }
+        V4 o0, o1;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = (E)y[e];
-        *reinterpret_cast<V8*>(static_cast<E*>(p.y[m]) + ((bt0 + tk) * p.heads[m] + hh) * D + d0) = out;
+        for (int e = 0; e < 4; ++e) {
+          o0[e] = (E)y[e];
+          o1[e] = (E)y[4 + e];
+        }
+        E* dst = (m ? y1 : y0) + (int64_t)(r - (m ? p.heads[0] : 0)) * D;
+        *reinterpret_cast<V4*>(dst + d0) = o0;
+        *reinterpret_cast<V4*>(dst + d1) = o1;
       }
     }
+    __builtin_amdgcn_wave_barrier();  // the table is read before the next token's is written
   }
   if (BWD && p.partial) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sums[((int)(threadIdx.x / LPR) * 2 + m) * D + d0 + e] = dw[m][e];
+      for (int e = 0; e < 8; ++e) sums[((w * RPW + sub) * 2 + m) * D + (e < 4 ? d0 : d1) + (e & 3)] = dw[m][e];
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * D; c += 256) {
       float x = 0.f;
-      for (int r = 0; r < RPP; ++r) x += sums[r * 2 * D + c];
+      for (int r = 0; r < 4 * RPW; ++r) x += sums[r * 2 * D + c];
       p.partial[(int64_t)blockIdx.x * 2 * D + c] = x;
     }
   }
 }
 
-// The weights' gradients from the workgroups' sums: 16 columns a workgroup, 16 threads a column, in a fixed order.
-__global__ __launch_bounds__(256) void gated_delta_qk_norm_rope_param_grad_kernel(const float* partial, int rows, int D,
-                                                                                 float* dqw, float* dkw) {
-  __shared__ float part[16][17];
+// The weights' gradients from the workgroups' sums: 16 columns a workgroup, 64 threads a column, in a fixed order.
+__global__ __launch_bounds__(1024) void gated_delta_qk_norm_rope_param_grad_kernel(const float* partial, int rows, int D,
+                                                                                  float* dqw, float* dkw) {
+  __shared__ float part[64][17];
   const int col = threadIdx.x % 16, at = blockIdx.x * 16 + col;
   float x = 0.f;
-  for (int r = threadIdx.x / 16; r < rows; r += 16) x += partial[(int64_t)r * 2 * D + at];
+#pragma unroll 8
+  for (int r = threadIdx.x / 16; r < rows; r += 64) x += partial[(int64_t)r * 2 * D + at];
   part[threadIdx.x / 16][col] = x;
   __syncthreads();
   if (threadIdx.x >= 16) return;
   x = 0.f;
-  for (int r = 0; r < 16; ++r) x += part[r][col];
+  for (int r = 0; r < 64; ++r) x += part[r][col];
   float* out = at < D ? dqw : dkw;
   if (out) out[at % D] = x;
 }
@@ -205,8 +232,7 @@ static int rope_check(const char* name, QkRopeParams& p, int64_t B, int64_t T, i
   p.heads[1] = (int)HK;
   p.rot = rot_dim;
   p.eps = eps;
-  // 4 tokens share a workgroup once 1,024 workgroups have work without that
-  p.step = p.tokens >= 1024 * kRopeTok ? kRopeTok : 1;
+  p.wpt = p.tokens <= kRopeShared ? 4 : 1;
   for (int f = 0; f < rot_dim / 2; ++f) p.turns[f] = pow(theta, -2. * f / rot_dim) / 6.283185307179586;
   return GDN_OK;
 }
@@ -227,10 +253,8 @@ static void launch_rope(const QkRopeParams& p, int64_t D, int dtype, int64_t blo
   else by_dim(float{});
 }
 
-static int64_t rope_bwd_blocks(int64_t tokens) {
-  const int64_t b = tokens >= 1024 * kRopeTok ? (tokens + kRopeTok - 1) / kRopeTok : tokens;
-  return b < kRopeBwdBlocks ? b : kRopeBwdBlocks;
-}
+static int64_t rope_blocks(int64_t tokens) { return tokens <= kRopeShared ? tokens : (tokens + 3) / 4; }
+static int64_t rope_bwd_blocks(int64_t tokens) { return rope_blocks(tokens) < kRopeBwdBlocks ? rope_blocks(tokens) : kRopeBwdBlocks; }
 
 }  // namespace gdn
 
@@ -252,8 +276,8 @@ extern "C" int gdn_qk_norm_rope_fwd(const void* q, int64_t q_batch_stride, int64
                  pos_token_stride, cu_seqlens, pos_i32, (flags & GDN_FLAG_CU_INT32) ? 1 : 0};
   if (int rc = rope_check("gdn_qk_norm_rope_fwd", p, B, T, HQ, HK, D, N, dtype, rot_dim, theta, eps)) return rc;
   if (T == 0) return GDN_OK;
-  const int64_t steps = (p.tokens + p.step - 1) / p.step;
-  launch_rope<false>(p, D, dtype, steps < 0x7fffffffLL ? steps : 0x7fffffffLL, static_cast<hipStream_t>(stream));
+  const int64_t blocks = rope_blocks(p.tokens);
+  launch_rope<false>(p, D, dtype, blocks < 0x3fffffffLL ? blocks : 0x3fffffffLL, static_cast<hipStream_t>(stream));
   return gdn_internal_check_launch("gated_delta_qk_norm_rope_kernel");
 }
 
@@ -291,7 +315,7 @@ extern "C" int gdn_qk_norm_rope_bwd(const void* q, int64_t q_batch_stride, int64
     if (int rc = gdn_internal_check_launch("gated_delta_qk_norm_rope_kernel(bwd)")) return rc;
   }
   if (params) {  // without tokens: zeros
-    hipLaunchKernelGGL(gated_delta_qk_norm_rope_param_grad_kernel, dim3((unsigned)(2 * D / 16)), dim3(256), 0, s, p.partial,
+    hipLaunchKernelGGL(gated_delta_qk_norm_rope_param_grad_kernel, dim3((unsigned)(2 * D / 16)), dim3(1024), 0, s, p.partial,
                        (int)blocks, (int)D, dq_weight, dk_weight);
     return gdn_internal_check_launch("gated_delta_qk_norm_rope_param_grad_kernel");
   }

@@ -29,9 +29,13 @@ __all__ = ["chunk_decay_linear_attention", "fused_recurrent_decay_linear_attenti
 
 def _launch(name: str, x: Tensor, *args) -> None:
     """``_lib.call`` on ``x``'s device and its current stream (a launch goes to the current device)."""
-    if x.is_cuda and x.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
-            _lib.call(name, *args, _lib.stream_of(x))
+    if x.is_cuda:
+        index = x.get_device()
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            return
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         _lib.call(name, *args, _lib.stream_of(x))
 
@@ -43,7 +47,10 @@ def _rows(x: Tensor) -> Tensor:
 
 
 def _state(x: Optional[Tensor]) -> Optional[Tensor]:
-    return None if x is None else _rows(x.float())
+    return None if x is None else _rows(x if x.dtype == torch.float32 else x.float())
+
+
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
 # ---------------------------------------------------------------------------------------------------
@@ -70,7 +77,7 @@ def states_bytes(b, t, hv, kd, vd, n, varlen: bool):
 
 def _gate_args(g: Optional[Tensor]):
     """dtype code and element strides of ``g`` ``[B, T, HV]`` (0 where it was expanded)."""
-    return (_lib.DTYPE_F32, 0, 0, 0) if g is None else (_lib.dtype_code(g.dtype), *g.stride())
+    return (_lib.DTYPE_F32, 0, 0, 0) if g is None else (_CODES[g.dtype], *g.stride())
 
 
 def attention_fwd_impl(q: Tensor, k: Tensor, v: Tensor, g: Optional[Tensor], initial_state: Optional[Tensor],
@@ -81,7 +88,7 @@ def attention_fwd_impl(q: Tensor, k: Tensor, v: Tensor, g: Optional[Tensor], ini
     qc, kc, vc = _rows(q), _rows(k), _rows(v)
     h0 = _state(initial_state)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    o = torch.empty(b, t, hv, vd, device=q.device, dtype=q.dtype)
+    o = torch.empty_like(vc)
     final = torch.empty((num_seqs, hv, kd, vd) if output_final_state else (0,), device=q.device, dtype=torch.float32)
     states = torch.empty(states_bytes(b, t, hv, kd, vd, num_seqs, cu is not None), device=q.device, dtype=torch.uint8)
     if t > 0:
@@ -250,12 +257,12 @@ def _recurrent(name, q, k, v, g, scale, initial_state, output_final_state, inpla
     final = h0 if inplace else None
     if output_final_state and not inplace:
         final = torch.empty(n, hv, kd, vd, device=q.device, dtype=torch.float32)
-    o = torch.empty(b, t, hv, vd, device=q.device, dtype=q.dtype)
+    o = torch.empty_like(v)
     if t > 0 or (final is not None and not inplace):
         cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-        _launch("gdn_decay_attn_recurrent_fwd", q, _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(g), _lib.ptr(h0),
-                _lib.ptr(o), _lib.ptr(final), _lib.ptr(cu), b, t, h, hv, kd, vd, n, _lib.dtype_code(q.dtype),
-                *_gate_args(g), scale, flags)
+        ptr = _lib.ptr
+        _launch("gdn_decay_attn_recurrent_fwd", q, ptr(q), ptr(k), ptr(v), ptr(g), ptr(h0), ptr(o), ptr(final), ptr(cu), b, t,
+                h, hv, kd, vd, n, _CODES[q.dtype], *_gate_args(g), scale, flags)
     return o, final
 
 
@@ -275,32 +282,32 @@ def fused_recurrent_decay_linear_attention(q: Tensor, k: Tensor, v: Tensor, g: T
 # ---------------------------------------------------------------------------------------------------
 # sorernn::qk_norm_rope_fwd / _bwd
 # ---------------------------------------------------------------------------------------------------
-def _strided(x: Tensor) -> Tensor:
-    """``x`` if its rows can be read where they are (contiguous, each on a 16-byte address), else a copy."""
-    unit = 16 // x.element_size()
-    if x.stride(3) == 1 and not x.data_ptr() & 15 and not (x.stride(0) % unit or x.stride(1) % unit or x.stride(2) % unit):
-        return x
-    return _rows(x)
+def _strided(x: Tensor):
+    """``x`` and its strides if its rows can be read where they are (contiguous, each on a 16-byte address), else a copy's."""
+    st = x.stride()
+    if st[3] != 1 or x.data_ptr() & 15 or (st[0] | st[1] | st[2]) & (16 // x.element_size() - 1):
+        x = _rows(x)
+        st = x.stride()
+    return x, st
 
 
-def _rope_args(q, k, q_weight, k_weight, positions):
-    w = tuple(None if x is None else x.float().contiguous() for x in (q_weight, k_weight))
-    ps = (0, 0, 0) if positions is None else (*positions.stride(), int(positions.dtype == torch.int32))
-    # the weights are returned to live until the launch
-    return w, (_lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(w[0]), _lib.ptr(w[1]),
-               _lib.ptr(positions), *ps)
+def _weight(w: Optional[Tensor]) -> Optional[Tensor]:
+    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.float().contiguous()
 
 
 def rope_fwd_impl(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], positions: Optional[Tensor],
                   cu_seqlens: Optional[Tensor], rot_dim: int, theta: float, eps: float, flags: int,
                   num_seqs: int) -> tuple[Tensor, Tensor]:
     b, t, hq, d = q.shape
-    qs, ks = _strided(q), _strided(k)
+    (qs, qst), (ks, kst) = _strided(q), _strided(k)
+    qw, kw = _weight(q_weight), _weight(k_weight)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    qo, ko = (torch.empty(x.shape, device=q.device, dtype=q.dtype) for x in (q, k))
-    w, args = _rope_args(qs, ks, q_weight, k_weight, positions)
-    _launch("gdn_qk_norm_rope_fwd", qs, *args, _lib.ptr(qo), _lib.ptr(ko), _lib.ptr(cu), b, t, hq, k.shape[2], d, num_seqs,
-            _lib.dtype_code(q.dtype), rot_dim, theta, eps, flags)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+    ptr = _lib.ptr
+    ps = (None, 0, 0, 0) if positions is None else (ptr(positions), *positions.stride(), positions.dtype == torch.int32)
+    _launch("gdn_qk_norm_rope_fwd", qs, ptr(qs), qst[0], qst[1], qst[2], ptr(ks), kst[0], kst[1], kst[2], ptr(qw), ptr(kw),
+            *ps, ptr(qo), ptr(ko), ptr(cu), b, t, hq, k.shape[2], d, num_seqs, _CODES[q.dtype], rot_dim, theta, eps, flags)
     return qo, ko
 
 
@@ -316,18 +323,20 @@ def rope_bwd_impl(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Op
                   cu_seqlens: Optional[Tensor], dq_out: Tensor, dk_out: Tensor, rot_dim: int, theta: float, eps: float,
                   flags: int, num_seqs: int, weight_grads: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     b, t, hq, d = q.shape
-    qs, ks, dqo, dko = _strided(q), _strided(k), _rows(dq_out.to(q.dtype)), _rows(dk_out.to(q.dtype))
+    (qs, qst), (ks, kst), dqo, dko = _strided(q), _strided(k), _rows(dq_out.to(q.dtype)), _rows(dk_out.to(q.dtype))
+    qw, kw = _weight(q_weight), _weight(k_weight)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    dev = q.device
-    dq, dk = (torch.empty(x.shape, device=dev, dtype=q.dtype) for x in (q, k))
-    dw = [torch.empty(d if weight_grads and x is not None else 0, device=dev, dtype=torch.float32)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    dw = [torch.empty(d if weight_grads and x is not None else 0, device=q.device, dtype=torch.float32)
           for x in (q_weight, k_weight)]
     nbytes = int(_lib.load().gdn_qk_norm_rope_bwd_workspace_size(b, t, d)) if weight_grads else 0
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    w, args = _rope_args(qs, ks, q_weight, k_weight, positions)
-    _launch("gdn_qk_norm_rope_bwd", qs, *args, _lib.ptr(dqo), _lib.ptr(dko), _lib.ptr(dq), _lib.ptr(dk),
-            *(_lib.ptr(x) if x.numel() else None for x in dw), _lib.ptr(cu), b, t, hq, k.shape[2], d, num_seqs,
-            _lib.dtype_code(q.dtype), rot_dim, theta, eps, flags, _lib.ptr(ws), nbytes)
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+    ptr = _lib.ptr
+    ps = (None, 0, 0, 0) if positions is None else (ptr(positions), *positions.stride(), positions.dtype == torch.int32)
+    _launch("gdn_qk_norm_rope_bwd", qs, ptr(qs), qst[0], qst[1], qst[2], ptr(ks), kst[0], kst[1], kst[2], ptr(qw), ptr(kw),
+            *ps, ptr(dqo), ptr(dko), ptr(dq), ptr(dk), *(ptr(x) if x.numel() else None for x in dw), ptr(cu), b, t, hq,
+            k.shape[2], d, num_seqs, _CODES[q.dtype], rot_dim, theta, eps, flags, ptr(ws), nbytes)
     return dq, dk, dw[0], dw[1]
 
 
@@ -389,7 +398,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor | None = None, k_weight:
     if not b or not hq or not k.shape[2]:
         raise ValueError(f"{name}: no batch or no heads in q {tuple(q.shape)}, k {tuple(k.shape)}")
     for w in (q_weight, k_weight):
-        if w is not None and tuple(w.shape) != (d,):
+        if w is not None and w.shape != (d,):
             raise ValueError(f"{name}: weights must be [{d}], got {tuple(w.shape)}")
     rot_dim = d if rot_dim is None else int(rot_dim)
     if d not in (64, 128, 256) or rot_dim < 0 or rot_dim > d or rot_dim % 16:
@@ -398,9 +407,10 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Tensor | None = None, k_weight:
     if positions is not None:
         if cu_seqlens is not None:
             raise ValueError(f"{name}: positions and cu_seqlens exclude each other")
-        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((b, t), (t,)):
+        if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((b, t), (t,)):
             raise ValueError(f"{name}: positions must be int32 or int64 {(b, t)} or {(t,)}, got {positions.dtype} "
                              f"{tuple(positions.shape)}")
-        positions = positions.expand(b, t)
+        if positions.dim() == 1:
+            positions = positions.expand(b, t)
     n, flags = _cu_info(name, cu_seqlens, cu_seqlens_cpu, b, t)
     return rope_fwd_call(q, k, q_weight, k_weight, positions, cu_seqlens, rot_dim, float(theta), float(eps), flags, n)

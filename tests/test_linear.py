@@ -134,7 +134,7 @@ def test_sizes_match_the_library():
     assert lib.gdn_decay_attn_states_size(0, 1, 1, 64, 64, 1, 0) == 0
     assert lib.gdn_decay_attn_bwd_workspace_size(1, 8, 2, 3, 64, 64, 1, 0) == 0
     assert lib.gdn_qk_norm_rope_bwd_workspace_size(1, 3, 64) == 3 * 2 * 64 * 4
-    assert lib.gdn_qk_norm_rope_bwd_workspace_size(4, 4096, 128) == 1024 * 2 * 128 * 4
+    assert lib.gdn_qk_norm_rope_bwd_workspace_size(4, 4096, 128) == 512 * 2 * 128 * 4
 
 
 def test_entry_points_check_their_arguments():
