@@ -13,11 +13,11 @@
 //                                      (k, q, do) and (v, do, q)
 //   dg_t = exp(g_t) <S_{t-1}, R_t> = sum over i >= t of (q_i . dq_i - k_i . dk_i), plus <S_T, dS_T>
 //
-// A workgroup of V / 16 waves walks one segment of a sequence for one value head. The state stays in fp32 MFMA
-// accumulators, wave w holding all K rows of 16 columns; it is the A operand of S^T Q^T as it stands, split into
-// bf16 parts in registers. Sequences are cut into segments so that few heads fill the chip: a first kernel walks
-// the segments for their own contribution to the state (k and v only), a scan over the segments turns these into the
-// states that enter them, and the walkers then run side by side.
+// The state stays in fp32 MFMA accumulators, a wave holding all K rows of its columns; it is the A operand of S^T Q^T as it
+// stands, split into bf16 parts in registers. A workgroup walks one segment of the flat token axis for one value head,
+// over the sequences' borders, so that 256 workgroups have the same number of tokens whatever the sequences' lengths are.
+// For the sequence that a segment's border cuts, a first kernel walks the segment for its own contribution to the state
+// (k and v only), a scan over the segments turns these into the states at the borders, and the walkers run side by side.
 //
 // Rounding: q, k, v and do are bf16 operands as they come. What is computed is split into bf16 parts that are multiplied
 // one by one: three (24 bits, as fp32 holds) where the result is an fp32 output (the state, and what dg sums), two
@@ -39,65 +39,87 @@ struct LinParams {
   int dg;
   int64_t gb, gt, gh;           // element strides of batch row, token and value head
   const float* init;            // [N][HV][K][V] state before the walk, or null: zeros
-  float* entry;                 // [slots][HV][K][V] states entering the segments, or null: one segment a sequence
-  float* decay;                 // [slots][HV] decay of a whole segment
+  float* entry;                 // [segments][HV][K][V] states entering the segments, or null where no border cuts a sequence
+  float* decay;                 // [segments][HV] decay of the sequence that goes on in the next segment; 0: it begins here
   int transposed;               // init and entry are read as [V][K]
   float* fin;                   // [N][HV][K][V] state after the walk, or null
   void* o;                      // [tokens][HV][V]
   float* dot;                   // [HV][tokens] with DOT
   const void* cu;
-  int cu_i32, shift;            // segments of 1 << shift tokens
-  int64_t T, N;
-  unsigned HV, spq;             // spq: segments of a sequence without cu
+  int cu_i32, T, N, tokens, L;  // segments of L tokens; without cu sequences of T
+  unsigned HV;
   float scale;
 };
 
-// Where a workgroup works: sequence n, the segment's first token (flat) and length, and its place in the sequence.
-struct Segment {
-  int64_t n, slot, tok, row, col;  // row, col: batch row and first token in it (the gate's strides)
-  int len;
-  bool first, last, some;
+// First token of sequence n; of n = N the number of tokens.
+__device__ __forceinline__ int seq_start(const LinParams& p, int n) {
+  return p.cu ? (int)load_index(p.cu, p.cu_i32, n) : n * p.T;
+}
+
+// The sequence of token t. All lanes of a wave search together.
+__device__ __forceinline__ int seq_of(const LinParams& p, int t) {
+  if (!p.cu) return (unsigned)t / (unsigned)p.T;
+  const int lane = threadIdx.x % kWave;
+  int lo = 0, hi = p.N;  // start of lo <= t < start of hi
+  while (hi - lo > 1) {
+    const int step = (hi - lo + kWave - 1) / kWave, i = lo + lane * step;
+    const bool in = i < hi && load_index(p.cu, p.cu_i32, i < hi ? i : lo) <= t;
+    const int cnt = __popcll(__ballot(in));  // one at least: lane 0's
+    lo += (cnt > 1 ? cnt - 1 : 0) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Up to 64 tokens of sequence n in walking order: fresh, the walk of the sequence begins with them; done, it ends.
+struct Chunk {
+  int t, len, n;  // len 0: none
+  bool fresh, done;
 };
 
-// Slots of a sequence: with cu, sequence n has the slots from (cu[n] >> shift) + n on, which leaves room for its
-// segments whatever the lengths are, so that the grid depends on T and N alone. All lanes of a wave search together.
-__device__ __forceinline__ Segment find_segment(const LinParams& p, unsigned slot) {
-  Segment s;
-  int64_t bos, len, local;
-  const int64_t L = (int64_t)1 << p.shift;
-  if (p.cu) {
-    const int lane = threadIdx.x % kWave;
-    int64_t lo = 0, hi = p.N;  // first slot of sequence lo <= slot < that of sequence hi
-    while (hi - lo > 1) {
-      const int64_t step = (hi - lo + kWave - 1) / kWave, i = lo + lane * step;
-      const bool in = i < hi && (load_index(p.cu, p.cu_i32, i < hi ? i : lo) >> p.shift) + i <= slot;
-      const int cnt = __popcll(__ballot(in));  // one at least: lane 0's
-      lo += (cnt > 1 ? cnt - 1 : 0) * step;
-      hi = lo + step < hi ? lo + step : hi;
-    }
-    s.n = lo;
-    bos = load_index(p.cu, p.cu_i32, lo);
-    len = load_index(p.cu, p.cu_i32, lo + 1) - bos;
-    local = slot - ((bos >> p.shift) + lo);
-    s.row = 0;
-    s.col = bos + local * L;
-  } else {
-    s.n = slot / p.spq;
-    local = slot % p.spq;
-    bos = s.n * p.T;
-    len = p.T;
-    s.row = s.n;
-    s.col = local * L;
+// The chunks of tokens [lo, hi) in walking order. Chunks begin where a sequence or the segment does.
+template <bool REV>
+struct ChunkWalk {
+  int lo, hi, n, bos, eos, t;  // t: REV, the end of what is left; else its start
+  __device__ __forceinline__ void start(const LinParams& p, int from, int to) {
+    lo = from;
+    hi = to;
+    n = seq_of(p, REV ? hi - 1 : lo);
+    bos = seq_start(p, n);
+    eos = seq_start(p, n + 1);
+    t = REV ? hi : lo;
   }
-  s.slot = slot;
-  s.tok = bos + local * L;
-  const int64_t left = len - local * L;
-  s.some = left > 0;
-  s.len = (int)(left < L ? left : L);
-  s.first = local == 0;
-  s.last = left <= L;
-  return s;
-}
+  __device__ __forceinline__ Chunk next(const LinParams& p) {
+    Chunk c{0, 0, n, false, false};
+    if (REV ? t <= lo : t >= hi) return c;
+    if (REV) {
+      const int first = bos > lo ? bos : lo;
+      c.t = first + ((t - 1 - first) & ~(kC - 1));
+      c.len = t - c.t;
+      c.fresh = t == eos;
+      c.done = c.t == bos;
+      t = c.t;
+      if (t == bos && t > lo) {
+        --n;
+        eos = bos;
+        bos = seq_start(p, n);
+      }
+    } else {
+      const int end = eos < hi ? eos : hi;
+      c.t = t;
+      c.len = end - t < kC ? end - t : kC;
+      c.fresh = t == bos;
+      c.done = t + c.len == eos;
+      t += c.len;
+      if (t == eos && t < hi) {
+        ++n;
+        bos = eos;
+        eos = seq_start(p, n + 1);
+      }
+    }
+    return c;
+  }
+};
 
 // Decay terms of a chunk, base-2 logarithms: b = h + l in two floats, the weight of a token in the state's update and
 // that of the state in a token's output (each with the factor it carries), and the decay of the whole chunk.
@@ -113,6 +135,19 @@ __device__ __forceinline__ double dpp_scan_step(double v) {
   return v + __hiloint2double(hi, lo);
 }
 
+__device__ __forceinline__ double wave_inclusive_sum64(double x) {
+  x = dpp_scan_step<0x111, 0xf>(x);
+  x = dpp_scan_step<0x112, 0xf>(x);
+  x = dpp_scan_step<0x114, 0xf>(x);
+  x = dpp_scan_step<0x118, 0xf>(x);
+  x = dpp_scan_step<0x142, 0xa>(x);
+  return dpp_scan_step<0x143, 0xc>(x);
+}
+__device__ __forceinline__ double last_lane(double x) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), kWave - 1),
+                          __builtin_amdgcn_readlane(__double2loint(x), kWave - 1));
+}
+
 // Log decays below -100 (exp of it is 0 beside any weight that counts) are taken as -100: a reset of -inf leaves the
 // differences of sums behind it finite.
 __device__ __forceinline__ double log2_decay(uint32_t raw, int dtype) {
@@ -123,14 +158,8 @@ __device__ __forceinline__ double log2_decay(uint32_t raw, int dtype) {
 // One wave, lane = token.
 template <bool REV>
 __device__ __forceinline__ void chunk_decays(Decays& d, double x, float scale, int lane) {
-  x = dpp_scan_step<0x111, 0xf>(x);
-  x = dpp_scan_step<0x112, 0xf>(x);
-  x = dpp_scan_step<0x114, 0xf>(x);
-  x = dpp_scan_step<0x118, 0xf>(x);
-  x = dpp_scan_step<0x142, 0xa>(x);
-  x = dpp_scan_step<0x143, 0xc>(x);
-  const double all = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), kWave - 1),
-                                      __builtin_amdgcn_readlane(__double2loint(x), kWave - 1));
+  x = wave_inclusive_sum64(x);
+  const double all = last_lane(x);
   const float head = __builtin_amdgcn_exp2f((float)x), tail = __builtin_amdgcn_exp2f((float)(all - x));
   d.h[lane] = (float)x;
   d.l[lane] = (float)(x - (double)(float)x);
@@ -244,7 +273,9 @@ struct State {
 #pragma unroll
       for (int ct = 0; ct < NCT; ++ct) s[a][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  __device__ __forceinline__ void load(const float* src, bool transposed, int w, int lane) {
+  // The addresses of load and store are computed where they are used, not kept in registers over the walk.
+  __device__ __forceinline__ void load(const float* src, int pitch, bool transposed, int w, int lane) {
+    lane = opaque_int(lane);
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
     for (int a = 0; a < NA; ++a)
@@ -254,11 +285,12 @@ struct State {
           s[a][ct] = *reinterpret_cast<const f32x4*>(src + col(w, ct, i) * KD + row0(a, g));
         } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[a][ct][r] = src[(row0(a, g) + r) * VD + col(w, ct, i)];
+          for (int r = 0; r < 4; ++r) s[a][ct][r] = src[(row0(a, g) + r) * pitch + col(w, ct, i)];
         }
       }
   }
   __device__ __forceinline__ void store(float* dst, int pitch, int w, int lane) const {
+    lane = opaque_int(lane);
     const int g = lane >> 4, i = lane & 15;
 #pragma unroll
     for (int a = 0; a < NA; ++a)
@@ -311,57 +343,67 @@ struct State {
   }
 };
 
-__device__ __forceinline__ uint32_t gate_raw(const LinParams& p, const Segment& sg, unsigned hv, int t) {
-  return load_raw32(p.g, p.dg, sg.row * p.gb + (sg.col + t) * p.gt + hv * p.gh);
-}
-
-// The gate of a segment's chunks in walking order, read by one wave: the raw values of the chunk after the next in flight.
-template <bool REV>
-struct GateWalk {
+// Raw gate values of a chunk's tokens, a lane each, read ahead of their use.
+struct GateRow {
   uint32_t raw = 0;
-  __device__ __forceinline__ void fetch(const LinParams& p, const Segment& sg, unsigned hv, int ci, int nc, int lane) {
-    const int t = (REV ? nc - 1 - ci : ci) * kC + lane;
-    raw = p.g && ci < nc && t < sg.len ? gate_raw(p, sg, hv, t) : 0u;
+  __device__ __forceinline__ void fetch(const LinParams& p, unsigned hv, const Chunk& c, int lane) {
+    const int64_t row = p.cu ? c.t * p.gt : c.n * p.gb + (c.t - c.n * p.T) * p.gt;
+    raw = p.g && lane < c.len ? load_raw32(p.g, p.dg, row + lane * p.gt + hv * p.gh) : 0u;
   }
   __device__ __forceinline__ double value(const LinParams& p) const { return p.g ? log2_decay(raw, p.dg) : 0.; }
 };
 
 // ------------------------------------------------------------------------------------------------
-// A segment's own contribution to the state: the walk without outputs, from a zero state. Forward walks leave it in
-// the next segment's slot, walks from the end in the one before; the sequence's last segment (first) has none to give.
-// Two workgroups share 128 columns, which doubles the waves in flight.
+// What a segment adds to the state of the sequence that its border cuts: the walk without outputs, from where the sequence
+// begins (with its initial state) or from the segment's other border (from zero). Forward walks leave it in the next
+// segment's place, walks from the end in that of the segment before. Two workgroups share 128 columns, which doubles the
+// waves in flight.
 template <int KD, bool REV>
 __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinParams p, int VD) {
   __shared__ __align__(16) bf16 Ks[kC * KD], Vs[kC * 64];
   __shared__ __align__(16) Decays d[2];
   const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const unsigned hv = blockIdx.x % p.HV;
-  const Segment sg = find_segment(p, blockIdx.x / p.HV);
-  if (!sg.some || (REV ? sg.first : sg.last)) return;
-  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD + blockIdx.y * 64;
-  const int nc = (sg.len + kC - 1) / kC;
+  const int seg = blockIdx.x / p.HV + (REV ? 1 : 0);  // without the last (first), whose border cuts nothing
+  int lo = seg * p.L, hi = lo + p.L < p.tokens ? lo + p.L : p.tokens;
+  const int n = seq_of(p, REV ? lo - 1 : hi), bos = seq_start(p, n), eos = seq_start(p, n + 1);
+  const bool whole = REV ? eos <= hi : bos >= lo;  // the sequence's walk begins in this segment
+  if (REV ? eos == lo : bos == hi) {               // no sequence is cut
+    if (threadIdx.x == 0 && blockIdx.y == 0) p.decay[(int64_t)seg * p.HV + hv] = 0.f;
+    return;
+  }
+  if (REV) hi = whole ? eos : hi;
+  else lo = whole ? bos : lo;
+  const bf16* k0 = p.k + lo * p.ks + hv / p.rk * KD;
+  const bf16* v0 = p.v + lo * p.vs + hv / p.rv * VD + blockIdx.y * 64;
+  const int nc = (hi - lo + kC - 1) / kC;
+  auto chunk = [&](int ci) {
+    Chunk c{lo + (REV ? nc - 1 - ci : ci) * kC, 0, n, false, false};
+    c.len = ci >= nc ? 0 : hi - c.t < kC ? hi - c.t : kC;
+    return c;
+  };
   Tile<KD> kt;
   Tile<64> vt;
-  GateWalk<REV> gate;
+  GateRow gate;
   const uint32_t koff = kt.offset(p.ks), voff = vt.offset(p.vs);
   auto fetch = [&](int ci) {
-    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
-    kt.fetch(k0 + t0 * p.ks, p.ks, koff, len);
-    vt.fetch(v0 + t0 * p.vs, p.vs, voff, len);
+    const Chunk c = chunk(ci);
+    kt.fetch(k0 + (c.t - lo) * p.ks, p.ks, koff, c.len);
+    vt.fetch(v0 + (c.t - lo) * p.vs, p.vs, voff, c.len);
   };
-  State<KD, 64, 4> st;
-  st.zero();
-  double total = 0.;
-  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
+  if (w == 0) gate.fetch(p, hv, chunk(0), lane);
   fetch(0);
+  State<KD, 64, 4> st;
+  if (whole && p.init) st.load(p.init + ((int64_t)n * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, false, w, lane);
+  else st.zero();
+  double total = 0.;
   if (w == 0) {
     total = gate.value(p);
     chunk_decays<REV>(d[0], total, p.scale, lane);
-    gate.fetch(p, sg, hv, 1, nc, lane);
+    gate.fetch(p, hv, chunk(1), lane);
   }
   for (int ci = 0; ci < nc; ++ci) {
-    const int t0 = (REV ? nc - 1 - ci : ci) * kC, len = sg.len - t0 < kC ? sg.len - t0 : kC;
+    const int len = chunk(ci).len;
     kt.put(Ks, len);
     vt.put(Vs, len);
     __syncthreads();
@@ -370,7 +412,7 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
       const double x = gate.value(p);
       total += x;
       chunk_decays<REV>(d[(ci + 1) & 1], x, p.scale, lane);
-      gate.fetch(p, sg, hv, ci + 2, nc, lane);
+      gate.fetch(p, hv, chunk(ci + 2), lane);
     }
     bf16x8 vf[2][1];
     st.columns(Vs, 0, w, lane, vf[0]);
@@ -378,49 +420,39 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
     st.update(d[ci & 1], Ks, vf, lane);
     __syncthreads();
   }
-  st.store(p.entry + ((sg.slot + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, w, lane);
+  st.store(p.entry + ((int64_t)(seg + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, w, lane);
   if (w == 0 && blockIdx.y == 0) {
     for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
-    if (lane == 0) p.decay[sg.slot * p.HV + hv] = __builtin_amdgcn_exp2f((float)total);
+    if (lane == 0) p.decay[(int64_t)seg * p.HV + hv] = whole ? 0.f : __builtin_amdgcn_exp2f((float)total);
   }
 }
 
 // The segments' contributions into the states entering them, in place: entry[s] += decay[s - 1] entry[s - 1] (from the
-// end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread.
+// end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread. Where a decay is 0 nothing of the other is read: it
+// may not have been written.
 template <bool REV>
-__global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, int64_t elems) {
-  const unsigned per = (unsigned)elems / 1024, chain = blockIdx.x / per, hv = chain % p.HV, n = chain / p.HV;
-  const int64_t at = (blockIdx.x % per) * 1024 + threadIdx.x * 4;
-  int64_t slot0, cnt;
-  if (p.cu) {
-    const int64_t bos = load_index(p.cu, p.cu_i32, n), eos = load_index(p.cu, p.cu_i32, (int64_t)n + 1);
-    slot0 = (bos >> p.shift) + n;
-    cnt = (eos - bos + ((int64_t)1 << p.shift) - 1) >> p.shift;
-  } else {
-    slot0 = (int64_t)n * p.spq;
-    cnt = p.spq;
-  }
-  if (cnt < 2) return;
+__global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, int elems, int segs) {
+  const unsigned per = elems / 1024, hv = blockIdx.x / per;
+  const int at = (blockIdx.x % per) * 1024 + threadIdx.x * 4;
   const int64_t step = (int64_t)p.HV * elems;
-  float* e = p.entry + (slot0 * p.HV + hv) * elems + at;
-  const float* dc = p.decay + slot0 * p.HV + hv;
+  float* e = p.entry + (int64_t)hv * elems + at;
+  const float* dc = p.decay + hv;
   f32x4 run = {0.f, 0.f, 0.f, 0.f};
-  if (p.init) run = *reinterpret_cast<const f32x4*>(p.init + chain * elems + at);
-  constexpr int U = 4;  // loads in flight
-  for (int64_t s0 = 0; s0 < cnt - 1; s0 += U) {
+  constexpr int U = 8;  // loads in flight
+  for (int s0 = 0; s0 < segs - 1; s0 += U) {
     f32x4 x[U];
     float c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t s = s0 + u < cnt - 1 ? s0 + u : cnt - 2;
-      x[u] = *reinterpret_cast<const f32x4*>(e + (REV ? cnt - 2 - s : s + 1) * step);
-      c[u] = dc[(REV ? cnt - 1 - s : s) * p.HV];
+      const int s = s0 + u < segs - 1 ? s0 + u : segs - 2;
+      x[u] = *reinterpret_cast<const f32x4*>(e + (REV ? segs - 2 - s : s + 1) * step);
+      c[u] = dc[(int64_t)(REV ? segs - 1 - s : s) * p.HV];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s0 + u >= cnt - 1) break;
-      run = run * c[u] + x[u];
-      *reinterpret_cast<f32x4*>(e + (REV ? cnt - 2 - s0 - u : s0 + u + 1) * step) = run;
+      if (s0 + u >= segs - 1) break;
+      run = c[u] == 0.f ? x[u] : run * c[u] + x[u];
+      *reinterpret_cast<f32x4*>(e + (REV ? segs - 2 - s0 - u : s0 + u + 1) * step) = run;
     }
   }
 }
@@ -444,34 +476,33 @@ struct WalkLds {
 };
 
 template <int KD, int VD, bool REV, int DOT, typename OT>
-__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams p) {
+__device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD, DOT>& lds) {
   constexpr int SW = 4, NCT = VD / 16 / SW, NU = KD / 32;
   constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
-  __shared__ __align__(16) WalkLds<KD, VD, DOT> lds;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, i = lane & 15;
-  const unsigned hv = blockIdx.x % p.HV;
-  const Segment sg = find_segment(p, blockIdx.x / p.HV);
-  if (!sg.some) return;
-  const int nc = (sg.len + kC - 1) / kC;
-  auto first_of = [&](int c) { return (REV ? nc - 1 - c : c) * kC; };  // first token of the walk's chunk c
-  auto len_of = [&](int c) { return sg.len - first_of(c) < kC ? sg.len - first_of(c) : kC; };
-  const bf16* e0 = DOT ? p.e + sg.tok * p.es + hv / p.re * VD : nullptr;
+  const unsigned hv = blockIdx.x % p.HV, seg = blockIdx.x / p.HV;
+  const int seg0 = seg * p.L, seg1 = p.tokens - seg0 < p.L ? p.tokens : seg0 + p.L;
+  const bf16* e0 = DOT ? p.e + hv / p.re * VD : nullptr;
+  ChunkWalk<REV> it;
+  it.start(p, seg0, seg1);
 
   if (wave < SW) {  // ------------------------------------------------------------------ the state's waves
     const int w = wave;
-    OT* o0 = static_cast<OT*>(p.o) + (sg.tok * p.HV + hv) * VD;
+    OT* o0 = static_cast<OT*>(p.o) + (int64_t)hv * VD;
     State<KD, VD, SW> st;
-    const bool inner = REV ? !sg.last : !sg.first;  // a segment of this sequence comes before
-    const float* src = inner ? p.entry + (sg.slot * p.HV + hv) * (KD * VD)
-                             : (p.init ? p.init + (sg.n * p.HV + hv) * (KD * VD) : nullptr);
-    if (src) st.load(src, p.transposed, w, lane);
-    else st.zero();
-    const bool wants_fin = p.fin && (REV ? sg.first : sg.last);
+    auto begin = [&](const Chunk& c) {
+      const float* src = !c.fresh ? p.entry + ((int64_t)seg * p.HV + hv) * (KD * VD)
+                                  : (p.init ? p.init + ((int64_t)c.n * p.HV + hv) * (KD * VD) : nullptr);
+      if (src) st.load(src, VD, p.transposed, w, lane);
+      else st.zero();
+    };
+    Chunk now = it.next(p), then = it.next(p);
+    begin(now);
     __syncthreads();
     __syncthreads();
-    for (int c = 0; c < nc; ++c) {
-      const int t0 = first_of(c), len = len_of(c);
+    for (int c = 0; now.len > 0; ++c) {
+      const int t0 = now.t, len = now.len;
       const Decays& d = lds.d[c % 3];
       const bf16 *Qs = lds.q[c % 3], *Ks = lds.k[c % 3], *Vs = lds.v[c & 1];
       bf16x4 ev[4][NCT];
@@ -479,7 +510,7 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int row = 16 * t + i;
-          const bf16* er = e0 + (t0 + (row < len ? row : 0)) * p.es + 16 * NCT * w + 4 * NCT * g;
+          const bf16* er = e0 + (int64_t)(t0 + (row < len ? row : 0)) * p.es + 16 * NCT * w + 4 * NCT * g;
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct) ev[t][ct] = *reinterpret_cast<const bf16x4*>(er + 4 * ct);
         }
@@ -587,45 +618,45 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
           *reinterpret_cast<bf16x4*>(dst) = to_bf16x4(acc[t][0][0], acc[t][0][1], acc[t][0][2], acc[t][0][3]);
         }
       }
-      if (c + 1 < nc || wants_fin) st.update(d, Ks, vf, lane);
+      if (now.done ? p.fin != nullptr : then.len > 0) st.update(d, Ks, vf, lane);
+      if (now.done && p.fin) st.store(p.fin + ((int64_t)now.n * p.HV + hv) * (KD * VD), VD, w, lane);
       __syncthreads();
+      now = then;
+      then = it.next(p);
+      if (now.len > 0 && now.fresh) begin(now);
     }
-    if (wants_fin) st.store(p.fin + (sg.n * p.HV + hv) * (KD * VD), VD, w, lane);
     return;
   }
 
   // ------------------------------------------------------------------------------------ the scores' waves
   const int w = wave - SW;
-  const bf16* q0 = p.q + sg.tok * p.qs + hv / p.rq * KD;
-  const bf16* k0 = p.k + sg.tok * p.ks + hv / p.rk * KD;
-  const bf16* v0 = p.v + sg.tok * p.vs + hv / p.rv * VD;
-  // Two sets of tiles in flight: a chunk's loads are issued two steps before their rows go to LDS. With one step between
-  // the two, a step lasted as long as the loads of all CUs took, and the memory had nothing to do meanwhile.
-  Tile<KD> qt[2], kt[2];
-  Tile<VD> vt[2];
-  const uint32_t qoff = qt[0].offset(p.qs), koff = kt[0].offset(p.ks), voff = vt[0].offset(p.vs);
-  auto fetch_qk = [&](int c, int set) {
-    if (c >= nc) return;
-    const int t0 = first_of(c), len = len_of(c);
-    qt[set].fetch(q0 + t0 * p.qs, p.qs, qoff, len);
-    kt[set].fetch(k0 + t0 * p.ks, p.ks, koff, len);
+  const bf16* q0 = p.q + hv / p.rq * KD;
+  const bf16* k0 = p.k + hv / p.rk * KD;
+  const bf16* v0 = p.v + hv / p.rv * VD;
+  Tile<KD> qt, kt;
+  Tile<VD> vt;
+  const uint32_t qoff = qt.offset(p.qs), koff = kt.offset(p.ks), voff = vt.offset(p.vs);
+  auto fetch_qk = [&](const Chunk& c) {
+    if (c.len == 0) return;
+    qt.fetch(q0 + c.t * p.qs, p.qs, qoff, c.len);
+    kt.fetch(k0 + c.t * p.ks, p.ks, koff, c.len);
   };
-  auto fetch_v = [&](int c, int set) {
-    if (c < nc) vt[set].fetch(v0 + first_of(c) * p.vs, p.vs, voff, len_of(c));
+  auto fetch_v = [&](const Chunk& c) {
+    if (c.len) vt.fetch(v0 + c.t * p.vs, p.vs, voff, c.len);
   };
-  auto put_qk = [&](int c, int set) {
-    if (c >= nc) return;
-    qt[set].put(lds.q[c % 3], len_of(c));
-    kt[set].put(lds.k[c % 3], len_of(c));
+  auto put_qk = [&](const Chunk& c, int slot) {
+    if (c.len == 0) return;
+    qt.put(lds.q[slot], c.len);
+    kt.put(lds.k[slot], c.len);
   };
-  auto put_v = [&](int c, int set) {
-    if (c < nc) vt[set].put(lds.v[c & 1], len_of(c));
+  auto put_v = [&](const Chunk& c, int half) {
+    if (c.len) vt.put(lds.v[half], c.len);
   };
-  GateWalk<REV> gate;
-  auto decays = [&](int c) {  // of chunk c, whose raw gate has been fetched; then the next chunk's
-    if (w != 0 || c >= nc) return;
-    chunk_decays<REV>(lds.d[c % 3], gate.value(p), p.scale, lane);
-    gate.fetch(p, sg, hv, c + 1, nc, lane);
+  GateRow gate;
+  auto decays = [&](const Chunk& c, int slot, const Chunk& after) {  // of c, whose gate has been fetched; then the next one's
+    if (w != 0 || c.len == 0) return;
+    chunk_decays<REV>(lds.d[slot], gate.value(p), p.scale, lane);
+    gate.fetch(p, hv, after, lane);
   };
   // 12 tiles of 16 keys x 16 queries are written (2 of zeros), 3 a wave: P^T, rows = keys j, column = query
   f32x4 pv[3];
@@ -634,11 +665,11 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
     ta = n == 0 ? sl >> 1 : 1 + n;
     ja = n == 0 ? sl & 1 : w;
   };
-  auto scores = [&](int c) {
-    if (c >= nc) return;
-    const bf16 *Qs = lds.q[c % 3], *Ks = lds.k[c % 3];
-    const Decays& d = lds.d[c % 3];
-    auto* ps = lds.ps[c & 1];
+  auto scores = [&](const Chunk& c, int slot, int half) {  // half: the chunk's number & 1
+    if (c.len == 0) return;
+    const bf16 *Qs = lds.q[slot], *Ks = lds.k[slot];
+    const Decays& d = lds.d[slot];
+    auto* ps = lds.ps[half];
     // the three tiles side by side, also where all of one is masked; tiles 1 and 2 have the same keys
     bf16x8 kf[2][NU], qf[3][NU];
 #pragma unroll
@@ -681,16 +712,16 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
     }
   };
   // DOT 2: the sums of W over the tiles whose scores this wave holds (pv, of the chunk before the one just scored)
-  auto score_dots = [&](int c, const f32x4 (&x)[3]) {
-    const int t0 = first_of(c), len = len_of(c);
-    const bf16* Vs = lds.v[c & 1];
+  auto score_dots = [&](const Chunk& c, int half, const f32x4 (&x)[3]) {
+    const int t0 = c.t, len = c.len;
+    const bf16* Vs = lds.v[half];
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
       int ta, ja;
       tile_of(n, ta, ja);
       if (ja > ta) continue;
       const int t = REV ? 3 - ta : ta, jt = REV ? 3 - ja : ja, iq = 16 * t + i;
-      const bf16* er = e0 + (t0 + (iq < len ? iq : 0)) * p.es + 8 * g;
+      const bf16* er = e0 + (int64_t)(t0 + (iq < len ? iq : 0)) * p.es + 8 * g;
       f32x4 a = {0.f, 0.f, 0.f, 0.f}, cs;
 #pragma unroll
       for (int u = 0; u < VD / 32; ++u) a = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), ld8(er + 32 * u), a);
@@ -703,15 +734,15 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
         cs[r] = group_sum<16>(ww);
       }
       rs = xor32_sum(xor16_sum(rs));
-      const int idx = ta * (ta + 1) / 2 + ja, sl = DOT == 2 ? c & 1 : 0;
+      const int idx = ta * (ta + 1) / 2 + ja, sl = DOT == 2 ? half : 0;
       if (g == 0) lds.rows[sl][idx][DOT == 2 ? i : 0] = rs;
       if (i == 0) *reinterpret_cast<f32x4*>(&lds.cols[sl][idx][DOT == 2 ? 4 * g : 0]) = cs;
     }
   };
-  // the gate's dot products of chunk c, all of whose shares are in LDS
-  auto finish_dots = [&](int c) {
-    if (!DOT || c < 0 || w != 1 || lane >= len_of(c)) return;
-    const int sl = DOT ? c & 1 : 0;
+  // the gate's dot products of a chunk, all of whose shares are in LDS
+  auto finish_dots = [&](const Chunk& c, int half) {
+    if (!DOT || w != 1 || lane >= c.len) return;
+    const int sl = DOT ? half : 0;
     float x = 0.f;
 #pragma unroll
     for (int ww = 0; ww < SW; ++ww) x += lds.dots[sl][ww][DOT ? lane : 0];
@@ -723,144 +754,188 @@ __global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams
         if (o >= ta) x -= lds.cols[DOT == 2 ? sl : 0][o * (o + 1) / 2 + ta][DOT == 2 ? i : 0];
       }
     }
-    const int64_t tokens = p.cu ? p.T : p.N * p.T;
-    p.dot[hv * tokens + sg.tok + first_of(c) + lane] = x;
+    p.dot[(int64_t)hv * p.tokens + c.t + lane] = x;
   };
-  if (w == 0) gate.fetch(p, sg, hv, 0, nc, lane);
-  fetch_qk(0, 0);
-  fetch_v(0, 0);
-  fetch_qk(1, 1);
-  fetch_v(1, 1);
-  decays(0);
-  decays(1);
-  put_qk(0, 0);
-  fetch_qk(2, 0);
-  put_v(0, 0);
-  fetch_v(2, 0);
-  put_qk(1, 1);
-  fetch_qk(3, 1);
+  // chunk c is at[1] in step c, and at[0] the one before
+  Chunk at[5] = {};
+#pragma unroll
+  for (int n = 1; n < 5; ++n) at[n] = it.next(p);
+  if (w == 0) gate.fetch(p, hv, at[1], lane);
+  fetch_qk(at[1]);
+  fetch_v(at[1]);
+  put_qk(at[1], 0);
+  fetch_qk(at[2]);
+  put_v(at[1], 0);
+  fetch_v(at[2]);
+  decays(at[1], 0, at[2]);
+  decays(at[2], 1, at[3]);
+  put_qk(at[2], 1);
+  fetch_qk(at[3]);
   __syncthreads();
-  scores(0);
+  scores(at[1], 0, 0);
   __syncthreads();
-  auto step = [&](int c, int set) {  // set: c & 1
-    put_v(c + 1, 1 - set);
-    fetch_v(c + 3, 1 - set);
-    put_qk(c + 2, set);
-    fetch_qk(c + 4, set);
-    decays(c + 2);
+  int slot = 0, half = 0;  // c % 3, c & 1
+  while (at[1].len > 0) {
+    const int s1 = slot == 2 ? 0 : slot + 1, s2 = slot == 0 ? 2 : slot - 1;  // of chunks c + 1 and c + 2
+    put_v(at[2], half ^ 1);
+    put_qk(at[3], s2);
+    fetch_v(at[3]);
+    fetch_qk(at[4]);
+    decays(at[3], s2, at[4]);
     f32x4 held[3];
     if (DOT == 2) {
 #pragma unroll
       for (int n = 0; n < 3; ++n) held[n] = pv[n];
     }
-    scores(c + 1);
-    if (DOT == 2) score_dots(c, held);
-    finish_dots(c - 1);
+    scores(at[2], s1, half ^ 1);
+    if (DOT == 2) score_dots(at[1], half, held);
+    finish_dots(at[0], half ^ 1);
     __syncthreads();
-  };
-  for (int c = 0; c < nc; c += 2) {
-    step(c, 0);
-    if (c + 1 < nc) step(c + 1, 1);
+    slot = s1;
+    half ^= 1;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) at[n] = at[n + 1];
+    at[4] = it.next(p);
   }
-  finish_dots(nc - 1);
+  finish_dots(at[0], half ^ 1);
+}
+
+template <int KD, int VD>
+__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams p) {
+  __shared__ __align__(16) WalkLds<KD, VD, 0> lds;
+  walk_segment<KD, VD, false, 0, bf16>(p, lds);
+}
+
+// The backward's three walks in one launch (K, V: those of the forward): y = 0 dq, 1 dk, 2 dv. OT: of dq and dk.
+template <int K, int V, bool GATE, typename OT>
+__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_bwd_kernel(LinParams dq, LinParams dk, LinParams dv) {
+  using Q = WalkLds<V, K, GATE ? 2 : 0>;
+  using R = WalkLds<V, K, GATE ? 1 : 0>;
+  using S = WalkLds<K, V, 0>;
+  constexpr size_t qr = sizeof(Q) > sizeof(R) ? sizeof(Q) : sizeof(R);
+  __shared__ __align__(16) char lds[qr > sizeof(S) ? qr : sizeof(S)];
+  if (blockIdx.y == 0) walk_segment<V, K, false, GATE ? 2 : 0, OT>(dq, *reinterpret_cast<Q*>(lds));
+  else if (blockIdx.y == 1) walk_segment<V, K, true, GATE ? 1 : 0, OT>(dk, *reinterpret_cast<R*>(lds));
+  else walk_segment<K, V, true, 0, bf16>(dv, *reinterpret_cast<S*>(lds));
 }
 
 // ------------------------------------------------------------------------------------------------
-// dg of a segment: what lies behind it is <S, R> at its end (the state entering the next segment with what the walk from
-// the end brings there; <S_T, dS_T> at the sequence's end), then the sum from the end of q . dq - k . dk.
-struct LinGateGrad {
+// dg of a segment: what lies behind each of its sequences is <S, R> at the segment's border (the state entering the next
+// segment with what the walk from the end brings there) or <S_T, dS_T> at the sequence's end, then the sum from the end
+// of q . dq - k . dk. The waves take the sequences in turn; the one at the border is the last.
+struct LinFinish {
   const float *x, *y;              // [HV][tokens] q . dq and k . dk
   const float *entry, *rentry;     // the states at the segments' borders, or null
   const float *fin, *dfin;         // at the sequences' ends; either may be null (dfin: a zero gradient)
-  void* out;                       // [tokens][HV]
-  int dtype;
-  int64_t elems;                   // K V
+  void* dg;                        // [tokens][HV], or null
+  int dtype, elems, segs;          // elems: K V
+  // dq and dk of the value heads that share a head, [tokens][HV][K] fp32, into [tokens][HV / rep][K]; or null
+  const float *dq_heads, *dk_heads;
+  bf16 *dq, *dk;
+  int rep, K;
 };
 
-__global__ __launch_bounds__(256) void gated_deltaless_gate_grad_kernel(LinParams p, LinGateGrad a) {
-  __shared__ double part[4];
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  const unsigned hv = blockIdx.x % p.HV;
-  const Segment sg = find_segment(p, blockIdx.x / p.HV);
-  if (!sg.some) return;
-  const float *s = nullptr, *r = nullptr;
-  if (!sg.last) {
-    s = a.entry + ((sg.slot + 1) * p.HV + hv) * a.elems;
-    r = a.rentry + (sg.slot * p.HV + hv) * a.elems;
-  } else if (a.fin && a.dfin) {
-    s = a.fin + (sg.n * p.HV + hv) * a.elems;
-    r = a.dfin + (sg.n * p.HV + hv) * a.elems;
-  }
+// Sum over the threads of `of` (a wave's 64 or a workgroup's 256) of the products of 4,096 m elements.
+__device__ __forceinline__ double state_product(const float* s, const float* r, int elems, int at, int of) {
   double sum = 0.;
-  if (s) {
-    for (int64_t at = threadIdx.x * 4; at < a.elems; at += 1024) {
-      const f32x4 u = *reinterpret_cast<const f32x4*>(s + at), v = *reinterpret_cast<const f32x4*>(r + at);
-      sum += (double)(u[0] * v[0] + u[1] * v[1]) + (double)(u[2] * v[2] + u[3] * v[3]);
+  for (int at0 = at * 4; at0 < elems; at0 += 16 * of) {
+    f32x4 u[4], v[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      u[n] = *reinterpret_cast<const f32x4*>(s + at0 + 4 * of * n);
+      v[n] = *reinterpret_cast<const f32x4*>(r + at0 + 4 * of * n);
     }
-    for (int m = 1; m < kWave; m <<= 1) sum += __shfl_xor(sum, m, kWave);
-    if (lane == 0) part[w] = sum;
-    __syncthreads();
-    sum = part[0] + part[1] + part[2] + part[3];
-    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      sum += (double)(u[n][0] * v[n][0] + u[n][1] * v[n][1]) + (double)(u[n][2] * v[n][2] + u[n][3] * v[n][3]);
   }
-  const int64_t tokens = p.cu ? p.T : p.N * p.T, base = hv * tokens + sg.tok;
-  for (int hi = sg.len; hi > 0; hi -= 256) {  // 256 tokens a step: wave w those from hi - 64 (w + 1) on
-    const int t = hi - kWave * (w + 1) + lane;
-    const double x = t >= 0 ? (double)a.x[base + t] - (double)a.y[base + t] : 0.;
-    double run = x;
-    for (int m = 1; m < kWave; m <<= 1) {
-      const double other = __shfl_down(run, m, kWave);
-      if (lane + m < kWave) run += other;
-    }
-    if (lane == 0) part[w] = run;
-    __syncthreads();
-    for (int ww = 0; ww < 4; ++ww) {
-      if (ww < w) run += part[ww];
-    }
-    if (t >= 0) store_from_f32(a.out, a.dtype, (sg.tok + t) * p.HV + hv, (float)(sum + run));
-    sum += part[0] + part[1] + part[2] + part[3];
-    __syncthreads();
-  }
+  for (int m = 1; m < kWave; m <<= 1) sum += __shfl_xor(sum, m, kWave);
+  return sum;
 }
 
-// Sums the gradients of the value heads that share a q/k head: [rows][rep][D] fp32 -> [rows][D] bf16.
-__global__ __launch_bounds__(256) void gated_deltaless_head_sum_kernel(const float* x, bf16* y, int64_t rows, int rep, int D) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (at >= rows * D) return;
-  const float* src = x + at / D * rep * D + at % D;
-  f32x4 sum = *reinterpret_cast<const f32x4*>(src);
-  for (int r = 1; r < rep; ++r) sum += *reinterpret_cast<const f32x4*>(src + (int64_t)r * D);
-  *reinterpret_cast<bf16x4*>(y + at) = to_bf16x4(sum[0], sum[1], sum[2], sum[3]);
+__global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p, LinFinish a) {
+  __shared__ double part[4];
+  const unsigned gates = a.dg ? (unsigned)a.segs * p.HV : 0u;
+  if (blockIdx.x >= gates) {  // the sums over the value heads that share a q/k head
+    const int64_t at = ((int64_t)(blockIdx.x - gates) * 256 + threadIdx.x) * 4, all = (int64_t)p.tokens * (p.HV / a.rep) * a.K;
+    if (at >= all) return;
+    const float* src = (blockIdx.y ? a.dk_heads : a.dq_heads) + at / a.K * a.rep * a.K + at % a.K;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(src);
+    for (int r = 1; r < a.rep; ++r) sum += *reinterpret_cast<const f32x4*>(src + (int64_t)r * a.K);
+    *reinterpret_cast<bf16x4*>((blockIdx.y ? a.dk : a.dq) + at) = to_bf16x4(sum[0], sum[1], sum[2], sum[3]);
+    return;
+  }
+  if (blockIdx.y) return;
+  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const unsigned hv = blockIdx.x % p.HV, seg = blockIdx.x / p.HV;
+  const int seg0 = seg * p.L, seg1 = p.tokens - seg0 < p.L ? p.tokens : seg0 + p.L;
+  const int first = seq_of(p, seg0), last = seq_of(p, seg1 - 1);
+  const bool cut = seq_start(p, last + 1) > seg1;  // the last sequence goes on in the next segment
+  double border = 0.;
+  if (cut) {
+    const int64_t at = ((int64_t)(seg + 1) * p.HV + hv) * a.elems;
+    const double sum = state_product(a.entry + at, a.rentry + at - (int64_t)p.HV * a.elems, a.elems, threadIdx.x, 256);
+    if (lane == 0) part[w] = sum;
+    __syncthreads();
+    border = part[0] + part[1] + part[2] + part[3];
+  }
+  for (int n = last - w; n >= first; n -= 4) {
+    const int bos = seq_start(p, n), eos = seq_start(p, n + 1);
+    const int lo = bos > seg0 ? bos : seg0, hi = eos < seg1 ? eos : seg1;
+    double sum = 0.;
+    if (eos > seg1) sum = border;
+    else if (a.fin && a.dfin) {
+      const int64_t at = ((int64_t)n * p.HV + hv) * a.elems;
+      sum = state_product(a.fin + at, a.dfin + at, a.elems, lane, kWave);
+    }
+    const int64_t base = (int64_t)hv * p.tokens;
+    auto load = [&](int end) {  // lane 0 the last of 64 tokens
+      const int t = end - 1 - lane;
+      return t >= lo ? (double)a.x[base + t] - (double)a.y[base + t] : 0.;
+    };
+    double next = load(hi);
+    for (int end = hi; end > lo; end -= kWave) {
+      const int t = end - 1 - lane;
+      const double run = wave_inclusive_sum64(next);
+      next = load(end - kWave);
+      if (t >= lo) store_from_f32(a.dg, a.dtype, (int64_t)t * p.HV + hv, (float)(sum + run));
+      sum += last_lane(run);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
 // host
 struct LinPlan {
-  int shift;
-  int64_t spq, slots;  // segments of a sequence without cu, slots in all
-  bool split;
+  int64_t L, segs;  // segments of L tokens of the flat token axis
+  bool split;       // a segment's border may cut a sequence
 };
 
-// Segments of a power of two of tokens, as short as gives kLinGroups workgroups and no shorter than kLinMinSegment.
-constexpr int64_t kLinGroups = 256, kLinMinSegment = 256;
+// Segments so that their number times the value heads is at most 256, a workgroup a CU (from 129 heads on one segment: more
+// are uneven, up to 170 heads three are less so). Short sequences stay whole, several a segment: a cut costs two launches
+// and a second pass over k and v, as much as walking 384 tokens (1 x 333 tokens, 4 heads of 64: XX us whole, 21 in 2).
+constexpr int64_t kLinGroups = 256, kLinMinSegment = 128, kLinWhole = 384;
 
-static LinPlan lin_plan(int64_t B, int64_t T, int64_t HV, int64_t N, bool varlen) {
+static LinPlan lin_plan(int64_t B, int64_t T, int64_t HV, bool varlen) {
+  const int64_t tokens = B * T, most = HV <= 128 ? kLinGroups / HV : HV <= 170 ? 3 : 1;
   LinPlan pl{};
-  int64_t L = kLinMinSegment;
-  pl.shift = 8;
-  while (L < T && (B * T / L) * HV > kLinGroups) {
-    L <<= 1;
-    ++pl.shift;
+  int64_t L = ((tokens + most - 1) / most + kC - 1) / kC * kC;
+  if (L < kLinMinSegment) L = kLinMinSegment;
+  if (!varlen && T <= (L > kLinWhole ? L : kLinWhole)) {
+    pl.L = (L + T - 1) / T * T;
+  } else if (tokens <= kLinWhole) {
+    pl.L = tokens;
+  } else {
+    pl.L = L;
   }
-  pl.spq = T > L ? (T + L - 1) / L : 1;
-  pl.slots = varlen ? (T >> pl.shift) + N : N * pl.spq;
-  pl.split = T > L;
+  pl.segs = (tokens + pl.L - 1) / pl.L;
+  pl.split = pl.segs > 1 && (varlen || T > pl.L);
   return pl;
 }
 
 static int64_t align256l(int64_t b) { return (b + 255) / 256 * 256; }
 static int64_t lin_states_bytes(const LinPlan& pl, int64_t HV, int64_t K, int64_t V) {
-  return pl.split ? align256l(pl.slots * HV * K * V * 4) + align256l(pl.slots * HV * 4) : 0;
+  return pl.split ? align256l(pl.segs * HV * K * V * 4) + align256l(pl.segs * HV * 4) : 0;
 }
 
 template <typename F>
@@ -875,19 +950,12 @@ static void lin_by_dims(int64_t K, int64_t V, F go) {
 
 template <bool REV>
 static void launch_segments(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  const dim3 grid((unsigned)(pl.slots * p.HV), (unsigned)(V / 64));
+  const dim3 grid((unsigned)((pl.segs - 1) * p.HV), (unsigned)(V / 64));
   if (K == 128) hipLaunchKernelGGL((gated_deltaless_segment_kernel<128, REV>), grid, dim3(256), 0, s, p, (int)V);
   else hipLaunchKernelGGL((gated_deltaless_segment_kernel<64, REV>), grid, dim3(256), 0, s, p, (int)V);
-  hipLaunchKernelGGL((gated_deltaless_scan_kernel<REV>), dim3((unsigned)(p.N * p.HV * (K * V / 1024))), dim3(256), 0, s, p,
-                     K * V);
-}
-
-template <bool REV, int DOT, typename OT>
-static void launch_walk(const LinParams& p, const LinPlan& pl, int64_t K, int64_t V, hipStream_t s) {
-  lin_by_dims(K, V, [&](auto k, auto v) {
-    hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k)::value, decltype(v)::value, REV, DOT, OT>),
-                       dim3((unsigned)(pl.slots * p.HV)), dim3(512), 0, s, p);
-  });
+  if (pl.segs > 2)
+    hipLaunchKernelGGL((gated_deltaless_scan_kernel<REV>), dim3((unsigned)(p.HV * (K * V / 1024))), dim3(256), 0, s, p,
+                       (int)(K * V), (int)pl.segs);
 }
 
 static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, int64_t N,
@@ -911,9 +979,8 @@ static int lin_check(const char* name, int64_t B, int64_t T, int64_t H, int64_t 
       gdn_internal_set_error("%s: tensors must be 16-byte aligned", name);
       return GDN_ERR_INVALID;
     }
-  const LinPlan pl = lin_plan(B, T, HV, N, varlen);
-  if (HV > 65536 || pl.slots * HV > 0x7fffffffLL || pl.spq > 0x7fffffffLL || N * HV * 16 > 0x7fffffffLL || B * T * HV > (1LL << 40)) {
-    gdn_internal_set_error("%s: too many sequences, heads or tokens for one launch", name);
+  if (HV > 65536 || N > 0x3fffffffLL || B > 0x3fffffffLL || T > 0x3fffffffLL || B * T > 0x3fffffffLL) {
+    gdn_internal_set_error("%s: too many sequences, heads or tokens for one call", name);
     return GDN_ERR_UNSUPPORTED;
   }
   return GDN_OK;
@@ -929,11 +996,11 @@ static LinParams lin_params(const LinPlan& pl, const void* g, int g_dtype, int64
   p.gh = gh;
   p.cu = cu;
   p.cu_i32 = (flags & GDN_FLAG_CU_INT32) ? 1 : 0;
-  p.shift = pl.shift;
-  p.T = T;
-  p.N = N;
+  p.T = (int)T;
+  p.N = (int)N;
+  p.tokens = (int)(cu ? T : N * T);
+  p.L = (int)pl.L;
   p.HV = (unsigned)HV;
-  p.spq = (unsigned)pl.spq;
   p.scale = scale;
   return p;
 }
@@ -957,7 +1024,7 @@ static void lin_roles(LinParams& p, const void* q, int rq, const void* k, int rk
 
 static void lin_states(LinParams& p, const LinPlan& pl, char* states, int64_t K, int64_t V) {
   p.entry = pl.split ? reinterpret_cast<float*>(states) : nullptr;
-  p.decay = pl.split ? reinterpret_cast<float*>(states + align256l(pl.slots * p.HV * K * V * 4)) : nullptr;
+  p.decay = pl.split ? reinterpret_cast<float*>(states + align256l(pl.segs * p.HV * K * V * 4)) : nullptr;
 }
 
 }  // namespace gdn
@@ -965,8 +1032,8 @@ static void lin_states(LinParams& p, const LinPlan& pl, char* states, int64_t K,
 using namespace gdn;
 
 extern "C" size_t gdn_decay_attn_states_size(int64_t B, int64_t T, int64_t HV, int64_t K, int64_t V, int64_t N, int varlen) {
-  if (B <= 0 || T < 0 || HV <= 0 || K <= 0 || V <= 0 || N <= 0) return 0;
-  return (size_t)lin_states_bytes(lin_plan(B, T, HV, N, varlen != 0), HV, K, V);
+  if (B <= 0 || T <= 0 || HV <= 0 || K <= 0 || V <= 0 || N <= 0) return 0;
+  return (size_t)lin_states_bytes(lin_plan(B, T, HV, varlen != 0), HV, K, V);
 }
 
 extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
@@ -980,13 +1047,13 @@ extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, c
   }
   const void* ptrs[] = {q, k, v, o, initial_state, final_state, states};
   if (int rc = lin_check("gdn_decay_attn_fwd", B, T, H, HV, K, V, N, cu_seqlens != nullptr, g_dtype, ptrs, 7)) return rc;
-  const LinPlan pl = lin_plan(B, T, HV, N, cu_seqlens != nullptr);
+  if (T == 0) return GDN_OK;
+  const LinPlan pl = lin_plan(B, T, HV, cu_seqlens != nullptr);
   const size_t need = (size_t)lin_states_bytes(pl, HV, K, V);
   if (need && (!states || states_bytes < need)) {
     gdn_internal_set_error("gdn_decay_attn_fwd: states of %zu bytes needed", need);
     return GDN_ERR_INVALID;
   }
-  if (T == 0) return GDN_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rep = (int)(HV / H);
   LinParams p = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N, HV, scale);
@@ -996,7 +1063,10 @@ extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, c
   if (pl.split) launch_segments<false>(p, pl, K, V, s);
   p.fin = final_state;
   p.o = o;
-  launch_walk<false, 0, bf16>(p, pl, K, V, s);
+  lin_by_dims(K, V, [&](auto k_, auto v_) {
+    hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k_)::value, decltype(v_)::value>),
+                       dim3((unsigned)(pl.segs * HV)), dim3(512), 0, s, p);
+  });
   return gdn_internal_check_launch("gated_deltaless_chunk_kernel");
 }
 
@@ -1014,8 +1084,8 @@ LinBwdSpace lin_bwd_space(const LinPlan& pl, int64_t B, int64_t T, int64_t HV, i
 
 extern "C" size_t gdn_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
                                                     int64_t N, int varlen) {
-  if (B <= 0 || T < 0 || H <= 0 || HV <= 0 || HV % H || K <= 0 || V <= 0 || N <= 0) return 0;
-  return (size_t)lin_bwd_space(lin_plan(B, T, HV, N, varlen != 0), B, T, HV, K, V).bytes(HV != H);
+  if (B <= 0 || T <= 0 || H <= 0 || HV <= 0 || HV % H || K <= 0 || V <= 0 || N <= 0) return 0;
+  return (size_t)lin_bwd_space(lin_plan(B, T, HV, varlen != 0), B, T, HV, K, V).bytes(HV != H);
 }
 
 extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
@@ -1035,7 +1105,8 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   const void* ptrs[] = {q, k, v, d_o, dq, dk, dv, initial_state, final_state, d_final_state, d_initial_state, states,
                         workspace};
   if (int rc = lin_check("gdn_decay_attn_bwd", B, T, H, HV, K, V, N, cu_seqlens != nullptr, g_dtype, ptrs, 13)) return rc;
-  const LinPlan pl = lin_plan(B, T, HV, N, cu_seqlens != nullptr);
+  if (T == 0) return GDN_OK;
+  const LinPlan pl = lin_plan(B, T, HV, cu_seqlens != nullptr);
   const bool shared = H != HV;
   const LinBwdSpace sp = lin_bwd_space(pl, B, T, HV, K, V);
   if ((pl.split && !states) || (sp.bytes(shared) && (!workspace || workspace_bytes < (size_t)sp.bytes(shared)))) {
@@ -1043,7 +1114,6 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
                            (long long)sp.bytes(shared));
     return GDN_ERR_INVALID;
   }
-  if (T == 0) return GDN_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rep = (int)(HV / H);
   char* ws = static_cast<char*>(workspace);
@@ -1053,43 +1123,43 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   float* dk_heads = reinterpret_cast<float*>(ws + sp.states + 2 * sp.dots + sp.heads);
   const LinParams base = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N,
                                     HV, scale);
-  // from the end: R's segments, then dv and dk
+  // from the end: the states R at the segments' borders, then dv and dk
   LinParams r = base;
   lin_roles(r, k, rep, q, rep, d_o, 1, nullptr, 1, K, V);
   lin_states(r, pl, ws, K, V);
   r.init = d_final_state;
   if (pl.split) launch_segments<true>(r, pl, K, V, s);
-  LinParams a = r;
-  a.o = dv;
-  a.fin = d_initial_state;
-  launch_walk<true, 0, bf16>(a, pl, K, V, s);
-  a = r;
-  lin_roles(a, v, 1, d_o, 1, q, rep, k, rep, V, K);
-  a.transposed = 1;
-  a.dot = dot_k;
-  a.o = shared ? static_cast<void*>(dk_heads) : dk;
-  if (shared) dg ? launch_walk<true, 1, float>(a, pl, V, K, s) : launch_walk<true, 0, float>(a, pl, V, K, s);
-  else dg ? launch_walk<true, 1, bf16>(a, pl, V, K, s) : launch_walk<true, 0, bf16>(a, pl, V, K, s);
+  LinParams v_ = r, k_ = r, q_ = base;
+  v_.o = dv;
+  v_.fin = d_initial_state;
+  lin_roles(k_, v, 1, d_o, 1, q, rep, k, rep, V, K);
+  k_.transposed = 1;
+  k_.dot = dot_k;
+  k_.o = shared ? static_cast<void*>(dk_heads) : dk;
   // from the start: dq
-  LinParams f = base;
-  lin_roles(f, d_o, 1, v, 1, k, rep, q, rep, V, K);
-  lin_states(f, pl, static_cast<char*>(const_cast<void*>(states)), K, V);
-  f.init = initial_state;
-  f.transposed = 1;
-  f.dot = dot_q;
-  f.o = shared ? static_cast<void*>(dq_heads) : dq;
-  if (shared) dg ? launch_walk<false, 2, float>(f, pl, V, K, s) : launch_walk<false, 0, float>(f, pl, V, K, s);
-  else dg ? launch_walk<false, 2, bf16>(f, pl, V, K, s) : launch_walk<false, 0, bf16>(f, pl, V, K, s);
-  if (dg) {
-    const LinGateGrad gg{dot_q, dot_k, f.entry, r.entry, final_state, d_final_state, dg, g_dtype, K * V};
-    hipLaunchKernelGGL(gated_deltaless_gate_grad_kernel, dim3((unsigned)(pl.slots * HV)), dim3(256), 0, s, base, gg);
+  lin_roles(q_, d_o, 1, v, 1, k, rep, q, rep, V, K);
+  lin_states(q_, pl, static_cast<char*>(const_cast<void*>(states)), K, V);
+  q_.init = initial_state;
+  q_.transposed = 1;
+  q_.dot = dot_q;
+  q_.o = shared ? static_cast<void*>(dq_heads) : dq;
+  const dim3 grid((unsigned)(pl.segs * HV), 3), nt(512);
+  lin_by_dims(K, V, [&](auto kd, auto vd) {
+    constexpr int KD = decltype(kd)::value, VD = decltype(vd)::value;
+    if (dg && shared) hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, true, float>), grid, nt, 0, s, q_, k_, v_);
+    else if (dg) hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, true, bf16>), grid, nt, 0, s, q_, k_, v_);
+    else if (shared) hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, false, float>), grid, nt, 0, s, q_, k_, v_);
+    else hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, false, bf16>), grid, nt, 0, s, q_, k_, v_);
+  });
+  if (dg || shared) {
+    const LinFinish fin{dot_q, dot_k, q_.entry, r.entry, final_state, d_final_state, dg, g_dtype, (int)(K * V),
+                        (int)pl.segs, dq_heads, dk_heads, static_cast<bf16*>(dq), static_cast<bf16*>(dk), rep, (int)K};
+    const int64_t blocks = (dg ? pl.segs * HV : 0) + (shared ? (B * T * H * K / 4 + 255) / 256 : 0);
+    if (blocks > 0x7fffffffLL) {
+      gdn_internal_set_error("gdn_decay_attn_bwd: too many tokens and heads for one launch");
+      return GDN_ERR_UNSUPPORTED;
+    }
+    hipLaunchKernelGGL(gated_deltaless_finish_kernel, dim3((unsigned)blocks, shared ? 2 : 1), dim3(256), 0, s, base, fin);
   }
-  if (shared) {
-    const int64_t rows = B * T * H, blocks = (rows * K / 4 + 255) / 256;
-    hipLaunchKernelGGL(gated_deltaless_head_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dq_heads,
-                       static_cast<bf16*>(dq), rows, rep, (int)K);
-    hipLaunchKernelGGL(gated_deltaless_head_sum_kernel, dim3((unsigned)blocks), dim3(256), 0, s, dk_heads,
-                       static_cast<bf16*>(dk), rows, rep, (int)K);
-  }
-  return gdn_internal_check_launch("gated_deltaless_chunk_kernel(bwd)");
+  return gdn_internal_check_launch("gated_deltaless_chunk_bwd_kernel");
 }

@@ -56,23 +56,19 @@ _CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.
 # ---------------------------------------------------------------------------------------------------
 # sorernn::chunk_decay_linear_attention_fwd / _bwd
 # ---------------------------------------------------------------------------------------------------
-_MIN_SEGMENT, _GROUPS = 256, 256
-
-
 def _align256(x):
     return (x + 255) // 256 * 256
 
 
-def states_bytes(b, t, hv, kd, vd, n, varlen: bool):
-    """``gdn_decay_attn_states_size`` in Python: the fp32 states entering the segments (a power of two of tokens, 256 at
-    least and as short as gives 256 workgroups) and the segments' decays."""
-    seg = _MIN_SEGMENT
-    while seg < t and (b * t // seg) * hv > _GROUPS:
-        seg *= 2
-    if t <= seg:
+def states_bytes(b, t, hv, kd, vd, varlen: bool):
+    """``gdn_decay_attn_states_size`` in Python: the fp32 states entering the segments of the flat token axis, and the
+    segments' decays; 0 where no segment's border cuts a sequence."""
+    tokens, most = b * t, 256 // hv if hv <= 128 else 3 if hv <= 170 else 1
+    seg = max(128, ((tokens + most - 1) // most + 63) // 64 * 64)
+    if (not varlen and t <= max(seg, 384)) or tokens <= 384:
         return 0
-    slots = (t // seg + n) if varlen else n * ((t + seg - 1) // seg)
-    return _align256(slots * hv * kd * vd * 4) + _align256(slots * hv * 4)
+    segs = (tokens + seg - 1) // seg
+    return 0 if segs == 1 else _align256(segs * hv * kd * vd * 4) + _align256(segs * hv * 4)
 
 
 def _gate_args(g: Optional[Tensor]):
@@ -90,7 +86,7 @@ def attention_fwd_impl(q: Tensor, k: Tensor, v: Tensor, g: Optional[Tensor], ini
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
     o = torch.empty_like(vc)
     final = torch.empty((num_seqs, hv, kd, vd) if output_final_state else (0,), device=q.device, dtype=torch.float32)
-    states = torch.empty(states_bytes(b, t, hv, kd, vd, num_seqs, cu is not None), device=q.device, dtype=torch.uint8)
+    states = torch.empty(states_bytes(b, t, hv, kd, vd, cu is not None), device=q.device, dtype=torch.uint8)
     if t > 0:
         _launch("gdn_decay_attn_fwd", qc, _lib.ptr(qc), _lib.ptr(kc), _lib.ptr(vc), _lib.ptr(g), _lib.ptr(h0), _lib.ptr(o),
                 _lib.ptr(final if output_final_state else None), _lib.ptr(cu), b, t, h, hv, kd, vd, num_seqs,
@@ -109,7 +105,7 @@ def _attention_fwd_fake(q, k, v, g, initial_state, cu_seqlens, scale, flags, num
     hv, vd = v.shape[2], v.shape[3]
     return (q.new_empty(b, t, hv, vd), q.new_empty((num_seqs, hv, kd, vd) if output_final_state else (0,),
                                                    dtype=torch.float32),
-            q.new_empty(states_bytes(b, t, hv, kd, vd, num_seqs, cu_seqlens is not None), dtype=torch.uint8))
+            q.new_empty(states_bytes(b, t, hv, kd, vd, cu_seqlens is not None), dtype=torch.uint8))
 
 
 def attention_bwd_impl(q: Tensor, k: Tensor, v: Tensor, g: Optional[Tensor], initial_state: Optional[Tensor],

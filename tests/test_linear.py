@@ -127,9 +127,10 @@ def test_no_second_derivative(launches):
 def test_sizes_match_the_library():
     lib = _lib.load()
     for b, t, hv, kd, vd, n, varlen in [(1, 1, 1, 64, 64, 1, 0), (4, 4096, 16, 128, 128, 4, 0), (1, 32768, 16, 128, 128, 8, 1),
-                                        (1, 257, 1, 64, 128, 1, 0), (1, 257, 1, 64, 128, 257, 1), (1, 256, 2, 64, 64, 3, 1),
+                                        (1, 257, 1, 64, 128, 1, 0), (1, 257, 1, 64, 128, 257, 1), (1, 385, 2, 64, 64, 3, 1),
+                                        (3, 385, 2, 64, 64, 3, 0), (2, 5000, 150, 64, 64, 2, 0), (2, 5000, 200, 64, 64, 2, 1), (64, 100, 16, 64, 64, 64, 0),
                                         (8, 300, 64, 128, 64, 8, 0), (1, 10**6, 1, 64, 64, 1, 0)]:
-        assert linear.states_bytes(b, t, hv, kd, vd, n, bool(varlen)) == lib.gdn_decay_attn_states_size(
+        assert linear.states_bytes(b, t, hv, kd, vd, bool(varlen)) == lib.gdn_decay_attn_states_size(
             b, t, hv, kd, vd, n, varlen)
     assert lib.gdn_decay_attn_states_size(0, 1, 1, 64, 64, 1, 0) == 0
     assert lib.gdn_decay_attn_bwd_workspace_size(1, 8, 2, 3, 64, 64, 1, 0) == 0
@@ -154,7 +155,7 @@ def test_entry_points_check_their_arguments():
     assert fwd(B=2, N=2, cu=P) == _lib.GDN_ERR_INVALID
     assert fwd(K=96) == _lib.GDN_ERR_UNSUPPORTED
     assert fwd(gd=3) == _lib.GDN_ERR_INVALID
-    assert fwd(T=1000) == _lib.GDN_ERR_INVALID and b"states" in lib.gdn_last_error()
+    assert fwd(T=1000, HV=1) == _lib.GDN_ERR_INVALID and b"states" in lib.gdn_last_error()
     assert fwd(T=0) == _lib.GDN_OK
     bwd = [P, P, P, P, None, None, P, None, None, None, 1, 8, 1, 1, 64, 64, 1, 0, 0, 0, 0, 1.0, 0, P, P, P, P, None, None, 0, None]
     assert lib.gdn_decay_attn_bwd(*bwd) == _lib.GDN_ERR_INVALID and b"workspace" in lib.gdn_last_error()
