@@ -357,10 +357,10 @@ struct GateRow {
 // What a segment adds to the state of the sequence that its border cuts: the walk without outputs, from where the sequence
 // begins (with its initial state) or from the segment's other border (from zero). Forward walks leave it in the next
 // segment's place, walks from the end in that of the segment before. Two workgroups share 128 columns, which doubles the
-// waves in flight.
+// waves in flight: at 4 x 4,096 tokens, 16 heads of 128, 37.5 us, 40.7 with eight waves of one workgroup for all columns.
 template <int KD, bool REV>
 __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinParams p, int VD) {
-  __shared__ __align__(16) bf16 Ks[kC * KD], Vs[kC * 64];
+  __shared__ __align__(16) bf16 Ks[2][kC * KD], Vs[2][kC * 64];
   __shared__ __align__(16) Decays d[2];
   const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const unsigned hv = blockIdx.x % p.HV;
@@ -397,27 +397,27 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
   if (whole && p.init) st.load(p.init + ((int64_t)n * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, false, w, lane);
   else st.zero();
   double total = 0.;
-  if (w == 0) {
-    total = gate.value(p);
-    chunk_decays<REV>(d[0], total, p.scale, lane);
-    gate.fetch(p, hv, chunk(1), lane);
-  }
-  for (int ci = 0; ci < nc; ++ci) {
+  auto bring = [&](int ci) {  // chunk ci, on its way, into LDS, and the next one's loads
+    if (ci >= nc) return;
     const int len = chunk(ci).len;
-    kt.put(Ks, len);
-    vt.put(Vs, len);
-    __syncthreads();
+    const double x = w == 0 ? gate.value(p) : 0.;  // ahead of the next loads: the wait for it would be for them too
+    kt.put(Ks[ci & 1], len);
+    vt.put(Vs[ci & 1], len);
+    if (w == 0) gate.fetch(p, hv, chunk(ci + 1), lane);
     if (ci + 1 < nc) fetch(ci + 1);
-    if (w == 0 && ci + 1 < nc) {
-      const double x = gate.value(p);
+    if (w == 0) {
       total += x;
-      chunk_decays<REV>(d[(ci + 1) & 1], x, p.scale, lane);
-      gate.fetch(p, hv, chunk(ci + 2), lane);
+      chunk_decays<REV>(d[ci & 1], x, p.scale, lane);
     }
+  };
+  bring(0);
+  __syncthreads();
+  for (int ci = 0; ci < nc; ++ci) {
+    bring(ci + 1);
     bf16x8 vf[2][1];
-    st.columns(Vs, 0, w, lane, vf[0]);
-    st.columns(Vs, 32, w, lane, vf[1]);
-    st.update(d[ci & 1], Ks, vf, lane);
+    st.columns(Vs[ci & 1], 0, w, lane, vf[0]);
+    st.columns(Vs[ci & 1], 32, w, lane, vf[1]);
+    st.update(d[ci & 1], Ks[ci & 1], vf, lane);
     __syncthreads();
   }
   st.store(p.entry + ((int64_t)(seg + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, w, lane);
@@ -459,25 +459,28 @@ __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, 
 
 // ------------------------------------------------------------------------------------------------
 // The walk. One workgroup a CU: waves 0-3 hold the state and make the outputs of chunk c, waves 4-7 meanwhile bring the
-// tiles of chunks c + 1 and c + 2 into LDS and make the scores of chunk c + 1; one barrier a chunk. At 4 x 4,096 tokens, 16 heads of 128, 82 us;
-// its loads and stores alone 59 us, the state's waves alone 64 us.
+// tiles of chunks c + 1 and c + 2 into LDS and make the scores of chunk c + 1; one barrier a chunk. At 4 x 4,096 tokens,
+// 16 heads of 128, 78 us; its loads and stores alone take 59, the state's waves alone 64. With eight waves for the state the
+// scores' waves are what a chunk waits for: 80 us.
 // DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums less the
 // column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.
 //
 // Scores are kept for the tiles that are not masked, in blocks of 16 queries x 32 keys (tok_col order): queries 0-15 and
 // 16-31 have one block, the others two (walks from the end: mirrored).
+constexpr int kStateWaves = 4, kScoreWaves = 4, kWalkThreads = (kStateWaves + kScoreWaves) * kWave;
+
 template <int KD, int VD, int DOT>
 struct WalkLds {
   bf16 q[3][kC * KD], k[3][kC * KD], v[2][kC * VD];
   bf16 ps[2][2][6 * 512];  // [slot][part]
   Decays d[3];
-  float dots[DOT ? 2 : 1][4][DOT ? kC : 1];
+  float dots[DOT ? 2 : 1][kStateWaves][DOT ? kC : 1];
   float rows[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1], cols[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1];
 };
 
 template <int KD, int VD, bool REV, int DOT, typename OT>
 __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD, DOT>& lds) {
-  constexpr int SW = 4, NCT = VD / 16 / SW, NU = KD / 32;
+  constexpr int NCT = VD / 16 / kStateWaves, NU = KD / 32;
   constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, i = lane & 15;
@@ -487,10 +490,10 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   ChunkWalk<REV> it;
   it.start(p, seg0, seg1);
 
-  if (wave < SW) {  // ------------------------------------------------------------------ the state's waves
+  if (wave < kStateWaves) {  // ------------------------------------------------------------------ the state's waves
     const int w = wave;
     OT* o0 = static_cast<OT*>(p.o) + (int64_t)hv * VD;
-    State<KD, VD, SW> st;
+    State<KD, VD, kStateWaves> st;
     auto begin = [&](const Chunk& c) {
       const float* src = !c.fresh ? p.entry + ((int64_t)seg * p.HV + hv) * (KD * VD)
                                   : (p.init ? p.init + ((int64_t)c.n * p.HV + hv) * (KD * VD) : nullptr);
@@ -564,7 +567,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
       float bad = 0.f;  // NaN where the wave's columns of v hold an infinity or NaN: a sum of products with zero
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
-        State<KD, VD, SW>::columns(Vs, 32 * k2, w, lane, vf[k2]);
+        State<KD, VD, kStateWaves>::columns(Vs, 32 * k2, w, lane, vf[k2]);
 #pragma unroll
         for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
@@ -629,7 +632,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   }
 
   // ------------------------------------------------------------------------------------ the scores' waves
-  const int w = wave - SW;
+  const int w = wave - kStateWaves;
   const bf16* q0 = p.q + hv / p.rq * KD;
   const bf16* k0 = p.k + hv / p.rk * KD;
   const bf16* v0 = p.v + hv / p.rv * VD;
@@ -653,10 +656,15 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
     if (c.len) vt.put(lds.v[half], c.len);
   };
   GateRow gate;
-  auto decays = [&](const Chunk& c, int slot, const Chunk& after) {  // of c, whose gate has been fetched; then the next one's
-    if (w != 0 || c.len == 0) return;
-    chunk_decays<REV>(lds.d[slot], gate.value(p), p.scale, lane);
-    gate.fetch(p, hv, after, lane);
+  // The gate's values and the rows of score_dots are taken before new loads are issued: a wait for them would be for
+  // those too.
+  auto gate_value = [&](const Chunk& c, const Chunk& after) {  // of c, which has been fetched; then the next one's loads
+    const double x = w == 0 && c.len ? gate.value(p) : 0.;
+    if (w == 0) gate.fetch(p, hv, after, lane);
+    return x;
+  };
+  auto decays = [&](const Chunk& c, int slot, double x) {
+    if (w == 0 && c.len) chunk_decays<REV>(lds.d[slot], x, p.scale, lane);
   };
   // 12 tiles of 16 keys x 16 queries are written (2 of zeros), 3 a wave: P^T, rows = keys j, column = query
   f32x4 pv[3];
@@ -712,8 +720,21 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
     }
   };
   // DOT 2: the sums of W over the tiles whose scores this wave holds (pv, of the chunk before the one just scored)
+  bf16x8 er[DOT == 2 ? 3 : 1][DOT == 2 ? VD / 32 : 1];
+  auto dot_rows = [&](const Chunk& c) {
+    if (DOT != 2 || c.len == 0) return;
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      int ta, ja;
+      tile_of(n, ta, ja);
+      const int iq = 16 * (REV ? 3 - ta : ta) + i;
+      const bf16* src = e0 + (int64_t)(c.t + (iq < c.len ? iq : 0)) * p.es + 8 * g;
+#pragma unroll
+      for (int u = 0; u < VD / 32; ++u) er[DOT == 2 ? n : 0][DOT == 2 ? u : 0] = ld8(src + 32 * u);
+    }
+  };
   auto score_dots = [&](const Chunk& c, int half, const f32x4 (&x)[3]) {
-    const int t0 = c.t, len = c.len;
+    const int len = c.len;
     const bf16* Vs = lds.v[half];
 #pragma unroll
     for (int n = 0; n < 3; ++n) {
@@ -721,10 +742,10 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
       tile_of(n, ta, ja);
       if (ja > ta) continue;
       const int t = REV ? 3 - ta : ta, jt = REV ? 3 - ja : ja, iq = 16 * t + i;
-      const bf16* er = e0 + (int64_t)(t0 + (iq < len ? iq : 0)) * p.es + 8 * g;
       f32x4 a = {0.f, 0.f, 0.f, 0.f}, cs;
 #pragma unroll
-      for (int u = 0; u < VD / 32; ++u) a = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), ld8(er + 32 * u), a);
+      for (int u = 0; u < VD / 32; ++u)
+        a = mma(ld_row<VD>(Vs, 16 * jt + i, 4 * u + g), er[DOT == 2 ? n : 0][DOT == 2 ? u : 0], a);
       float rs = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -745,7 +766,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
     const int sl = DOT ? half : 0;
     float x = 0.f;
 #pragma unroll
-    for (int ww = 0; ww < SW; ++ww) x += lds.dots[sl][ww][DOT ? lane : 0];
+    for (int ww = 0; ww < kStateWaves; ++ww) x += lds.dots[sl][ww][DOT ? lane : 0];
     if (DOT == 2) {
       const int ta = REV ? 3 - g : g;  // the token's tile, as query and as key
 #pragma unroll
@@ -763,25 +784,29 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   if (w == 0) gate.fetch(p, hv, at[1], lane);
   fetch_qk(at[1]);
   fetch_v(at[1]);
+  const double x0 = gate_value(at[1], at[2]);
   put_qk(at[1], 0);
   fetch_qk(at[2]);
   put_v(at[1], 0);
   fetch_v(at[2]);
-  decays(at[1], 0, at[2]);
-  decays(at[2], 1, at[3]);
+  decays(at[1], 0, x0);
+  const double x1 = gate_value(at[2], at[3]);
   put_qk(at[2], 1);
   fetch_qk(at[3]);
+  decays(at[2], 1, x1);
   __syncthreads();
   scores(at[1], 0, 0);
   __syncthreads();
   int slot = 0, half = 0;  // c % 3, c & 1
   while (at[1].len > 0) {
     const int s1 = slot == 2 ? 0 : slot + 1, s2 = slot == 0 ? 2 : slot - 1;  // of chunks c + 1 and c + 2
+    dot_rows(at[1]);
+    const double x = gate_value(at[3], at[4]);
     put_v(at[2], half ^ 1);
     put_qk(at[3], s2);
     fetch_v(at[3]);
     fetch_qk(at[4]);
-    decays(at[3], s2, at[4]);
+    decays(at[3], s2, x);
     f32x4 held[3];
     if (DOT == 2) {
 #pragma unroll
@@ -801,14 +826,14 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
 }
 
 template <int KD, int VD>
-__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_kernel(LinParams p) {
+__global__ __launch_bounds__(kWalkThreads, 2) void gated_deltaless_chunk_kernel(LinParams p) {
   __shared__ __align__(16) WalkLds<KD, VD, 0> lds;
   walk_segment<KD, VD, false, 0, bf16>(p, lds);
 }
 
 // The backward's three walks in one launch (K, V: those of the forward): y = 0 dq, 1 dk, 2 dv. OT: of dq and dk.
 template <int K, int V, bool GATE, typename OT>
-__global__ __launch_bounds__(512, 2) void gated_deltaless_chunk_bwd_kernel(LinParams dq, LinParams dk, LinParams dv) {
+__global__ __launch_bounds__(kWalkThreads, 2) void gated_deltaless_chunk_bwd_kernel(LinParams dq, LinParams dk, LinParams dv) {
   using Q = WalkLds<V, K, GATE ? 2 : 0>;
   using R = WalkLds<V, K, GATE ? 1 : 0>;
   using S = WalkLds<K, V, 0>;
@@ -889,17 +914,23 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
       sum = state_product(a.fin + at, a.dfin + at, a.elems, lane, kWave);
     }
     const int64_t base = (int64_t)hv * p.tokens;
-    auto load = [&](int end) {  // lane 0 the last of 64 tokens
-      const int t = end - 1 - lane;
-      return t >= lo ? (double)a.x[base + t] - (double)a.y[base + t] : 0.;
-    };
-    double next = load(hi);
-    for (int end = hi; end > lo; end -= kWave) {
-      const int t = end - 1 - lane;
-      const double run = wave_inclusive_sum64(next);
-      next = load(end - kWave);
-      if (t >= lo) store_from_f32(a.dg, a.dtype, (int64_t)t * p.HV + hv, (float)(sum + run));
-      sum += last_lane(run);
+    constexpr int U = 8;  // loads in flight
+    for (int end0 = hi; end0 > lo; end0 -= U * kWave) {
+      float x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // lane 0 the last of 64 tokens
+        const int t = end0 - u * kWave - 1 - lane;
+        x[u] = a.x[base + (t >= lo ? t : lo)];
+        y[u] = a.y[base + (t >= lo ? t : lo)];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = end0 - u * kWave - 1 - lane;
+        if (end0 - u * kWave <= lo) break;
+        const double run = wave_inclusive_sum64(t >= lo ? (double)x[u] - (double)y[u] : 0.);
+        if (t >= lo) store_from_f32(a.dg, a.dtype, (int64_t)t * p.HV + hv, (float)(sum + run));
+        sum += last_lane(run);
+      }
     }
   }
 }
@@ -913,7 +944,8 @@ struct LinPlan {
 
 // Segments so that their number times the value heads is at most 256, a workgroup a CU (from 129 heads on one segment: more
 // are uneven, up to 170 heads three are less so). Short sequences stay whole, several a segment: a cut costs two launches
-// and a second pass over k and v, as much as walking 384 tokens (1 x 333 tokens, 4 heads of 64: XX us whole, 21 in 2).
+// and a second pass over k and v, as much as walking 384 tokens (1 x 384 tokens, 4 heads of 64: 15.5 us whole; 448, the
+// first length that is cut: 15.1, and about 5 us of the host's time for the launches).
 constexpr int64_t kLinGroups = 256, kLinMinSegment = 128, kLinWhole = 384;
 
 static LinPlan lin_plan(int64_t B, int64_t T, int64_t HV, bool varlen) {
@@ -1065,7 +1097,7 @@ extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, c
   p.o = o;
   lin_by_dims(K, V, [&](auto k_, auto v_) {
     hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k_)::value, decltype(v_)::value>),
-                       dim3((unsigned)(pl.segs * HV)), dim3(512), 0, s, p);
+                       dim3((unsigned)(pl.segs * HV)), dim3(kWalkThreads), 0, s, p);
   });
   return gdn_internal_check_launch("gated_deltaless_chunk_kernel");
 }
@@ -1143,7 +1175,7 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   q_.transposed = 1;
   q_.dot = dot_q;
   q_.o = shared ? static_cast<void*>(dq_heads) : dq;
-  const dim3 grid((unsigned)(pl.segs * HV), 3), nt(512);
+  const dim3 grid((unsigned)(pl.segs * HV), 3), nt(kWalkThreads);
   lin_by_dims(K, V, [&](auto kd, auto vd) {
     constexpr int KD = decltype(kd)::value, VD = decltype(vd)::value;
     if (dg && shared) hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, true, float>), grid, nt, 0, s, q_, k_, v_);
