@@ -520,6 +520,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
       }
       // the state's share: O^T = S^T Q^T, columns = tokens
       f32x4 acc[4][NCT];
+      f32x4 low[DOT ? 4 : 1][DOT ? NCT : 1] = {};  // the small parts' products apart: fewer roundings of the whole
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -542,7 +543,16 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
 #pragma unroll
           for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int ct = 0; ct < NCT; ++ct) acc[t][ct] = mma(part[ct][n], qf[t], acc[t][ct]);
+            for (int ct = 0; ct < NCT; ++ct) {
+              if (DOT && n > 0) low[DOT ? t : 0][DOT ? ct : 0] = mma(part[ct][n], qf[t], low[DOT ? t : 0][DOT ? ct : 0]);
+              else acc[t][ct] = mma(part[ct][n], qf[t], acc[t][ct]);
+            }
+      }
+      if (DOT) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) acc[t][ct] += low[DOT ? t : 0][DOT ? ct : 0];
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -553,13 +563,14 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
       if (DOT) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          float x = 0.f;
+          double x = 0.;  // dg sums thousands of these, which mostly cancel
 #pragma unroll
           for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x += acc[t][ct][r] * (float)ev[t][ct][r];
-          x = xor32_sum(xor16_sum(x));
-          if (g == 0) lds.dots[DOT ? c & 1 : 0][w][DOT ? 16 * t + i : 0] = x;
+            for (int r = 0; r < 4; ++r) x += (double)acc[t][ct][r] * (double)(float)ev[t][ct][r];
+          x += __shfl_xor(x, 16);
+          x += __shfl_xor(x, 32);
+          if (g == 0) lds.dots[DOT ? c & 1 : 0][w][DOT ? 16 * t + i : 0] = (float)x;
         }
       }
       // the scores' share: O^T += V^T P^T
@@ -764,7 +775,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   auto finish_dots = [&](const Chunk& c, int half) {
     if (!DOT || w != 1 || lane >= c.len) return;
     const int sl = DOT ? half : 0;
-    float x = 0.f;
+    double x = 0.;
 #pragma unroll
     for (int ww = 0; ww < kStateWaves; ++ww) x += lds.dots[sl][ww][DOT ? lane : 0];
     if (DOT == 2) {
@@ -775,7 +786,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
         if (o >= ta) x -= lds.cols[DOT == 2 ? sl : 0][o * (o + 1) / 2 + ta][DOT == 2 ? i : 0];
       }
     }
-    p.dot[(int64_t)hv * p.tokens + c.t + lane] = x;
+    p.dot[(int64_t)hv * p.tokens + c.t + lane] = (float)x;
   };
   // chunk c is at[1] in step c, and at[0] the one before
   Chunk at[5] = {};
@@ -847,11 +858,14 @@ __global__ __launch_bounds__(kWalkThreads, 2) void gated_deltaless_chunk_bwd_ker
 // ------------------------------------------------------------------------------------------------
 // dg of a segment: what lies behind each of its sequences is <S, R> at the segment's border (the state entering the next
 // segment with what the walk from the end brings there) or <S_T, dS_T> at the sequence's end, then the sum from the end
-// of q . dq - k . dk. The waves take the sequences in turn; the one at the border is the last.
+// of q . dq - k . dk. The sum over a whole piece is known as well, from <S, R> at the border before it or <S_0, dS_0>: what
+// it misses, the rounding of all the dot products, is spread over the piece in proportion to |q . dq| + |k . dk|, which
+// leaves 1/sqrt(3) of the error of a plain sum. The waves take the sequences in turn; the one at the border is the last.
 struct LinFinish {
   const float *x, *y;              // [HV][tokens] q . dq and k . dk
   const float *entry, *rentry;     // the states at the segments' borders, or null
   const float *fin, *dfin;         // at the sequences' ends; either may be null (dfin: a zero gradient)
+  const float *init, *dinit;       // at their beginnings, or null (init: zeros)
   void* dg;                        // [tokens][HV], or null
   int dtype, elems, segs;          // elems: K V
   // dq and dk of the value heads that share a head, [tokens][HV][K] fp32, into [tokens][HV / rep][K]; or null
@@ -879,7 +893,7 @@ __device__ __forceinline__ double state_product(const float* s, const float* r, 
 }
 
 __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p, LinFinish a) {
-  __shared__ double part[4];
+  __shared__ double part[2][4];
   const unsigned gates = a.dg ? (unsigned)a.segs * p.HV : 0u;
   if (blockIdx.x >= gates) {  // the sums over the value heads that share a q/k head
     const int64_t at = ((int64_t)(blockIdx.x - gates) * 256 + threadIdx.x) * 4, all = (int64_t)p.tokens * (p.HV / a.rep) * a.K;
@@ -896,13 +910,20 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
   const int seg0 = seg * p.L, seg1 = p.tokens - seg0 < p.L ? p.tokens : seg0 + p.L;
   const int first = seq_of(p, seg0), last = seq_of(p, seg1 - 1);
   const bool cut = seq_start(p, last + 1) > seg1;  // the last sequence goes on in the next segment
-  double border = 0.;
-  if (cut) {
-    const int64_t at = ((int64_t)(seg + 1) * p.HV + hv) * a.elems;
-    const double sum = state_product(a.entry + at, a.rentry + at - (int64_t)p.HV * a.elems, a.elems, threadIdx.x, 256);
-    if (lane == 0) part[w] = sum;
+  const bool begun = seq_start(p, first) < seg0;           // the first one began in an earlier segment
+  const int64_t next = (int64_t)p.HV * a.elems, at0 = ((int64_t)seg * p.HV + hv) * a.elems;
+  double border = 0., before = 0.;
+  if (cut || begun) {
+    double r = 0., l = 0.;
+    if (cut) r = state_product(a.entry + at0 + next, a.rentry + at0, a.elems, threadIdx.x, 256);
+    if (begun) l = state_product(a.entry + at0, a.rentry + at0 - next, a.elems, threadIdx.x, 256);
+    if (lane == 0) {
+      part[0][w] = r;
+      part[1][w] = l;
+    }
     __syncthreads();
-    border = part[0] + part[1] + part[2] + part[3];
+    border = part[0][0] + part[0][1] + part[0][2] + part[0][3];
+    before = part[1][0] + part[1][1] + part[1][2] + part[1][3];
   }
   for (int n = last - w; n >= first; n -= 4) {
     const int bos = seq_start(p, n), eos = seq_start(p, n + 1);
@@ -913,21 +934,55 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
       const int64_t at = ((int64_t)n * p.HV + hv) * a.elems;
       sum = state_product(a.fin + at, a.dfin + at, a.elems, lane, kWave);
     }
-    const int64_t base = (int64_t)hv * p.tokens;
+    const float *xs = a.x + (int64_t)hv * p.tokens, *ys = a.y + (int64_t)hv * p.tokens;
+    // what the sum over the piece misses, for a unit of |x| + |y|
+    double first_sum = before;
+    bool known = true;
+    if (bos >= seg0) {
+      first_sum = 0.;
+      known = !a.init || a.dinit;
+      if (a.init && a.dinit) {
+        const int64_t at = ((int64_t)n * p.HV + hv) * a.elems;
+        first_sum = state_product(a.init + at, a.dinit + at, a.elems, lane, kWave);
+      }
+    }
+    double all = 0., weight = 0.;
     constexpr int U = 8;  // loads in flight
+    for (int t0 = known ? lo + lane : hi; t0 < hi; t0 += U * kWave) {
+      float x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kWave;
+        x[u] = xs[t < hi ? t : lo];
+        y[u] = ys[t < hi ? t : lo];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (t0 + u * kWave >= hi) break;
+        all += (double)x[u] - (double)y[u];
+        weight += fabs((double)x[u]) + fabs((double)y[u]);
+      }
+    }
+    for (int m = 1; m < kWave; m <<= 1) {
+      all += __shfl_xor(all, m, kWave);
+      weight += __shfl_xor(weight, m, kWave);
+    }
+    double miss = known && weight > 0. ? (first_sum - sum - all) / weight : 0.;
+    if (!(fabs(miss) < 1e30)) miss = 0.;  // infinities and NaN stay with the tokens before them
     for (int end0 = hi; end0 > lo; end0 -= U * kWave) {
       float x[U], y[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // lane 0 the last of 64 tokens
         const int t = end0 - u * kWave - 1 - lane;
-        x[u] = a.x[base + (t >= lo ? t : lo)];
-        y[u] = a.y[base + (t >= lo ? t : lo)];
+        x[u] = xs[t >= lo ? t : lo];
+        y[u] = ys[t >= lo ? t : lo];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int t = end0 - u * kWave - 1 - lane;
         if (end0 - u * kWave <= lo) break;
-        const double run = wave_inclusive_sum64(t >= lo ? (double)x[u] - (double)y[u] : 0.);
+        const double xx = x[u], yy = y[u];
+        const double run = wave_inclusive_sum64(t >= lo ? xx - yy + miss * (fabs(xx) + fabs(yy)) : 0.);
         if (t >= lo) store_from_f32(a.dg, a.dtype, (int64_t)t * p.HV + hv, (float)(sum + run));
         sum += last_lane(run);
       }
@@ -1184,8 +1239,9 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
     else hipLaunchKernelGGL((gated_deltaless_chunk_bwd_kernel<KD, VD, false, bf16>), grid, nt, 0, s, q_, k_, v_);
   });
   if (dg || shared) {
-    const LinFinish fin{dot_q, dot_k, q_.entry, r.entry, final_state, d_final_state, dg, g_dtype, (int)(K * V),
-                        (int)pl.segs, dq_heads, dk_heads, static_cast<bf16*>(dq), static_cast<bf16*>(dk), rep, (int)K};
+    const LinFinish fin{dot_q, dot_k, q_.entry, r.entry, final_state, d_final_state, initial_state, d_initial_state, dg, g_dtype,
+                        (int)(K * V), (int)pl.segs, dq_heads, dk_heads, static_cast<bf16*>(dq), static_cast<bf16*>(dk), rep,
+                        (int)K};
     const int64_t blocks = (dg ? pl.segs * HV : 0) + (shared ? (B * T * H * K / 4 + 255) / 256 : 0);
     if (blocks > 0x7fffffffLL) {
       gdn_internal_set_error("gdn_decay_attn_bwd: too many tokens and heads for one launch");
