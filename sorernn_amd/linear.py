@@ -259,6 +259,8 @@ def _recurrent(name, q, k, v, g, scale, initial_state, output_final_state, inpla
         ptr = _lib.ptr
         _launch("gdn_decay_attn_recurrent_fwd", q, ptr(q), ptr(k), ptr(v), ptr(g), ptr(h0), ptr(o), ptr(final), ptr(cu), b, t,
                 h, hv, kd, vd, n, _CODES[q.dtype], *_gate_args(g), scale, flags)
+        if inplace:  # a graph that saved the state must not use what it holds now
+            torch.autograd.graph.increment_version(h0)
     return o, final
 
 

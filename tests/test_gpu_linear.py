@@ -203,6 +203,50 @@ def test_chunk_non_finite_token_leaves_others_alone(which, bad):
         assert not torch.isfinite(s).all()
 
 
+@pytest.mark.parametrize("how", ["whole", "cut", "docs"])
+def test_chunk_gate_gradient_without_the_states_gradient(how):
+    """An initial state that needs no gradient: its product with the gradient is not known at the sequence's start."""
+    t, lens = {"whole": (200, None), "cut": (1500, None), "docs": (1500, [700, 1, 799])}[how]
+    x = _inputs(1, t, 1, 2, 64, 128, "token", True, lens, train=True, seed=11)
+    x["g"].requires_grad_(True)
+    o, s = _call(chunk_decay_linear_attention, x, 0.2)
+    (dg,) = torch.autograd.grad([o, s], [x["g"]], [x["do"], x["dht"]])
+    with torch.no_grad():
+        check(dg, decay_attention(x["q"], x["k"], x["v"], x["g"], 0.2, x["h0"], x["cu"], x["do"], x["dht"]), "dg", GATE)
+
+
+@pytest.mark.parametrize("t", [200, 1500])
+def test_chunk_non_finite_gradient_leaves_later_tokens_alone(t):
+    x = _inputs(1, t, 1, 1, 64, 64, "token", True, train=True, seed=12)
+    names, at = ["q", "k", "v", "g", "h0"], t // 2
+    for n in names:
+        x[n].requires_grad_(True)
+    o, s = _call(chunk_decay_linear_attention, x, 0.2)
+    up = x["do"].clone()
+    up[0, at, 0, 3] = float("nan")
+    got = torch.autograd.grad([o, s], [x[n] for n in names], [up, x["dht"]])
+    with torch.no_grad():
+        ref = decay_attention(x["q"], x["k"], x["v"], x["g"], 0.2, x["h0"], None, x["do"], x["dht"])
+    for n, y, per in zip(("dq", "dk", "dv", "dg"), got, (OUT, OUT, OUT, GATE)):
+        check(y[:, at + 1:], {m: ref[m][:, at + 1:] for m in (n, n + "_mag")}, n, per)
+        assert torch.isnan(y[:, at].float()).any()
+    assert torch.isnan(got[4]).any()
+
+
+def test_chunk_gate_gradient_over_a_long_segment():
+    """dg is a running sum of differences of dot products D. Rounded at random, each is off by 1.6 u of its root mean square
+    (the state 0.8 u, the products' sum 0.9 u, weights 1 u, for either of the two): 2 u; over 1,024 tokens whose sum is known
+    at both ends that grows to sqrt(1024 / 6) of it in the mean."""
+    x = _inputs(1, 2048, 128, 128, 64, 64, "token", False, train=True, seed=13)
+    x["g"].requires_grad_(True)
+    o, _ = _call(chunk_decay_linear_attention, x, 0.125, final=False)
+    (dg,) = torch.autograd.grad(o, [x["g"]], x["do"])
+    with torch.no_grad():
+        ref = decay_attention(x["q"], x["k"], x["v"], x["g"], 0.125, None, None, x["do"])["dg"]
+        err = (dg.double() - ref).square().mean().sqrt().item()
+        assert err <= 2 * U * (1024 / 6)**0.5 * ref.diff(dim=1).square().mean().sqrt().item()
+
+
 def test_chunk_strided_and_unaligned_inputs():
     x = _inputs(2, 130, 2, 2, 64, 64, "token", True, seed=2)
     want = _call(chunk_decay_linear_attention, x, 0.1)

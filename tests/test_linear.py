@@ -124,6 +124,19 @@ def test_no_second_derivative(launches):
         torch.autograd.grad(dq.float().sum(), [k])
 
 
+def test_a_state_overwritten_in_place_is_not_used_by_an_earlier_graph(launches):
+    q, k, v, g = (x.requires_grad_(True) for x in _x())
+    o, s = chunk_decay_linear_attention(q, k, v, g, output_final_state=True)
+    with torch.no_grad():
+        _, s2 = fused_recurrent_decay_linear_attention(q, k, v, g, initial_state=s, inplace_final_state=True)
+        assert s2 is s
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad([o, s], [q], [torch.ones_like(o), torch.ones_like(s)])
+    with torch.inference_mode():
+        h0 = torch.zeros(1, 2, 64, 64)
+        assert fused_recurrent_decay_linear_attention(q, k, v, g, initial_state=h0, inplace_final_state=True)[1] is h0
+
+
 def test_sizes_match_the_library():
     lib = _lib.load()
     for b, t, hv, kd, vd, n, varlen in [(1, 1, 1, 64, 64, 1, 0), (4, 4096, 16, 128, 128, 4, 0), (1, 32768, 16, 128, 128, 8, 1),
