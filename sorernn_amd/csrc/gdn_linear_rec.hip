@@ -3,7 +3,8 @@
 // A workgroup of 4 waves holds 64 columns of one (sequence, value head) state in registers: thread t the columns
 // 4 (t % 16) .. + 3 of the rows t / 16 + 16 i. The state is read once and written once, which is what bounds the step of
 // one token; the tokens' rows pass through LDS 16 at a time. A token's output is a sum over all rows: 4 row groups by
-// lane swaps, the 4 waves through LDS after the 16 tokens, so that 16 tokens take two barriers.
+// lane swaps, the 4 waves through LDS after the 16 tokens, so that 16 tokens take two barriers. A token for 64 sequences of 16
+// heads of 128: 25 us for 135 MB, 5.4 TB/s; for one sequence 4.5 us.
 
 #include <type_traits>
 
