@@ -520,6 +520,63 @@ def test_graph_replays_of_the_forward_and_a_step():
             assert torch.equal(a, b)
 
 
+def test_graph_of_documents_takes_other_lengths():
+    """What a captured call launches depends on the number of tokens and documents alone."""
+    first, lens = [300, 1, 399], [[300, 1, 399], [64, 635, 1], [1, 1, 698]]
+    x = _inputs(1, 700, 2, 4, 128, 64, "token", True, first, seed=14, train=True)
+    cu, leaves = x["cu"].to(DEV), ["q", "k", "v", "g", "h0"]
+
+    def step(cu_dev, host):
+        a = {m: x[m].detach().requires_grad_(True) for m in leaves}
+        q, k = qk_norm_rope(a["q"], a["k"], rot_dim=32, cu_seqlens=cu_dev, cu_seqlens_cpu=host)
+        o, s = chunk_decay_linear_attention(q, k, a["v"], a["g"], 0.1, a["h0"], True, cu_dev, host)
+        grads = torch.autograd.grad([o, s], [a[m] for m in leaves], [x["do"], x["dht"]])
+        with torch.no_grad():
+            o2, s2 = fused_recurrent_decay_linear_attention(q, k, a["v"], a["g"], 0.1, s, True, cu_seqlens=cu_dev,
+                                                            cu_seqlens_cpu=host)
+        return [o, s, *grads, o2, s2]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(cu, x["cu"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(cu, x["cu"])
+    for n in lens:
+        now = _cu(n)
+        cu.copy_(now)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step(now.to(DEV), now)):
+            assert torch.equal(a, b)
+
+
+def test_elements_past_32_bits():
+    """2^31 and more elements a tensor. The inputs repeat every 1,024 tokens and a weight of e^-100 is nothing beside the
+    others, so tokens 1,024 apart have the same results: two roundings of them apart."""
+    t, h, d, back = 2**20 + 700, 16, 128, 1024 * 1000
+    x = _inputs(1, 1024, h, h, d, d, "token", False, train=True, seed=15)
+    reps = t // 1024 + 1
+    big = {m: x[m].repeat(1, reps, 1, 1)[:, :t].contiguous() for m in ("q", "k", "v", "do")}
+    assert big["q"].numel() > 2**31
+    g = torch.full((h,), -1.0, device=DEV, requires_grad=True).expand(1, t, h)
+    for m in ("q", "k", "v"):
+        big[m].requires_grad_(True)
+    o, s = chunk_decay_linear_attention(big["q"], big["k"], big["v"], g, 0.1, output_final_state=True)
+    got = [o, *torch.autograd.grad(o, [big["q"], big["k"], big["v"], g], big["do"])]
+    assert torch.isfinite(s).all()
+    for y in got:
+        late, early = (y[:, a:a + 400].detach().double() for a in (t - 1000, t - 1000 - back))
+        assert late.any() and (late - early).norm() <= 2.0**-8 * early.norm()
+    del got, o, y
+    with torch.no_grad():
+        a, _ = qk_norm_rope(big["q"], big["k"], rot_dim=64)
+        want, _ = qk_norm_rope(big["q"][:, -300:], big["k"][:, -300:], rot_dim=64,
+                               positions=torch.arange(t - 300, t, device=DEV))
+        assert torch.equal(a[:, -300:], want)
+
+
 def test_graph_of_a_training_step():
     x = _inputs(2, 300, 1, 2, 64, 128, "token", False, seed=8, train=True)
     leaves = ["q", "k", "v", "g"]
