@@ -51,9 +51,12 @@ struct LinParams {
   float scale;
 };
 
-// First token of sequence n; of n = N the number of tokens.
+// First token of sequence n; of n = N the number of tokens. Captured and compiled calls do not check the bounds: whatever
+// they hold, nothing outside the tensors is touched, and tokens of no sequence are left out.
 __device__ __forceinline__ int seq_start(const LinParams& p, int n) {
-  return p.cu ? (int)load_index(p.cu, p.cu_i32, n) : n * p.T;
+  if (!p.cu) return n * p.T;
+  const int64_t x = load_index(p.cu, p.cu_i32, n);
+  return x < 0 ? 0 : x > p.tokens ? p.tokens : (int)x;
 }
 
 // The sequence of token t. All lanes of a wave search together.
@@ -87,34 +90,33 @@ struct ChunkWalk {
     n = seq_of(p, REV ? hi - 1 : lo);
     bos = seq_start(p, n);
     eos = seq_start(p, n + 1);
-    t = REV ? hi : lo;
+    t = REV ? (eos < hi ? eos : hi) : (bos > lo ? bos : lo);
   }
   __device__ __forceinline__ Chunk next(const LinParams& p) {
     Chunk c{0, 0, n, false, false};
-    if (REV ? t <= lo : t >= hi) return c;
     if (REV) {
       const int first = bos > lo ? bos : lo;
+      if (t <= first) return c;
       c.t = first + ((t - 1 - first) & ~(kC - 1));
       c.len = t - c.t;
       c.fresh = t == eos;
       c.done = c.t == bos;
       t = c.t;
       if (t == bos && t > lo) {
-        --n;
-        eos = bos;
-        bos = seq_start(p, n);
+        eos = t;
+        while (bos >= t && --n >= 0) bos = seq_start(p, n);
       }
     } else {
       const int end = eos < hi ? eos : hi;
+      if (t >= end) return c;
       c.t = t;
       c.len = end - t < kC ? end - t : kC;
       c.fresh = t == bos;
       c.done = t + c.len == eos;
       t += c.len;
       if (t == eos && t < hi) {
-        ++n;
-        bos = eos;
-        eos = seq_start(p, n + 1);
+        bos = t;
+        while (eos <= t && ++n < p.N) eos = seq_start(p, n + 1);
       }
     }
     return c;
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
   int lo = seg * p.L, hi = lo + p.L < p.tokens ? lo + p.L : p.tokens;
   const int n = seq_of(p, REV ? lo - 1 : hi), bos = seq_start(p, n), eos = seq_start(p, n + 1);
   const bool whole = REV ? eos <= hi : bos >= lo;  // the sequence's walk begins in this segment
-  if (REV ? eos == lo : bos == hi) {               // no sequence is cut
+  if (REV ? bos >= lo || eos <= lo : bos >= hi || eos <= hi) {  // no sequence is cut
     if (threadIdx.x == 0 && blockIdx.y == 0) p.decay[(int64_t)seg * p.HV + hv] = 0.f;
     return;
   }

@@ -36,8 +36,10 @@ __global__ __launch_bounds__(256) void gated_deltaless_recurrent_kernel(LinRecPa
   const int64_t VD = p.slices * 64, h = hv / (p.HV / p.H);
   int64_t tok0 = n * p.T, len = p.T;
   if (p.cu) {
-    tok0 = load_index(p.cu, p.cu_i32, n);
-    len = load_index(p.cu, p.cu_i32, n + 1) - tok0;
+    // captured calls do not check the bounds: nothing outside the tensors is touched whatever they hold
+    const int64_t a = load_index(p.cu, p.cu_i32, n), e = load_index(p.cu, p.cu_i32, n + 1);
+    tok0 = a < 0 ? 0 : a > p.T ? p.T : a;
+    len = (e > p.T ? p.T : e) - tok0;
   }
   const int64_t st0 = (n * p.HV + hv) * KD * VD + sl * 64 + 4 * cg;
   float4 s[RPT];

@@ -552,6 +552,49 @@ def test_graph_of_documents_takes_other_lengths():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bounds, docs", [
+    ([0, 300, 301, 650], [(0, 300), (300, 301), (301, 650)]),  # rows behind the last document
+    ([0, 64, 64, 699], [(0, 64), (64, 699)]),                  # an empty document
+    ([130, 131, 131, 5000], [(130, 131), (131, 700)]),         # rows before the first one, an end past the tokens
+    ([-7, 0, 0, 0], []),
+    ([0, 650, 300, 700], None),                                # out of order
+])
+def test_bounds_that_no_call_checked(bounds, docs):
+    """Captured and compiled calls take the documents' bounds as they are. In ascending order the documents come out right
+    and other tokens stay as they were; whatever the bounds hold, nothing outside the tensors is written."""
+    from sorernn_amd import _lib, linear
+
+    x = _inputs(1, 700, 1, 2, 64, 64, "token", True, [300, 1, 399], seed=16, train=True)
+    cu = torch.tensor(bounds, device=DEV)
+    wide = torch.full((5, 2, 64, 64), 7.0, device=DEV)
+    o = torch.full((3, 700, 2, 64), 7.0, device=DEV, dtype=torch.bfloat16)
+    need = _lib.load().gdn_decay_attn_states_size(1, 700, 2, 64, 64, 3, 1)
+    states = torch.full((need + 256,), 3, device=DEV, dtype=torch.uint8)
+    _lib.call("gdn_decay_attn_fwd", x["q"].data_ptr(), x["k"].data_ptr(), x["v"].data_ptr(), x["g"].data_ptr(),
+              x["h0"].data_ptr(), o[1].data_ptr(), wide[1].data_ptr(), cu.data_ptr(), 1, 700, 1, 2, 64, 64, 3, 0,
+              *x["g"].stride(), 0.1, 0, states.data_ptr(), need, _lib.stream_of(o))
+    grads = linear.attention_bwd_impl(x["q"], x["k"], x["v"], x["g"], x["h0"], None, x["do"], None, states[:need], cu, 0.1, 0, 3,
+                                      True, True)
+    rec = torch.full((3, 700, 2, 64), 7.0, device=DEV, dtype=torch.bfloat16)
+    _lib.call("gdn_decay_attn_recurrent_fwd", x["q"].data_ptr(), x["k"].data_ptr(), x["v"].data_ptr(), x["g"].data_ptr(), None,
+              rec[1].data_ptr(), None, cu.data_ptr(), 1, 700, 1, 2, 64, 64, 3, 1, 0, *x["g"].stride(), 0.1, 0,
+              _lib.stream_of(o))
+    torch.cuda.synchronize()
+    for y in (wide[0], wide[4], o[0], o[2], rec[0], rec[2]):
+        assert bool((y == 7).all())
+    assert bool((states[need:] == 3).all())
+    inside = torch.zeros(700, dtype=torch.bool, device=DEV)
+    for a, e in docs or []:
+        inside[a:e] = True
+        n = max(i for i in range(3) if bounds[i] <= a)  # the last of those that begin there
+        part = {m: x[m][:, a:e] for m in ("q", "k", "v", "g", "do")}
+        ref = decay_attention(*(part[m] for m in ("q", "k", "v", "g")), 0.1, x["h0"][n:n + 1], None, part["do"])
+        check(o[1:2, a:e], ref, "o", OUT)
+        for name, y in zip(("dq", "dk", "dv", "dg"), grads):
+            check(y[:, a:e], ref, name, GATE if name == "dg" else OUT)
+    assert docs is None or bool((o[1][~inside] == 7).all() and (rec[1][~inside] == 7).all())
+
+
 def test_elements_past_32_bits():
     """2^31 and more elements a tensor. The inputs repeat every 1,024 tokens and a weight of e^-100 is nothing beside the
     others, so tokens 1,024 apart have the same results: two roundings of them apart."""
