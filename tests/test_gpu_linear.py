@@ -552,6 +552,26 @@ def test_graph_of_documents_takes_other_lengths():
             assert torch.equal(a, b)
 
 
+def test_compiled_for_any_length():
+    """One compiled function over lengths on both sides of the split, with documents and their states."""
+    def f(q, k, v, g, h0, cu):
+        q, k = qk_norm_rope(q, k, rot_dim=32, cu_seqlens=cu)
+        return chunk_decay_linear_attention(q, k, v, g, 0.1, h0, True, cu)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, fullgraph=True, dynamic=True, backend="aot_eager")
+    for lens in ([60, 40], [300, 500], [1000, 37]):
+        x = _inputs(1, sum(lens), 1, 2, 64, 128, "token", True, lens, train=True, seed=17)
+        outs = []
+        for fn in (f, compiled):
+            a = [x[m].detach().requires_grad_(True) for m in ("q", "k", "v", "g", "h0")]
+            o, s = fn(*a, x["cu"].to(DEV))
+            outs.append([o, s, *torch.autograd.grad([o, s], a, [x["do"], x["dht"]])])
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)
+    torch._dynamo.reset()
+
+
 @pytest.mark.parametrize("bounds, docs", [
     ([0, 300, 301, 650], [(0, 300), (300, 301), (301, 650)]),  # rows behind the last document
     ([0, 64, 64, 699], [(0, 64), (64, 699)]),                  # an empty document
