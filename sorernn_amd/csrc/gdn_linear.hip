@@ -51,77 +51,20 @@ struct LinParams {
   float scale;
 };
 
-// First token of sequence n; of n = N the number of tokens. Captured and compiled calls do not check the bounds: whatever
-// they hold, nothing outside the tensors is touched, and tokens of no sequence are left out.
-__device__ __forceinline__ int seq_start(const LinParams& p, int n) {
-  if (!p.cu) return n * p.T;
-  const int64_t x = load_index(p.cu, p.cu_i32, n);
-  return x < 0 ? 0 : x > p.tokens ? p.tokens : (int)x;
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ int starts_up_to(const LinParams& p, int lo, int hi, int step, int t) {
+  const int i = lo + (int)(threadIdx.x % kWave) * step;
+  return __popcll(__ballot(i < hi && load_index(p.cu, p.cu_i32, i < hi ? i : lo) <= t));
 }
 
-// The sequence of token t. All lanes of a wave search together.
-__device__ __forceinline__ int seq_of(const LinParams& p, int t) {
-  if (!p.cu) return (unsigned)t / (unsigned)p.T;
-  const int lane = threadIdx.x % kWave;
-  int lo = 0, hi = p.N;  // start of lo <= t < start of hi
-  while (hi - lo > 1) {
-    const int step = (hi - lo + kWave - 1) / kWave, i = lo + lane * step;
-    const bool in = i < hi && load_index(p.cu, p.cu_i32, i < hi ? i : lo) <= t;
-    const int cnt = __popcll(__ballot(in));  // one at least: lane 0's
-    lo += (cnt > 1 ? cnt - 1 : 0) * step;
-    hi = lo + step < hi ? lo + step : hi;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
+}  // namespace gdn
 
-// Up to 64 tokens of sequence n in walking order: fresh, the walk of the sequence begins with them; done, it ends.
-struct Chunk {
-  int t, len, n;  // len 0: none
-  bool fresh, done;
-};
+#include "gdn_linear_walk.h"
 
-// The chunks of tokens [lo, hi) in walking order. Chunks begin where a sequence or the segment does.
-template <bool REV>
-struct ChunkWalk {
-  int lo, hi, n, bos, eos, t;  // t: REV, the end of what is left; else its start
-  __device__ __forceinline__ void start(const LinParams& p, int from, int to) {
-    lo = from;
-    hi = to;
-    n = seq_of(p, REV ? hi - 1 : lo);
-    bos = seq_start(p, n);
-    eos = seq_start(p, n + 1);
-    t = REV ? (eos < hi ? eos : hi) : (bos > lo ? bos : lo);
-  }
-  __device__ __forceinline__ Chunk next(const LinParams& p) {
-    Chunk c{0, 0, n, false, false};
-    if (REV) {
-      const int first = bos > lo ? bos : lo;
-      if (t <= first) return c;
-      c.t = first + ((t - 1 - first) & ~(kC - 1));
-      c.len = t - c.t;
-      c.fresh = t == eos;
-      c.done = c.t == bos;
-      t = c.t;
-      if (t == bos && t > lo) {
-        eos = t;
-        while (bos >= t && --n >= 0) bos = seq_start(p, n);
-      }
-    } else {
-      const int end = eos < hi ? eos : hi;
-      if (t >= end) return c;
-      c.t = t;
-      c.len = end - t < kC ? end - t : kC;
-      c.fresh = t == bos;
-      c.done = t + c.len == eos;
-      t += c.len;
-      if (t == eos && t < hi) {
-        bos = t;
-        while (eos <= t && ++n < p.N) eos = seq_start(p, n + 1);
-      }
-    }
-    return c;
-  }
-};
+namespace gdn {
+
+static_assert(kLinChunk == kC && kLinLanes == kWave, "the walk's chunks and lanes");
 
 // Decay terms of a chunk, base-2 logarithms: b = h + l in two floats, the weight of a token in the state's update and
 // that of the state in a token's output (each with the factor it carries), and the decay of the whole chunk.
@@ -503,7 +446,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
       else st.zero();
     };
     Chunk now = it.next(p), then = it.next(p);
-    begin(now);
+    if (now.len > 0) begin(now);
     __syncthreads();
     __syncthreads();
     for (int c = 0; now.len > 0; ++c) {
@@ -912,9 +855,11 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
   const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const unsigned hv = blockIdx.x % p.HV, seg = blockIdx.x / p.HV;
   const int seg0 = seg * p.L, seg1 = p.tokens - seg0 < p.L ? p.tokens : seg0 + p.L;
-  const int first = seq_of(p, seg0), last = seq_of(p, seg1 - 1);
+  const Span span = span_of(p, seg0, seg1);
+  if (span.t0 >= span.t1) return;
+  const int first = span.first, last = span.last;
   const bool cut = seq_start(p, last + 1) > seg1;  // the last sequence goes on in the next segment
-  const bool begun = seq_start(p, first) < seg0;           // the first one began in an earlier segment
+  const bool begun = seq_start(p, first) < seg0;   // the first one began in an earlier segment
   const int64_t next = (int64_t)p.HV * a.elems, at0 = ((int64_t)seg * p.HV + hv) * a.elems;
   double border = 0., before = 0.;
   if (cut || begun) {
@@ -932,6 +877,7 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
   for (int n = last - w; n >= first; n -= 4) {
     const int bos = seq_start(p, n), eos = seq_start(p, n + 1);
     const int lo = bos > seg0 ? bos : seg0, hi = eos < seg1 ? eos : seg1;
+    if (lo >= hi) continue;
     double sum = 0.;
     if (eos > seg1) sum = border;
     else if (a.fin && a.dfin) {

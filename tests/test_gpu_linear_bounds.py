@@ -1,0 +1,55 @@
+"""GPU: documents' bounds as captured and compiled calls take them, unchecked: empty documents, tokens of none.
+
+Error bounds: those of tests/test_gpu_linear.py.
+"""
+import pytest
+import torch
+
+from sorernn_amd import linear
+from tests.linear_ref import check, decay_attention
+from tests.test_gpu_linear import DEV, GATE, OUT, STATE, _inputs
+
+pytestmark = pytest.mark.gpu
+
+BOUNDS = [
+    # tokens, bounds: sequences that stay whole (up to 384 tokens) and that are cut
+    (300, [0, 200, 200]),                 # an empty document at the end, tokens behind it
+    (300, [0, 1, 200, 200, 200, 200]),    # a call filled up to a fixed number of documents
+    (300, [70, 70, 300]),                 # an empty one at the beginning, tokens before it
+    (300, [0, 0, 130, 130, 131, 131]),
+    (300, [0, 0, 0]),                     # no tokens at all
+    (300, [300, 300, 300]),
+    (700, [0, 300, 650, 650]),
+    (700, [0, 650] + [650] * 200),
+    (700, [130, 130, 390, 390, 390, 700]),
+    (700, [0, 0, 0, 700, 700]),
+    (700, [200, 200, 200]),
+]
+IDS = [f"{t}-{'.'.join(map(str, b[:6]))}" for t, b in BOUNDS]
+
+
+def _run(t, bounds, h=1, hv=2, kd=64, vd=128, seed=21):
+    """A forward and backward without checks, as a replay runs them."""
+    n = len(bounds) - 1
+    x = _inputs(1, t, h, hv, kd, vd, "token", True, [t // n] * (n - 1) + [t - t // n * (n - 1)], seed=seed, train=True)
+    cu = torch.tensor(bounds, device=DEV)
+    args = [x[m] for m in ("q", "k", "v", "g", "h0")]
+    o, final, states = linear.attention_fwd_impl(*args, cu, 0.1, 0, n, True)
+    grads = linear.attention_bwd_impl(*args, final, x["do"], x["dht"], states, cu, 0.1, 0, n, True, True)
+    torch.cuda.synchronize()
+    return x, o, final, grads
+
+
+@pytest.mark.parametrize("t, bounds", BOUNDS, ids=IDS)
+def test_documents_among_empty_ones_and_loose_tokens(t, bounds):
+    x, o, final, grads = _run(t, bounds)
+    for n, (a, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        if a == e:
+            continue
+        part = [x[m][:, a:e] for m in ("q", "k", "v", "g")]
+        ref = decay_attention(*part, 0.1, x["h0"][n:n + 1], None, x["do"][:, a:e], x["dht"][n:n + 1])
+        check(o[:, a:e], ref, "o", OUT)
+        check(final[n:n + 1], ref, "state", STATE)
+        for name, y in zip(("dq", "dk", "dv", "dg"), grads):
+            check(y[:, a:e], ref, name, GATE if name == "dg" else OUT)
+        check(grads[4][n:n + 1], ref, "dh0", STATE)
