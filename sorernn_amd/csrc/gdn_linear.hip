@@ -423,6 +423,21 @@ struct WalkLds {
   float rows[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1], cols[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1];
 };
 
+// The states of sequences without tokens go through a walk as they are. One wave; the segments take the sequences in turn.
+template <int KD, int VD>
+__device__ __forceinline__ void pass_states(const LinParams& p, unsigned hv, int seg, int segs, int lane) {
+  for (int64_t n0 = seg; n0 < p.N; n0 += (int64_t)segs * kWave) {
+    const int64_t n = n0 + (int64_t)lane * segs;
+    const bool empty = n < p.N && seq_start(p, (int)n) >= seq_start(p, (int)n + 1);
+    for (uint64_t m = __ballot(empty); m; m &= m - 1) {
+      const int64_t at = ((n0 + (int64_t)(__ffsll((unsigned long long)m) - 1) * segs) * p.HV + hv) * (KD * VD) + lane * 4;
+      for (int i = 0; i < KD * VD; i += 4 * kWave)
+        *reinterpret_cast<f32x4*>(p.fin + at + i) =
+            p.init ? *reinterpret_cast<const f32x4*>(p.init + at + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+}
+
 template <int KD, int VD, bool REV, int DOT, typename OT>
 __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD, DOT>& lds) {
   constexpr int NCT = VD / 16 / kStateWaves, NU = KD / 32;
@@ -740,6 +755,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   if (w == 0) gate.fetch(p, hv, at[1], lane);
   fetch_qk(at[1]);
   fetch_v(at[1]);
+  if (w == 3 && p.fin && p.cu) pass_states<KD, VD>(p, hv, seg, gridDim.x / p.HV, lane);
   const double x0 = gate_value(at[1], at[2]);
   put_qk(at[1], 0);
   fetch_qk(at[2]);

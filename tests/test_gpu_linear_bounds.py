@@ -28,14 +28,16 @@ BOUNDS = [
 IDS = [f"{t}-{'.'.join(map(str, b[:6]))}" for t, b in BOUNDS]
 
 
-def _run(t, bounds, h=1, hv=2, kd=64, vd=128, seed=21):
+def _run(t, bounds, h=1, hv=2, kd=64, vd=128, seed=21, states=True):
     """A forward and backward without checks, as a replay runs them."""
     n = len(bounds) - 1
     x = _inputs(1, t, h, hv, kd, vd, "token", True, [t // n] * (n - 1) + [t - t // n * (n - 1)], seed=seed, train=True)
+    if not states:
+        x["h0"] = x["dht"] = None
     cu = torch.tensor(bounds, device=DEV)
     args = [x[m] for m in ("q", "k", "v", "g", "h0")]
-    o, final, states = linear.attention_fwd_impl(*args, cu, 0.1, 0, n, True)
-    grads = linear.attention_bwd_impl(*args, final, x["do"], x["dht"], states, cu, 0.1, 0, n, True, True)
+    o, final, kept = linear.attention_fwd_impl(*args, cu, 0.1, 0, n, True)
+    grads = linear.attention_bwd_impl(*args, final, x["do"], x["dht"], kept, cu, 0.1, 0, n, True, True)
     torch.cuda.synchronize()
     return x, o, final, grads
 
@@ -53,3 +55,23 @@ def test_documents_among_empty_ones_and_loose_tokens(t, bounds):
         for name, y in zip(("dq", "dk", "dv", "dg"), grads):
             check(y[:, a:e], ref, name, GATE if name == "dg" else OUT)
         check(grads[4][n:n + 1], ref, "dh0", STATE)
+
+
+@pytest.fixture
+def unwritten_is_nan():
+    """Memory that nothing has written holds NaN."""
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    yield
+    torch.use_deterministic_algorithms(False)
+
+
+@pytest.mark.parametrize("states", [True, False], ids=["states", "zeros"])
+@pytest.mark.parametrize("t, bounds", BOUNDS, ids=IDS)
+def test_states_of_empty_documents_go_through(t, bounds, states, unwritten_is_nan):
+    """A document without tokens ends with its initial state, whose gradient is the final state's."""
+    x, _, final, grads = _run(t, bounds, states=states)
+    for n, (a, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        if a == e:
+            assert torch.equal(final[n], x["h0"][n] if states else torch.zeros_like(final[n])), n
+            assert torch.equal(grads[4][n], x["dht"][n] if states else torch.zeros_like(final[n])), n
+    assert torch.isfinite(final).all() and torch.isfinite(grads[4]).all()
