@@ -47,6 +47,7 @@ struct LinParams {
   float* dot;                   // [HV][tokens] with DOT
   const void* cu;
   int cu_i32, T, N, tokens, L;  // segments of L tokens; without cu sequences of T
+  int zero_rest;                // write zeros to the rows of o whose tokens belong to no sequence
   unsigned HV;
   float scale;
 };
@@ -423,6 +424,14 @@ struct WalkLds {
   float rows[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1], cols[DOT == 2 ? 2 : 1][10][DOT == 2 ? 16 : 1];
 };
 
+// Zeros in rows [t0, t1) of o (pitch in elements), by the 256 threads of the scores' waves.
+template <int VD, typename OT>
+__device__ __forceinline__ void zero_rows(OT* o, int64_t pitch, int t0, int t1) {
+  constexpr int PER = 16 / sizeof(OT), LPR = VD / PER, RP = kScoreWaves * kWave / LPR;
+  const int at = threadIdx.x % (kScoreWaves * kWave);
+  for (int t = t0 + at / LPR; t < t1; t += RP) *reinterpret_cast<f32x4*>(o + t * pitch + at % LPR * PER) = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 // The states of sequences without tokens go through a walk as they are. One wave; the segments take the sequences in turn.
 template <int KD, int VD>
 __device__ __forceinline__ void pass_states(const LinParams& p, unsigned hv, int seg, int segs, int lane) {
@@ -449,6 +458,7 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
   const bf16* e0 = DOT ? p.e + hv / p.re * VD : nullptr;
   ChunkWalk<REV> it;
   it.start(p, seg0, seg1);
+  const int first = it.t;  // with REV the end of the first chunk
 
   if (wave < kStateWaves) {  // ------------------------------------------------------------------ the state's waves
     const int w = wave;
@@ -795,6 +805,11 @@ __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD,
     at[4] = it.next(p);
   }
   finish_dots(at[0], half ^ 1);
+  if (p.zero_rest) {
+    OT* o = static_cast<OT*>(p.o) + (int64_t)hv * VD;
+    zero_rows<VD>(o, (int64_t)p.HV * VD, seg0, REV ? it.t : first);
+    zero_rows<VD>(o, (int64_t)p.HV * VD, REV ? first : it.t, seg1);
+  }
 }
 
 template <int KD, int VD>
@@ -872,6 +887,9 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
   const unsigned hv = blockIdx.x % p.HV, seg = blockIdx.x / p.HV;
   const int seg0 = seg * p.L, seg1 = p.tokens - seg0 < p.L ? p.tokens : seg0 + p.L;
   const Span span = span_of(p, seg0, seg1);
+  if (p.zero_rest)  // tokens of no sequence
+    for (int t = seg0 + threadIdx.x; t < seg1; t += 256)
+      if (t < span.t0 || t >= span.t1) store_from_f32(a.dg, a.dtype, (int64_t)t * p.HV + hv, 0.f);
   if (span.t0 >= span.t1) return;
   const int first = span.first, last = span.last;
   const bool cut = seq_start(p, last + 1) > seg1;  // the last sequence goes on in the next segment
@@ -1174,8 +1192,9 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
   float* dot_k = reinterpret_cast<float*>(ws + sp.states + sp.dots);
   float* dq_heads = reinterpret_cast<float*>(ws + sp.states + 2 * sp.dots);
   float* dk_heads = reinterpret_cast<float*>(ws + sp.states + 2 * sp.dots + sp.heads);
-  const LinParams base = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N,
+  LinParams base = lin_params(pl, g, g_dtype, g_batch_stride, g_token_stride, g_head_stride, cu_seqlens, flags, T, N,
                                     HV, scale);
+  base.zero_rest = cu_seqlens != nullptr;
   // from the end: the states R at the segments' borders, then dv and dk
   LinParams r = base;
   lin_roles(r, k, rep, q, rep, d_o, 1, nullptr, 1, K, V);

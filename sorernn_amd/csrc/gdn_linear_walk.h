@@ -74,7 +74,8 @@ struct Chunk {
 };
 
 // The chunks of tokens [lo, hi) in walking order. Chunks begin where a sequence or the segment does. The first is not fresh
-// only if it lies at a border inside the token axis.
+// only if it lies at a border inside the token axis. They cover all tokens from t after start() to t after the last of them;
+// the others of [lo, hi) belong to no sequence.
 template <bool REV>
 struct ChunkWalk {
   int lo, hi, n, bos, eos, t;  // t: REV, the end of what is left; else its start
@@ -84,6 +85,7 @@ struct ChunkWalk {
     hi = to;
     t = REV ? hi : lo;
     n = REV ? span_back(p, t, lo) : span_front(p, t, hi);
+    t = t < lo ? lo : t > hi ? hi : t;
     bos = seq_start(p, n);
     eos = seq_start(p, n + 1);
     if (REV && t < hi) eos = t;

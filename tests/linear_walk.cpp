@@ -38,23 +38,26 @@ inline int starts_up_to(const Bounds& p, int lo, int hi, int step, int t) {
 #include "../sorernn_amd/csrc/gdn_linear_walk.h"
 
 template <bool REV>
-static int walk(const gdn::Bounds& p, int lo, int hi, int* out, int most) {
+static int walk(const gdn::Bounds& p, int lo, int hi, int* out, int most, int* ends) {
   gdn::ChunkWalk<REV> it;
   it.start(p, lo, hi);
+  ends[0] = it.t;
   int count = 0;
   for (gdn::Chunk c = it.next(p); c.len > 0 && count < most; c = it.next(p), ++count) {
     const int row[] = {c.t, c.len, c.n, c.fresh, c.done};
     for (int i = 0; i < 5; ++i) out[5 * count + i] = row[i];
   }
+  ends[1] = it.t;
   return count;
 }
 
-// Chunks (t, len, n, fresh, done) of tokens [lo, hi) into out; their number, or -1 after a read outside the bounds.
-extern "C" int linear_walk(const int64_t* cu, int n, int tokens, int seq, int rev, int lo, int hi, int* out, int most) {
+// Chunks (t, len, n, fresh, done) of tokens [lo, hi) into out, and where they begin and end in walking order; their number,
+// or -1 after a read outside the bounds.
+extern "C" int linear_walk(const int64_t* cu, int n, int tokens, int seq, int rev, int lo, int hi, int* out, int most, int* ends) {
   const gdn::Bounds p{cu, 0, seq, n, tokens};
   gdn::g_outside = 0;
   gdn::g_entries = n + 1;
-  const int count = rev ? walk<true>(p, lo, hi, out, most) : walk<false>(p, lo, hi, out, most);
+  const int count = rev ? walk<true>(p, lo, hi, out, most, ends) : walk<false>(p, lo, hi, out, most, ends);
   return gdn::g_outside ? -1 : count;
 }
 

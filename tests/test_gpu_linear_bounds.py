@@ -75,3 +75,19 @@ def test_states_of_empty_documents_go_through(t, bounds, states, unwritten_is_na
             assert torch.equal(final[n], x["h0"][n] if states else torch.zeros_like(final[n])), n
             assert torch.equal(grads[4][n], x["dht"][n] if states else torch.zeros_like(final[n])), n
     assert torch.isfinite(final).all() and torch.isfinite(grads[4]).all()
+
+
+def _loose(t, bounds):
+    out = torch.ones(t, dtype=torch.bool, device=DEV)
+    for a, e in zip(bounds[:-1], bounds[1:]):
+        out[a:e] = False
+    return out
+
+
+@pytest.mark.parametrize("heads", [(1, 2), (2, 2)], ids=["shared", "own"])
+@pytest.mark.parametrize("t, bounds", BOUNDS, ids=IDS)
+def test_gradients_of_loose_tokens_are_zero(t, bounds, heads, unwritten_is_nan):
+    _, _, _, grads = _run(t, bounds, *heads)
+    loose = _loose(t, bounds)
+    for name, y in zip(("dq", "dk", "dv", "dg"), grads):
+        assert not y[:, loose].any() and torch.isfinite(y.float()).all(), name

@@ -24,13 +24,21 @@ def lib(tmp_path_factory):
 
 def _chunks(lib, cu, tokens, rev, lo, hi, seq=0):
     most = tokens + 2
-    out = np.zeros(5 * most, np.int32)
+    out, ends = np.zeros(5 * most, np.int32), np.zeros(2, np.int32)
     bounds = None if cu is None else np.array(cu, np.int64)
     n = len(cu) - 1 if cu is not None else tokens // seq
     count = lib.linear_walk(None if cu is None else bounds.ctypes.data_as(ctypes.c_void_p), n, tokens, seq, int(rev), lo, hi,
-                            out.ctypes.data_as(ctypes.c_void_p), most)
+                            out.ctypes.data_as(ctypes.c_void_p), most, ends.ctypes.data_as(ctypes.c_void_p))
     assert 0 <= count < most, (cu, tokens, rev, lo, hi, count)
-    return out[:5 * count].reshape(count, 5).tolist()
+    chunks = out[:5 * count].reshape(count, 5).tolist()
+    first, last = ends.tolist()
+    assert lo <= min(first, last) and max(first, last) <= hi, (cu, tokens, rev, lo, hi, first, last)
+    at = first  # they cover what lies between their ends
+    for t, ln, *_ in chunks:
+        assert (t + ln if rev else t) == at, (cu, tokens, rev, lo, hi, first, last, t, ln)
+        at = t if rev else t + ln
+    assert at == last
+    return chunks
 
 
 def _span(lib, cu, tokens, lo, hi, seq=0):
