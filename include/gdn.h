@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 8
+#define GDN_ABI_VERSION 9
 
 #if defined(__GNUC__) || defined(__clang__)
 #define GDN_API __attribute__((visibility("default")))
@@ -47,6 +47,7 @@ extern "C" {
 #define GDN_FLAG_BETA_SIGMOID 0x2u /* beta holds logits: use sigmoid(beta) */
 #define GDN_FLAG_GATE_IN_KERNEL 0x4u /* g holds a: use g = -exp(A_log[h]) * softplus(a + dt_bias[h]) */
 #define GDN_FLAG_CU_INT32 0x8u /* cu_seqlens is int32 (default int64) */
+#define GDN_FLAG_ZERO_REST 0x10u /* zeros in the rows of o whose tokens lie outside cu_seqlens (default: left as they are) */
 
 /* activation codes for the conv and the gated norm */
 #define GDN_ACT_NONE 0
@@ -354,7 +355,8 @@ GDN_API int gdn_attn_fwd(const void* q, const void* k, const void* v, int64_t v_
  * o_t = scale S_t^T q_t. bf16 q, k, v, o; initial_state (or NULL: zeros) and final_state (or NULL: not written)
  * fp32. g: log decays in g_dtype, element strides for the batch row, the token and the value head (0 where it does
  * not vary: one decay a head is 0, 0, 1), or NULL: no decay. With cu_seqlens the batch stride is not used. Values
- * below -100 are taken as -100. K and V each 64 or 128; tensors 16-byte aligned. flags: GDN_FLAG_CU_INT32.
+ * below -100 are taken as -100. K and V each 64 or 128; tensors 16-byte aligned. flags: GDN_FLAG_CU_INT32,
+ * GDN_FLAG_ZERO_REST. cu_seqlens ascends; a document without tokens passes its state on.
  * states: gdn_decay_attn_states_size(B, T, HV, K, V, N, cu_seqlens != NULL) bytes (0: may be NULL), contents on
  * entry irrelevant: the states entering the segments that the call cuts its sequences into. gdn_decay_attn_bwd
  * reads them. Calls that share them must not overlap.
@@ -371,7 +373,7 @@ GDN_API size_t gdn_decay_attn_states_size(int64_t B, int64_t T, int64_t HV, int6
 /*
  * Backward of gdn_decay_attn_fwd: its inputs and the states it left, d_o [B,T,HV,V] bf16, d_final_state or NULL (zero).
  * dq, dk [B,T,H,K] and dv [B,T,HV,V] bf16; dg [B,T,HV] contiguous in g_dtype or NULL (not wanted); d_initial_state or
- * NULL. final_state (the forward's) is read for dg where d_final_state is given. workspace:
+ * NULL. Rows of tokens outside cu_seqlens are zero. final_state (the forward's) is read for dg where d_final_state is given. workspace:
  * gdn_decay_attn_bwd_workspace_size bytes.
  */
 GDN_API int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
@@ -388,7 +390,7 @@ GDN_API size_t gdn_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H
 
 /*
  * The recurrence of gdn_decay_attn_fwd token by token in fp32, q, k, v, o in qkv_dtype: the step of single tokens.
- * final_state may equal initial_state (in-place update). g and its strides as there, without the bound of -100.
+ * The same flags. final_state may equal initial_state (in-place update). g and its strides as there, without the bound of -100.
  */
 GDN_API int gdn_decay_attn_recurrent_fwd(const void* q, const void* k, const void* v, const void* g,
                                          const float* initial_state, void* o, float* final_state,

@@ -20,8 +20,9 @@ FLAG_QK_L2NORM = 0x1
 FLAG_BETA_SIGMOID = 0x2
 FLAG_GATE_IN_KERNEL = 0x4
 FLAG_CU_INT32 = 0x8
+FLAG_ZERO_REST = 0x10
 ACT_NONE, ACT_SILU, ACT_SILU_ROUNDED = 0, 1, 2
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64

@@ -1134,6 +1134,7 @@ extern "C" int gdn_decay_attn_fwd(const void* q, const void* k, const void* v, c
   if (pl.split) launch_segments<false>(p, pl, K, V, s);
   p.fin = final_state;
   p.o = o;
+  p.zero_rest = cu_seqlens && (flags & GDN_FLAG_ZERO_REST);
   lin_by_dims(K, V, [&](auto k_, auto v_) {
     hipLaunchKernelGGL((gated_deltaless_chunk_kernel<decltype(k_)::value, decltype(v_)::value>),
                        dim3((unsigned)(pl.segs * HV)), dim3(kWalkThreads), 0, s, p);

@@ -18,9 +18,9 @@ struct LinRecParams {
   void* o;
   float* ht;
   const void* cu;
-  int cu_i32, dg;
+  int cu_i32, dg, zero_rest;  // zero_rest: write zeros to the rows of o outside all sequences
   int64_t gb, gt, gh;
-  int64_t T, H, HV, slices;  // slices: V / 64
+  int64_t T, N, H, HV, slices;  // slices: V / 64
   float scale;
 };
 
@@ -34,12 +34,20 @@ __global__ __launch_bounds__(256) void gated_deltaless_recurrent_kernel(LinRecPa
   const int t = threadIdx.x, cg = t % 16, rg = t / 16, lane = t % kWave, w = t / kWave;
   const int64_t sl = blockIdx.x % p.slices, hv = blockIdx.x / p.slices % p.HV, n = blockIdx.x / p.slices / p.HV;
   const int64_t VD = p.slices * 64, h = hv / (p.HV / p.H);
+  E* o = static_cast<E*>(p.o);
   int64_t tok0 = n * p.T, len = p.T;
   if (p.cu) {
     // captured calls do not check the bounds: nothing outside the tensors is touched whatever they hold
     const int64_t a = load_index(p.cu, p.cu_i32, n), e = load_index(p.cu, p.cu_i32, n + 1);
     tok0 = a < 0 ? 0 : a > p.T ? p.T : a;
-    len = (e > p.T ? p.T : e) - tok0;
+    const int64_t end = e < 0 ? 0 : e > p.T ? p.T : e;
+    len = end - tok0;
+    if (p.zero_rest) {  // the rows before the first sequence and behind the last
+      if (n == 0)
+        for (int64_t c = t; c < tok0 * 64; c += 256) o[(c / 64 * p.HV + hv) * VD + sl * 64 + c % 64] = (E)0.f;
+      if (n == p.N - 1)
+        for (int64_t c = end * 64 + t; c < p.T * 64; c += 256) o[(c / 64 * p.HV + hv) * VD + sl * 64 + c % 64] = (E)0.f;
+    }
   }
   const int64_t st0 = (n * p.HV + hv) * KD * VD + sl * 64 + 4 * cg;
   float4 s[RPT];
@@ -47,7 +55,6 @@ __global__ __launch_bounds__(256) void gated_deltaless_recurrent_kernel(LinRecPa
   for (int i = 0; i < RPT; ++i)
     s[i] = p.h0 ? *reinterpret_cast<const float4*>(p.h0 + st0 + (rg + 16 * i) * VD) : float4{0.f, 0.f, 0.f, 0.f};
   const E *q = static_cast<const E*>(p.q), *k = static_cast<const E*>(p.k), *v = static_cast<const E*>(p.v);
-  E* o = static_cast<E*>(p.o);
   const int64_t g0 = p.cu ? tok0 * p.gt : n * p.gb;
   for (int64_t t0 = 0; t0 < len; t0 += kLinRecTok) {
     const int nt = len - t0 < kLinRecTok ? (int)(len - t0) : kLinRecTok;
@@ -134,7 +141,7 @@ extern "C" int gdn_decay_attn_recurrent_fwd(const void* q, const void* k, const 
     return GDN_ERR_UNSUPPORTED;
   }
   LinRecParams p{q, k, v, g, initial_state, o, final_state, cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, g_dtype,
-                 g_batch_stride, g_token_stride, g_head_stride, T, H, HV, V / 64, scale};
+                 (flags & GDN_FLAG_ZERO_REST) ? 1 : 0, g_batch_stride, g_token_stride, g_head_stride, T, N, H, HV, V / 64, scale};
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto e) {
     using E = decltype(e);

@@ -200,6 +200,8 @@ def _attention_args(name, q, k, v, g, scale, initial_state, cu_seqlens, cu_seqle
         if tuple(g.shape) != (b, t, hv):
             raise ValueError(f"{name}: g must be [B,T,HV] = {(b, t, hv)} or [HV], got {tuple(g.shape)}")
     n, flags = _cu_info(name, cu_seqlens, cu_seqlens_cpu, b, t)
+    if cu_seqlens is not None:  # a replayed or compiled call may leave tokens out
+        flags |= _lib.FLAG_ZERO_REST
     if initial_state is not None and tuple(initial_state.shape) != (n, hv, kd, vd):
         raise ValueError(f"{name}: initial_state must be [N,HV,K,V] = {(n, hv, kd, vd)}, got {tuple(initial_state.shape)}")
     return g, n, flags, float(kd**-0.5 if scale is None else scale)

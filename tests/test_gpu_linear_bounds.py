@@ -5,9 +5,9 @@ Error bounds: those of tests/test_gpu_linear.py.
 import pytest
 import torch
 
-from sorernn_amd import linear
+from sorernn_amd import fused_recurrent_decay_linear_attention, linear
 from tests.linear_ref import check, decay_attention
-from tests.test_gpu_linear import DEV, GATE, OUT, STATE, _inputs
+from tests.test_gpu_linear import DEV, GATE, OUT, STATE, _block, _block_params, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,46 @@ def test_gradients_of_loose_tokens_are_zero(t, bounds, heads, unwritten_is_nan):
     loose = _loose(t, bounds)
     for name, y in zip(("dq", "dk", "dv", "dg"), grads):
         assert not y[:, loose].any() and torch.isfinite(y.float()).all(), name
+
+
+def test_graph_of_a_training_step_with_loose_tokens(unwritten_is_nan):
+    """Captured with whole bounds and replayed with padded ones, over memory full of NaN: the outputs of tokens in no
+    document are zero, and the parameters' gradients those of the documents alone."""
+    t, p = 700, _block_params(2)
+    gen = torch.Generator(DEV).manual_seed(5)
+    x, up = (torch.randn(1, t, 192, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    for w in p.values():
+        w.requires_grad_(True)
+
+    def step(x, up, cu, host):
+        y, s = _block(x, p, cu, host)
+        with torch.no_grad():  # the rows of the recurrent form too
+            q = torch.ones(1, x.shape[1], 1, 64, device=DEV, dtype=x.dtype)
+            o, _ = fused_recurrent_decay_linear_attention(q, q, q, cu_seqlens=cu, cu_seqlens_cpu=host)
+        return [y, s, o, *torch.autograd.grad(y, list(p.values()), up)]
+
+    host = torch.tensor([0, 100, 300, 700])
+    cu, static = host.to(DEV), up.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(x, static, cu, host)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(x, static, cu, host)
+    for bounds in ([0, 200, 500, 500], [64, 64, 300, 650], [0, 100, 300, 700]):
+        cu.copy_(torch.tensor(bounds))
+        static.copy_(up)
+        static[:, _loose(t, bounds)] = 0
+        graph.replay()
+        torch.cuda.synchronize()
+        loose = _loose(t, bounds)
+        for z in (outs[0], outs[2]):
+            assert torch.isfinite(z).all() and not z[:, loose].any()
+        a, e = bounds[0], bounds[-1]
+        alone = sorted({b - a for b in bounds})
+        want = step(x[:, a:e], up[:, a:e], torch.tensor(alone, device=DEV), torch.tensor(alone))
+        for name, g, w in zip(p, outs[3:], want[3:]):
+            assert torch.isfinite(g).all(), name
+            if name in ("w", "wo"):  # a few roundings to bf16 on the way, each of half a step at most
+                assert (g.double() - w.double()).norm() <= 8 * 2.0**-8 * w.double().norm(), name
