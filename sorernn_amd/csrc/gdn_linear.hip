@@ -25,6 +25,8 @@
 // rounding of the output itself. The decays are summed in 64 bits: a difference of two sums in 32 would carry the
 // rounding of the sums into every weight.
 
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "gdn_mfma.h"
@@ -69,10 +71,11 @@ static_assert(kLinChunk == kC && kLinLanes == kWave, "the walk's chunks and lane
 
 // Decay terms of a chunk, base-2 logarithms: b = h + l in two floats, the weight of a token in the state's update and
 // that of the state in a token's output (each with the factor it carries), and the decay of the whole chunk.
-struct Decays {
+struct alignas(16) Decays {
   float h[kC], l[kC], wst[kC], win[kC];
   float all;
 };
+static_assert(sizeof(Decays) % 16 == 0, "arrays of it are read 16 bytes at a time");
 
 template <int CTRL, int ROW_MASK>
 __device__ __forceinline__ double dpp_scan_step(double v) {
@@ -451,6 +454,9 @@ template <int KD, int VD, bool REV, int DOT, typename OT>
 __device__ __forceinline__ void walk_segment(const LinParams& p, WalkLds<KD, VD, DOT>& lds) {
   constexpr int NCT = VD / 16 / kStateWaves, NU = KD / 32;
   constexpr int NS = DOT ? 3 : 2;  // parts of the state under o
+  using Lds = WalkLds<KD, VD, DOT>;
+  static_assert(offsetof(Lds, ps) % 16 == 0 && offsetof(Lds, d) % 16 == 0 && (DOT < 2 || offsetof(Lds, cols) % 16 == 0),
+                "accessed 16 bytes at a time");
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int g = lane >> 4, i = lane & 15;
   const unsigned hv = blockIdx.x % p.HV, seg = blockIdx.x / p.HV;
