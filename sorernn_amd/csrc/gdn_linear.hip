@@ -33,6 +33,10 @@
 
 namespace gdn {
 
+// In place of a segment's decay: the sequence that goes on in the next segment begins in this one, or none does. No decay is
+// negative.
+constexpr float kBegins = -1.f;
+
 struct LinParams {
   const bf16 *q, *k, *v, *e;    // [tokens][heads][K or V]: the walk's q, k, v and the rows of the gate's dot products
   int64_t qs, ks, vs, es;       // elements between tokens
@@ -42,7 +46,7 @@ struct LinParams {
   int64_t gb, gt, gh;           // element strides of batch row, token and value head
   const float* init;            // [N][HV][K][V] state before the walk, or null: zeros
   float* entry;                 // [segments][HV][K][V] states entering the segments, or null where no border cuts a sequence
-  float* decay;                 // [segments][HV] decay of the sequence that goes on in the next segment; 0: it begins here
+  float* decay;                 // [segments][HV] decay of the sequence that goes on in the next segment, or kBegins
   int transposed;               // init and entry are read as [V][K]
   float* fin;                   // [N][HV][K][V] state after the walk, or null
   void* o;                      // [tokens][HV][V]
@@ -318,7 +322,7 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
   const int n = seq_of(p, REV ? lo - 1 : hi), bos = seq_start(p, n), eos = seq_start(p, n + 1);
   const bool whole = REV ? eos <= hi : bos >= lo;  // the sequence's walk begins in this segment
   if (REV ? bos >= lo || eos <= lo : bos >= hi || eos <= hi) {  // no sequence is cut
-    if (threadIdx.x == 0 && blockIdx.y == 0) p.decay[(int64_t)seg * p.HV + hv] = 0.f;
+    if (threadIdx.x == 0 && blockIdx.y == 0) p.decay[(int64_t)seg * p.HV + hv] = kBegins;
     return;
   }
   if (REV) hi = whole ? eos : hi;
@@ -372,13 +376,13 @@ __global__ __launch_bounds__(256, 3) void gated_deltaless_segment_kernel(LinPara
   st.store(p.entry + ((int64_t)(seg + (REV ? -1 : 1)) * p.HV + hv) * (KD * VD) + blockIdx.y * 64, VD, w, lane);
   if (w == 0 && blockIdx.y == 0) {
     for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m, kWave);
-    if (lane == 0) p.decay[(int64_t)seg * p.HV + hv] = whole ? 0.f : __builtin_amdgcn_exp2f((float)total);
+    if (lane == 0) p.decay[(int64_t)seg * p.HV + hv] = whole ? kBegins : __builtin_amdgcn_exp2f((float)total);
   }
 }
 
 // The segments' contributions into the states entering them, in place: entry[s] += decay[s - 1] entry[s - 1] (from the
-// end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread. Where a decay is 0 nothing of the other is read: it
-// may not have been written.
+// end: decay[s + 1] entry[s + 1]), four neighbouring elements a thread. Where a decay is kBegins nothing of the other is
+// taken: it may not have been written. A decay that is 0 is multiplied: 0 times an infinity or NaN is NaN, as in a walk.
 template <bool REV>
 __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, int elems, int segs) {
   const unsigned per = elems / 1024, hv = blockIdx.x / per;
@@ -400,7 +404,7 @@ __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s0 + u >= segs - 1) break;
-      run = c[u] == 0.f ? x[u] : run * c[u] + x[u];
+      run = c[u] == kBegins ? x[u] : run * c[u] + x[u];
       *reinterpret_cast<f32x4*>(e + (REV ? segs - 2 - s0 - u : s0 + u + 1) * step) = run;
     }
   }

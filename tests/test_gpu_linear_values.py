@@ -1,0 +1,36 @@
+"""GPU: the decay linear attention's values where a call is cut into segments and where types meet."""
+import pytest
+import torch
+
+from sorernn_amd import chunk_decay_linear_attention
+from tests.test_gpu_linear import DEV, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("t", [200, 2000], ids=["whole", "cut"])
+def test_non_finite_token_stays_over_segments_that_decay_to_nothing(t, bad):
+    """exp(-256) over a segment's 128 tokens is 0 in fp32, and 0 times an infinity or NaN is NaN: how a call is cut does not
+    decide whether a bad token shows behind it (its column) and, in the backward, before it."""
+    x = _inputs(1, t, 1, 1, 64, 64, "none", True, train=True, seed=31)
+    x["v"][0, 10, 0, 5] = bad
+    g = torch.full((1,), -2.0, device=DEV)
+    o, s = chunk_decay_linear_attention(x["q"], x["k"], x["v"], g, 0.2, x["h0"], True)
+    assert not torch.isfinite(o[0, 10:, 0, 5].float()).any() and not torch.isfinite(s[..., 5]).any()
+    rest = [c for c in range(64) if c != 5]
+    assert torch.isfinite(o[..., rest].float()).all() and torch.isfinite(s[..., rest]).all()
+    assert torch.isfinite(o[:, :10].float()).all()
+
+    y = _inputs(1, t, 1, 1, 64, 64, "none", True, train=True, seed=31)
+    names = ("q", "k", "v", "h0")
+    for n in names:
+        y[n].requires_grad_(True)
+    o, s = chunk_decay_linear_attention(y["q"], y["k"], y["v"], g, 0.2, y["h0"], True)
+    up = y["do"].clone()
+    up[0, t - 10, 0, 3] = bad
+    dq, dk, dv, dh0 = torch.autograd.grad([o, s], [y[n] for n in names], [up, y["dht"]])
+    assert not torch.isfinite(dv[0, :t - 9, 0, 3].float()).any() and not torch.isfinite(dh0[..., 3]).any()
+    assert not torch.isfinite(dk[0, :t - 9].float()).any()
+    for z in (dq, dk, dv):
+        assert torch.isfinite(z[:, t - 9:].float()).all()
