@@ -287,7 +287,8 @@ def _strided(x: Tensor):
     st = x.stride()
     if st[3] != 1 or x.data_ptr() & 15 or (st[0] | st[1] | st[2]) & (16 // x.element_size() - 1):
         x = _rows(x)
-        st = x.stride()
+        _, t, h, d = x.shape
+        st = (t * h * d, h * d, d, 1)  # where a size is 1, a contiguous tensor may have any stride
     return x, st
 
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from sorernn_amd import chunk_decay_linear_attention
+from sorernn_amd import chunk_decay_linear_attention, qk_norm_rope
 from tests.test_gpu_linear import DEV, _inputs
 
 pytestmark = pytest.mark.gpu
@@ -34,3 +34,11 @@ def test_non_finite_token_stays_over_segments_that_decay_to_nothing(t, bad):
     assert not torch.isfinite(dk[0, :t - 9].float()).any()
     for z in (dq, dk, dv):
         assert torch.isfinite(z[:, t - 9:].float()).all()
+
+
+def test_norm_rope_of_one_padded_row():
+    wide = torch.randn(1, 1, 1, 131, device=DEV).bfloat16()
+    x, rows = wide[..., :128], wide[..., :128].clone(memory_format=torch.contiguous_format)
+    pos = torch.tensor([5], device=DEV)
+    for a, b in zip(qk_norm_rope(x, x, positions=pos), qk_norm_rope(rows, rows, positions=pos)):
+        assert torch.equal(a, b)

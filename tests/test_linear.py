@@ -191,3 +191,26 @@ def test_entry_points_check_their_arguments():
     for kw in ({"D": 96}, {"rot": 24}, {"rot": 80}):
         assert rope(**kw) == _lib.GDN_ERR_UNSUPPORTED, kw
     assert rope(T=0) == _lib.GDN_OK
+
+
+@pytest.mark.parametrize("shape, pad", [((1, 1, 1), 131), ((1, 1, 3), 131), ((1, 4, 1), 131), ((2, 1, 1), 129)])
+def test_padded_rows_are_copied_to_aligned_ones(shape, pad):
+    """Also where the odd strides belong to dimensions of size 1, which a contiguous copy may keep."""
+    x = torch.zeros(*shape, pad, dtype=torch.bfloat16)[..., :128]
+    y, strides = linear._strided(x)
+    assert torch.equal(x, y) and y.data_ptr() % 16 == 0 and strides[3] == 1
+    assert all(st % 8 == 0 for st in strides[:3]) and all(n == 1 or st == s for n, st, s in zip(x.shape, strides, y.stride()))
+
+
+def test_one_padded_row_reaches_the_kernels(launches, monkeypatch):
+    """The C entry's own rule of alignment, for one token of one head."""
+    def call(name, *a):
+        launches.append(name)
+        for at in (1, 2, 3, 5, 6, 7):
+            assert a[at] % 8 == 0, (name, at, a[at])
+
+    monkeypatch.setattr(_lib, "call", call)
+    x = torch.zeros(1, 1, 1, 131, dtype=torch.bfloat16)[..., :128].requires_grad_(True)
+    a, b = qk_norm_rope(x, x)
+    torch.autograd.grad([a, b], [x], [torch.ones_like(a), torch.ones_like(b)])
+    assert launches == ["gdn_qk_norm_rope_fwd", "gdn_qk_norm_rope_bwd"]
