@@ -196,6 +196,8 @@ def _attention_args(name, q, k, v, g, scale, initial_state, cu_seqlens, cu_seqle
     if g is not None:
         _lib.dtype_code(g.dtype)
         if g.dim() == 1 and g.shape[0] == hv:
+            if g.dtype != torch.float32 and g.requires_grad and torch.is_grad_enabled():
+                g = g.float()  # its gradient is a sum over the tokens: summed in fp32, rounded once
             g = g.expand(b, t, hv)
         if tuple(g.shape) != (b, t, hv):
             raise ValueError(f"{name}: g must be [B,T,HV] = {(b, t, hv)} or [HV], got {tuple(g.shape)}")

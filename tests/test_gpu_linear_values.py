@@ -42,3 +42,20 @@ def test_norm_rope_of_one_padded_row():
     pos = torch.tensor([5], device=DEV)
     for a, b in zip(qk_norm_rope(x, x, positions=pos), qk_norm_rope(rows, rows, positions=pos)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_one_gate_a_head_in_16_bits_has_one_rounding_of_its_gradient(dtype):
+    """The gradient of a decay for each head is a sum over all tokens in fp32, rounded once to the gate's type, also where
+    most of it cancels: the second row's gradient is nearly the first's negative."""
+    x = _inputs(2, 600, 1, 8, 64, 64, "head", False, train=True, seed=33)
+    for m in ("q", "k", "v", "do"):
+        x[m][1] = x[m][0]
+    x["do"][1] *= -1.0078125
+    gate = x["g"].to(dtype)
+    grads = []
+    for g in (gate, gate.float()):
+        g = g.detach().requires_grad_(True)
+        o, _ = chunk_decay_linear_attention(x["q"], x["k"], x["v"], g, 0.1)
+        grads.append(torch.autograd.grad(o, [g], [x["do"]])[0])
+    assert grads[0].dtype == dtype and torch.equal(grads[0], grads[1].to(dtype))
