@@ -20,6 +20,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWave = 64;
 
+// Workgroups of 256 threads along x that a launch takes: a grid of 2^32 threads or more is launched with their number modulo
+// 2^32, without an error unless that is 0.
+constexpr int64_t kMaxGroups256 = 0xffffff;
+
 // ---------------------------------------------------------------- element access by runtime dtype
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
   switch (dtype) {

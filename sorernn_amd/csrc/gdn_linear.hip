@@ -1196,6 +1196,12 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
                            (long long)sp.bytes(shared));
     return GDN_ERR_INVALID;
   }
+  // the last kernel's: the gate's segments, and dq and dk of shared heads
+  const int64_t blocks = (dg ? pl.segs * HV : 0) + (shared ? (B * T * H * K / 4 + 255) / 256 : 0);
+  if (blocks > kMaxGroups256) {
+    gdn_internal_set_error("gdn_decay_attn_bwd: too many tokens and heads for one launch");
+    return GDN_ERR_UNSUPPORTED;
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int rep = (int)(HV / H);
   char* ws = static_cast<char*>(workspace);
@@ -1238,11 +1244,6 @@ extern "C" int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, c
     const LinFinish fin{dot_q, dot_k, q_.entry, r.entry, final_state, d_final_state, initial_state, d_initial_state, dg, g_dtype,
                         (int)(K * V), (int)pl.segs, dq_heads, dk_heads, static_cast<bf16*>(dq), static_cast<bf16*>(dk), rep,
                         (int)K};
-    const int64_t blocks = (dg ? pl.segs * HV : 0) + (shared ? (B * T * H * K / 4 + 255) / 256 : 0);
-    if (blocks > 0x7fffffffLL) {
-      gdn_internal_set_error("gdn_decay_attn_bwd: too many tokens and heads for one launch");
-      return GDN_ERR_UNSUPPORTED;
-    }
     hipLaunchKernelGGL(gated_deltaless_finish_kernel, dim3((unsigned)blocks, shared ? 2 : 1), dim3(256), 0, s, base, fin);
   }
   return gdn_internal_check_launch("gated_deltaless_chunk_bwd_kernel");

@@ -136,7 +136,7 @@ extern "C" int gdn_decay_attn_recurrent_fwd(const void* q, const void* k, const 
     return GDN_ERR_INVALID;
   }
   const int64_t blocks = N * HV * (V / 64);
-  if (blocks > 0x7fffffffLL) {
+  if (blocks > kMaxGroups256) {
     gdn_internal_set_error("%s: too many sequences and heads for one launch", name);
     return GDN_ERR_UNSUPPORTED;
   }

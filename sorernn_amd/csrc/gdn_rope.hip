@@ -282,7 +282,7 @@ extern "C" int gdn_qk_norm_rope_fwd(const void* q, int64_t q_batch_stride, int64
   if (int rc = rope_check("gdn_qk_norm_rope_fwd", p, B, T, HQ, HK, D, N, dtype, rot_dim, theta, eps)) return rc;
   if (T == 0) return GDN_OK;
   const int64_t blocks = rope_blocks(p.tokens);
-  launch_rope<false>(p, D, dtype, blocks < 0x3fffffffLL ? blocks : 0x3fffffffLL, static_cast<hipStream_t>(stream));
+  launch_rope<false>(p, D, dtype, blocks < kMaxGroups256 ? blocks : kMaxGroups256, static_cast<hipStream_t>(stream));
   return gdn_internal_check_launch("gated_delta_qk_norm_rope_kernel");
 }
 

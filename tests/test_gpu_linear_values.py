@@ -59,3 +59,13 @@ def test_one_gate_a_head_in_16_bits_has_one_rounding_of_its_gradient(dtype):
         o, _ = chunk_decay_linear_attention(x["q"], x["k"], x["v"], g, 0.1)
         grads.append(torch.autograd.grad(o, [g], [x["do"]])[0])
     assert grads[0].dtype == dtype and torch.equal(grads[0], grads[1].to(dtype))
+
+
+def test_norm_rope_of_2_26_tokens():
+    """A workgroup for every four tokens would be 2^32 threads, which no launch takes."""
+    t = 2**26
+    x = torch.randn(1, 4096, 1, 64, device=DEV).bfloat16().repeat(1, t // 4096, 1, 1)
+    q, k = qk_norm_rope(x, x, rot_dim=64)
+    for a, e in ((0, 300), (t // 2, t // 2 + 300), (t - 300, t)):
+        want, _ = qk_norm_rope(x[:, a:e], x[:, a:e], rot_dim=64, positions=torch.arange(a, e, device=DEV))
+        assert torch.equal(q[:, a:e], want) and torch.equal(k[:, a:e], want)

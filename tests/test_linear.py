@@ -214,3 +214,19 @@ def test_one_padded_row_reaches_the_kernels(launches, monkeypatch):
     a, b = qk_norm_rope(x, x)
     torch.autograd.grad([a, b], [x], [torch.ones_like(a), torch.ones_like(b)])
     assert launches == ["gdn_qk_norm_rope_fwd", "gdn_qk_norm_rope_bwd"]
+
+
+def test_launches_past_2_32_threads_are_refused():
+    """A grid of more threads than 32 bits count is launched with what their number is modulo 2^32: most of the rows would
+    silently stay as they were."""
+    lib = _lib.load()
+    P = 1 << 20
+    for n, hv in ((2**18 + 3, 64), (2**24, 1), (2**18, 64)):
+        assert lib.gdn_decay_attn_recurrent_fwd(P, P, P, None, None, P, None, None, n, 1, hv, hv, 64, 64, n, 1, 0, 0, 0, 0, 1.0, 0,
+                                                None) == _lib.GDN_ERR_UNSUPPORTED, (n, hv)
+    # dq and dk of the value heads that share a head: 1,024 elements a workgroup
+    for t, h, hv in ((2**28, 1, 2), (2**26 + 5, 4, 8)):
+        states = lib.gdn_decay_attn_states_size(1, t, hv, 64, 64, 1, 0)
+        need = lib.gdn_decay_attn_bwd_workspace_size(1, t, h, hv, 64, 64, 1, 0)
+        assert lib.gdn_decay_attn_bwd(P, P, P, None, None, None, P, None, P if states else None, None, 1, t, h, hv, 64, 64, 1, 0, 0,
+                                      0, 0, 1.0, 0, P, P, P, None, None, P, need, None) == _lib.GDN_ERR_UNSUPPORTED, (t, h, hv)
