@@ -18,12 +18,18 @@
 
 namespace gdn {
 
-// Workgroups of the backward, at most: each leaves one row of weight gradient sums. 16 + 16 heads of 128, bf16, with 256,
-// 512 and 1,024 of them: 4,096 tokens 29, 26 and 27 us, 16,384 tokens 90, 73 and 70.
+// Workgroups of the backward, at most: each leaves one row of weight gradient sums, which a second kernel adds. bf16, with
+// 256, 512 and 1,024 of them, both kernels: 16 + 16 heads of 128, 4,096 tokens 31, 28 and 28 us, 16,384 tokens 108, 89 and
+// 86; 1 + 1 heads of 64, 4,096 tokens 13, 11 and 14, 16,384 tokens 32, 22 and 23.
 constexpr int64_t kRopeBwdBlocks = 512;
-// Up to this many tokens the 4 waves of a workgroup share one. Forward of such rows, shared and a wave each: 256 tokens 4.8
-// and 6.4 us, 512 tokens 6.9 and 6.7, 1,024 tokens 10.8 and 7.3.
-constexpr int64_t kRopeShared = 512;
+// Up to this many tokens the 4 waves of a workgroup share one: a workgroup a CU. Shared and a wave each, bf16, us:
+//   heads x D       256 tokens: forward   backward      512 tokens: forward   backward
+//   16 + 16 x 128             4.6, 6.3    9.3, 11.0               6.8, 6.6   11.7, 11.6
+//   16 + 2 x 128              4.5, 5.5    8.8, 9.8                6.3, 5.6   11.2, 10.2
+//   8 + 8 x 256               4.8, 6.4    9.3, 10.9               7.1, 6.7   12.4, 11.7
+//   1 + 1 x 128               4.1, 4.1    8.3, 7.6                5.7, 4.1   10.5, 7.9
+// With few heads three of the waves have no rows, which costs the backward 0.7 us from 128 tokens on.
+constexpr int64_t kRopeShared = 256;
 
 struct QkRopeParams {
   const void* x[2];              // q, k [B, T, heads, D] by strides (elements), last axis contiguous

@@ -230,3 +230,9 @@ def test_launches_past_2_32_threads_are_refused():
         need = lib.gdn_decay_attn_bwd_workspace_size(1, t, h, hv, 64, 64, 1, 0)
         assert lib.gdn_decay_attn_bwd(P, P, P, None, None, None, P, None, P if states else None, None, 1, t, h, hv, 64, 64, 1, 0, 0,
                                       0, 0, 1.0, 0, P, P, P, None, None, P, need, None) == _lib.GDN_ERR_UNSUPPORTED, (t, h, hv)
+
+
+def test_waves_share_a_token_up_to_a_workgroup_a_cu():
+    """The norm's backward leaves a row of sums for each workgroup: one a token up to 256 tokens, then one for four."""
+    size = _lib.load().gdn_qk_norm_rope_bwd_workspace_size
+    assert [size(1, t, 64) // (2 * 64 * 4) for t in (1, 256, 257, 512, 2048, 4096)] == [1, 256, 65, 128, 512, 512]
