@@ -921,7 +921,6 @@ __global__ __launch_bounds__(256) void gated_deltaless_finish_kernel(LinParams p
   for (int n = last - w; n >= first; n -= 4) {
     const int bos = seq_start(p, n), eos = seq_start(p, n + 1);
     const int lo = bos > seg0 ? bos : seg0, hi = eos < seg1 ? eos : seg1;
-    if (lo >= hi) continue;
     double sum = 0.;
     if (eos > seg1) sum = border;
     else if (a.fin && a.dfin) {
