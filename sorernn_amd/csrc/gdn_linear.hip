@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256) void gated_deltaless_scan_kernel(LinParams p, 
 // ------------------------------------------------------------------------------------------------
 // The walk. One workgroup a CU: waves 0-3 hold the state and make the outputs of chunk c, waves 4-7 meanwhile bring the
 // tiles of chunks c + 1 and c + 2 into LDS and make the scores of chunk c + 1; one barrier a chunk. At 4 x 4,096 tokens,
-// 16 heads of 128, 78 us; its loads and stores alone take 59, the state's waves alone 64. With eight waves for the state the
+// 16 heads of 128, 79 us; its loads and stores alone take 59, the state's waves alone 64. With eight waves for the state the
 // scores' waves are what a chunk waits for: 80 us.
 // DOT 1 also gives e_i . (the state's share of o_i) for every token; DOT 2 adds the scores' share, the row sums less the
 // column sums of W_ij = P_ij (e_i . v_j), exact bf16 products summed in fp32.

@@ -4,7 +4,7 @@
 //   lo = y[0 : rot / 2], hi = y[rot / 2 : rot], c, s = cos, sin(position theta^(-2f / rot)), f = 0 .. rot / 2 - 1
 //
 // fp32 throughout, one rounding at the end. Bound by the bytes of the rows: 16,384 tokens of 16 + 16 heads of 128 in bf16 take
-// 62 us forward and 90 backward from memory, 4.3 and 4.5 TB/s. A wave takes a token (with few tokens a
+// 62 us forward and 92 backward as slices of a projection in memory, 4.3 and 4.4 TB/s. A wave takes a token (with few tokens a
 // workgroup's 4 waves share one) and its heads D / 8 lanes each; a lane holds two pieces of 4 elements that turn with one
 // another, so that nothing is exchanged between lanes but the sum of squares. Angles are taken in turns in 64 bits,
 // position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.

@@ -223,7 +223,12 @@ def chunk_decay_linear_attention(q: Tensor, k: Tensor, v: Tensor, g: Tensor | No
     ``cu_seqlens`` (``[N+1]``, needs ``B == 1``) the state restarts at every document; ``cu_seqlens_cpu`` lets the bounds
     be checked without a device sync. Differentiable in q, k, v, g and initial_state. Decays may exceed 1; weights past
     fp32's range (``exp`` of the sum of g over a sequence) are infinite. An infinity or NaN in a token reaches that token
-    and those after it (in the backward, the gradients of those before it), not the others.
+    and those after it (in the backward, the gradients of those before it), not the others. The gradient of g is a sum
+    over the tokens from there on, rounded as such: next to 0, where a decay leaves nothing of the state, it is noise of
+    about 1e-6 of the terms.
+
+    Replayed and compiled calls take ``cu_seqlens`` unchecked, in ascending order: a document may be empty (its state goes
+    through), and tokens before the first or behind the last have zeros in ``o`` and in the gradients.
 
     fp32 and fp16 q/k/v run on the recurrent kernel, forward only (a ``RuntimeWarning`` says so once per dtype).
     """
