@@ -5,7 +5,7 @@ Error bounds: those of tests/test_gpu_linear.py.
 import pytest
 import torch
 
-from sorernn_amd import fused_recurrent_decay_linear_attention, linear
+from sorernn_amd import chunk_decay_linear_attention, fused_recurrent_decay_linear_attention, linear
 from tests.linear_ref import check, decay_attention
 from tests.test_gpu_linear import DEV, GATE, OUT, STATE, _block, _block_params, _inputs
 
@@ -96,13 +96,12 @@ def test_gradients_of_loose_tokens_are_zero(t, bounds, heads, unwritten_is_nan):
 def test_graph_of_a_training_step_with_loose_tokens(unwritten_is_nan):
     """Captured with whole bounds and replayed with padded ones, over memory full of NaN: the outputs of tokens in no
     document are zero, and the parameters' gradients those of the documents alone."""
-    t, p = 700, _block_params(2)
+    t, params = 700, _block_params(2)
     gen = torch.Generator(DEV).manual_seed(5)
     x, up = (torch.randn(1, t, 192, generator=gen, device=DEV).bfloat16() for _ in range(2))
-    for w in p.values():
-        w.requires_grad_(True)
 
     def step(x, up, cu, host):
+        p = {n: w.detach().requires_grad_(True) for n, w in params.items()}  # leaves of this step's stream
         y, s = _block(x, p, cu, host)
         with torch.no_grad():  # the rows of the recurrent form too
             q = torch.ones(1, x.shape[1], 1, 64, device=DEV, dtype=x.dtype)
@@ -130,7 +129,34 @@ def test_graph_of_a_training_step_with_loose_tokens(unwritten_is_nan):
         a, e = bounds[0], bounds[-1]
         alone = sorted({b - a for b in bounds})
         want = step(x[:, a:e], up[:, a:e], torch.tensor(alone, device=DEV), torch.tensor(alone))
-        for name, g, w in zip(p, outs[3:], want[3:]):
+        for name, g, w in zip(params, outs[3:], want[3:]):
             assert torch.isfinite(g).all(), name
             if name in ("w", "wo"):  # a few roundings to bf16 on the way, each of half a step at most
                 assert (g.double() - w.double()).norm() <= 8 * 2.0**-8 * w.double().norm(), name
+
+
+def test_compiled_call_with_loose_tokens(unwritten_is_nan):
+    """A compiled function does not read the bounds: padded ones give what a replay gives."""
+    def f(q, k, v, g, h0, cu):
+        return chunk_decay_linear_attention(q, k, v, g, 0.1, h0, True, cu)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(f, fullgraph=True, backend="aot_eager")
+    t, bounds = 700, [64, 64, 300, 650, 650]
+    x = _inputs(1, t, 1, 2, 64, 128, "token", True, [100, 100, 100, 400], seed=23, train=True)
+    leaves = [x[m].requires_grad_(True) for m in ("q", "k", "v", "g", "h0")]
+    o, s = compiled(*leaves, torch.tensor(bounds, device=DEV))
+    grads = torch.autograd.grad([o, s], leaves, [x["do"], x["dht"]])
+    loose = _loose(t, bounds)
+    for y in (o, *grads[:4]):
+        assert torch.isfinite(y).all() and not y[:, loose].any()
+    with torch.no_grad():
+        for n in (0, 3):
+            assert torch.equal(s[n], x["h0"][n]) and torch.equal(grads[4][n], x["dht"][n])
+        for n, (a, e) in ((1, (64, 300)), (2, (300, 650))):
+            part = [x[m][:, a:e] for m in ("q", "k", "v", "g")]
+            ref = decay_attention(*part, 0.1, x["h0"][n:n + 1], None, x["do"][:, a:e], x["dht"][n:n + 1])
+            check(o[:, a:e], ref, "o", OUT)
+            for name, y in zip(("dq", "dk", "dv", "dg"), grads):
+                check(y[:, a:e], ref, name, GATE if name == "dg" else OUT)
+    torch._dynamo.reset()
