@@ -47,7 +47,7 @@ extern "C" {
 #define GDN_FLAG_BETA_SIGMOID 0x2u /* beta holds logits: use sigmoid(beta) */
 #define GDN_FLAG_GATE_IN_KERNEL 0x4u /* g holds a: use g = -exp(A_log[h]) * softplus(a + dt_bias[h]) */
 #define GDN_FLAG_CU_INT32 0x8u /* cu_seqlens is int32 (default int64) */
-#define GDN_FLAG_ZERO_REST 0x10u /* zeros in the rows of o whose tokens lie outside cu_seqlens (default: left as they are) */
+#define GDN_FLAG_ZERO_REST 0x10u /* gdn_decay_attn_*: zeros in the rows of o of tokens outside cu_seqlens (default: left) */
 
 /* activation codes for the conv and the gated norm */
 #define GDN_ACT_NONE 0
@@ -373,8 +373,8 @@ GDN_API size_t gdn_decay_attn_states_size(int64_t B, int64_t T, int64_t HV, int6
 /*
  * Backward of gdn_decay_attn_fwd: its inputs and the states it left, d_o [B,T,HV,V] bf16, d_final_state or NULL (zero).
  * dq, dk [B,T,H,K] and dv [B,T,HV,V] bf16; dg [B,T,HV] contiguous in g_dtype or NULL (not wanted); d_initial_state or
- * NULL. Rows of tokens outside cu_seqlens are zero. final_state (the forward's) is read for dg where d_final_state is given. workspace:
- * gdn_decay_attn_bwd_workspace_size bytes.
+ * NULL. Rows of tokens outside cu_seqlens are zero. final_state (the forward's) is read for dg where d_final_state is
+ * given. workspace: gdn_decay_attn_bwd_workspace_size bytes.
  */
 GDN_API int gdn_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const float* initial_state,
                                const float* final_state, const void* d_o, const float* d_final_state,
@@ -390,7 +390,8 @@ GDN_API size_t gdn_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H
 
 /*
  * The recurrence of gdn_decay_attn_fwd token by token in fp32, q, k, v, o in qkv_dtype: the step of single tokens.
- * The same flags. final_state may equal initial_state (in-place update). g and its strides as there, without the bound of -100.
+ * The same flags. final_state may equal initial_state (in-place update). g and its strides as there, without the bound
+ * of -100.
  */
 GDN_API int gdn_decay_attn_recurrent_fwd(const void* q, const void* k, const void* v, const void* g,
                                          const float* initial_state, void* o, float* final_state,

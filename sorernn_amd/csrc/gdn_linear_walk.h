@@ -1,4 +1,5 @@
 // Which tokens a workgroup of the decay linear attention walks, in chunks: index arithmetic only, the same on the host.
+// Included after the definitions of load_index, uniform and starts_up_to.
 //
 // P has cu, cu_i32, T, N and tokens. starts_up_to(p, lo, hi, step, t) counts the lanes i of a wave with
 // lo + i step < hi and start of sequence lo + i step <= t.
