@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 9
+#define GDN_ABI_VERSION 10
 
 #if defined(__GNUC__) || defined(__clang__)
 #define GDN_API __attribute__((visibility("default")))
@@ -431,6 +431,86 @@ GDN_API int gdn_qk_norm_rope_bwd(const void* q, int64_t q_batch_stride, int64_t 
 
 /* Workspace bytes gdn_qk_norm_rope_bwd needs (0 for invalid sizes). */
 GDN_API size_t gdn_qk_norm_rope_bwd_workspace_size(int64_t B, int64_t T, int64_t D);
+
+/*
+ * Causal attention with a sliding window and sinks over whole sequences: token i of a sequence sees token j <= i if
+ * i - j < window or j < sinks; o = softmax(scale q k^T) v, q head i reading kv head i / (HQ / HKV). q [B, T, HQ, D],
+ * k, v [B, T, HKV, D] in dtype (bf16 or fp16) by element strides (the last axis contiguous; multiples of 8 elements, tensors
+ * 16-byte aligned, at most 2^23 elements between tokens); o [B, T, HQ, D] contiguous; lse [HQ, B T] fp32 or NULL (log2 of a
+ * row's sum of 2^(scale log2(e) q.k); infinity for a row that sees nothing), which the backward reads. window 0: none.
+ * cu_seqlens ascends (empty sequences allowed); rows of tokens in no sequence are zero. D = 64 or 128, T < 2^28.
+ */
+GDN_API int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                void* o, float* lse, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
+                                int64_t D, int64_t N, int dtype, int64_t window, int64_t sinks, float scale, unsigned flags,
+                                void* stream);
+
+/*
+ * Backward of gdn_window_attn_fwd in bf16: its inputs, o and lse, and d_o [B, T, HQ, D] contiguous, into contiguous dq
+ * [B, T, HQ, D], dk, dv [B, T, HKV, D]. Rows of tokens in no sequence are zero. workspace:
+ * gdn_window_attn_bwd_workspace_size bytes, 16-byte aligned.
+ */
+GDN_API int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                const void* o, const float* lse, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
+                                int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t window, int64_t sinks, float scale,
+                                unsigned flags, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* Workspace bytes gdn_window_attn_bwd needs (0 for invalid sizes). */
+GDN_API size_t gdn_window_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                                                  int64_t window, int64_t sinks, int varlen);
+
+/*
+ * A paged cache of keys and values [pages, HKV, page_size, D] by strides (pages, heads, tokens; the last axis contiguous).
+ * Token s of sequence n lies at row s % page_size of page page_table[n * table_stride + s / page_size] (int32, width numbers
+ * a row). lengths [N] int64 (int32 with lengths_i32): a sequence's tokens in the cache with the call's new ones counted; new
+ * token t of T_n is at place lengths[n] - T_n + t. Page numbers outside [0, pages), places below 0 and lengths over
+ * width * page_size are safe: such tokens are not written and not seen. page_size a power of two from 16 to 65536; D 64 or
+ * 128; bf16 or fp16.
+ *
+ * gdn_paged_append: k and v [B, T, HKV, D] by element strides into their places, k normed (k_weight [D] fp32, NULL: not) and
+ * rotated over its first rot_dim entries (element f with f + rot_dim / 2, angle position * theta^(-2f / rot_dim)) on the way;
+ * and q [B, T, HQ, D] (or NULL) likewise into q_out, contiguous. fp32 inside, one rounding. positions: [B, T] int64 (int32
+ * with pos_i32) by strides, or NULL: the tokens' places. With cu_seqlens (B == 1) N sequences of uneven lengths; rows of q_out
+ * of tokens in none are zero. No two new tokens may have one place.
+ */
+GDN_API int gdn_paged_append(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                             const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                             const float* q_weight, const float* k_weight, void* q_out, void* k_cache, int64_t kc_page_stride,
+                             int64_t kc_head_stride, int64_t kc_token_stride, void* v_cache, int64_t vc_page_stride,
+                             int64_t vc_head_stride, int64_t vc_token_stride, const int32_t* page_table,
+                             int64_t table_stride, const void* lengths, int lengths_i32, const void* positions,
+                             int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, const void* cu_seqlens,
+                             int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t pages,
+                             int64_t page_size, int64_t width, int dtype, int rot_dim, double theta, float eps,
+                             unsigned flags, void* stream);
+
+/*
+ * Attention of the call's new tokens over the cache that holds their keys and values too: q [B, T, HQ, D] by strides, o
+ * contiguous. A token at place i sees place j <= i if i - j < window (0: none) or j < sinks. tree: [B, T] by strides, T_n at
+ * most 64, or NULL: bit t of a token's word says that it sees the sequence's new token t; the tokens before the new ones are
+ * then seen from place lengths[n] - T_n + (bits set) - 1. Rows that see nothing are zero. workspace:
+ * gdn_paged_attn_workspace_size bytes, 16-byte aligned (0: may be NULL), contents irrelevant; calls that share it must not
+ * overlap.
+ */
+GDN_API int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k_cache, int64_t kc_page_stride, int64_t kc_head_stride, int64_t kc_token_stride,
+                               const void* v_cache, int64_t vc_page_stride, int64_t vc_head_stride, int64_t vc_token_stride,
+                               const int32_t* page_table, int64_t table_stride, const void* lengths, int lengths_i32,
+                               const int64_t* tree, int64_t tree_batch_stride, int64_t tree_token_stride, void* o,
+                               const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                               int64_t pages, int64_t page_size, int64_t width, int dtype, int64_t window, int64_t sinks,
+                               float scale, unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes gdn_paged_attn_fwd needs (0 for invalid sizes, or where none is). */
+GDN_API size_t gdn_paged_attn_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                                             int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen,
+                                             int tree);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,8 @@ from sorernn_amd.linear import (  # noqa: F401
     fused_recurrent_decay_linear_attention,
     qk_norm_rope,
 )
+from sorernn_amd.paged import paged_attention, paged_kv_append  # noqa: F401
+from sorernn_amd.window import window_attention  # noqa: F401
 from sorernn_amd.range_guard import check_chunk_range, range_guard, set_range_guard  # noqa: F401
 
 __version__ = "0.1.0"

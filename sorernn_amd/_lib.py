@@ -22,7 +22,7 @@ FLAG_GATE_IN_KERNEL = 0x4
 FLAG_CU_INT32 = 0x8
 FLAG_ZERO_REST = 0x10
 ACT_NONE, ACT_SILU, ACT_SILU_ROUNDED = 0, 1, 2
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -72,6 +72,14 @@ SIGNATURES = {
     "gdn_qk_norm_rope_bwd": ([_P] + [_I64] * 3) * 2 + [_P] * 3 + [_I64] * 2 + [_INT] + [_P] * 7 + [_I64] * 6
     + [_INT, _INT, _D, _F, _U, _P, _SZ, _P],
     "gdn_qk_norm_rope_bwd_workspace_size": [_I64] * 3,
+    "gdn_window_attn_fwd": ([_P] + [_I64] * 3) * 3 + [_P] * 3 + [_I64] * 6 + [_INT] + [_I64] * 2 + [_F, _U, _P],
+    "gdn_window_attn_bwd": ([_P] + [_I64] * 3) * 3 + [_P] * 4 + [_I64] * 8 + [_F, _U] + [_P] * 4 + [_SZ, _P],
+    "gdn_window_attn_bwd_workspace_size": [_I64] * 8 + [_INT],
+    "gdn_paged_append": ([_P] + [_I64] * 3) * 3 + [_P] * 3 + ([_P] + [_I64] * 3) * 2 + [_P, _I64, _P, _INT, _P, _I64, _I64, _INT]
+    + [_P] + [_I64] * 9 + [_INT, _INT, _D, _F, _U, _P],
+    "gdn_paged_attn_fwd": ([_P] + [_I64] * 3) * 3 + [_P, _I64, _P, _INT, _P, _I64, _I64, _P, _P] + [_I64] * 9 + [_INT]
+    + [_I64] * 2 + [_F, _U, _P, _SZ, _P],
+    "gdn_paged_attn_workspace_size": [_I64] * 10 + [_INT] * 2,
 }
 
 RESTYPES = {
@@ -86,6 +94,8 @@ RESTYPES = {
     "gdn_decay_attn_states_size": ctypes.c_size_t,
     "gdn_decay_attn_bwd_workspace_size": ctypes.c_size_t,
     "gdn_qk_norm_rope_bwd_workspace_size": ctypes.c_size_t,
+    "gdn_window_attn_bwd_workspace_size": ctypes.c_size_t,
+    "gdn_paged_attn_workspace_size": ctypes.c_size_t,
 }
 
 _lib = None

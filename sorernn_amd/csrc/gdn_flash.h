@@ -1,0 +1,529 @@
+// What the attention kernels with a window and sinks share (gdn_window.hip: whole sequences with their backward;
+// gdn_paged.hip: a paged cache): which keys a query sees, the walk of sequences in tiles, tiles of rows in LDS, the
+// softmax of a block, and the rows that are computed one by one where infinities or NaN lie in places they must not see.
+//
+//   A query at place i of its sequence sees key j iff j <= i and (i - j < window or j < sinks).
+//
+// v_mfma_f32_32x32x16 layouts (lane = 32 hh + li): A lane holds row li, k = 8 hh .. 8 hh + 7; B lane column li, same k;
+// the accumulator's element e of a lane is column li, row 8 (e / 4) + 4 hh + e % 4.
+#pragma once
+
+#include "gdn_mfma.h"
+
+namespace gdn {
+
+template <typename E> struct Pack;
+template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; };
+template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; };
+
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kFar = 1 << 29;  // no window; also the bound on a sequence's length, so that places and their differences fit 32 bits
+constexpr int64_t kMaxRowBytes = 1 << 24;  // bytes between two tokens of an operand read through 32-bit offsets inside a block
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int imin(int a, int b) { return a < b ? a : b; }
+__device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int s = 1; s < kWave; s <<= 1) x = fmaxf(x, __shfl_xor(x, s, kWave));
+  return x;
+}
+
+// ------------------------------------------------------------------------------------------------ sequences in tiles
+// Tokens of a packed axis, cut where a sequence ends: N sequences and, for bounds that nobody checked, the tokens before
+// the first and behind the last as sequences 0 and N + 1 that see nothing. Bounds are taken as between 0 and T: whatever they
+// hold, no token outside is touched.
+struct Packed {
+  const void* cu;
+  int cu_i32;
+  int64_t N, T;
+  __device__ __forceinline__ int64_t bound(int64_t j) const {
+    if (j <= 0) return 0;
+    if (j > N + 1) return T;
+    const int64_t x = load_index(cu, cu_i32, j - 1);
+    return x < 0 ? 0 : x > T ? T : x;
+  }
+};
+
+// Tile `t` of rows of the sequences, `mul` rows a token and M rows a tile. A sequence from row b0 to row b1 has the tiles
+// b0 / M + j to b1 / M + j of the list, j its number: as many as it can need, without a scan of the lengths. One wave reads
+// 64 bounds at a time.
+struct Seq {
+  int64_t row;   // the batch row
+  int64_t start; // first token inside it
+  int len;       // tokens
+  int num;       // number of the sequence, -1: tokens that belong to none
+  int tile;      // tile of the sequence
+};
+__device__ __forceinline__ Seq packed_tile(const Packed& s, int64_t t, int mul, int M) {
+  const int lane = threadIdx.x % kWave;
+  int64_t count = 0;
+  for (int64_t base = 0; base < s.N + 2; base += kWave) {
+    const int64_t j = base + lane;
+    const uint64_t below = __ballot(j < s.N + 2 && s.bound(j) * mul / M + j <= t);
+    count += __popcll(below);
+    if (below != ~0ull) break;
+  }
+  const int64_t j = uniform64(count > 0 ? count - 1 : 0);
+  const int64_t b0 = uniform64(s.bound(j)), b1 = uniform64(s.bound(j + 1));
+  Seq r;
+  r.row = 0;
+  r.start = b0;
+  r.len = (int)(b1 > b0 ? b1 - b0 : 0);
+  r.num = j == 0 || j == s.N + 1 ? -1 : (int)(j - 1);
+  const int64_t tile = t - (b0 * mul / M + j);
+  r.tile = tile < 0 || tile > kFar ? kFar / M : (int)tile;
+  return r;
+}
+inline int64_t packed_tiles(int64_t T, int64_t N, int mul, int M) { return T * mul / M + N + 2; }
+
+// Workgroup `idx` of a flat grid as (kv head, q head of it, tile). Workgroup i runs on XCD i % 8: the q heads of one kv head
+// and neighbouring tiles share an XCD and its L2 as far as the heads divide over the eight; the tiles are dealt out in turn
+// among the `parts` XCDs that share a head.
+struct Job {
+  int hkv, hm;
+  int64_t tile;
+};
+__device__ __forceinline__ bool job_of(int64_t idx, int hkv, int rep, int parts, int64_t tiles, Job& job) {
+  const int x = (int)(idx & 7), per = hkv * parts / 8 * rep;
+  const int64_t j = idx >> 3, rank = j / per;
+  const int m = (int)(j - rank * per), vg = x + 8 * (m / rep);
+  job.hm = m % rep;
+  job.hkv = vg % hkv;
+  job.tile = rank * parts + vg / hkv;
+  return job.tile < tiles;
+}
+inline int job_parts(int64_t hkv) { return hkv % 8 == 0 ? 1 : hkv % 4 == 0 ? 2 : hkv % 2 == 0 ? 4 : 8; }
+inline int64_t job_groups(int64_t hkv, int64_t rep, int64_t tiles) {
+  const int64_t parts = job_parts(hkv);
+  return hkv * parts * rep * ((tiles + parts - 1) / parts);
+}
+
+// The blocks of BK keys that queries at places first .. last see: those with sinks before the window's, then the window's.
+struct Blocks {
+  int sinks, from, count;  // block n is n < sinks ? n : n - sinks + from
+  __device__ __forceinline__ int at(int n) const { return n < sinks ? n : n - sinks + from; }
+};
+template <int BK>
+__device__ __forceinline__ Blocks blocks_of(int first, int last, int window, int sinks) {
+  Blocks b;
+  const int lo = imax(0, first - window + 1);
+  b.from = lo / BK;
+  b.sinks = imin((sinks + BK - 1) / BK, b.from);
+  const int end = last >= 0 ? last / BK + 1 : 0;
+  b.count = imax(0, b.sinks + end - b.from);
+  return b;
+}
+
+__device__ __forceinline__ bool sees(int q, int k, int window, int sinks) { return k <= q && (q - k < window || k < sinks); }
+// of keys k0 .. k1 and queries q0 .. q1: all see all; none sees any
+__device__ __forceinline__ bool all_see(int q0, int q1, int k0, int k1, int window, int sinks) {
+  return k1 <= q0 && (q1 - k0 < window || k1 < sinks);
+}
+__device__ __forceinline__ bool none_sees(int q0, int q1, int k0, int k1, int window, int sinks) {
+  return k0 > q1 || (q0 - k1 >= window && k0 >= sinks);
+}
+
+// ------------------------------------------------------------------------------------------------ tiles in LDS
+// Rows of D elements lie unpadded (a load straight into LDS fills 1 KB contiguously); the 16-byte chunk c of row r is stored
+// at chunk c ^ swz(r), which keeps both the row fragments' and the transposed reads free of bank conflicts.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : (((r & 3) << 1) | ((r >> 2) & 1));
+}
+
+template <int D>
+struct TileReads {
+  int row[D / 16];     // row fragments: row li, chunk 2 st + hh; + 32 D for the next 32 rows
+  int tr[D / 32][2];   // transposed: rows 4 hh + m (+ 8), 32 columns from 32 d; + 16 D for the next 16 rows
+  __device__ __forceinline__ void init(int lane) {
+    const int hh = lane >> 5, li = lane & 31, gsub = (lane >> 4) & 1, lm = (lane & 15) >> 2, lq = lane & 3;
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) row[st] = li * D + (((2 * st + hh) ^ swz<D>(li)) << 3);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int h8 = 0; h8 < 2; ++h8) {
+        const int r = 4 * hh + lm + 8 * h8;
+        tr[d][h8] = r * D + (((4 * d + 2 * gsub + (lq >> 1)) ^ swz<D>(r)) << 3) + 4 * (lq & 1);
+      }
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ typename Pack<E>::x8 row_frag(const E* tile, int off) {
+  return *reinterpret_cast<const typename Pack<E>::x8*>(tile + off);
+}
+// A operand of the transposed tile's 16 rows from `rows` (in elements: 16 D per step): lane li holds column 32 d + li, k in the
+// order 4 hh + r, 8 + 4 hh + r, which is the accumulator's own row order
+template <typename E>
+__device__ __forceinline__ typename Pack<E>::x8 tr_frag(const E* tile, const int (&off)[2]) {
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off[0]));
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off[1]));
+  return __builtin_bit_cast(typename Pack<E>::x8, bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+}
+
+// 16 accumulator elements as the two B operands of their 32 rows
+template <typename E>
+__device__ __forceinline__ void pack16(const f32x16& s, typename Pack<E>::x8 (&out)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[h][e] = (E)s[8 * h + e];
+}
+
+// One 16-byte load a lane straight into LDS (lane l's at `to` + 16 l bytes).
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, void* to, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
+
+// ------------------------------------------------------------------------------------------------ softmax
+// Online softmax of KT x 32 keys of the wave's 32 queries (raw scores s, masked ones -inf) and O^T += V^T P^T.
+// p = 2^(s c - m c), c = scale log2(e) > 0. The row's m moves only when a block's maximum exceeds it by more than `slack` =
+// 8 / c: p <= 2^8 meanwhile, which costs no precision, and O^T is rescaled rarely. A row that saw no key yet keeps m = -inf and
+// uses 0. P is rounded to the inputs' type for the product (off by half a step of it a term, as the output itself is); the
+// row sum adds p in fp32, so that the backward's logarithm of it is exact to fp32.
+template <int KT, int D, typename E>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 32], float& m, float& l, float c, float slack,
+                                             const E* vb, const TileReads<D>& rd) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kt][e]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+  const bool grow = mx > m + slack;
+  if (!__all(!grow)) {
+    const float alpha = grow ? __builtin_amdgcn_exp2f((m - mx) * c) : 1.f;  // 0 while no key was seen
+    m = grow ? mx : m;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
+  }
+  const float nmc = m == -INFINITY ? 0.f : -m * c;
+  float sum = 0.f;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[kt][e] = __builtin_amdgcn_exp2f(fmaf(s[kt][e], c, nmc));
+      sum += s[kt][e];
+    }
+  }
+  l += sum;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    typename Pack<E>::x8 pb[2];
+    pack16<E>(s[kt], pb);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] = mma32(tr_frag(vb + (2 * kt + h) * 16 * D, rd.tr[d]), pb[h], acc[d]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows one by one
+// The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
+// reach rows that do not see it. Such a row's result is not finite, so rows with finite results are right, and the others
+// are computed again here, key by key, over the keys that they see. A wave a row; lane l holds columns l and l + 64.
+template <int D, typename E>
+__device__ __forceinline__ float dot_row(const E* a, const E* b) {
+  float x = 0.f;
+  for (int d = 0; d < D; d += 8) {
+    const auto u = *reinterpret_cast<const typename Pack<E>::x8*>(a + d), w = *reinterpret_cast<const typename Pack<E>::x8*>(b + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x += (float)u[e] * (float)w[e];
+  }
+  return x;
+}
+
+// Adds keys [key0, key1) to a row's running maximum, sum and output. key(j): K row j or null (not to be seen); val(j): V row j.
+template <int D, typename E, typename Key, typename Val, typename Seen>
+__device__ __forceinline__ void slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float& m, float& l,
+                                      float (&acc)[D / 64]) {
+  const int lane = threadIdx.x % kWave;
+  for (int base = key0; base < key1; base += kWave) {
+    const int j = base + lane;
+    const E* kr = j < key1 && seen(j) ? key(j) : nullptr;
+    const uint64_t live = __ballot(kr != nullptr);
+    if (!live) continue;
+    const float s = kr ? dot_row<D>(q, kr) : -INFINITY;
+    const float top = fmaxf(m, wave_max(s));
+    const float alpha = top == m ? 1.f : __builtin_amdgcn_exp2f((m - top) * c);
+    m = top;
+    const float p = kr ? __builtin_amdgcn_exp2f(s * c - (m == -INFINITY ? 0.f : m * c)) : 0.f;
+    l = l * alpha + wave_xor_sum(p, 1);
+    for (int i = 0; i < D / 64; ++i) acc[i] *= alpha;
+    for (int n = 0; n < kWave; ++n) {
+      if (!(live >> n & 1)) continue;
+      const float pn = __shfl(p, n, kWave);
+      const E* vr = val(base + n);
+      for (int i = 0; i < D / 64; ++i) acc[i] += pn * (float)vr[lane + 64 * i];
+    }
+  }
+}
+
+__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// whether a lane's accumulators are all finite: 0 x stays 0 unless x is not
+template <int N>
+__device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
+  float z = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z = fmaf(a[n][e], 0.f, z);
+  return z == 0.f;
+}
+
+// ------------------------------------------------------------------------------------------------ forward over whole tiles
+// Strides in elements; k and v of a paged cache: between pages, tokens of a page, heads.
+struct FlashParams {
+  const void *q, *k, *v;
+  int64_t qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh;
+  void* o;       // [B, T, HQ, D]
+  float* lse;    // [HQ, B T] or null: log2 of the sum of 2^(c s)
+  Packed seqs;   // cu null: batch rows of T tokens
+  int64_t B, tiles;
+  int HQ, HKV, parts, window, sinks;
+  float scale_log2;
+  // paged
+  const int* table;
+  int64_t table_stride;
+  const void* lengths;
+  int len_i32, width, shift, pages;
+};
+
+// Entry `at` of a row of a page table, `at` the same in every lane: through the scalar cache, apart from the vector loads that
+// are under way.
+__device__ __forceinline__ int page_at(const int* table, int at) {
+  typedef const __attribute__((address_space(4))) int* Constant;
+  return ((Constant)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(at)];
+}
+
+// the sequence's length in the cache, within what its row of the table can hold
+__device__ __forceinline__ int cache_length(const void* lengths, int i32, int seq, int width, int shift) {
+  const int64_t x = uniform64(load_index(lengths, i32, seq)), most = (int64_t)width << shift;
+  return (int)(x < 0 ? 0 : x > most ? most : x);
+}
+
+constexpr int kBQ = 128;  // queries a workgroup: 32 a wave
+constexpr int kBK = 64;   // keys a block
+
+// O = softmax(scale Q K^T) V over the keys that a query sees. A workgroup of 4 waves takes 128 queries of one head, a wave 32
+// of them in registers; blocks of 64 keys pass through LDS, loaded straight from memory one block ahead. S^T = K Q^T puts one
+// query into each lane's column: maximum, sum and rescaling are a lane's own, and P^T is the next product's operand as it is.
+template <int D, typename E, bool PAGED>
+__device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* Ks1, E* Vs0, E* Vs1) {
+  using X8 = typename Pack<E>::x8;
+  using X4 = typename Pack<E>::x4;
+  constexpr int DS = D / 16, DT = D / 32, CPR = D / 8, RPL = 512 / D, LPT = kBK / (4 * RPL);
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+  const int rep = p.HQ / p.HKV;
+  Job job;
+  if (!job_of(blockIdx.x, p.HKV, rep, p.parts, p.tiles, job)) return;
+  Seq sq;
+  if (p.seqs.cu) {
+    sq = packed_tile(p.seqs, job.tile, 1, kBQ);
+  } else {  // the last tiles, which see most, first
+    const int64_t per = (p.seqs.T + kBQ - 1) / kBQ;
+    sq.row = job.tile % p.B;
+    sq.start = 0;
+    sq.len = (int)p.seqs.T;
+    sq.num = (int)sq.row;
+    sq.tile = (int)(per - 1 - job.tile / p.B);
+  }
+  const int q0 = sq.tile * kBQ, hq = job.hkv * rep + job.hm;
+  if (q0 >= sq.len) return;
+  const int q1 = imin(q0 + kBQ, sq.len) - 1;
+  int klen = sq.num < 0 ? 0 : sq.len, pos0 = 0;
+  const int* table = nullptr;
+  if (PAGED) {
+    klen = sq.num < 0 ? 0 : cache_length(p.lengths, p.len_i32, sq.num, p.width, p.shift);
+    pos0 = klen - sq.len;
+    if (sq.num >= 0) table = p.table + sq.num * p.table_stride;
+  }
+  Blocks bl = blocks_of<kBK>(pos0 + q0, pos0 + q1, p.window, p.sinks);
+  if (sq.num < 0) bl.count = 0;
+
+  const int qr = q0 + 32 * w + li, qi = pos0 + qr;  // the lane's query: row of the sequence, place
+  const int wq0 = pos0 + q0 + 32 * w, wq1 = imin(wq0 + 31, pos0 + q1);
+  const bool wave_live = wq0 <= wq1;
+  const int64_t tok = sq.row * p.seqs.T + sq.start;  // flat number of the sequence's first token
+  const E* qrow = static_cast<const E*>(p.q) + sq.row * p.qsb + (sq.start + imin(qr, sq.len - 1)) * p.qst + hq * p.qsh;
+  X8 qf[DS];
+#pragma unroll
+  for (int s = 0; s < DS; ++s) qf[s] = *reinterpret_cast<const X8*>(qrow + 16 * s + 8 * hh);
+
+  // load u of wave w fills LDS bytes [(w + 4u) KB, + 1 KB) of a block: rows (w + 4u) RPL + lane / CPR. The lane's chunk does not
+  // depend on u.
+  const char* const kbase = reinterpret_cast<const char*>(static_cast<const E*>(p.k) + (PAGED ? 0 : sq.row * p.ksb + sq.start * p.kst) + job.hkv * p.ksh);
+  const char* const vbase = reinterpret_cast<const char*>(static_cast<const E*>(p.v) + (PAGED ? 0 : sq.row * p.vsb + sq.start * p.vst) + job.hkv * p.vsh);
+  const int kst = (int)p.kst * 2, vst = (int)p.vst * 2;  // bytes
+  const int drow = w * RPL + lane / CPR, dch = (lane % CPR) ^ swz<D>(drow);
+  const int grow = PAGED ? drow & 15 : drow;  // paged: the row inside its 16 keys, which share a page
+  const uint32_t koff = (uint32_t)(grow * kst + dch * 16), voff = (uint32_t)(grow * vst + dch * 16);
+  int pid[4];  // paged: pages of a block's four groups of 16 keys, -1: none
+  auto look_up = [&](int jb) {
+    if (!PAGED) return;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int key = jb * kBK + 16 * g, at = key >> p.shift;
+      const int id = key < klen ? page_at(table, at) : -1;
+      pid[g] = id >= 0 && id < p.pages ? id : -1;
+    }
+  };
+  auto ok_bits = [&]() {
+    int b = 15;
+    if (PAGED) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (pid[g] < 0) b &= ~(1 << g);
+    }
+    return b;
+  };
+  auto fetch = [&](int jb, E* kd, E* vd) {
+    const int key0 = jb * kBK;
+    if (PAGED) {
+#pragma unroll
+      for (int u = 0; u < LPT; ++u) {
+        const int g = D == 128 ? u : 2 * u + (w >> 1), id = D == 128 ? pid[u] : (w >> 1) ? pid[2 * u + 1] : pid[2 * u];
+        const int key = key0 + 16 * g, rows = imin(16, klen - key), in = key & ((1 << p.shift) - 1);
+        const int64_t page = id < 0 ? 0 : id;
+        const auto rk = make_rsrc(kbase + page * p.ksb * 2 + (int64_t)in * kst, id < 0 || rows <= 0 ? 0u : (uint32_t)((rows - 1) * kst + 2 * D));
+        const auto rv = make_rsrc(vbase + page * p.vsb * 2 + (int64_t)in * vst, id < 0 || rows <= 0 ? 0u : (uint32_t)((rows - 1) * vst + 2 * D));
+        load_lds16(rk, kd + (w + 4 * u) * 512, koff);
+        load_lds16(rv, vd + (w + 4 * u) * 512, voff);
+      }
+    } else {
+      const int rows = imin(kBK, klen - key0);
+      const auto rk = make_rsrc(kbase + (int64_t)key0 * kst, (uint32_t)((rows - 1) * kst + 2 * D));
+      const auto rv = make_rsrc(vbase + (int64_t)key0 * vst, (uint32_t)((rows - 1) * vst + 2 * D));
+#pragma unroll
+      for (int u = 0; u < LPT; ++u) {
+        load_lds16(rk, kd + (w + 4 * u) * 512, koff + u * 4 * RPL * kst);
+        load_lds16(rv, vd + (w + 4 * u) * 512, voff + u * 4 * RPL * vst);
+      }
+    }
+  };
+  // rows of a block behind the sequence's end or on no page: zeros among the values (their weight is 0, and 0 times whatever
+  // lies there has to be 0). The wave's own loads have landed.
+  auto clean = [&](int jb, int ok, E* vd) {
+    if ((jb + 1) * kBK <= klen && ok == 15) return;
+#pragma unroll
+    for (int u = 0; u < LPT; ++u) {
+      const int row = (w + 4 * u) * RPL + lane / CPR;
+      if (jb * kBK + row >= klen || !(ok >> (row >> 4) & 1)) *reinterpret_cast<X8*>(vd + (w + 4 * u) * 512 + lane * 8) = X8{};
+    }
+  };
+
+  TileReads<D> rd;
+  rd.init(lane);
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale_log2, slack = 8.f / c;
+
+  auto block = [&](bool masked, int ok, const E* kb, const E* vb, int k0) {
+    f32x16 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = f32x16{};
+#pragma unroll
+      for (int st = 0; st < DS; ++st) s[kt] = mma32(row_frag(kb + 32 * kt * D, rd.row[st]), qf[st], s[kt]);
+    }
+    if (masked) {
+      const int hi = qi - k0, lo = qi - p.window - k0, sk = p.sinks - k0;  // seen: <= hi and (> lo or < sk)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
+          if (ko > hi || (ko <= lo && ko >= sk) || (PAGED && !(ok >> (2 * kt + (e >> 3)) & 1))) s[kt][e] = -INFINITY;
+        }
+    }
+    softmax_step<2, D, E>(s, acc, m, l, c, slack, vb, rd);
+  };
+  int ok = 15, ok_next = 15;  // of the block being used and of the one being loaded
+  auto step = [&](int n, const E* kc, const E* vc, E* kn, E* vn) {
+    const int jb = bl.at(n), next = bl.at(n + 1);
+    const bool more = n + 1 < bl.count;
+    if (more) {
+      ok_next = ok_bits();
+      fetch(next, kn, vn);
+      if (n + 2 < bl.count) look_up(bl.at(n + 2));
+    }
+    const int k0 = jb * kBK, k1 = k0 + kBK - 1;
+    if (wave_live && !none_sees(wq0, wq1, k0, k1, p.window, p.sinks))
+      block(ok != 15 || !all_see(wq0, wq1, k0, k1, p.window, p.sinks), ok, kc, vc, k0);
+    wait_loads();
+    if (more) clean(next, ok_next, vn);
+    ok = ok_next;
+    __syncthreads();
+  };
+  if (bl.count > 0) {
+    look_up(bl.at(0));
+    ok = ok_bits();
+    fetch(bl.at(0), Ks0, Vs0);
+    if (bl.count > 1) look_up(bl.at(1));
+    wait_loads();
+    clean(bl.at(0), ok, Vs0);
+    __syncthreads();
+    for (int n = 0; n < bl.count; n += 2) {
+      step(n, Ks0, Vs0, Ks1, Vs1);
+      if (n + 1 < bl.count) step(n + 1, Ks1, Vs1, Ks0, Vs0);
+    }
+  }
+
+  // O = O^T / l; the lane holds its query's columns 32 d + 8 j + 4 hh + r
+  l += __shfl_xor(l, 32, kWave);
+  const bool row_ok = qr < sq.len && wave_live;
+  bool fine = finite_all(acc) && finite_f(l);
+  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  E* orow = static_cast<E*>(p.o) + ((tok + qr) * p.HQ + hq) * D;
+  if (row_ok && fine) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        X4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = (E)(acc[d][4 * j + r] * inv);
+        *reinterpret_cast<X4*>(orow + 32 * d + 8 * j + 4 * hh) = x;
+      }
+    if (p.lse && hh == 0) p.lse[hq * p.B * p.seqs.T + tok + qr] = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : INFINITY;
+  }
+  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
+  while (redo) {
+    const int n = __ffsll((unsigned long long)redo) - 1;
+    redo &= redo - 1;
+    const int r = q0 + 32 * w + n, place = pos0 + r;
+    const E* qp = static_cast<const E*>(p.q) + sq.row * p.qsb + (sq.start + r) * p.qst + hq * p.qsh;
+    auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
+      if (!PAGED) return reinterpret_cast<const E*>(base + j * row_bytes);
+      const int id = table[j >> p.shift];
+      return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
+                                     : reinterpret_cast<const E*>(base + id * page_bytes + (j & ((1 << p.shift) - 1)) * row_bytes);
+    };
+    float mr = -INFINITY, lr = 0.f, a[D / 64] = {};
+    slow_row<D, E>(qp, 0, place + 1, [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
+                   [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); },
+                   [&](int j) { return sees(place, j, p.window, p.sinks); }, c, mr, lr, a);
+    E* to = static_cast<E*>(p.o) + ((tok + r) * p.HQ + hq) * D;
+    for (int i = 0; i < D / 64; ++i) to[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+    if (p.lse && lane == 0) p.lse[hq * p.B * p.seqs.T + tok + r] = lr == 0.f ? INFINITY : mr * c + __builtin_amdgcn_logf(lr);
+  }
+}
+
+}  // namespace gdn

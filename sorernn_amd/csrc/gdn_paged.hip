@@ -1,0 +1,700 @@
+// A paged cache of keys and values: new tokens' rows normed, rotated and put into their pages, and the attention that reads
+// them: single tokens, pieces of a prompt, and trees of drafted tokens, causal at the cache's end, with a window and sinks.
+//
+//   cache [pages, HKV, page, D]; token s of sequence n lies at row s % page of page table[n][s / page]
+//   lengths[n]: the sequence's tokens with the T_n new ones counted: new token t is at place lengths[n] - T_n + t
+//
+// Nothing that the table, the lengths or the bounds hold leads outside the tensors: a page number that is none is read as
+// keys that nobody sees and is not written, a length as at most what a row of the table can hold.
+
+#include <math.h>
+
+#include <type_traits>
+
+#include "gdn_flash.h"
+
+namespace gdn {
+
+// ------------------------------------------------------------------------------------------------ append
+// k' = rotate(norm(k)) and v into their places, q' = rotate(norm(q)) beside them, fp32 with one rounding. Bound by the rows'
+// bytes, or by the launch where tokens are few. A wave takes a token (with few tokens four share one) and its heads D / 8 lanes
+// each; a lane holds two pieces of 4 elements that turn with one another. Angles are taken in turns in 64 bits,
+// position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.
+struct AppendParams {
+  const void* x[3];                // q (or null), k, v [B, T, heads, D] by strides (elements)
+  int64_t sb[3], st[3], sh[3];
+  const float* w[2];               // RMSNorm weights of q, k [D], null: not normed
+  void* q_out;                     // [B, T, HQ, D]
+  void* cache[2];                  // k, v
+  int64_t cp[2], ch[2], ct[2];     // strides between pages, heads, tokens (elements)
+  const int* table;
+  int64_t table_stride;
+  const void *lengths, *pos;       // pos: rotation's positions [B, T] by strides, or null: the tokens' places
+  int64_t pb, pt;
+  const void* cu;
+  int len_i32, pos_i32, cu_i32, width, shift, pages;
+  int64_t T, N, tokens;
+  int HQ, HKV, rot, wpt;           // HQ 0 without q; wpt: waves that share a token
+  float eps;
+  double turns[64];                // theta^(-2f / rot) / 2 pi
+};
+
+// Up to this many tokens the 4 waves of a workgroup share one.
+constexpr int64_t kAppendShared = 256;
+
+template <int D, typename E>
+__global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendParams p) {
+  constexpr int LPR = D / 8, RPW = kWave / LPR, U = 4;  // lanes a row, rows a pass, passes in flight
+  using X4 = typename Pack<E>::x4;
+  __shared__ __align__(16) float tab[4][2][D / 2];
+  const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int li = lane % LPR, sub = lane / LPR, half = p.rot >> 1, np = half >> 2;
+  const bool in_rot = li < np;
+  const int d0 = in_rot ? 4 * li : p.rot + 8 * (li - np), d1 = in_rot ? d0 + half : d0 + 4;  // the lane's two pieces
+  const int rows = p.HQ + 2 * p.HKV, r_first = (w % p.wpt) * RPW + sub, r_step = p.wpt * RPW;
+  const int64_t stride = (int64_t)gridDim.x * 4 / p.wpt;
+  for (int64_t bt = ((int64_t)blockIdx.x * 4 + w) / p.wpt; bt < p.tokens; bt += stride) {
+    const int64_t bi = bt / p.T, ti = bt - bi * p.T;
+    auto kind = [&](int r) { return r < p.HQ ? 0 : r < p.HQ + p.HKV ? 1 : 2; };
+    auto head = [&](int r, int m) { return r - (m == 0 ? 0 : m == 1 ? p.HQ : p.HQ + p.HKV); };
+    X4 xv[U][2];
+    auto load = [&](int r0) {  // U passes' rows; past the last the last again
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = imin(r0 + u * r_step, rows - 1), m = kind(r);
+        const int64_t sb = m == 0 ? p.sb[0] : m == 1 ? p.sb[1] : p.sb[2], st = m == 0 ? p.st[0] : m == 1 ? p.st[1] : p.st[2];
+        const E* base = static_cast<const E*>(m == 0 ? p.x[0] : m == 1 ? p.x[1] : p.x[2]);
+        const E* src = base + bi * sb + ti * st + head(r, m) * (m == 0 ? p.sh[0] : m == 1 ? p.sh[1] : p.sh[2]);
+        xv[u][0] = *reinterpret_cast<const X4*>(src + d0);
+        xv[u][1] = *reinterpret_cast<const X4*>(src + d1);
+      }
+    };
+    load(r_first);
+    // the token's sequence, its place there and its row of the cache
+    int64_t num = bi, first = 0, count = p.T;
+    bool member = true;
+    if (p.cu) {
+      int64_t below = 0;
+      for (int64_t base = 0; base <= p.N; base += kWave) {
+        const int64_t j = base + lane;
+        const uint64_t m = __ballot(j <= p.N && load_index(p.cu, p.cu_i32, j) <= bt);
+        below += __popcll(m);
+        if (m != ~0ull) break;
+      }
+      num = uniform64(below) - 1;
+      member = num >= 0 && num < p.N;
+      if (member) {
+        first = uniform64(load_index(p.cu, p.cu_i32, num));
+        count = uniform64(load_index(p.cu, p.cu_i32, num + 1)) - first;
+        member = bt - first < count;
+      }
+    }
+    const int64_t length = member ? uniform64(load_index(p.lengths, p.len_i32, num)) : 0;
+    const int64_t place = length - count + (p.cu ? bt - first : ti);
+    int64_t page = -1;
+    if (member && place >= 0 && place < (int64_t)p.width << p.shift && length <= (int64_t)p.width << p.shift) {
+      page = __builtin_amdgcn_readfirstlane(p.table[num * p.table_stride + (place >> p.shift)]);
+      if (page >= p.pages) page = -1;
+    }
+    const int64_t in = place & ((1 << p.shift) - 1);
+    const int64_t pos = p.pos ? load_index(p.pos, p.pos_i32, bi * p.pb + ti * p.pt) : place;
+    for (int f = lane; f < half; f += kWave) {
+      const double turn = (double)pos * p.turns[f];
+      float sv, cv;
+      sincospif(2.f * (float)(turn - rint(turn)), &sv, &cv);
+      tab[w][0][f] = cv;
+      tab[w][1][f] = sv;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the table is the wave's own
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    float c[4], s[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = in_rot ? tab[w][0][d0 + e] : 1.f;
+      s[e] = in_rot ? tab[w][1][d0 + e] : 0.f;
+    }
+    for (int r0 = r_first; r0 < rows; r0 += U * r_step) {  // uniform inside a row's lanes
+      if (r0 != r_first) load(r0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * r_step;
+        if (r >= rows) break;
+        const int m = kind(r), h = head(r, m);
+        X4 o0 = xv[u][0], o1 = xv[u][1];
+        if (m < 2) {
+          const float* wt = m ? p.w[1] : p.w[0];
+          float x[8], ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = (float)xv[u][e >> 2][e & 3];
+            ss += x[e] * x[e];
+          }
+          if (wt) {
+            const float rr = 1.f / sqrtf(group_sum<LPR>(ss) / (float)D + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * rr * wt[(e < 4 ? d0 : d1) + (e & 3)];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = x[e], b = x[4 + e];
+            o0[e] = (E)(a * c[e] - b * s[e]);
+            o1[e] = (E)(b * c[e] + a * s[e]);
+          }
+        }
+        E* dst;
+        if (m == 0) {
+          dst = static_cast<E*>(p.q_out) + (bt * p.HQ + h) * D;
+          if (!member) o0 = X4{}, o1 = X4{};
+        } else {
+          if (page < 0) continue;
+          const int i = m - 1;
+          dst = static_cast<E*>(i ? p.cache[1] : p.cache[0]) + page * (i ? p.cp[1] : p.cp[0]) + h * (i ? p.ch[1] : p.ch[0]) +
+                in * (i ? p.ct[1] : p.ct[0]);
+        }
+        *reinterpret_cast<X4*>(dst + d0) = o0;
+        *reinterpret_cast<X4*>(dst + d1) = o1;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // the table is read before the next token's is written
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ attention, many new tokens
+template <int D, typename E>
+__global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashParams p) {
+  __shared__ __align__(16) E Ks0[kBK * D];
+  __shared__ __align__(16) E Ks1[kBK * D];
+  __shared__ __align__(16) E Vs0[kBK * D];
+  __shared__ __align__(16) E Vs1[kBK * D];
+  flash_forward<D, E, true>(p, Ks0, Ks1, Vs0, Vs1);
+}
+
+// ------------------------------------------------------------------------------------------------ attention, few new tokens
+// A kv head's new rows (token, q head of the group) in tiles of 32; the keys that they see in blocks of 32, cut into `splits`
+// runs, a workgroup each. Every wave takes blocks of its own, loaded straight into its own LDS one ahead: no barrier until the
+// four waves' sums meet, 128 KB a CU under way. Bound by the cache's bytes.
+struct FewParams : FlashParams {
+  const int64_t* tree;  // [B, T] bits of the sequence's drafted tokens that each sees, or null
+  int64_t tb, tt;
+  int splits;
+  float* part;          // [tiles HKV][splits][32][D], then [tiles HKV][splits][2][32]
+};
+
+constexpr int kFewRows = 32, kFewKeys = 32;
+
+struct FewPlan {
+  Seq sq;
+  int hkv, row0, rows, klen, base;  // rows of this tile; keys; place of the first new token
+  Blocks bl;
+  int per, used;                    // blocks a split, splits with any
+  int64_t job;
+};
+__device__ __forceinline__ bool few_plan(const FewParams& p, int64_t job, FewPlan& f) {
+  const int rep = p.HQ / p.HKV;
+  f.job = job;
+  const int64_t t = job / p.HKV;
+  f.hkv = (int)(job - t * p.HKV);
+  if (p.seqs.cu) {
+    f.sq = packed_tile(p.seqs, t, rep, kFewRows);
+  } else {
+    const int64_t per = (p.seqs.T * rep + kFewRows - 1) / kFewRows, row = t / per;
+    f.sq = Seq{row, 0, (int)p.seqs.T, (int)row, (int)(t - row * per)};
+  }
+  if (f.sq.tile >= kFar / kFewRows) return false;
+  f.row0 = f.sq.tile * kFewRows;
+  f.rows = (int)((int64_t)f.sq.len * rep - f.row0 < kFewRows ? (int64_t)f.sq.len * rep - f.row0 : kFewRows);
+  if (f.rows <= 0) return false;
+  f.klen = f.sq.num < 0 ? 0 : cache_length(p.lengths, p.len_i32, f.sq.num, p.width, p.shift);
+  f.base = f.klen - f.sq.len;
+  // a drafted token stands behind as many others as it sees; a row of the tree without bits at the committed tokens' end
+  const int first = p.tree ? f.base - 1 : f.base + f.row0 / rep, last = p.tree ? f.klen - 1 : f.base + (f.row0 + f.rows - 1) / rep;
+  f.bl = blocks_of<kFewKeys>(first, last, p.window, p.sinks);
+  if (f.sq.num < 0) f.bl.count = 0;
+  f.per = imax((f.bl.count + p.splits - 1) / p.splits, 4);
+  f.used = imax((f.bl.count + f.per - 1) / f.per, 1);
+  return true;
+}
+
+// What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
+struct RowView {
+  int place, base;
+  uint64_t bits;
+  bool tree;
+  __device__ __forceinline__ bool operator()(int j, int window, int sinks) const {
+    if (!tree) return sees(place, j, window, sinks);
+    const int n = j - base;
+    return n < 0 ? sees(place, j, window, sinks) : n < 64 && (bits >> n & 1);
+  }
+};
+__device__ __forceinline__ RowView few_view(const FewParams& p, const FewPlan& f, int row) {
+  const int token = row / (p.HQ / p.HKV);
+  RowView v{f.base + token, f.base, 0, p.tree != nullptr};
+  if (p.tree) {
+    v.bits = (uint64_t)p.tree[f.sq.row * p.tb + (f.sq.start + token) * p.tt];
+    if (f.sq.len < 64) v.bits &= (1ull << f.sq.len) - 1;
+    v.place = f.base + __popcll(v.bits) - 1;
+  }
+  return v;
+}
+
+template <int D, typename E>
+__global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewParams p) {
+  using X8 = typename Pack<E>::x8;
+  constexpr int DS = D / 16, DT = D / 32, CPR = D / 8, RPL = 512 / D, LPB = kFewKeys / RPL, TILE = kFewKeys * D, CH = D / 4;
+  __shared__ __align__(16) E K0[4 * TILE];
+  __shared__ __align__(16) E K1[4 * TILE];
+  __shared__ __align__(16) E V0[4 * TILE];
+  __shared__ __align__(16) E V1[4 * TILE];
+  __shared__ float ml[4][2][kFewRows];
+  __shared__ uint32_t redo_rows;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+  const int rep = p.HQ / p.HKV;
+  FewPlan f;
+  const int split = blockIdx.x % p.splits;
+  if (!few_plan(p, blockIdx.x / p.splits, f) || split >= f.used) return;
+  const int n0 = split * f.per, n1 = imin(n0 + f.per, f.bl.count);
+  const int* const table = f.sq.num >= 0 ? p.table + f.sq.num * p.table_stride : nullptr;
+  const int row = f.row0 + imin(li, f.rows - 1);  // the lane's query: token row / rep, head row % rep of the group
+  const RowView view = few_view(p, f, row);
+  auto q_at = [&](int r) {
+    return static_cast<const E*>(p.q) + f.sq.row * p.qsb + (f.sq.start + r / rep) * p.qst + (f.hkv * rep + r % rep) * p.qsh;
+  };
+  X8 qf[DS];
+  {
+    const E* q = q_at(row);
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = *reinterpret_cast<const X8*>(q + 16 * s + 8 * hh);
+  }
+  const char* const kbase = reinterpret_cast<const char*>(static_cast<const E*>(p.k) + f.hkv * p.ksh);
+  const char* const vbase = reinterpret_cast<const char*>(static_cast<const E*>(p.v) + f.hkv * p.vsh);
+  const int kst = (int)p.kst * 2, vst = (int)p.vst * 2, in_page = (1 << p.shift) - 1;
+  int pid[2];
+  auto look_up = [&](int n) {
+    const int jb = f.bl.at(n);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = jb * kFewKeys + 16 * g;
+      const int id = key < f.klen ? page_at(table, key >> p.shift) : -1;
+      pid[g] = id >= 0 && id < p.pages ? id : -1;
+    }
+  };
+  auto fetch = [&](int n, E* kd, E* vd) {
+    const int jb = f.bl.at(n);
+    __amdgpu_buffer_rsrc_t rk[2], rv[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int key = jb * kFewKeys + 16 * g, left = imin(16, f.klen - key), in = key & in_page;
+      const bool any = pid[g] >= 0 && left > 0;
+      const int64_t page = any ? pid[g] : 0;
+      rk[g] = make_rsrc(kbase + page * p.ksb * 2 + (int64_t)in * kst, any ? (uint32_t)((left - 1) * kst + 2 * D) : 0u);
+      rv[g] = make_rsrc(vbase + page * p.vsb * 2 + (int64_t)in * vst, any ? (uint32_t)((left - 1) * vst + 2 * D) : 0u);
+    }
+#pragma unroll
+    for (int u = 0; u < LPB; ++u) {
+      const int r = RPL * u + lane / CPR, ch = (lane % CPR) ^ swz<D>(r);
+      load_lds16(rk[RPL * u / 16], kd + u * 512, (uint32_t)((r & 15) * kst + ch * 16));
+      load_lds16(rv[RPL * u / 16], vd + u * 512, (uint32_t)((r & 15) * vst + ch * 16));
+    }
+  };
+  auto ok_bits = [&]() { return (pid[0] >= 0 ? 1 : 0) | (pid[1] >= 0 ? 2 : 0); };
+  TileReads<D> rd;
+  rd.init(lane);
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale_log2, slack = 8.f / c;
+  const int first = p.tree ? f.base - 1 : f.base + f.row0 / rep, last = p.tree ? f.klen - 1 : f.base + (f.row0 + f.rows - 1) / rep;
+  int ok = 3, ok_next = 3;
+  auto step = [&](int n, const E* kc, E* vc, E* kn, E* vn) {
+    const int k0 = f.bl.at(n) * kFewKeys, k1 = k0 + kFewKeys - 1;
+    if (n + 4 < n1) {
+      ok_next = ok_bits();
+      fetch(n + 4, kn, vn);
+      if (n + 8 < n1) look_up(n + 8);
+      if (LPB == 8) __builtin_amdgcn_s_waitcnt(0x4F70);  // vmcnt(16): all but the loads just issued have landed
+      else __builtin_amdgcn_s_waitcnt(0x0F78);           // vmcnt(8)
+    } else {
+      wait_loads();
+    }
+    asm volatile("" ::: "memory");
+    const bool partial = k1 >= f.klen || ok != 3;
+    if (partial) {  // rows behind the end or on no page: zeros among the values
+#pragma unroll
+      for (int u = 0; u < LPB; ++u) {
+        const int r = RPL * u + lane / CPR;
+        if (k0 + r >= f.klen || !(ok >> (r >> 4) & 1)) *reinterpret_cast<X8*>(vc + u * 512 + lane * 8) = X8{};
+      }
+    }
+    f32x16 s[1] = {f32x16{}};
+#pragma unroll
+    for (int st = 0; st < DS; ++st) s[0] = mma32(row_frag(kc, rd.row[st]), qf[st], s[0]);
+    if (partial || (p.tree && k1 >= f.base) || !all_see(first, last, k0, k1, p.window, p.sinks)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int j = k0 + 8 * (e >> 2) + 4 * hh + (e & 3);
+        if (j >= f.klen || !(ok >> (e >> 3) & 1) || !view(j, p.window, p.sinks)) s[0][e] = -INFINITY;
+      }
+    }
+    softmax_step<1, D, E>(s, acc, m, l, c, slack, vc, rd);
+    ok = ok_next;
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this block's reads are done before its buffer is loaded again
+    asm volatile("" ::: "memory");
+  };
+  E *const k0p = K0 + w * TILE, *const k1p = K1 + w * TILE, *const v0p = V0 + w * TILE, *const v1p = V1 + w * TILE;
+  if (n0 + w < n1) {
+    look_up(n0 + w);
+    ok = ok_bits();
+    fetch(n0 + w, k0p, v0p);
+    if (n0 + w + 4 < n1) look_up(n0 + w + 4);
+    for (int n = n0 + w; n < n1; n += 8) {
+      step(n, k0p, v0p, k1p, v1p);
+      if (n + 4 < n1) step(n + 4, k1p, v1p, k0p, v0p);
+    }
+  }
+
+  // The four waves' sums at one maximum. A row's 16-byte piece i lies at i ^ (row & 31) of its D floats.
+  l += __shfl_xor(l, 32, kWave);
+  if (hh == 0) {
+    ml[w][0][li] = m;
+    ml[w][1][li] = l;
+  }
+  if (t == 0) redo_rows = 0;
+  __syncthreads();  // every wave is done with its tiles, which take the sums
+  const float top = fmaxf(fmaxf(ml[0][0][li], ml[1][0][li]), fmaxf(ml[2][0][li], ml[3][0][li]));
+  const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
+  float* const red = reinterpret_cast<float*>(w < 2 ? K0 : K1) + (w & 1) * kFewRows * D;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int piece = (8 * d + 2 * j + hh) ^ (li & (CH - 1));
+      *reinterpret_cast<f32x4*>(red + li * D + 4 * piece) =
+          f32x4{acc[d][4 * j] * mine, acc[d][4 * j + 1] * mine, acc[d][4 * j + 2] * mine, acc[d][4 * j + 3] * mine};
+    }
+  __syncthreads();
+  const int64_t place = f.job * p.splits + split;
+  float* const po = p.part + place * kFewRows * D;
+  float* const pml = p.part + p.tiles * p.HKV * p.splits * kFewRows * D + place * 2 * kFewRows;
+  auto out_row = [&](int r) {
+    return static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + r / rep) * p.HQ) + f.hkv * rep + r % rep) * D;
+  };
+  for (int i = t; i < f.rows * CH; i += 256) {
+    const int r = i / CH, piece = i % CH;
+    const float tm = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
+    float sum = 0.f;
+    f32x4 x{};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float mv = ml[v][0][r];
+      if (mv != -INFINITY) sum += ml[v][1][r] * __builtin_amdgcn_exp2f((mv - tm) * c);
+      x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
+                                           4 * (piece ^ (r & (CH - 1))));
+    }
+    if (!finite_f(sum) || !finite_f(x[0]) || !finite_f(x[1]) || !finite_f(x[2]) || !finite_f(x[3])) {
+      atomicOr(&redo_rows, 1u << r);
+      continue;
+    }
+    if (f.used == 1) {
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      typename Pack<E>::x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
+      *reinterpret_cast<typename Pack<E>::x4*>(out_row(f.row0 + r) + 4 * piece) = y;
+    } else {
+      *reinterpret_cast<f32x4*>(po + r * D + 4 * piece) = x;
+      if (piece == 0) {
+        pml[r] = tm;
+        pml[kFewRows + r] = sum;
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t redo = redo_rows; redo; redo &= redo - 1) {  // over the keys that the row sees only
+    const int r = __ffs(redo) - 1;
+    if (r % 4 != w) continue;
+    const RowView v = few_view(p, f, f.row0 + r);
+    auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
+      const int id = table[j >> p.shift];
+      return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
+                                     : reinterpret_cast<const E*>(base + id * page_bytes + (j & in_page) * row_bytes);
+    };
+    float mr = -INFINITY, lr = 0.f, a[D / 64] = {};
+    for (int n = n0; n < n1; ++n) {
+      const int k0 = f.bl.at(n) * kFewKeys;
+      slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
+                     [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); }, c,
+                     mr, lr, a);
+    }
+    if (f.used == 1) {
+      for (int i = 0; i < D / 64; ++i) out_row(f.row0 + r)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+    } else {
+      for (int i = 0; i < D / 64; ++i) po[r * D + lane + 64 * i] = a[i];
+      if (lane == 0) {
+        pml[r] = mr;
+        pml[kFewRows + r] = lr;
+      }
+    }
+  }
+}
+
+// The runs' sums of each row at one maximum, in order. A workgroup a tile of rows.
+template <int D, typename E>
+__global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(FewParams p) {
+  constexpr int CH = D / 4;
+  FewPlan f;
+  if (!few_plan(p, blockIdx.x, f) || f.used == 1) return;
+  const int rep = p.HQ / p.HKV;
+  const float* const po = p.part + f.job * p.splits * kFewRows * D;
+  const float* const pml = p.part + p.tiles * p.HKV * p.splits * kFewRows * D + f.job * p.splits * 2 * kFewRows;
+  for (int i = threadIdx.x; i < f.rows * CH; i += 256) {
+    const int r = i / CH, piece = i % CH;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < f.used; ++s) top = fmaxf(top, pml[s * 2 * kFewRows + r]);
+    f32x4 x{};
+#pragma unroll 8
+    for (int s = 0; s < f.used; ++s) {
+      const float ms = pml[s * 2 * kFewRows + r], a = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - top) * p.scale_log2);
+      sum += a * pml[(s * 2 + 1) * kFewRows + r];
+      x += a * *reinterpret_cast<const f32x4*>(po + (s * kFewRows + r) * D + 4 * piece);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    typename Pack<E>::x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
+    const int row = f.row0 + r;
+    *reinterpret_cast<typename Pack<E>::x4*>(static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + row / rep) * p.HQ) +
+                                                                     f.hkv * rep + row % rep) * D + 4 * piece) = y;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int log2_of(int64_t x) {
+  int s = 0;
+  while (((int64_t)1 << s) < x) ++s;
+  return s;
+}
+
+static int paged_check(const char* name, int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, const void* cu,
+                       int64_t pages, int64_t page_size, int64_t width, int dtype) {
+  if (B <= 0 || T < 0 || HQ < 0 || HKV <= 0 || N <= 0 || (cu ? B != 1 : N != B) || pages <= 0 || width <= 0 || page_size <= 0) {
+    gdn_internal_set_error("%s: bad sizes B=%lld T=%lld HQ=%lld HKV=%lld N=%lld pages=%lld page_size=%lld table width=%lld "
+                           "(cu_seqlens requires B == 1)", name, (long long)B, (long long)T, (long long)HQ, (long long)HKV,
+                           (long long)N, (long long)pages, (long long)page_size, (long long)width);
+    return GDN_ERR_INVALID;
+  }
+  if (D != 64 && D != 128) {
+    gdn_internal_set_error("%s: head dim %lld unsupported (64 or 128)", name, (long long)D);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (dtype != GDN_DTYPE_BF16 && dtype != GDN_DTYPE_F16) {
+    gdn_internal_set_error("%s: dtype %d unsupported (bf16 or fp16)", name, dtype);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1))) {
+    gdn_internal_set_error("%s: page size %lld unsupported (a power of two from 16 to 65536)", name, (long long)page_size);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (T >= kFar / 2 || width >= kFar || width * page_size >= kFar / 2 || N >= kFar || pages > 0x7fffffff || HQ > 65536 ||
+      HKV > 65536 || B * T > (1LL << 40)) {
+    gdn_internal_set_error("%s: too many tokens, pages or heads (B=%lld T=%lld N=%lld pages=%lld table width=%lld HQ=%lld HKV=%lld)",
+                           name, (long long)B, (long long)T, (long long)N, (long long)pages, (long long)width, (long long)HQ,
+                           (long long)HKV);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  return GDN_OK;
+}
+
+// every stride of rows a multiple of 8 elements and none negative, every pointer on 16 bytes
+static bool rows_ok(const int64_t* st, int n, uintptr_t all) {
+  for (int i = 0; i < n; ++i)
+    if (st[i] < 0 || st[i] % 8) return false;
+  return !(all & 15);
+}
+
+struct FewSize {
+  int64_t tiles;
+  int splits;
+};
+// Runs of keys a tile: about kFewGroups workgroups in all, each with 4 blocks at least, one a wave.
+constexpr int64_t kFewGroups = 1024;
+static FewSize few_size(int64_t T, int64_t B, int64_t HQ, int64_t HKV, int64_t N, bool varlen, int64_t keys) {
+  const int64_t rep = HQ / HKV;
+  const int64_t tiles = varlen ? packed_tiles(T, N, (int)rep, kFewRows) : B * ((T * rep + kFewRows - 1) / kFewRows);
+  const int64_t busy = varlen ? (T * rep + kFewRows - 1) / kFewRows + N : tiles;
+  const int64_t blocks = (keys + kFewKeys - 1) / kFewKeys + 1;
+  int64_t splits = (kFewGroups + busy * HKV - 1) / (busy * HKV);
+  if (splits > (blocks + 3) / 4) splits = (blocks + 3) / 4;
+  if (splits < 1) splits = 1;
+  return {tiles, (int)splits};
+}
+
+// Whole tiles of queries a head share what they load among 128 of them; few new tokens' rows are taken together with their
+// group's heads and the keys cut into runs instead.
+static bool takes_few(int64_t T, int64_t HQ, int64_t HKV, int64_t N, bool varlen, bool tree) {
+  const int64_t tokens = varlen ? (T + N - 1) / N : T;
+  return tree || tokens * (HQ / HKV) <= 256;
+}
+
+// keys that a row can see at most
+static int64_t most_keys(int64_t T, int64_t width, int64_t page_size, int64_t window, int64_t sinks) {
+  const int64_t all = width * page_size;
+  if (window <= 0 || window >= all) return all;
+  const int64_t some = window + T + (sinks < all ? sinks : all);
+  return some < all ? some : all;
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_paged_append(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                const float* q_weight, const float* k_weight, void* q_out, void* k_cache, int64_t kc_page_stride,
+                                int64_t kc_head_stride, int64_t kc_token_stride, void* v_cache, int64_t vc_page_stride,
+                                int64_t vc_head_stride, int64_t vc_token_stride, const int32_t* page_table,
+                                int64_t table_stride, const void* lengths, int lengths_i32, const void* positions,
+                                int64_t pos_batch_stride, int64_t pos_token_stride, int pos_i32, const void* cu_seqlens,
+                                int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t pages,
+                                int64_t page_size, int64_t width, int dtype, int rot_dim, double theta, float eps,
+                                unsigned flags, void* stream) {
+  const char* name = "gdn_paged_append";
+  if (int rc = paged_check(name, B, T, q ? HQ : 0, HKV, D, N, cu_seqlens, pages, page_size, width, dtype)) return rc;
+  if (rot_dim < 0 || rot_dim > D || rot_dim % 16) {
+    gdn_internal_set_error("%s: rot_dim=%d unsupported (a multiple of 16 up to D)", name, rot_dim);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (!(theta > 0.) || !(theta < 1e300) || !(eps >= 0.f) || (q && HQ <= 0)) {
+    gdn_internal_set_error("%s: bad arguments HQ=%lld theta=%g eps=%g", name, (long long)HQ, theta, (double)eps);
+    return GDN_ERR_INVALID;
+  }
+  if (T == 0) return GDN_OK;
+  const int64_t st[15] = {k_batch_stride, k_token_stride, k_head_stride, v_batch_stride, v_token_stride, v_head_stride,
+                          kc_page_stride, kc_head_stride, kc_token_stride, vc_page_stride, vc_head_stride, vc_token_stride,
+                          q ? q_batch_stride : 0, q ? q_token_stride : 0, q ? q_head_stride : 0};
+  if (!k || !v || !k_cache || !v_cache || !page_table || !lengths || (q && !q_out) ||
+      !rows_ok(st, 15, reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                           reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
+                           (q ? reinterpret_cast<uintptr_t>(q_out) : 0))) {
+    gdn_internal_set_error("%s: null tensor pointer, or rows not 16-byte aligned", name);
+    return GDN_ERR_INVALID;
+  }
+  AppendParams p{{q, k, v}, {q_batch_stride, k_batch_stride, v_batch_stride}, {q_token_stride, k_token_stride, v_token_stride},
+                 {q_head_stride, k_head_stride, v_head_stride}, {q_weight, k_weight}, q_out, {k_cache, v_cache},
+                 {kc_page_stride, vc_page_stride}, {kc_head_stride, vc_head_stride}, {kc_token_stride, vc_token_stride},
+                 page_table, table_stride, lengths, positions, pos_batch_stride, pos_token_stride, cu_seqlens,
+                 lengths_i32, pos_i32, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, (int)width, log2_of(page_size), (int)pages,
+                 T, N, B * T, q ? (int)HQ : 0, (int)HKV, rot_dim, B * T <= kAppendShared ? 4 : 1, eps};
+  for (int f = 0; f < rot_dim / 2; ++f) p.turns[f] = pow(theta, -2. * f / rot_dim) / 6.283185307179586;
+  const int64_t want = p.wpt == 4 ? p.tokens : (p.tokens + 3) / 4;
+  const dim3 grid((unsigned)(want < kMaxGroups256 ? want : kMaxGroups256)), block(256);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == GDN_DTYPE_BF16) {
+    if (D == 128) hipLaunchKernelGGL((gated_delta_paged_append_kernel<128, bf16>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_delta_paged_append_kernel<64, bf16>), grid, block, 0, s, p);
+  } else {
+    if (D == 128) hipLaunchKernelGGL((gated_delta_paged_append_kernel<128, f16>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_delta_paged_append_kernel<64, f16>), grid, block, 0, s, p);
+  }
+  return gdn_internal_check_launch("gated_delta_paged_append_kernel");
+}
+
+extern "C" size_t gdn_paged_attn_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                                                int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen,
+                                                int tree) {
+  if (B <= 0 || T <= 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || D <= 0 || N <= 0 || page_size <= 0 || width <= 0) return 0;
+  if (!takes_few(T, HQ, HKV, N, varlen != 0, tree != 0)) return 0;
+  const FewSize f = few_size(T, B, HQ, HKV, N, varlen != 0, most_keys(T, width, page_size, window, sinks));
+  return f.splits == 1 ? 0 : (size_t)f.tiles * HKV * f.splits * kFewRows * (D + 2) * 4;
+}
+
+extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                  const void* k_cache, int64_t kc_page_stride, int64_t kc_head_stride, int64_t kc_token_stride,
+                                  const void* v_cache, int64_t vc_page_stride, int64_t vc_head_stride, int64_t vc_token_stride,
+                                  const int32_t* page_table, int64_t table_stride, const void* lengths, int lengths_i32,
+                                  const int64_t* tree, int64_t tree_batch_stride, int64_t tree_token_stride, void* o,
+                                  const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                                  int64_t pages, int64_t page_size, int64_t width, int dtype, int64_t window, int64_t sinks,
+                                  float scale, unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "gdn_paged_attn_fwd";
+  if (int rc = paged_check(name, B, T, HQ, HKV, D, N, cu_seqlens, pages, page_size, width, dtype)) return rc;
+  if (HQ <= 0 || HQ % HKV || window < 0 || sinks < 0) {
+    gdn_internal_set_error("%s: bad arguments HQ=%lld HKV=%lld window=%lld sinks=%lld (HQ a multiple of HKV)", name,
+                           (long long)HQ, (long long)HKV, (long long)window, (long long)sinks);
+    return GDN_ERR_INVALID;
+  }
+  if (!(scale > 0.f) || scale > 3.0e38f) {
+    gdn_internal_set_error("%s: scale %g unsupported (a positive finite softmax scale)", name, (double)scale);
+    return GDN_ERR_INVALID;
+  }
+  if (T == 0) return GDN_OK;
+  const int64_t st[9] = {q_batch_stride, q_token_stride, q_head_stride, kc_page_stride, kc_head_stride, kc_token_stride,
+                         vc_page_stride, vc_head_stride, vc_token_stride};
+  if (!q || !k_cache || !v_cache || !page_table || !lengths || !o ||
+      !rows_ok(st, 9, reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
+                          reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(o)) ||
+      kc_token_stride * 2 > kMaxRowBytes || vc_token_stride * 2 > kMaxRowBytes) {
+    gdn_internal_set_error("%s: null tensor pointer, rows not 16-byte aligned, or cache rows more than %lld bytes apart", name,
+                           (long long)kMaxRowBytes);
+    return GDN_ERR_INVALID;
+  }
+  FewParams p{};
+  p.q = q, p.k = k_cache, p.v = v_cache, p.o = o;
+  p.qsb = q_batch_stride, p.qst = q_token_stride, p.qsh = q_head_stride;
+  p.ksb = kc_page_stride, p.ksh = kc_head_stride, p.kst = kc_token_stride;
+  p.vsb = vc_page_stride, p.vsh = vc_head_stride, p.vst = vc_token_stride;
+  p.seqs = Packed{cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, N, T};
+  p.B = B;
+  p.HQ = (int)HQ, p.HKV = (int)HKV, p.parts = job_parts(HKV);
+  p.window = window <= 0 || window > kFar ? kFar : (int)window;
+  p.sinks = window <= 0 ? 0 : sinks > kFar ? kFar : (int)sinks;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.table = page_table, p.table_stride = table_stride, p.lengths = lengths, p.len_i32 = lengths_i32;
+  p.width = (int)width, p.shift = log2_of(page_size), p.pages = (int)pages;
+  p.tree = tree, p.tb = tree_batch_stride, p.tt = tree_token_stride;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 block(256);
+  auto by_type = [&](auto go) {
+    if (dtype == GDN_DTYPE_BF16) D == 128 ? go(bf16{}, std::integral_constant<int, 128>{}) : go(bf16{}, std::integral_constant<int, 64>{});
+    else D == 128 ? go(f16{}, std::integral_constant<int, 128>{}) : go(f16{}, std::integral_constant<int, 64>{});
+  };
+  if (!takes_few(T, HQ, HKV, N, cu_seqlens != nullptr, tree != nullptr)) {
+    p.tiles = cu_seqlens ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ);
+    const int64_t groups = job_groups(HKV, HQ / HKV, p.tiles);
+    if (groups > kMaxGroups256) {
+      gdn_internal_set_error("%s: grid too large", name);
+      return GDN_ERR_UNSUPPORTED;
+    }
+    const FlashParams fp = p;
+    by_type([&](auto e, auto d) {
+      hipLaunchKernelGGL((gated_delta_paged_attn_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)groups), block, 0, s, fp);
+    });
+    return gdn_internal_check_launch("gated_delta_paged_attn_kernel");
+  }
+  const FewSize f = few_size(T, B, HQ, HKV, N, cu_seqlens != nullptr, most_keys(T, width, page_size, window, sinks));
+  p.tiles = f.tiles, p.splits = f.splits, p.part = static_cast<float*>(workspace);
+  const size_t need = gdn_paged_attn_workspace_size(B, T, HQ, HKV, D, N, page_size, width, window, sinks, cu_seqlens != nullptr,
+                                                    tree != nullptr);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) {
+    gdn_internal_set_error("%s: workspace of %zu bytes needed, 16-byte aligned", name, need);
+    return GDN_ERR_INVALID;
+  }
+  const int64_t jobs = f.tiles * HKV;
+  if (jobs * f.splits > kMaxGroups256) {
+    gdn_internal_set_error("%s: grid too large", name);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  by_type([&](auto e, auto d) {
+    hipLaunchKernelGGL((gated_delta_paged_attn_few_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)(jobs * f.splits)),
+                       block, 0, s, p);
+  });
+  if (int rc = gdn_internal_check_launch("gated_delta_paged_attn_few_kernel")) return rc;
+  if (f.splits == 1) return GDN_OK;
+  by_type([&](auto e, auto d) {
+    hipLaunchKernelGGL((gated_delta_paged_attn_merge_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)jobs), block, 0, s, p);
+  });
+  return gdn_internal_check_launch("gated_delta_paged_attn_merge_kernel");
+}

@@ -1,0 +1,635 @@
+// Attention with a sliding window and a few first tokens that stay visible (sinks), over whole sequences, and its backward.
+//
+//   p_ij = softmax_j(scale q_i . k_j) over the keys that i sees;  o_i = sum_j p_ij v_j
+//   delta_i = do_i . o_i;  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j;  dk_j = scale sum_i ds_ij q_i;  dv_j = sum_i p_ij do_i
+//
+// Bound by the matrix units and by the LDS reads that feed them: one operand of every product comes from LDS, 1 KB for the 32
+// cycles of a 32x32x16 product, which is what four waves' reads reach. The backward computes S and dP again from the row's
+// logarithm: one kernel holds 32 queries a wave and walks their keys (dq, and delta on the way), the other holds 32 keys and
+// walks their queries (dk, dv, summed over the q heads of the kv head in fp32). No atomics.
+
+#include "gdn_flash.h"
+
+namespace gdn {
+
+template <int D, typename E>
+__global__ __launch_bounds__(256, 2) void gated_delta_window_attn_fwd_kernel(FlashParams p) {
+  __shared__ __align__(16) E Ks0[kBK * D];
+  __shared__ __align__(16) E Ks1[kBK * D];
+  __shared__ __align__(16) E Vs0[kBK * D];
+  __shared__ __align__(16) E Vs1[kBK * D];
+  flash_forward<D, E, false>(p, Ks0, Ks1, Vs0, Vs1);
+}
+
+struct WindowBwdParams {
+  const bf16 *q, *k, *v, *o, *d_o;  // o, d_o [B, T, HQ, D]
+  int64_t qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh;
+  const float* lse;                 // [HQ, B T]
+  float* delta;                     // [HQ, B T]
+  bf16 *dq, *dk, *dv;               // contiguous
+  Packed seqs;
+  int64_t B, q_tiles, k_tiles, pieces;
+  int HQ, HKV, parts, window, sinks;
+  float scale, scale_log2;
+  // far queries of the sinks: a slot for each piece of `far` queries and one a sequence for the near ones, per kv head and tile
+  // of 128 sinks: [slots][HKV][sink tiles][2][sink rows][D]
+  float* part;
+  int far, sink_tiles, sink_rows;
+};
+
+// Loads of 64 rows of `stride` bytes from `base` (the block's first row) into a tile, `rows` of them there.
+template <int D>
+struct BlockLoad {
+  int w, lane;
+  static constexpr int CPR = D / 8, RPL = 512 / D, LPT = kBK / (4 * RPL);
+  __device__ __forceinline__ void load(const char* base, int stride, int rows, bf16* to) const {
+    const auto r = make_rsrc(base, rows <= 0 ? 0u : (uint32_t)((rows - 1) * stride + 2 * D));
+    const int drow = w * RPL + lane / CPR;
+    const uint32_t off = (uint32_t)(drow * stride + ((lane % CPR) ^ swz<D>(drow)) * 16);
+#pragma unroll
+    for (int u = 0; u < LPT; ++u) load_lds16(r, to + (w + 4 * u) * 512, off + u * 4 * RPL * stride);
+  }
+  // the rows of the wave's own loads from `rows` on: zeros
+  __device__ __forceinline__ void clean(int rows, bf16* to) const {
+#pragma unroll
+    for (int u = 0; u < LPT; ++u)
+      if ((w + 4 * u) * RPL + lane / CPR >= rows) *reinterpret_cast<bf16x8*>(to + (w + 4 * u) * 512 + lane * 8) = bf16x8{};
+  }
+};
+
+template <int D>
+__device__ __forceinline__ float dot8(bf16x8 a, bf16x8 b) {
+  float x = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x += (float)a[e] * (float)b[e];
+  return x;
+}
+
+// dq and delta: 128 queries of one head a workgroup, as the forward's.
+template <int D>
+__global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(WindowBwdParams p) {
+  constexpr int DS = D / 16, DT = D / 32;
+  __shared__ __align__(16) bf16 Ks0[kBK * D];
+  __shared__ __align__(16) bf16 Ks1[kBK * D];
+  __shared__ __align__(16) bf16 Vs0[kBK * D];
+  __shared__ __align__(16) bf16 Vs1[kBK * D];
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+  const int rep = p.HQ / p.HKV;
+  Job job;
+  if (!job_of(blockIdx.x, p.HKV, rep, p.parts, p.q_tiles, job)) return;
+  Seq sq;
+  if (p.seqs.cu) {
+    sq = packed_tile(p.seqs, job.tile, 1, kBQ);
+  } else {
+    const int64_t per = (p.seqs.T + kBQ - 1) / kBQ;
+    sq = Seq{job.tile % p.B, 0, (int)p.seqs.T, 0, (int)(per - 1 - job.tile / p.B)};
+  }
+  const int q0 = sq.tile * kBQ, hq = job.hkv * rep + job.hm;
+  if (q0 >= sq.len) return;
+  const int q1 = imin(q0 + kBQ, sq.len) - 1, qi = q0 + 32 * w + li, wq0 = q0 + 32 * w, wq1 = imin(wq0 + 31, q1);
+  const bool wave_live = wq0 <= wq1, row_ok = wave_live && qi < sq.len;
+  Blocks bl = blocks_of<kBK>(q0, q1, p.window, p.sinks);
+  if (sq.num < 0) bl.count = 0;
+  const int64_t tok = sq.row * p.seqs.T + sq.start, all = p.B * p.seqs.T;
+  const int qc = imin(qi, sq.len - 1);
+  const bf16* qrow = p.q + sq.row * p.qsb + (sq.start + qc) * p.qst + hq * p.qsh;
+  const int64_t orow = ((tok + qc) * p.HQ + hq) * D;
+  bf16x8 qf[DS], df[DS];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < DS; ++s) {
+    qf[s] = *reinterpret_cast<const bf16x8*>(qrow + 16 * s + 8 * hh);
+    df[s] = *reinterpret_cast<const bf16x8*>(p.d_o + orow + 16 * s + 8 * hh);
+    delta += dot8<D>(df[s], *reinterpret_cast<const bf16x8*>(p.o + orow + 16 * s + 8 * hh));
+  }
+  delta += __shfl_xor(delta, 32, kWave);
+  const float lse = p.lse[hq * all + tok + qc];
+  if (row_ok && hh == 0) p.delta[hq * all + tok + qi] = delta;
+
+  const char* const kbase = reinterpret_cast<const char*>(p.k + sq.row * p.ksb + sq.start * p.kst + job.hkv * p.ksh);
+  const char* const vbase = reinterpret_cast<const char*>(p.v + sq.row * p.vsb + sq.start * p.vst + job.hkv * p.vsh);
+  const int kst = (int)p.kst * 2, vst = (int)p.vst * 2;
+  const BlockLoad<D> io{w, lane};
+  auto fetch = [&](int jb, bf16* kd, bf16* vd) {
+    io.load(kbase + (int64_t)jb * kBK * kst, kst, imin(kBK, sq.len - jb * kBK), kd);
+    io.load(vbase + (int64_t)jb * kBK * vst, vst, imin(kBK, sq.len - jb * kBK), vd);
+  };
+  TileReads<D> rd;
+  rd.init(lane);
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  const float c = p.scale_log2;
+  auto block = [&](bool masked, const bf16* kb, const bf16* vb, int k0) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(kb + 32 * kt * D, rd.row[st]), qf[st], s);
+#pragma unroll
+      for (int st = 0; st < DS; ++st) dp = mma32(row_frag(vb + 32 * kt * D, rd.row[st]), df[st], dp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - delta);
+      if (masked) {
+        const int hi = qi - k0, lo = qi - p.window - k0, sk = p.sinks - k0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
+          if (ko > hi || (ko <= lo && ko >= sk)) s[e] = 0.f;
+        }
+      }
+      bf16x8 pb[2];
+      pack16<bf16>(s, pb);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = mma32(tr_frag(kb + (2 * kt + h) * 16 * D, rd.tr[d]), pb[h], acc[d]);
+    }
+  };
+  auto arrive = [&](int jb, bf16* kd) {  // the wave's loads of block jb have landed; keys behind the end: zeros
+    wait_loads();
+    if ((jb + 1) * kBK > sq.len) io.clean(sq.len - jb * kBK, kd);
+  };
+  auto step = [&](int n, const bf16* kc, const bf16* vc, bf16* kn, bf16* vn) {
+    const int jb = bl.at(n), next = bl.at(n + 1);
+    if (n + 1 < bl.count) fetch(next, kn, vn);
+    const int k0 = jb * kBK, k1 = k0 + kBK - 1;
+    if (wave_live && !none_sees(wq0, wq1, k0, k1, p.window, p.sinks))
+      block(!all_see(wq0, wq1, k0, k1, p.window, p.sinks), kc, vc, k0);
+    if (n + 1 < bl.count) arrive(next, kn);
+    __syncthreads();
+  };
+  if (bl.count > 0) {
+    fetch(bl.at(0), Ks0, Vs0);
+    arrive(bl.at(0), Ks0);
+    __syncthreads();
+    for (int n = 0; n < bl.count; n += 2) {
+      step(n, Ks0, Vs0, Ks1, Vs1);
+      if (n + 1 < bl.count) step(n + 1, Ks1, Vs1, Ks0, Vs0);
+    }
+  }
+  bool fine = finite_all(acc);
+  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  if (row_ok && fine) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<bf16x4*>(p.dq + orow + 32 * d + 8 * j + 4 * hh) =
+            to_bf16x4(acc[d][4 * j] * p.scale, acc[d][4 * j + 1] * p.scale, acc[d][4 * j + 2] * p.scale, acc[d][4 * j + 3] * p.scale);
+  }
+  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
+  while (redo) {  // over the keys that the row sees only
+    const int n = __ffsll((unsigned long long)redo) - 1, r = wq0 + n;
+    redo &= redo - 1;
+    const bf16* qp = p.q + sq.row * p.qsb + (sq.start + r) * p.qst + hq * p.qsh;
+    const int64_t at = ((tok + r) * p.HQ + hq) * D;
+    const float lr = __shfl(lse, n, kWave), dr = __shfl(delta, n, kWave);
+    float a[D / 64] = {};
+    for (int base = 0; base <= r; base += kWave) {
+      const int j = base + lane;
+      const bool see = j <= r && sees(r, j, p.window, p.sinks);
+      const uint64_t live = __ballot(see);
+      float ds = 0.f;
+      if (see) {
+        const float s = dot_row<D>(qp, reinterpret_cast<const bf16*>(kbase + (int64_t)j * kst));
+        ds = __builtin_amdgcn_exp2f(fmaf(s, c, -lr)) * (dot_row<D>(p.d_o + at, reinterpret_cast<const bf16*>(vbase + (int64_t)j * vst)) - dr);
+      }
+      for (int i = 0; i < kWave; ++i) {
+        if (!(live >> i & 1)) continue;
+        const float x = __shfl(ds, i, kWave);
+        const bf16* kr = reinterpret_cast<const bf16*>(kbase + (int64_t)(base + i) * kst);
+        for (int e = 0; e < D / 64; ++e) a[e] += x * (float)kr[lane + 64 * e];
+      }
+    }
+    for (int e = 0; e < D / 64; ++e) p.dq[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
+  }
+}
+
+// The queries of a key tile end here: near ones, which see keys through the window. Those behind see sinks only.
+__device__ __forceinline__ int near_end(int tile, int window, int len) { return imin(len, tile * kBQ + kBQ - 1 + window); }
+
+// dk and dv: 128 keys of one kv head a workgroup, 32 a wave in registers; blocks of 64 queries with their do pass through LDS,
+// head after head. Sinks are seen by far queries too: the first k_tiles jobs are every tile's near queries, the others a piece
+// of the far queries for one tile of sinks. A tile's sums over those meet in gated_delta_window_attn_sinks_kernel.
+template <int D>
+__global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(WindowBwdParams p) {
+  constexpr int DS = D / 16, DT = D / 32;
+  __shared__ __align__(16) bf16 Qs0[kBK * D];
+  __shared__ __align__(16) bf16 Qs1[kBK * D];
+  __shared__ __align__(16) bf16 Ds0[kBK * D];
+  __shared__ __align__(16) bf16 Ds1[kBK * D];
+  __shared__ __align__(16) float Ls0[2 * kBK];  // lse, delta
+  __shared__ __align__(16) float Ls1[2 * kBK];
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+  const int rep = p.HQ / p.HKV;
+  Job job;
+  if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles + p.pieces * p.sink_tiles, job)) return;
+  Seq sq;
+  int tile, from, to;
+  int64_t slot;  // where sums over part of a sink's queries go
+  if (job.tile < p.k_tiles) {
+    if (p.seqs.cu) sq = packed_tile(p.seqs, job.tile, 1, kBQ);
+    else sq = Seq{job.tile % p.B, 0, (int)p.seqs.T, (int)(job.tile % p.B), (int)(job.tile / p.B)};  // those that most see first
+    tile = sq.tile;
+    if (tile * kBQ >= sq.len) return;
+    from = tile * kBQ;
+    to = sq.num < 0 ? from : near_end(tile, p.window, sq.len);
+    slot = to < sq.len && sq.num >= 0 ? p.pieces + sq.num : -1;
+  } else {
+    const int64_t f = job.tile - p.k_tiles;
+    slot = f / p.sink_tiles;
+    tile = (int)(f - slot * p.sink_tiles);
+    if (p.seqs.cu) sq = packed_tile(p.seqs, slot, 1, p.far);
+    else sq = Seq{slot % p.B, 0, (int)p.seqs.T, 0, (int)(slot / p.B)};
+    if (sq.num < 0 || tile * kBQ >= sq.len || sq.tile > sq.len / p.far) return;
+    from = imax(near_end(tile, p.window, sq.len), sq.tile * p.far);
+    to = imin(sq.len, (sq.tile + 1) * p.far);
+    if (from >= to) return;
+  }
+  const bool far_job = job.tile >= p.k_tiles;
+  const int wk0 = tile * kBQ + 32 * w, key = wk0 + li, kc = imin(key, sq.len - 1);
+  const bool wave_live = wk0 < sq.len && !(far_job && wk0 >= p.sinks);
+  const bool row_ok = key < sq.len && !(far_job && key >= p.sinks);
+  const int64_t tok = sq.row * p.seqs.T + sq.start, all = p.B * p.seqs.T;
+  const bf16* const krow = p.k + sq.row * p.ksb + (sq.start + kc) * p.kst + job.hkv * p.ksh;
+  const bf16* const vrow = p.v + sq.row * p.vsb + (sq.start + kc) * p.vst + job.hkv * p.vsh;
+  bf16x8 kf[DS], vf[DS];
+#pragma unroll
+  for (int s = 0; s < DS; ++s) {
+    kf[s] = *reinterpret_cast<const bf16x8*>(krow + 16 * s + 8 * hh);
+    vf[s] = *reinterpret_cast<const bf16x8*>(vrow + 16 * s + 8 * hh);
+  }
+  const char* const qbase = reinterpret_cast<const char*>(p.q + sq.row * p.qsb + sq.start * p.qst + (int64_t)job.hkv * rep * p.qsh);
+  const char* const dbase = reinterpret_cast<const char*>(p.d_o + (tok * p.HQ + job.hkv * rep) * D);
+  const int qst = (int)p.qst * 2, dst = p.HQ * D * 2;
+  const BlockLoad<D> io{w, lane};
+  auto fetch = [&](int g, int qb, bf16* qd, bf16* dd, float* ld) {
+    const int rows = imin(kBK, sq.len - qb * kBK);
+    io.load(qbase + g * p.qsh * 2 + (int64_t)qb * kBK * qst, qst, rows, qd);
+    io.load(dbase + (int64_t)g * D * 2 + (int64_t)qb * kBK * dst, dst, rows, dd);
+    if (w < 2) {
+      const float* src = (w ? p.delta : p.lse) + (job.hkv * rep + g) * all + tok + qb * kBK;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(src, (uint32_t)(rows * 4)),
+                                               (__attribute__((address_space(3))) void*)(ld + w * kBK), 4, lane * 4, 0, 0, 0);
+    }
+  };
+  TileReads<D> rd;
+  rd.init(lane);
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) dk[d] = f32x16{}, dv[d] = f32x16{};
+  const float c = p.scale_log2;
+  // the lane's key is seen by queries lo_q .. hi_q - 1 of the job
+  const int lo_q = imax(key, from), hi_q = key < p.sinks ? to : imin(to, key + p.window);
+  auto block = [&](bool masked, const bf16* qb, const bf16* db, const float* lb, int q0) {
+    const int lo = lo_q - q0, hi = hi_q - q0;
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      f32x16 s{}, dp{};
+#pragma unroll
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(qb + 32 * qt * D, rd.row[st]), kf[st], s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 ls = ld4f(lb + 32 * qt + 8 * j + 4 * hh);
+        s[4 * j] = __builtin_amdgcn_exp2f(fmaf(s[4 * j], c, -ls.x));
+        s[4 * j + 1] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 1], c, -ls.y));
+        s[4 * j + 2] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 2], c, -ls.z));
+        s[4 * j + 3] = __builtin_amdgcn_exp2f(fmaf(s[4 * j + 3], c, -ls.w));
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
+          if (qo < lo || qo >= hi) s[e] = 0.f;
+        }
+      }
+      bf16x8 pb[2];
+      pack16<bf16>(s, pb);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dv[d] = mma32(tr_frag(db + (2 * qt + h) * 16 * D, rd.tr[d]), pb[h], dv[d]);
+#pragma unroll
+      for (int st = 0; st < DS; ++st) dp = mma32(row_frag(db + 32 * qt * D, rd.row[st]), vf[st], dp);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 de = ld4f(lb + kBK + 32 * qt + 8 * j + 4 * hh);
+        s[4 * j] *= dp[4 * j] - de.x;
+        s[4 * j + 1] *= dp[4 * j + 1] - de.y;
+        s[4 * j + 2] *= dp[4 * j + 2] - de.z;
+        s[4 * j + 3] *= dp[4 * j + 3] - de.w;
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
+          if (qo < lo || qo >= hi) s[e] = 0.f;
+        }
+      }
+      pack16<bf16>(s, pb);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[d] = mma32(tr_frag(qb + (2 * qt + h) * 16 * D, rd.tr[d]), pb[h], dk[d]);
+    }
+  };
+  auto arrive = [&](int qb, bf16* qd, bf16* dd) {
+    wait_loads();
+    if ((qb + 1) * kBK > sq.len) {
+      io.clean(sq.len - qb * kBK, qd);
+      io.clean(sq.len - qb * kBK, dd);
+    }
+  };
+  const int qb0 = from / kBK, qb1 = from < to ? (to - 1) / kBK + 1 : qb0;
+  int g = 0, qb = qb0;  // the block being used
+  auto step = [&](const bf16* qc, const bf16* dc, const float* lc, bf16* qn, bf16* dn, float* ln) {
+    const int gn = qb + 1 < qb1 ? g : g + 1, qn_b = qb + 1 < qb1 ? qb + 1 : qb0;
+    if (gn < rep) fetch(gn, qn_b, qn, dn, ln);
+    const int q0 = qb * kBK, q1 = q0 + kBK - 1;
+    if (wave_live && !none_sees(q0, q1, wk0, wk0 + 31, p.window, p.sinks))
+      block(q0 < from || q1 >= to || !all_see(q0, q1, wk0, wk0 + 31, p.window, p.sinks), qc, dc, lc, q0);
+    if (gn < rep) arrive(qn_b, qn, dn);
+    g = gn;
+    qb = qn_b;
+    __syncthreads();
+  };
+  if (qb0 < qb1) {
+    fetch(0, qb0, Qs0, Ds0, Ls0);
+    arrive(qb0, Qs0, Ds0);
+    __syncthreads();
+    while (g < rep) {
+      step(Qs0, Ds0, Ls0, Qs1, Ds1, Ls1);
+      if (g < rep) step(Qs1, Ds1, Ls1, Qs0, Ds0, Ls0);
+    }
+  }
+  bool fine = finite_all(dk) && finite_all(dv);
+  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  const int64_t out = ((tok + kc) * p.HKV + job.hkv) * D;
+  const bool to_part = slot >= 0 && key < p.sinks;
+  float* const part = p.part + (((slot >= 0 ? slot : 0) * p.HKV + job.hkv) * p.sink_tiles + tile) * 2 * p.sink_rows * D;
+  if (row_ok && fine) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 32 * d + 8 * j + 4 * hh;
+        const f32x4 a = {dk[d][4 * j], dk[d][4 * j + 1], dk[d][4 * j + 2], dk[d][4 * j + 3]};
+        const f32x4 b = {dv[d][4 * j], dv[d][4 * j + 1], dv[d][4 * j + 2], dv[d][4 * j + 3]};
+        if (to_part) {
+          *reinterpret_cast<f32x4*>(part + (32 * w + li) * D + at) = a;
+          *reinterpret_cast<f32x4*>(part + (p.sink_rows + 32 * w + li) * D + at) = b;
+        } else {
+          *reinterpret_cast<bf16x4*>(p.dk + out + at) = to_bf16x4(a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
+          *reinterpret_cast<bf16x4*>(p.dv + out + at) = to_bf16x4(b[0], b[1], b[2], b[3]);
+        }
+      }
+  }
+  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
+  while (redo) {  // over the queries that see the key only
+    const int n = __ffsll((unsigned long long)redo) - 1, j = wk0 + n;
+    redo &= redo - 1;
+    const bf16* kr = p.k + sq.row * p.ksb + (sq.start + j) * p.kst + job.hkv * p.ksh;
+    const bf16* vr = p.v + sq.row * p.vsb + (sq.start + j) * p.vst + job.hkv * p.vsh;
+    float a[D / 64] = {}, b[D / 64] = {};
+    for (int h = 0; h < rep; ++h)
+      for (int base = from; base < to; base += kWave) {
+        const int i = base + lane;
+        const bool see = i < to && sees(i, j, p.window, p.sinks);
+        const uint64_t live = __ballot(see);
+        if (!live) continue;
+        auto q_at = [&](int x) { return reinterpret_cast<const bf16*>(qbase + h * p.qsh * 2 + (int64_t)x * qst); };
+        auto d_at = [&](int x) { return reinterpret_cast<const bf16*>(dbase + (int64_t)h * D * 2 + (int64_t)x * dst); };
+        const int64_t at = (job.hkv * rep + h) * all + tok + i;
+        float pr = 0.f, ds = 0.f;
+        if (see) {
+          pr = __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q_at(i), kr), c, -p.lse[at]));
+          ds = pr * (dot_row<D>(d_at(i), vr) - p.delta[at]);
+        }
+        for (int x = 0; x < kWave; ++x) {
+          if (!(live >> x & 1)) continue;
+          const float px = __shfl(pr, x, kWave), dx = __shfl(ds, x, kWave);
+          for (int e = 0; e < D / 64; ++e) {
+            a[e] += dx * (float)q_at(base + x)[lane + 64 * e];
+            b[e] += px * (float)d_at(base + x)[lane + 64 * e];
+          }
+        }
+      }
+    const int64_t at = ((tok + j) * p.HKV + job.hkv) * D;
+    for (int e = 0; e < D / 64; ++e) {
+      if (slot >= 0 && j < p.sinks) {
+        part[(32 * w + n) * D + lane + 64 * e] = a[e];
+        part[(p.sink_rows + 32 * w + n) * D + lane + 64 * e] = b[e];
+      } else {
+        p.dk[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
+        p.dv[at + lane + 64 * e] = (bf16)b[e];
+      }
+    }
+  }
+}
+
+// dk and dv of sinks that far queries see: the near queries' sums and each piece's, in order. A workgroup a sequence, kv head
+// and tile of sinks.
+__global__ __launch_bounds__(256) void gated_delta_window_attn_sinks_kernel(WindowBwdParams p, int D) {
+  const int tile = blockIdx.x % p.sink_tiles, hkv = blockIdx.x / p.sink_tiles % p.HKV;
+  const int64_t num = blockIdx.x / p.sink_tiles / p.HKV;
+  int64_t row = 0, start = 0, first = num, step = p.B;  // slots of the sequence's pieces
+  int len = (int)p.seqs.T;
+  if (p.seqs.cu) {
+    const int64_t b0 = p.seqs.bound(num + 1), b1 = p.seqs.bound(num + 2);
+    start = b0;
+    len = (int)(b1 > b0 ? b1 - b0 : 0);
+    first = b0 / p.far + num + 1;
+    step = 1;
+  } else {
+    row = num;
+  }
+  const int near = near_end(tile, p.window, len), rows = imin(imin(p.sinks, len) - tile * kBQ, kBQ);
+  if (near >= len || rows <= 0) return;  // written where it was computed
+  const int quads = D / 4;
+  const int64_t one = (int64_t)2 * p.sink_rows * D, per = p.HKV * p.sink_tiles * one, here = (hkv * p.sink_tiles + tile) * one;
+  for (int i = threadIdx.x; i < 2 * rows * quads; i += 256) {
+    const int which = i / (rows * quads), r = i / quads % rows, d = i % quads * 4;
+    const int64_t at = here + (which * p.sink_rows + r) * D + d;
+    f32x4 x = *reinterpret_cast<const f32x4*>(p.part + (p.pieces + num) * per + at);
+    for (int n = near / p.far; n <= (len - 1) / p.far; ++n) x += *reinterpret_cast<const f32x4*>(p.part + (first + n * step) * per + at);
+    if (!which) x *= p.scale;
+    bf16* to = (which ? p.dv : p.dk) + ((row * p.seqs.T + start + tile * kBQ + r) * p.HKV + hkv) * D + d;
+    *reinterpret_cast<bf16x4*>(to) = to_bf16x4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int window_check(const char* name, int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, const void* cu,
+                        const int64_t* st, int64_t window, int64_t sinks, float scale) {
+  if (B <= 0 || T < 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || N <= 0 || (cu ? B != 1 : N != B) || window < 0 || sinks < 0) {
+    gdn_internal_set_error("%s: bad sizes B=%lld T=%lld HQ=%lld HKV=%lld N=%lld window=%lld sinks=%lld (HQ a multiple of HKV; "
+                           "cu_seqlens requires B == 1)", name, (long long)B, (long long)T, (long long)HQ, (long long)HKV,
+                           (long long)N, (long long)window, (long long)sinks);
+    return GDN_ERR_INVALID;
+  }
+  if (D != 64 && D != 128) {
+    gdn_internal_set_error("%s: head dim %lld unsupported (64 or 128)", name, (long long)D);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (!(scale > 0.f) || scale > 3.0e38f) {
+    gdn_internal_set_error("%s: scale %g unsupported (a positive finite softmax scale)", name, (double)scale);
+    return GDN_ERR_INVALID;
+  }
+  if (T >= kFar / 2 || N >= kFar || HQ > 65536 || B * T > (1LL << 40)) {
+    gdn_internal_set_error("%s: too many tokens or heads (B=%lld T=%lld N=%lld HQ=%lld)", name, (long long)B, (long long)T,
+                           (long long)N, (long long)HQ);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  for (int i = 0; i < 9; ++i)
+    if (st[i] < 0 || st[i] % 8 || (i % 3 == 1 && st[i] * 2 > kMaxRowBytes)) {
+      gdn_internal_set_error("%s: strides must be multiples of 8 elements, between tokens at most %lld bytes", name,
+                             (long long)kMaxRowBytes);
+      return GDN_ERR_INVALID;
+    }
+  if (HQ * D * 2 > kMaxRowBytes) {
+    gdn_internal_set_error("%s: HQ * D = %lld too large", name, (long long)(HQ * D));
+    return GDN_ERR_UNSUPPORTED;
+  }
+  return GDN_OK;
+}
+
+static int far_window(int64_t window) { return window <= 0 || window > kFar ? kFar : (int)window; }
+// without a window sinks say nothing; sinks as far as the first window reaches neither change who sees what, nor are they cut
+static int far_sinks(int64_t window, int64_t sinks) { return window <= 0 ? 0 : sinks > kFar ? kFar : (int)sinks; }
+
+// A piece of the far queries: as many as a tile's near ones, so that the jobs are of one length, and 512 at least.
+static int far_piece(int window) { return window >= kFar / 2 ? kFar : (window + kBQ > 512 ? window + kBQ : 512) / kBK * kBK; }
+
+struct FarPlan {
+  int far, sink_tiles, sink_rows;
+  int64_t pieces;
+};
+static FarPlan far_plan(int64_t B, int64_t T, int64_t N, bool varlen, int window, int sinks) {
+  FarPlan f{far_piece(window), 0, 0, 0};
+  if (!sinks || (int64_t)window + 1 >= T) return f;  // every query is a near one
+  const int64_t some = sinks < T ? sinks : T;
+  f.sink_tiles = (int)((some + kBQ - 1) / kBQ);
+  f.sink_rows = f.sink_tiles > 1 ? kBQ : (int)((some + 31) / 32 * 32);
+  f.pieces = varlen ? packed_tiles(T, N, 1, f.far) : B * ((T + f.far - 1) / f.far);
+  return f;
+}
+
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                   const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                   const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                   void* o, float* lse, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
+                                   int64_t D, int64_t N, int dtype, int64_t window, int64_t sinks, float scale, unsigned flags,
+                                   void* stream) {
+  const int64_t st[9] = {q_batch_stride, q_token_stride, q_head_stride, k_batch_stride, k_token_stride, k_head_stride,
+                         v_batch_stride, v_token_stride, v_head_stride};
+  if (int rc = window_check("gdn_window_attn_fwd", B, T, HQ, HKV, D, N, cu_seqlens, st, window, sinks, scale)) return rc;
+  if (dtype != GDN_DTYPE_BF16 && dtype != GDN_DTYPE_F16) {
+    gdn_internal_set_error("gdn_window_attn_fwd: dtype %d unsupported (bf16 or fp16)", dtype);
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (T == 0) return GDN_OK;
+  if (!q || !k || !v || !o || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                                reinterpret_cast<uintptr_t>(o)) & 15)) {
+    gdn_internal_set_error("gdn_window_attn_fwd: null or misaligned (16 bytes) tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  FlashParams p{};
+  p.q = q, p.k = k, p.v = v, p.o = o, p.lse = lse;
+  p.qsb = st[0], p.qst = st[1], p.qsh = st[2], p.ksb = st[3], p.kst = st[4], p.ksh = st[5], p.vsb = st[6], p.vst = st[7], p.vsh = st[8];
+  p.seqs = Packed{cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, N, T};
+  p.B = B;
+  p.tiles = cu_seqlens ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ);
+  p.HQ = (int)HQ, p.HKV = (int)HKV, p.parts = job_parts(HKV);
+  p.window = far_window(window), p.sinks = far_sinks(window, sinks);
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const int64_t groups = job_groups(HKV, HQ / HKV, p.tiles);
+  if (groups > kMaxGroups256) {
+    gdn_internal_set_error("gdn_window_attn_fwd: grid too large");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)groups), block(256);
+  if (dtype == GDN_DTYPE_BF16) {
+    if (D == 128) hipLaunchKernelGGL((gated_delta_window_attn_fwd_kernel<128, bf16>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_delta_window_attn_fwd_kernel<64, bf16>), grid, block, 0, s, p);
+  } else {
+    if (D == 128) hipLaunchKernelGGL((gated_delta_window_attn_fwd_kernel<128, f16>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((gated_delta_window_attn_fwd_kernel<64, f16>), grid, block, 0, s, p);
+  }
+  return gdn_internal_check_launch("gated_delta_window_attn_fwd_kernel");
+}
+
+extern "C" size_t gdn_window_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
+                                                     int64_t window, int64_t sinks, int varlen) {
+  if (B <= 0 || T <= 0 || HQ <= 0 || HKV <= 0 || D <= 0 || N <= 0 || window < 0 || sinks < 0) return 0;
+  const FarPlan f = far_plan(B, T, N, varlen != 0, far_window(window), far_sinks(window, sinks));
+  const size_t delta = ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256;
+  return delta + (size_t)(f.sink_tiles ? f.pieces + N : 0) * HKV * f.sink_tiles * 2 * f.sink_rows * D * 4;
+}
+
+extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                                   const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                   const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
+                                   const void* o, const float* lse, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
+                                   int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t window, int64_t sinks, float scale,
+                                   unsigned flags, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  const int64_t st[9] = {q_batch_stride, q_token_stride, q_head_stride, k_batch_stride, k_token_stride, k_head_stride,
+                         v_batch_stride, v_token_stride, v_head_stride};
+  if (int rc = window_check("gdn_window_attn_bwd", B, T, HQ, HKV, D, N, cu_seqlens, st, window, sinks, scale)) return rc;
+  if (T == 0) return GDN_OK;
+  uintptr_t every = 0;
+  bool null = !lse;
+  const void* const all[] = {q, k, v, o, d_o, dq, dk, dv, workspace};
+  for (const void* x : all) every |= reinterpret_cast<uintptr_t>(x), null |= !x;
+  if (null || (every & 15)) {
+    gdn_internal_set_error("gdn_window_attn_bwd: null or misaligned (16 bytes) tensor pointer");
+    return GDN_ERR_INVALID;
+  }
+  const size_t need = gdn_window_attn_bwd_workspace_size(B, T, HQ, HKV, D, N, window, sinks, cu_seqlens != nullptr);
+  if (workspace_bytes < need) {
+    gdn_internal_set_error("gdn_window_attn_bwd: workspace of %zu bytes needed", need);
+    return GDN_ERR_INVALID;
+  }
+  WindowBwdParams p{};
+  p.q = static_cast<const bf16*>(q), p.k = static_cast<const bf16*>(k), p.v = static_cast<const bf16*>(v);
+  p.o = static_cast<const bf16*>(o), p.d_o = static_cast<const bf16*>(d_o), p.lse = lse;
+  p.qsb = st[0], p.qst = st[1], p.qsh = st[2], p.ksb = st[3], p.kst = st[4], p.ksh = st[5], p.vsb = st[6], p.vst = st[7], p.vsh = st[8];
+  p.dq = static_cast<bf16*>(dq), p.dk = static_cast<bf16*>(dk), p.dv = static_cast<bf16*>(dv);
+  p.delta = static_cast<float*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256);
+  p.seqs = Packed{cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, N, T};
+  p.B = B;
+  p.q_tiles = p.k_tiles = cu_seqlens ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ);
+  p.HQ = (int)HQ, p.HKV = (int)HKV, p.parts = job_parts(HKV);
+  p.window = far_window(window), p.sinks = far_sinks(window, sinks);
+  p.scale = scale, p.scale_log2 = scale * 1.4426950408889634f;
+  const FarPlan f = far_plan(B, T, N, cu_seqlens != nullptr, p.window, p.sinks);
+  p.far = f.far, p.sink_tiles = f.sink_tiles, p.sink_rows = f.sink_rows, p.pieces = f.pieces;
+  const int64_t q_groups = job_groups(HKV, HQ / HKV, p.q_tiles);
+  const int64_t k_groups = job_groups(HKV, 1, p.k_tiles + p.pieces * p.sink_tiles), s_groups = N * HKV * p.sink_tiles;
+  if (q_groups > kMaxGroups256 || k_groups > kMaxGroups256 || s_groups > kMaxGroups256) {
+    gdn_internal_set_error("gdn_window_attn_bwd: grid too large");
+    return GDN_ERR_UNSUPPORTED;
+  }
+  if (!f.sink_tiles) p.sink_tiles = 1, p.pieces = 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 block(256);
+  if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<128>, dim3((unsigned)q_groups), block, 0, s, p);
+  else hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<64>, dim3((unsigned)q_groups), block, 0, s, p);
+  if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dq_kernel")) return rc;
+  if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<128>, dim3((unsigned)k_groups), block, 0, s, p);
+  else hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<64>, dim3((unsigned)k_groups), block, 0, s, p);
+  if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dkv_kernel")) return rc;
+  if (f.sink_tiles) {
+    hipLaunchKernelGGL(gated_delta_window_attn_sinks_kernel, dim3((unsigned)s_groups), block, 0, s, p, (int)D);
+    return gdn_internal_check_launch("gated_delta_window_attn_sinks_kernel");
+  }
+  return GDN_OK;
+}
