@@ -449,7 +449,8 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          if (ko > hi || (ko <= lo && ko >= sk) || (PAGED && !(ok >> (2 * kt + (e >> 3)) & 1))) s[kt][e] = -INFINITY;
+          const bool seen = (ko <= hi) & ((ko > lo) | (ko < sk)) & (!PAGED | ((ok >> (2 * kt + (e >> 3)) & 1) != 0));
+          s[kt][e] = seen ? s[kt][e] : -INFINITY;
         }
     }
     softmax_step<2, D, E>(s, acc, m, l, c, slack, vb, rd);

@@ -218,19 +218,19 @@ __device__ __forceinline__ bool few_plan(const FewParams& p, int64_t job, FewPla
 
 // What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
 struct RowView {
-  int place, base;
+  int place, base;  // base: the first drafted token's place; without a tree behind every place
   uint64_t bits;
-  bool tree;
   __device__ __forceinline__ bool operator()(int j, int window, int sinks) const {
-    if (!tree) return sees(place, j, window, sinks);
     const int n = j - base;
-    return n < 0 ? sees(place, j, window, sinks) : n < 64 && (bits >> n & 1);
+    const bool by_place = (j <= place) & ((place - j < window) | (j < sinks));
+    return ((n < 0) & by_place) | ((n >= 0) & (n < 64) & ((bits >> (n & 63) & 1) != 0));
   }
 };
 __device__ __forceinline__ RowView few_view(const FewParams& p, const FewPlan& f, int row) {
   const int token = row / (p.HQ / p.HKV);
-  RowView v{f.base + token, f.base, 0, p.tree != nullptr};
+  RowView v{f.base + token, kFar, 0};
   if (p.tree) {
+    v.base = f.base;
     v.bits = (uint64_t)p.tree[f.sq.row * p.tb + (f.sq.start + token) * p.tt];
     if (f.sq.len < 64) v.bits &= (1ull << f.sq.len) - 1;
     v.place = f.base + __popcll(v.bits) - 1;
@@ -334,7 +334,8 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int j = k0 + 8 * (e >> 2) + 4 * hh + (e & 3);
-        if (j >= f.klen || !(ok >> (e >> 3) & 1) || !view(j, p.window, p.sinks)) s[0][e] = -INFINITY;
+        const bool seen = view(j, p.window, p.sinks) & (j < f.klen) & ((ok >> (e >> 3) & 1) != 0);
+        s[0][e] = seen ? s[0][e] : -INFINITY;
       }
     }
     softmax_step<1, D, E>(s, acc, m, l, c, slack, vc, rd);

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          if (ko > hi || (ko <= lo && ko >= sk)) s[e] = 0.f;
+          s[e] = ((ko <= hi) & ((ko > lo) | (ko < sk))) ? s[e] : 0.f;
         }
       }
       bf16x8 pb[2];
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(Win
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          if (qo < lo || qo >= hi) s[e] = 0.f;
+          s[e] = ((qo >= lo) & (qo < hi)) ? s[e] : 0.f;
         }
       }
       bf16x8 pb[2];
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(Win
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          if (qo < lo || qo >= hi) s[e] = 0.f;
+          s[e] = ((qo >= lo) & (qo < hi)) ? s[e] : 0.f;
         }
       }
       pack16<bf16>(s, pb);

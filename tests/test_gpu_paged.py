@@ -185,8 +185,10 @@ def _normed(x, w):
 
 
 def test_a_prompt_in_pieces_then_single_tokens():
-    """Appends and attention as a server makes them give what the whole sequence gives at once."""
+    """Appends and attention as a server makes them, and what the whole sequence gives at once. Both round the rotated rows
+    once from fp32, but sum a product pair in either order, so they are compared with 64 bits and not with one another."""
     from sorernn_amd import qk_norm_rope, window_attention
+    from tests.window_ref import window_attention as whole_reference
 
     gen = torch.Generator(DEV).manual_seed(5)
     total, hq, hkv, d, win, sinks = 700, 4, 2, 128, 150, 3
@@ -195,15 +197,19 @@ def test_a_prompt_in_pieces_then_single_tokens():
     qr, kr = qk_norm_rope(q, k, qw, kw, rot_dim=32)
     whole = window_attention(qr, kr, v, window=win, sinks=sinks)
     kc, vc, table = _cache(1, total, hkv, d, 16, torch.bfloat16, gen)
-    at, pieces = 0, []
+    at, rows, pieces = 0, [], []
     for t in (300, 1, 257, 5) + (1,) * 137:
         part = slice(at, at + t)
         at += t
         lengths = torch.tensor([at], device=DEV)
-        qn = paged_kv_append(k[:, part], v[:, part], kc, vc, table, lengths, q=q[:, part], q_weight=qw, k_weight=kw, rot_dim=32)
-        assert torch.equal(qn, qr[:, part])
-        pieces.append(paged_attention(qn, kc, vc, table, lengths, window=win, sinks=sinks))
-    assert at == total and torch.equal(gather(kc, table[0], total), kr[0]) and torch.equal(gather(vc, table[0], total), v[0])
-    ref = reference(qr, kc, vc, table, torch.tensor([total]), win, sinks, d**-0.5)
-    check(torch.cat(pieces, 1), ref, "o")
-    check(whole, ref, "o")
+        rows.append(paged_kv_append(k[:, part], v[:, part], kc, vc, table, lengths, q=q[:, part], q_weight=qw, k_weight=kw,
+                                    rot_dim=32))
+        pieces.append(paged_attention(rows[-1], kc, vc, table, lengths, window=win, sinks=sinks))
+    assert at == total and torch.equal(gather(vc, table[0], total), v[0])
+    place = torch.arange(total, device=DEV)[None]
+    cached = gather(kc, table[0], total)[None]
+    rows = torch.cat(rows, 1)
+    check_rows(rows, norm_rope(q, qw, place, 32, 1e7, 1e-6), "y", (d + 24) * U)
+    check_rows(cached, norm_rope(k, kw, place, 32, 1e7, 1e-6), "y", (d + 24) * U)
+    check(torch.cat(pieces, 1), reference(rows, kc, vc, table, torch.tensor([total]), win, sinks, d**-0.5), "o")
+    check(whole, whole_reference(qr, kr, v, win, sinks, d**-0.5), "o")
