@@ -509,8 +509,7 @@ GDN_API int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_
 
 /* Workspace bytes gdn_paged_attn_fwd needs (0 for invalid sizes, or where none is). */
 GDN_API size_t gdn_paged_attn_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
-                                             int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen,
-                                             int tree);
+                                             int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen);
 
 #ifdef __cplusplus
 }

@@ -79,7 +79,7 @@ SIGNATURES = {
     + [_P] + [_I64] * 9 + [_INT, _INT, _D, _F, _U, _P],
     "gdn_paged_attn_fwd": ([_P] + [_I64] * 3) * 3 + [_P, _I64, _P, _INT, _P, _I64, _I64, _P, _P] + [_I64] * 9 + [_INT]
     + [_I64] * 2 + [_F, _U, _P, _SZ, _P],
-    "gdn_paged_attn_workspace_size": [_I64] * 10 + [_INT] * 2,
+    "gdn_paged_attn_workspace_size": [_I64] * 10 + [_INT],
 }
 
 RESTYPES = {

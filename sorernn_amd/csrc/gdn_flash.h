@@ -141,34 +141,32 @@ __device__ __forceinline__ int swz(int r) {
   return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : (((r & 3) << 1) | ((r >> 2) & 1));
 }
 
+// Where a lane reads a tile: the XOR of a chunk number is the XOR of the address, so that three registers hold all of them.
 template <int D>
 struct TileReads {
-  int row[D / 16];     // row fragments: row li, chunk 2 st + hh; + 32 D for the next 32 rows
-  int tr[D / 32][2];   // transposed: rows 4 hh + m (+ 8), 32 columns from 32 d; + 16 D for the next 16 rows
+  int row, tr0, tr1;
   __device__ __forceinline__ void init(int lane) {
     const int hh = lane >> 5, li = lane & 31, gsub = (lane >> 4) & 1, lm = (lane & 15) >> 2, lq = lane & 3;
-#pragma unroll
-    for (int st = 0; st < D / 16; ++st) row[st] = li * D + (((2 * st + hh) ^ swz<D>(li)) << 3);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int h8 = 0; h8 < 2; ++h8) {
-        const int r = 4 * hh + lm + 8 * h8;
-        tr[d][h8] = r * D + (((4 * d + 2 * gsub + (lq >> 1)) ^ swz<D>(r)) << 3) + 4 * (lq & 1);
-      }
+    row = li * D + ((hh ^ swz<D>(li)) << 3);
+    const int r = 4 * hh + lm, ch = 2 * gsub + (lq >> 1);
+    tr0 = r * D + ((ch ^ swz<D>(r)) << 3) + 4 * (lq & 1);
+    tr1 = (r + 8) * D + ((ch ^ swz<D>(r + 8)) << 3) + 4 * (lq & 1);
   }
+  // the same, with the addresses made where they are used instead of being kept in registers over a loop
+  __device__ __forceinline__ TileReads here() const { return TileReads{opaque_int(row), opaque_int(tr0), opaque_int(tr1)}; }
 };
 
-template <typename E>
-__device__ __forceinline__ typename Pack<E>::x8 row_frag(const E* tile, int off) {
-  return *reinterpret_cast<const typename Pack<E>::x8*>(tile + off);
+// A operand: row li of the 32 from `tile`, k-step st
+template <int D, typename E>
+__device__ __forceinline__ typename Pack<E>::x8 row_frag(const E* tile, const TileReads<D>& rd, int st) {
+  return *reinterpret_cast<const typename Pack<E>::x8*>(tile + (rd.row ^ (16 * st)));
 }
-// A operand of the transposed tile's 16 rows from `rows` (in elements: 16 D per step): lane li holds column 32 d + li, k in the
-// order 4 hh + r, 8 + 4 hh + r, which is the accumulator's own row order
-template <typename E>
-__device__ __forceinline__ typename Pack<E>::x8 tr_frag(const E* tile, const int (&off)[2]) {
-  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off[0]));
-  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + off[1]));
+// A operand of the transposed 16 rows from `tile`: lane li holds column 32 d + li, k in the order 4 hh + r, 8 + 4 hh + r, which
+// is the accumulator's own row order
+template <int D, typename E>
+__device__ __forceinline__ typename Pack<E>::x8 tr_frag(const E* tile, const TileReads<D>& rd, int d) {
+  const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + (rd.tr0 ^ (32 * d))));
+  const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + (rd.tr1 ^ (32 * d))));
   return __builtin_bit_cast(typename Pack<E>::x8, bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
@@ -228,7 +226,7 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] = mma32(tr_frag(vb + (2 * kt + h) * 16 * D, rd.tr[d]), pb[h], acc[d]);
+      for (int d = 0; d < D / 32; ++d) acc[d] = mma32(tr_frag(vb + (2 * kt + h) * 16 * D, rd, d), pb[h], acc[d]);
   }
 }
 
@@ -285,7 +283,7 @@ __device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
   return z == 0.f;
 }
 
-// ------------------------------------------------------------------------------------------------ forward over whole tiles
+// ------------------------------------------------------------------------------------------------ parameters and plans
 // Strides in elements; k and v of a paged cache: between pages, tokens of a page, heads.
 struct FlashParams {
   const void *q, *k, *v;
@@ -296,11 +294,15 @@ struct FlashParams {
   int64_t B, tiles;
   int HQ, HKV, parts, window, sinks;
   float scale_log2;
-  // paged
+  // paged: the table, the sequences' lengths, and how the work on their keys is cut
   const int* table;
   int64_t table_stride;
   const void* lengths;
   int len_i32, width, shift, pages;
+  const int64_t* tree;  // [B, T] bits of the sequence's drafted tokens that each sees, or null
+  int64_t tb, tt;
+  int splits;
+  float* part;          // [tiles HKV][splits][rows a tile][D], then [tiles HKV][splits][2][rows a tile]: O, maximum and sum
 };
 
 // Entry `at` of a row of a page table, `at` the same in every lane: through the scalar cache, apart from the vector loads that
@@ -316,12 +318,75 @@ __device__ __forceinline__ int cache_length(const void* lengths, int i32, int se
   return (int)(x < 0 ? 0 : x > most ? most : x);
 }
 
-constexpr int kBQ = 128;  // queries a workgroup: 32 a wave
+// A tile of ROWS rows (token, q head of the group) of a sequence's new tokens over a kv head of the cache: the blocks of BK
+// keys that they see, cut into runs.
+struct PagedPlan {
+  Seq sq;
+  int hkv, row0, rows;     // rows of this tile
+  int klen, base;          // keys; place of the first new token
+  int first, last;         // places that its rows see from: all of them lie between
+  Blocks bl;
+  int per, used;           // blocks a run, runs with any
+  int64_t job;
+};
+template <int ROWS, int BK>
+__device__ __forceinline__ bool paged_plan(const FlashParams& p, int64_t t, int hkv, PagedPlan& f) {
+  const int rep = p.HQ / p.HKV;
+  f.job = t * p.HKV + hkv;
+  f.hkv = hkv;
+  if (p.seqs.cu) {
+    f.sq = packed_tile(p.seqs, t, rep, ROWS);
+  } else {
+    const int64_t per = (p.seqs.T * rep + ROWS - 1) / ROWS, row = t / per;
+    f.sq = Seq{row, 0, (int)p.seqs.T, (int)row, (int)(t - row * per)};
+  }
+  if (f.sq.tile >= kFar / ROWS) return false;
+  f.row0 = f.sq.tile * ROWS;
+  const int64_t left = (int64_t)f.sq.len * rep - f.row0;
+  f.rows = (int)(left < ROWS ? left : ROWS);
+  if (f.rows <= 0) return false;
+  f.klen = f.sq.num < 0 ? 0 : cache_length(p.lengths, p.len_i32, f.sq.num, p.width, p.shift);
+  f.base = f.klen - f.sq.len;
+  // a drafted token stands behind as many others as it sees; one that sees none at the committed tokens' end
+  f.first = p.tree ? f.base - 1 : f.base + f.row0 / rep;
+  f.last = p.tree ? f.klen - 1 : f.base + (f.row0 + f.rows - 1) / rep;
+  f.bl = blocks_of<BK>(f.first, f.last, p.window, p.sinks);
+  if (f.sq.num < 0) f.bl.count = 0;
+  f.per = imax((f.bl.count + p.splits - 1) / p.splits, 4);
+  f.used = imax((f.bl.count + f.per - 1) / f.per, 1);
+  return true;
+}
+
+// What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
+struct RowView {
+  int place, base;  // base: the first drafted token's place; without a tree behind every place
+  uint64_t bits;
+  __device__ __forceinline__ bool operator()(int j, int window, int sinks) const {
+    const int n = j - base;
+    const bool by_place = (j <= place) & ((place - j < window) | (j < sinks));
+    return ((n < 0) & by_place) | ((n >= 0) & (n < 64) & ((bits >> (n & 63) & 1) != 0));
+  }
+};
+__device__ __forceinline__ RowView row_view(const FlashParams& p, const PagedPlan& f, int row) {
+  const int token = row / (p.HQ / p.HKV);
+  RowView v{f.base + token, kFar, 0};
+  if (p.tree) {
+    v.base = f.base;
+    v.bits = (uint64_t)p.tree[f.sq.row * p.tb + (f.sq.start + token) * p.tt];
+    if (f.sq.len < 64) v.bits &= (1ull << f.sq.len) - 1;
+    v.place = f.base + __popcll(v.bits) - 1;
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------------ forward over whole tiles
+constexpr int kBQ = 128;  // rows a workgroup: 32 a wave
 constexpr int kBK = 64;   // keys a block
 
-// O = softmax(scale Q K^T) V over the keys that a query sees. A workgroup of 4 waves takes 128 queries of one head, a wave 32
-// of them in registers; blocks of 64 keys pass through LDS, loaded straight from memory one block ahead. S^T = K Q^T puts one
-// query into each lane's column: maximum, sum and rescaling are a lane's own, and P^T is the next product's operand as it is.
+// O = softmax(scale Q K^T) V over the keys that a row sees. A workgroup of 4 waves takes 128 rows, a wave 32 of them in
+// registers: queries of one head, or of a paged cache new tokens with the heads of a group. Blocks of 64 keys pass through LDS,
+// loaded straight from memory one block ahead. S^T = K Q^T puts one row into each lane's column: maximum, sum and rescaling
+// are a lane's own, and P^T is the next product's operand as it is.
 template <int D, typename E, bool PAGED>
 __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* Ks1, E* Vs0, E* Vs1) {
   using X8 = typename Pack<E>::x8;
@@ -330,39 +395,66 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
   const int rep = p.HQ / p.HKV;
   Job job;
-  if (!job_of(blockIdx.x, p.HKV, rep, p.parts, p.tiles, job)) return;
+  PagedPlan f;
   Seq sq;
-  if (p.seqs.cu) {
-    sq = packed_tile(p.seqs, job.tile, 1, kBQ);
-  } else {  // the last tiles, which see most, first
-    const int64_t per = (p.seqs.T + kBQ - 1) / kBQ;
-    sq.row = job.tile % p.B;
-    sq.start = 0;
-    sq.len = (int)p.seqs.T;
-    sq.num = (int)sq.row;
-    sq.tile = (int)(per - 1 - job.tile / p.B);
-  }
-  const int q0 = sq.tile * kBQ, hq = job.hkv * rep + job.hm;
-  if (q0 >= sq.len) return;
-  const int q1 = imin(q0 + kBQ, sq.len) - 1;
-  int klen = sq.num < 0 ? 0 : sq.len, pos0 = 0;
+  int row0, rows, klen, split = 0, n0 = 0, n1;
+  Blocks bl;
   const int* table = nullptr;
-  if (PAGED) {
-    klen = sq.num < 0 ? 0 : cache_length(p.lengths, p.len_i32, sq.num, p.width, p.shift);
-    pos0 = klen - sq.len;
+  RowView view;
+  int wq0, wq1;  // places of the wave's first and last row
+  bool tree = false;
+  if constexpr (PAGED) {
+    const int64_t jobs = gridDim.x / p.splits;
+    split = (int)(blockIdx.x / jobs);
+    if (!job_of(blockIdx.x - split * jobs, p.HKV, 1, p.parts, p.tiles, job)) return;
+    if (!paged_plan<kBQ, kBK>(p, job.tile, job.hkv, f) || split >= f.used) return;
+    sq = f.sq;
+    row0 = f.row0;
+    rows = f.rows;
+    klen = f.klen;
+    bl = f.bl;
+    n0 = split * f.per;
+    n1 = imin(n0 + f.per, bl.count);
     if (sq.num >= 0) table = p.table + sq.num * p.table_stride;
+    tree = p.tree != nullptr;
+    view = row_view(p, f, row0 + imin(32 * w + li, rows - 1));
+    wq0 = tree ? f.first : f.base + (row0 + 32 * w) / rep;
+    wq1 = tree ? f.last : f.base + (row0 + imin(32 * w + 31, rows - 1)) / rep;
+  } else {
+    if (!job_of(blockIdx.x, p.HKV, rep, p.parts, p.tiles, job)) return;
+    if (p.seqs.cu) {
+      sq = packed_tile(p.seqs, job.tile, 1, kBQ);
+    } else {  // the last tiles, which see most, first
+      const int64_t per = (p.seqs.T + kBQ - 1) / kBQ;
+      sq = Seq{job.tile % p.B, 0, (int)p.seqs.T, 0, (int)(per - 1 - job.tile / p.B)};
+    }
+    row0 = sq.tile * kBQ;
+    rows = imin(kBQ, sq.len - row0);
+    if (rows <= 0) return;
+    klen = sq.num < 0 ? 0 : sq.len;
+    wq0 = row0 + 32 * w;
+    wq1 = row0 + imin(32 * w + 31, rows - 1);
+    view = RowView{row0 + imin(32 * w + li, rows - 1), kFar, 0};
+    bl = blocks_of<kBK>(row0, row0 + rows - 1, p.window, p.sinks);
+    if (sq.num < 0) bl.count = 0;
+    n1 = bl.count;
   }
-  Blocks bl = blocks_of<kBK>(pos0 + q0, pos0 + q1, p.window, p.sinks);
-  if (sq.num < 0) bl.count = 0;
-
-  const int qr = q0 + 32 * w + li, qi = pos0 + qr;  // the lane's query: row of the sequence, place
-  const int wq0 = pos0 + q0 + 32 * w, wq1 = imin(wq0 + 31, pos0 + q1);
-  const bool wave_live = wq0 <= wq1;
-  const int64_t tok = sq.row * p.seqs.T + sq.start;  // flat number of the sequence's first token
-  const E* qrow = static_cast<const E*>(p.q) + sq.row * p.qsb + (sq.start + imin(qr, sq.len - 1)) * p.qst + hq * p.qsh;
+  const bool wave_live = 32 * w < rows, row_ok = 32 * w + li < rows;
+  // row r of the tile: which token and q head
+  auto token_of = [&](int r) { return PAGED ? (row0 + r) / rep : row0 + r; };
+  auto head_of = [&](int r) { return job.hkv * rep + (PAGED ? (row0 + r) % rep : job.hm); };
+  auto q_at = [&](int r) {
+    return static_cast<const E*>(p.q) + sq.row * p.qsb + (sq.start + token_of(r)) * p.qst + head_of(r) * p.qsh;
+  };
+  auto o_at = [&](int r) {
+    return static_cast<E*>(p.o) + ((sq.row * p.seqs.T + sq.start + token_of(r)) * p.HQ + head_of(r)) * D;
+  };
   X8 qf[DS];
+  {
+    const E* q = q_at(imin(32 * w + li, rows - 1));
 #pragma unroll
-  for (int s = 0; s < DS; ++s) qf[s] = *reinterpret_cast<const X8*>(qrow + 16 * s + 8 * hh);
+    for (int s = 0; s < DS; ++s) qf[s] = *reinterpret_cast<const X8*>(q + 16 * s + 8 * hh);
+  }
 
   // load u of wave w fills LDS bytes [(w + 4u) KB, + 1 KB) of a block: rows (w + 4u) RPL + lane / CPR. The lane's chunk does not
   // depend on u.
@@ -397,17 +489,18 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
       for (int u = 0; u < LPT; ++u) {
         const int g = D == 128 ? u : 2 * u + (w >> 1), id = D == 128 ? pid[u] : (w >> 1) ? pid[2 * u + 1] : pid[2 * u];
-        const int key = key0 + 16 * g, rows = imin(16, klen - key), in = key & ((1 << p.shift) - 1);
-        const int64_t page = id < 0 ? 0 : id;
-        const auto rk = make_rsrc(kbase + page * p.ksb * 2 + (int64_t)in * kst, id < 0 || rows <= 0 ? 0u : (uint32_t)((rows - 1) * kst + 2 * D));
-        const auto rv = make_rsrc(vbase + page * p.vsb * 2 + (int64_t)in * vst, id < 0 || rows <= 0 ? 0u : (uint32_t)((rows - 1) * vst + 2 * D));
+        const int key = key0 + 16 * g, left = imin(16, klen - key), in = key & ((1 << p.shift) - 1);
+        const bool any = id >= 0 && left > 0;
+        const int64_t page = any ? id : 0;
+        const auto rk = make_rsrc(kbase + page * p.ksb * 2 + (int64_t)in * kst, any ? (uint32_t)((left - 1) * kst + 2 * D) : 0u);
+        const auto rv = make_rsrc(vbase + page * p.vsb * 2 + (int64_t)in * vst, any ? (uint32_t)((left - 1) * vst + 2 * D) : 0u);
         load_lds16(rk, kd + (w + 4 * u) * 512, koff);
         load_lds16(rv, vd + (w + 4 * u) * 512, voff);
       }
     } else {
-      const int rows = imin(kBK, klen - key0);
-      const auto rk = make_rsrc(kbase + (int64_t)key0 * kst, (uint32_t)((rows - 1) * kst + 2 * D));
-      const auto rv = make_rsrc(vbase + (int64_t)key0 * vst, (uint32_t)((rows - 1) * vst + 2 * D));
+      const int left = imin(kBK, klen - key0);
+      const auto rk = make_rsrc(kbase + (int64_t)key0 * kst, (uint32_t)((left - 1) * kst + 2 * D));
+      const auto rv = make_rsrc(vbase + (int64_t)key0 * vst, (uint32_t)((left - 1) * vst + 2 * D));
 #pragma unroll
       for (int u = 0; u < LPT; ++u) {
         load_lds16(rk, kd + (w + 4 * u) * 512, koff + u * 4 * RPL * kst);
@@ -440,16 +533,20 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     for (int kt = 0; kt < 2; ++kt) {
       s[kt] = f32x16{};
 #pragma unroll
-      for (int st = 0; st < DS; ++st) s[kt] = mma32(row_frag(kb + 32 * kt * D, rd.row[st]), qf[st], s[kt]);
+      for (int st = 0; st < DS; ++st) s[kt] = mma32(row_frag(kb + 32 * kt * D, rd, st), qf[st], s[kt]);
     }
-    if (masked) {
-      const int hi = qi - k0, lo = qi - p.window - k0, sk = p.sinks - k0;  // seen: <= hi and (> lo or < sk)
+    if (masked) {  // selects throughout: branches a lane apart cost more than the comparisons
+      const int hi = view.place - k0, lo = hi - p.window, sk = p.sinks - k0;  // seen: <= hi and (> lo or < sk)
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          const bool seen = (ko <= hi) & ((ko > lo) | (ko < sk)) & (!PAGED | ((ok >> (2 * kt + (e >> 3)) & 1) != 0));
+          bool seen = (ko <= hi) & ((ko > lo) | (ko < sk));
+          if (PAGED) {
+            if (tree) seen = view(k0 + ko, p.window, p.sinks);
+            seen &= (k0 + ko < klen) & ((ok >> (2 * kt + (e >> 3)) & 1) != 0);
+          }
           s[kt][e] = seen ? s[kt][e] : -INFINITY;
         }
     }
@@ -458,11 +555,11 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   int ok = 15, ok_next = 15;  // of the block being used and of the one being loaded
   auto step = [&](int n, const E* kc, const E* vc, E* kn, E* vn) {
     const int jb = bl.at(n), next = bl.at(n + 1);
-    const bool more = n + 1 < bl.count;
+    const bool more = n + 1 < n1;
     if (more) {
       ok_next = ok_bits();
       fetch(next, kn, vn);
-      if (n + 2 < bl.count) look_up(bl.at(n + 2));
+      if (n + 2 < n1) look_up(bl.at(n + 2));
     }
     const int k0 = jb * kBK, k1 = k0 + kBK - 1;
     if (wave_live && !none_sees(wq0, wq1, k0, k1, p.window, p.sinks))
@@ -472,45 +569,65 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     ok = ok_next;
     __syncthreads();
   };
-  if (bl.count > 0) {
-    look_up(bl.at(0));
+  if (n0 < n1) {
+    look_up(bl.at(n0));
     ok = ok_bits();
-    fetch(bl.at(0), Ks0, Vs0);
-    if (bl.count > 1) look_up(bl.at(1));
+    fetch(bl.at(n0), Ks0, Vs0);
+    if (n0 + 1 < n1) look_up(bl.at(n0 + 1));
     wait_loads();
-    clean(bl.at(0), ok, Vs0);
+    clean(bl.at(n0), ok, Vs0);
     __syncthreads();
-    for (int n = 0; n < bl.count; n += 2) {
+    for (int n = n0; n < n1; n += 2) {
       step(n, Ks0, Vs0, Ks1, Vs1);
-      if (n + 1 < bl.count) step(n + 1, Ks1, Vs1, Ks0, Vs0);
+      if (n + 1 < n1) step(n + 1, Ks1, Vs1, Ks0, Vs0);
     }
   }
 
-  // O = O^T / l; the lane holds its query's columns 32 d + 8 j + 4 hh + r
+  // O = O^T / l; the lane holds its row's columns 32 d + 8 j + 4 hh + r. Of several runs each leaves O, m and l.
+  const bool whole = !PAGED || f.used == 1;
+  float *po = nullptr, *pml = nullptr;
+  if constexpr (PAGED) {
+    po = p.part + (f.job * p.splits + split) * kBQ * D;
+    pml = p.part + p.tiles * p.HKV * p.splits * kBQ * D + (f.job * p.splits + split) * 2 * kBQ;
+  }
   l += __shfl_xor(l, 32, kWave);
-  const bool row_ok = qr < sq.len && wave_live;
   bool fine = finite_all(acc) && finite_f(l);
   fine = __shfl_xor((int)fine, 32, kWave) && fine;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  E* orow = static_cast<E*>(p.o) + ((tok + qr) * p.HQ + hq) * D;
+  const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;
+  const int r = 32 * w + li;
   if (row_ok && fine) {
+    if (whole) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      E* const to = o_at(r);
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        X4 x;
+        for (int j = 0; j < 4; ++j) {
+          X4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = (E)(acc[d][4 * j + r] * inv);
-        *reinterpret_cast<X4*>(orow + 32 * d + 8 * j + 4 * hh) = x;
+          for (int e = 0; e < 4; ++e) x[e] = (E)(acc[d][4 * j + e] * inv);
+          *reinterpret_cast<X4*>(to + 32 * d + 8 * j + 4 * hh) = x;
+        }
+      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : INFINITY;
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4*>(po + r * D + 32 * d + 8 * j + 4 * hh) =
+              f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+      if (hh == 0) {
+        pml[r] = m;
+        pml[kBQ + r] = l;
       }
-    if (p.lse && hh == 0) p.lse[hq * p.B * p.seqs.T + tok + qr] = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : INFINITY;
+    }
   }
   uint64_t redo = __ballot(row_ok && !fine && hh == 0);
   while (redo) {
-    const int n = __ffsll((unsigned long long)redo) - 1;
+    const int n = __ffsll((unsigned long long)redo) - 1, rr = 32 * w + n;
     redo &= redo - 1;
-    const int r = q0 + 32 * w + n, place = pos0 + r;
-    const E* qp = static_cast<const E*>(p.q) + sq.row * p.qsb + (sq.start + r) * p.qst + hq * p.qsh;
+    RowView v{row0 + rr, kFar, 0};
+    if constexpr (PAGED) v = row_view(p, f, row0 + rr);
     auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
       if (!PAGED) return reinterpret_cast<const E*>(base + j * row_bytes);
       const int id = table[j >> p.shift];
@@ -518,12 +635,23 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
                                      : reinterpret_cast<const E*>(base + id * page_bytes + (j & ((1 << p.shift) - 1)) * row_bytes);
     };
     float mr = -INFINITY, lr = 0.f, a[D / 64] = {};
-    slow_row<D, E>(qp, 0, place + 1, [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
-                   [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); },
-                   [&](int j) { return sees(place, j, p.window, p.sinks); }, c, mr, lr, a);
-    E* to = static_cast<E*>(p.o) + ((tok + r) * p.HQ + hq) * D;
-    for (int i = 0; i < D / 64; ++i) to[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
-    if (p.lse && lane == 0) p.lse[hq * p.B * p.seqs.T + tok + r] = lr == 0.f ? INFINITY : mr * c + __builtin_amdgcn_logf(lr);
+    for (int b = n0; b < n1; ++b) {
+      const int k0 = bl.at(b) * kBK;
+      slow_row<D, E>(q_at(rr), k0, imin(k0 + kBK, klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
+                     [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); }, c,
+                     mr, lr, a);
+    }
+    if (whole) {
+      for (int i = 0; i < D / 64; ++i) o_at(rr)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+      if (!PAGED && p.lse && lane == 0)
+        p.lse[head_of(rr) * all + tok + token_of(rr)] = lr == 0.f ? INFINITY : mr * c + __builtin_amdgcn_logf(lr);
+    } else {
+      for (int i = 0; i < D / 64; ++i) po[rr * D + lane + 64 * i] = a[i];
+      if (lane == 0) {
+        pml[rr] = mr;
+        pml[kBQ + rr] = lr;
+      }
+    }
   }
 }
 

@@ -160,7 +160,8 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
   }
 }
 
-// ------------------------------------------------------------------------------------------------ attention, many new tokens
+// ------------------------------------------------------------------------------------------------ attention, many rows
+// Tiles of 128 rows (token, q head of the group) of a kv head; where they are few their keys are cut into `splits` runs.
 template <int D, typename E>
 __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashParams p) {
   __shared__ __align__(16) E Ks0[kBK * D];
@@ -174,72 +175,10 @@ __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashPar
 // A kv head's new rows (token, q head of the group) in tiles of 32; the keys that they see in blocks of 32, cut into `splits`
 // runs, a workgroup each. Every wave takes blocks of its own, loaded straight into its own LDS one ahead: no barrier until the
 // four waves' sums meet, 128 KB a CU under way. Bound by the cache's bytes.
-struct FewParams : FlashParams {
-  const int64_t* tree;  // [B, T] bits of the sequence's drafted tokens that each sees, or null
-  int64_t tb, tt;
-  int splits;
-  float* part;          // [tiles HKV][splits][32][D], then [tiles HKV][splits][2][32]
-};
-
 constexpr int kFewRows = 32, kFewKeys = 32;
 
-struct FewPlan {
-  Seq sq;
-  int hkv, row0, rows, klen, base;  // rows of this tile; keys; place of the first new token
-  Blocks bl;
-  int per, used;                    // blocks a split, splits with any
-  int64_t job;
-};
-__device__ __forceinline__ bool few_plan(const FewParams& p, int64_t job, FewPlan& f) {
-  const int rep = p.HQ / p.HKV;
-  f.job = job;
-  const int64_t t = job / p.HKV;
-  f.hkv = (int)(job - t * p.HKV);
-  if (p.seqs.cu) {
-    f.sq = packed_tile(p.seqs, t, rep, kFewRows);
-  } else {
-    const int64_t per = (p.seqs.T * rep + kFewRows - 1) / kFewRows, row = t / per;
-    f.sq = Seq{row, 0, (int)p.seqs.T, (int)row, (int)(t - row * per)};
-  }
-  if (f.sq.tile >= kFar / kFewRows) return false;
-  f.row0 = f.sq.tile * kFewRows;
-  f.rows = (int)((int64_t)f.sq.len * rep - f.row0 < kFewRows ? (int64_t)f.sq.len * rep - f.row0 : kFewRows);
-  if (f.rows <= 0) return false;
-  f.klen = f.sq.num < 0 ? 0 : cache_length(p.lengths, p.len_i32, f.sq.num, p.width, p.shift);
-  f.base = f.klen - f.sq.len;
-  // a drafted token stands behind as many others as it sees; a row of the tree without bits at the committed tokens' end
-  const int first = p.tree ? f.base - 1 : f.base + f.row0 / rep, last = p.tree ? f.klen - 1 : f.base + (f.row0 + f.rows - 1) / rep;
-  f.bl = blocks_of<kFewKeys>(first, last, p.window, p.sinks);
-  if (f.sq.num < 0) f.bl.count = 0;
-  f.per = imax((f.bl.count + p.splits - 1) / p.splits, 4);
-  f.used = imax((f.bl.count + f.per - 1) / f.per, 1);
-  return true;
-}
-
-// What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
-struct RowView {
-  int place, base;  // base: the first drafted token's place; without a tree behind every place
-  uint64_t bits;
-  __device__ __forceinline__ bool operator()(int j, int window, int sinks) const {
-    const int n = j - base;
-    const bool by_place = (j <= place) & ((place - j < window) | (j < sinks));
-    return ((n < 0) & by_place) | ((n >= 0) & (n < 64) & ((bits >> (n & 63) & 1) != 0));
-  }
-};
-__device__ __forceinline__ RowView few_view(const FewParams& p, const FewPlan& f, int row) {
-  const int token = row / (p.HQ / p.HKV);
-  RowView v{f.base + token, kFar, 0};
-  if (p.tree) {
-    v.base = f.base;
-    v.bits = (uint64_t)p.tree[f.sq.row * p.tb + (f.sq.start + token) * p.tt];
-    if (f.sq.len < 64) v.bits &= (1ull << f.sq.len) - 1;
-    v.place = f.base + __popcll(v.bits) - 1;
-  }
-  return v;
-}
-
 template <int D, typename E>
-__global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewParams p) {
+__global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FlashParams p) {
   using X8 = typename Pack<E>::x8;
   constexpr int DS = D / 16, DT = D / 32, CPR = D / 8, RPL = 512 / D, LPB = kFewKeys / RPL, TILE = kFewKeys * D, CH = D / 4;
   __shared__ __align__(16) E K0[4 * TILE];
@@ -250,13 +189,14 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
   __shared__ uint32_t redo_rows;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
   const int rep = p.HQ / p.HKV;
-  FewPlan f;
-  const int split = blockIdx.x % p.splits;
-  if (!few_plan(p, blockIdx.x / p.splits, f) || split >= f.used) return;
+  PagedPlan f;
+  const int64_t jobs = p.tiles * p.HKV, job = blockIdx.x % jobs;
+  const int split = (int)(blockIdx.x / jobs);
+  if (!paged_plan<kFewRows, kFewKeys>(p, job / p.HKV, (int)(job % p.HKV), f) || split >= f.used) return;
   const int n0 = split * f.per, n1 = imin(n0 + f.per, f.bl.count);
   const int* const table = f.sq.num >= 0 ? p.table + f.sq.num * p.table_stride : nullptr;
   const int row = f.row0 + imin(li, f.rows - 1);  // the lane's query: token row / rep, head row % rep of the group
-  const RowView view = few_view(p, f, row);
+  const RowView view = row_view(p, f, row);
   auto q_at = [&](int r) {
     return static_cast<const E*>(p.q) + f.sq.row * p.qsb + (f.sq.start + r / rep) * p.qst + (f.hkv * rep + r % rep) * p.qsh;
   };
@@ -305,7 +245,6 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float m = -INFINITY, l = 0.f;
   const float c = p.scale_log2, slack = 8.f / c;
-  const int first = p.tree ? f.base - 1 : f.base + f.row0 / rep, last = p.tree ? f.klen - 1 : f.base + (f.row0 + f.rows - 1) / rep;
   int ok = 3, ok_next = 3;
   auto step = [&](int n, const E* kc, E* vc, E* kn, E* vn) {
     const int k0 = f.bl.at(n) * kFewKeys, k1 = k0 + kFewKeys - 1;
@@ -329,8 +268,8 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
     }
     f32x16 s[1] = {f32x16{}};
 #pragma unroll
-    for (int st = 0; st < DS; ++st) s[0] = mma32(row_frag(kc, rd.row[st]), qf[st], s[0]);
-    if (partial || (p.tree && k1 >= f.base) || !all_see(first, last, k0, k1, p.window, p.sinks)) {
+    for (int st = 0; st < DS; ++st) s[0] = mma32(row_frag(kc, rd, st), qf[st], s[0]);
+    if (partial || (p.tree && k1 >= f.base) || !all_see(f.first, f.last, k0, k1, p.window, p.sinks)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int j = k0 + 8 * (e >> 2) + 4 * hh + (e & 3);
@@ -415,7 +354,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
   for (uint32_t redo = redo_rows; redo; redo &= redo - 1) {  // over the keys that the row sees only
     const int r = __ffs(redo) - 1;
     if (r % 4 != w) continue;
-    const RowView v = few_view(p, f, f.row0 + r);
+    const RowView v = row_view(p, f, f.row0 + r);
     auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
       const int id = table[j >> p.shift];
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
@@ -440,35 +379,54 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(FewP
   }
 }
 
-// The runs' sums of each row at one maximum, in order. A workgroup a tile of rows.
-template <int D, typename E>
-__global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(FewParams p) {
+// The runs' sums of each row at one maximum: D / 4 threads a row, each in `groups` groups that take every groups-th run, so that
+// many runs' loads are under way at once. In a fixed order.
+template <int D, typename E, int ROWS, int BK>
+__global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(FlashParams p, int groups, int passes) {
   constexpr int CH = D / 4;
-  FewPlan f;
-  if (!few_plan(p, blockIdx.x, f) || f.used == 1) return;
-  const int rep = p.HQ / p.HKV;
-  const float* const po = p.part + f.job * p.splits * kFewRows * D;
-  const float* const pml = p.part + p.tiles * p.HKV * p.splits * kFewRows * D + f.job * p.splits * 2 * kFewRows;
-  for (int i = threadIdx.x; i < f.rows * CH; i += 256) {
-    const int r = i / CH, piece = i % CH;
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < f.used; ++s) top = fmaxf(top, pml[s * 2 * kFewRows + r]);
-    f32x4 x{};
-#pragma unroll 8
-    for (int s = 0; s < f.used; ++s) {
-      const float ms = pml[s * 2 * kFewRows + r], a = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - top) * p.scale_log2);
-      sum += a * pml[(s * 2 + 1) * kFewRows + r];
-      x += a * *reinterpret_cast<const f32x4*>(po + (s * kFewRows + r) * D + 4 * piece);
+  __shared__ __align__(16) float xs[256 * 4];
+  __shared__ float ms[256], ls[256];
+  PagedPlan f;
+  const int64_t job = blockIdx.x / passes;
+  if (!paged_plan<ROWS, BK>(p, job / p.HKV, (int)(job % p.HKV), f) || f.used == 1) return;
+  const int t = threadIdx.x, piece = t % CH, g = t / CH % groups, rep = p.HQ / p.HKV;
+  const int r = (int)(blockIdx.x % passes) * (256 / CH / groups) + t / CH / groups;
+  const float* const po = p.part + f.job * p.splits * ROWS * D;
+  const float* const pml = p.part + p.tiles * p.HKV * p.splits * ROWS * D + f.job * p.splits * 2 * ROWS;
+  float top = -INFINITY, sum = 0.f;
+  f32x4 x{};
+  if (r < f.rows) {
+#pragma unroll 4
+    for (int s = g; s < f.used; s += groups) {
+      const float m = pml[s * 2 * ROWS + r], l = pml[(s * 2 + 1) * ROWS + r];
+      const f32x4 y = *reinterpret_cast<const f32x4*>(po + (int64_t)(s * ROWS + r) * D + 4 * piece);
+      const float now = fmaxf(top, m), a = now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2);
+      const float b = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
+      sum = sum * a + l * b;
+      x = x * a + y * b;
+      top = now;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    typename Pack<E>::x4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
-    const int row = f.row0 + r;
-    *reinterpret_cast<typename Pack<E>::x4*>(static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + row / rep) * p.HQ) +
-                                                                     f.hkv * rep + row % rep) * D + 4 * piece) = y;
   }
+  ms[t] = top;
+  ls[t] = sum;
+  *reinterpret_cast<f32x4*>(xs + 4 * t) = x;
+  __syncthreads();
+  if (g || r >= f.rows) return;
+  for (int i = 1; i < groups; ++i) {
+    const int o = t + i * CH;
+    const float m = ms[o], now = fmaxf(top, m), a = now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2);
+    const float b = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
+    sum = sum * a + ls[o] * b;
+    x = x * a + *reinterpret_cast<const f32x4*>(xs + 4 * o) * b;
+    top = now;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  typename Pack<E>::x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
+  const int row = f.row0 + r;
+  *reinterpret_cast<typename Pack<E>::x4*>(static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + row / rep) * p.HQ) +
+                                                                   f.hkv * rep + row % rep) * D + 4 * piece) = y;
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -515,36 +473,34 @@ static bool rows_ok(const int64_t* st, int n, uintptr_t all) {
   return !(all & 15);
 }
 
-struct FewSize {
+// How a call is cut: tiles of `rows` rows, blocks of `keys` keys, `splits` runs of them a tile.
+struct PagedCut {
+  int rows, keys, splits;
   int64_t tiles;
-  int splits;
 };
-// Runs of keys a tile: about kFewGroups workgroups in all, each with 4 blocks at least, one a wave.
-constexpr int64_t kFewGroups = 1024;
-static FewSize few_size(int64_t T, int64_t B, int64_t HQ, int64_t HKV, int64_t N, bool varlen, int64_t keys) {
-  const int64_t rep = HQ / HKV;
-  const int64_t tiles = varlen ? packed_tiles(T, N, (int)rep, kFewRows) : B * ((T * rep + kFewRows - 1) / kFewRows);
-  const int64_t busy = varlen ? (T * rep + kFewRows - 1) / kFewRows + N : tiles;
-  const int64_t blocks = (keys + kFewKeys - 1) / kFewKeys + 1;
-  int64_t splits = (kFewGroups + busy * HKV - 1) / (busy * HKV);
-  if (splits > (blocks + 3) / 4) splits = (blocks + 3) / 4;
-  if (splits < 1) splits = 1;
-  return {tiles, (int)splits};
-}
-
-// Whole tiles of queries a head share what they load among 128 of them; few new tokens' rows are taken together with their
-// group's heads and the keys cut into runs instead.
-static bool takes_few(int64_t T, int64_t HQ, int64_t HKV, int64_t N, bool varlen, bool tree) {
-  const int64_t tokens = varlen ? (T + N - 1) / N : T;
-  return tree || tokens * (HQ / HKV) <= 256;
-}
-
-// keys that a row can see at most
-static int64_t most_keys(int64_t T, int64_t width, int64_t page_size, int64_t window, int64_t sinks) {
-  const int64_t all = width * page_size;
-  if (window <= 0 || window >= all) return all;
-  const int64_t some = window + T + (sinks < all ? sinks : all);
-  return some < all ? some : all;
+// Up to this many rows (new tokens times heads of a group) a sequence, tiles of 32 with a run of keys a wave; else tiles of 128
+// that share what they load.
+constexpr int64_t kFewMost = 64;
+// Workgroups that the runs are to make, in all; a run has 4 blocks at least.
+constexpr int64_t kFewGroups = 1024, kManyGroups = 1024;
+static PagedCut paged_cut(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t N, bool varlen, int64_t page_size, int64_t width,
+                          int64_t window, int64_t sinks) {
+  const int64_t rep = HQ / HKV, tokens = varlen ? (T + N - 1) / N : T;
+  PagedCut c{};
+  const bool few = tokens * rep <= kFewMost;
+  c.rows = few ? kFewRows : kBQ;
+  c.keys = few ? kFewKeys : kBK;
+  c.tiles = varlen ? packed_tiles(T, N, (int)rep, c.rows) : B * ((T * rep + c.rows - 1) / c.rows);
+  const int64_t busy = (varlen ? (T * rep + c.rows - 1) / c.rows + N : c.tiles) * HKV;  // about as many do anything
+  int64_t keys = width * page_size;  // that a tile sees at most
+  if (window > 0 && window < keys) {
+    const int64_t some = window + c.rows / rep + 1 + (sinks < keys ? sinks : keys);
+    if (some < keys) keys = some;
+  }
+  const int64_t blocks = (keys + c.keys - 1) / c.keys + 1, most = (blocks + 3) / 4;
+  int64_t splits = ((few ? kFewGroups : kManyGroups) + busy - 1) / busy;
+  c.splits = (int)(splits > most ? most : splits);
+  return c;
 }
 
 }  // namespace gdn
@@ -604,12 +560,10 @@ extern "C" int gdn_paged_append(const void* q, int64_t q_batch_stride, int64_t q
 }
 
 extern "C" size_t gdn_paged_attn_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
-                                                int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen,
-                                                int tree) {
+                                                int64_t page_size, int64_t width, int64_t window, int64_t sinks, int varlen) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || D <= 0 || N <= 0 || page_size <= 0 || width <= 0) return 0;
-  if (!takes_few(T, HQ, HKV, N, varlen != 0, tree != 0)) return 0;
-  const FewSize f = few_size(T, B, HQ, HKV, N, varlen != 0, most_keys(T, width, page_size, window, sinks));
-  return f.splits == 1 ? 0 : (size_t)f.tiles * HKV * f.splits * kFewRows * (D + 2) * 4;
+  const PagedCut c = paged_cut(B, T, HQ, HKV, N, varlen != 0, page_size, width, window, sinks);
+  return c.splits == 1 ? 0 : (size_t)c.tiles * HKV * c.splits * c.rows * (D + 2) * 4;
 }
 
 extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -642,7 +596,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t
                            (long long)kMaxRowBytes);
     return GDN_ERR_INVALID;
   }
-  FewParams p{};
+  FlashParams p{};
   p.q = q, p.k = k_cache, p.v = v_cache, p.o = o;
   p.qsb = q_batch_stride, p.qst = q_token_stride, p.qsh = q_head_stride;
   p.ksb = kc_page_stride, p.ksh = kc_head_stride, p.kst = kc_token_stride;
@@ -662,40 +616,37 @@ extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t
     if (dtype == GDN_DTYPE_BF16) D == 128 ? go(bf16{}, std::integral_constant<int, 128>{}) : go(bf16{}, std::integral_constant<int, 64>{});
     else D == 128 ? go(f16{}, std::integral_constant<int, 128>{}) : go(f16{}, std::integral_constant<int, 64>{});
   };
-  if (!takes_few(T, HQ, HKV, N, cu_seqlens != nullptr, tree != nullptr)) {
-    p.tiles = cu_seqlens ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ);
-    const int64_t groups = job_groups(HKV, HQ / HKV, p.tiles);
-    if (groups > kMaxGroups256) {
-      gdn_internal_set_error("%s: grid too large", name);
-      return GDN_ERR_UNSUPPORTED;
-    }
-    const FlashParams fp = p;
-    by_type([&](auto e, auto d) {
-      hipLaunchKernelGGL((gated_delta_paged_attn_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)groups), block, 0, s, fp);
-    });
-    return gdn_internal_check_launch("gated_delta_paged_attn_kernel");
-  }
-  const FewSize f = few_size(T, B, HQ, HKV, N, cu_seqlens != nullptr, most_keys(T, width, page_size, window, sinks));
-  p.tiles = f.tiles, p.splits = f.splits, p.part = static_cast<float*>(workspace);
-  const size_t need = gdn_paged_attn_workspace_size(B, T, HQ, HKV, D, N, page_size, width, window, sinks, cu_seqlens != nullptr,
-                                                    tree != nullptr);
+  const PagedCut cut = paged_cut(B, T, HQ, HKV, N, cu_seqlens != nullptr, page_size, width, window, sinks);
+  p.tiles = cut.tiles, p.splits = cut.splits, p.part = static_cast<float*>(workspace);
+  const size_t need = gdn_paged_attn_workspace_size(B, T, HQ, HKV, D, N, page_size, width, window, sinks, cu_seqlens != nullptr);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) {
     gdn_internal_set_error("%s: workspace of %zu bytes needed, 16-byte aligned", name, need);
     return GDN_ERR_INVALID;
   }
-  const int64_t jobs = f.tiles * HKV;
-  if (jobs * f.splits > kMaxGroups256) {
+  const bool few = cut.rows == kFewRows;
+  const int64_t jobs = cut.tiles * HKV, groups = (few ? jobs : job_groups(HKV, 1, cut.tiles)) * cut.splits;
+  // the merge: a row's threads in 8 groups where there are many runs
+  const int merge_groups = cut.splits > 8 ? 8 : 1, merge_rows = (int)(256 / (D / 4) / merge_groups);
+  const int64_t tile_rows = cu_seqlens || T * (HQ / HKV) > cut.rows ? cut.rows : T * (HQ / HKV);
+  const int merge_passes = (int)((tile_rows + merge_rows - 1) / merge_rows);
+  if (groups > kMaxGroups256 || (cut.splits > 1 && jobs * merge_passes > kMaxGroups256)) {
     gdn_internal_set_error("%s: grid too large", name);
     return GDN_ERR_UNSUPPORTED;
   }
   by_type([&](auto e, auto d) {
-    hipLaunchKernelGGL((gated_delta_paged_attn_few_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)(jobs * f.splits)),
-                       block, 0, s, p);
+    constexpr int kD = decltype(d)::value;
+    using E = decltype(e);
+    if (few) hipLaunchKernelGGL((gated_delta_paged_attn_few_kernel<kD, E>), dim3((unsigned)groups), block, 0, s, p);
+    else hipLaunchKernelGGL((gated_delta_paged_attn_kernel<kD, E>), dim3((unsigned)groups), block, 0, s, p);
   });
-  if (int rc = gdn_internal_check_launch("gated_delta_paged_attn_few_kernel")) return rc;
-  if (f.splits == 1) return GDN_OK;
+  if (int rc = gdn_internal_check_launch("gated_delta_paged_attn_kernel")) return rc;
+  if (cut.splits == 1) return GDN_OK;
   by_type([&](auto e, auto d) {
-    hipLaunchKernelGGL((gated_delta_paged_attn_merge_kernel<decltype(d)::value, decltype(e)>), dim3((unsigned)jobs), block, 0, s, p);
+    constexpr int kD = decltype(d)::value;
+    using E = decltype(e);
+    const dim3 grid((unsigned)(jobs * merge_passes));
+    if (few) hipLaunchKernelGGL((gated_delta_paged_attn_merge_kernel<kD, E, kFewRows, kFewKeys>), grid, block, 0, s, p, merge_groups, merge_passes);
+    else hipLaunchKernelGGL((gated_delta_paged_attn_merge_kernel<kD, E, kBQ, kBK>), grid, block, 0, s, p, merge_groups, merge_passes);
   });
   return gdn_internal_check_launch("gated_delta_paged_attn_merge_kernel");
 }

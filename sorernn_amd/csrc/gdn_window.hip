@@ -126,9 +126,9 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
     for (int kt = 0; kt < 2; ++kt) {
       f32x16 s{}, dp{};
 #pragma unroll
-      for (int st = 0; st < DS; ++st) s = mma32(row_frag(kb + 32 * kt * D, rd.row[st]), qf[st], s);
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(kb + 32 * kt * D, rd, st), qf[st], s);
 #pragma unroll
-      for (int st = 0; st < DS; ++st) dp = mma32(row_frag(vb + 32 * kt * D, rd.row[st]), df[st], dp);
+      for (int st = 0; st < DS; ++st) dp = mma32(row_frag(vb + 32 * kt * D, rd, st), df[st], dp);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - delta);
       if (masked) {
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = mma32(tr_frag(kb + (2 * kt + h) * 16 * D, rd.tr[d]), pb[h], acc[d]);
+        for (int d = 0; d < DT; ++d) acc[d] = mma32(tr_frag(kb + (2 * kt + h) * 16 * D, rd, d), pb[h], acc[d]);
     }
   };
   auto arrive = [&](int jb, bf16* kd) {  // the wave's loads of block jb have landed; keys behind the end: zeros
@@ -211,18 +211,24 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 __device__ __forceinline__ int near_end(int tile, int window, int len) { return imin(len, tile * kBQ + kBQ - 1 + window); }
 
 // dk and dv: 128 keys of one kv head a workgroup, 32 a wave in registers; blocks of 64 queries with their do pass through LDS,
-// head after head. Sinks are seen by far queries too: the first k_tiles jobs are every tile's near queries, the others a piece
-// of the far queries for one tile of sinks. A tile's sums over those meet in gated_delta_window_attn_sinks_kernel.
+// head after head. Two teams of four waves take every other block and add their sums at the end: two waves a SIMD also where a
+// layer has no more key tiles than there are CUs. Sinks are seen by far queries too: the first k_tiles jobs are every tile's
+// near queries, the others a piece of the far queries for one tile of sinks. A tile's sums over those meet in
+// gated_delta_window_attn_sinks_kernel.
 template <int D>
-__global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(WindowBwdParams p) {
-  constexpr int DS = D / 16, DT = D / 32;
-  __shared__ __align__(16) bf16 Qs0[kBK * D];
-  __shared__ __align__(16) bf16 Qs1[kBK * D];
-  __shared__ __align__(16) bf16 Ds0[kBK * D];
-  __shared__ __align__(16) bf16 Ds1[kBK * D];
-  __shared__ __align__(16) float Ls0[2 * kBK];  // lse, delta
-  __shared__ __align__(16) float Ls1[2 * kBK];
-  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+__global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(WindowBwdParams p) {
+  // of D = 128 half of each wave's V fragments lie in LDS (VL k-steps): with all of them in registers the loop reloads spilled
+  // ones, and waits for the tiles under way with them
+  constexpr int DS = D / 16, DT = D / 32, VL = D == 128 ? DS / 2 : 0, VR = DS - VL;
+  __shared__ __align__(16) bf16 Qs0[2 * kBK * D];
+  __shared__ __align__(16) bf16 Qs1[2 * kBK * D];
+  __shared__ __align__(16) bf16 Ds0[2 * kBK * D];
+  __shared__ __align__(16) bf16 Ds1[2 * kBK * D];
+  __shared__ __align__(16) float Ls0[2][2 * kBK];  // lse, delta
+  __shared__ __align__(16) float Ls1[2][2 * kBK];
+  __shared__ __align__(16) bf16 Vs[VL ? 4 * VL * kWave * 8 : 8];
+  const int t = threadIdx.x, lane = t & 63, w8 = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
+  const int w = w8 & 3, team = w8 >> 2;
   const int rep = p.HQ / p.HKV;
   Job job;
   if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles + p.pieces * p.sink_tiles, job)) return;
@@ -255,41 +261,47 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(Win
   const int64_t tok = sq.row * p.seqs.T + sq.start, all = p.B * p.seqs.T;
   const bf16* const krow = p.k + sq.row * p.ksb + (sq.start + kc) * p.kst + job.hkv * p.ksh;
   const bf16* const vrow = p.v + sq.row * p.vsb + (sq.start + kc) * p.vst + job.hkv * p.vsh;
-  bf16x8 kf[DS], vf[DS];
+  bf16x8 kf[DS], vf[VR];
 #pragma unroll
-  for (int s = 0; s < DS; ++s) {
-    kf[s] = *reinterpret_cast<const bf16x8*>(krow + 16 * s + 8 * hh);
-    vf[s] = *reinterpret_cast<const bf16x8*>(vrow + 16 * s + 8 * hh);
+  for (int s = 0; s < DS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(krow + 16 * s + 8 * hh);
+#pragma unroll
+  for (int s = 0; s < VR; ++s) vf[s] = *reinterpret_cast<const bf16x8*>(vrow + 16 * s + 8 * hh);
+  bf16* const vl = Vs + (w * VL * kWave + lane) * 8;
+  if (!team) {  // read behind the first barrier
+#pragma unroll
+    for (int s = 0; s < VL; ++s) *reinterpret_cast<bf16x8*>(vl + s * kWave * 8) = *reinterpret_cast<const bf16x8*>(vrow + 16 * (VR + s) + 8 * hh);
   }
   const char* const qbase = reinterpret_cast<const char*>(p.q + sq.row * p.qsb + sq.start * p.qst + (int64_t)job.hkv * rep * p.qsh);
   const char* const dbase = reinterpret_cast<const char*>(p.d_o + (tok * p.HQ + job.hkv * rep) * D);
   const int qst = (int)p.qst * 2, dst = p.HQ * D * 2;
   const BlockLoad<D> io{w, lane};
-  auto fetch = [&](int g, int qb, bf16* qd, bf16* dd, float* ld) {
-    const int rows = imin(kBK, sq.len - qb * kBK);
-    io.load(qbase + g * p.qsh * 2 + (int64_t)qb * kBK * qst, qst, rows, qd);
-    io.load(dbase + (int64_t)g * D * 2 + (int64_t)qb * kBK * dst, dst, rows, dd);
+  auto fetch = [&](int h, int blk, bf16* qd, bf16* dd, float* ld) {
+    const int rows = imin(kBK, sq.len - blk * kBK);
+    io.load(qbase + h * p.qsh * 2 + (int64_t)blk * kBK * qst, qst, rows, qd);
+    io.load(dbase + (int64_t)h * D * 2 + (int64_t)blk * kBK * dst, dst, rows, dd);
     if (w < 2) {
-      const float* src = (w ? p.delta : p.lse) + (job.hkv * rep + g) * all + tok + qb * kBK;
+      const float* src = (w ? p.delta : p.lse) + (job.hkv * rep + h) * all + tok + blk * kBK;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(src, (uint32_t)(rows * 4)),
                                                (__attribute__((address_space(3))) void*)(ld + w * kBK), 4, lane * 4, 0, 0, 0);
     }
   };
-  TileReads<D> rd;
-  rd.init(lane);
+  TileReads<D> reads;
+  reads.init(lane);
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) dk[d] = f32x16{}, dv[d] = f32x16{};
   const float c = p.scale_log2;
-  // the lane's key is seen by queries lo_q .. hi_q - 1 of the job
-  const int lo_q = imax(key, from), hi_q = key < p.sinks ? to : imin(to, key + p.window);
   auto block = [&](bool masked, const bf16* qb, const bf16* db, const float* lb, int q0) {
-    const int lo = lo_q - q0, hi = hi_q - q0;
+    const bf16* const vh = vl + opaque_int(0);
+    // the lane's key is seen by the block's queries lo .. hi - 1 (made here: registers are short)
+    const int kk = wk0 + (opaque_int(lane) & 31);
+    const int lo = imax(kk, from) - q0, hi = (kk < p.sinks ? to : imin(to, kk + p.window)) - q0;
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       f32x16 s{}, dp{};
+      TileReads<D> rd = reads.here();
 #pragma unroll
-      for (int st = 0; st < DS; ++st) s = mma32(row_frag(qb + 32 * qt * D, rd.row[st]), kf[st], s);
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(qb + 32 * qt * D, rd, st), kf[st], s);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float4 ls = ld4f(lb + 32 * qt + 8 * j + 4 * hh);
@@ -307,12 +319,15 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(Win
       }
       bf16x8 pb[2];
       pack16<bf16>(s, pb);
+      rd = reads.here();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dv[d] = mma32(tr_frag(db + (2 * qt + h) * 16 * D, rd.tr[d]), pb[h], dv[d]);
+        for (int d = 0; d < DT; ++d) dv[d] = mma32(tr_frag(db + (2 * qt + h) * 16 * D, rd, d), pb[h], dv[d]);
+      rd = reads.here();
 #pragma unroll
-      for (int st = 0; st < DS; ++st) dp = mma32(row_frag(db + 32 * qt * D, rd.row[st]), vf[st], dp);
+      for (int st = 0; st < DS; ++st)
+        dp = mma32(row_frag(db + 32 * qt * D, rd, st), st < VR ? vf[st < VR ? st : 0] : ld8(vh + (st - VR) * kWave * 8), dp);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float4 de = ld4f(lb + kBK + 32 * qt + 8 * j + 4 * hh);
@@ -329,41 +344,72 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dkv_kernel(Win
         }
       }
       pack16<bf16>(s, pb);
+      rd = reads.here();
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) dk[d] = mma32(tr_frag(qb + (2 * qt + h) * 16 * D, rd.tr[d]), pb[h], dk[d]);
+        for (int d = 0; d < DT; ++d) dk[d] = mma32(tr_frag(qb + (2 * qt + h) * 16 * D, rd, d), pb[h], dk[d]);
     }
   };
-  auto arrive = [&](int qb, bf16* qd, bf16* dd) {
+  auto arrive = [&](int blk, bf16* qd, bf16* dd) {
     wait_loads();
-    if ((qb + 1) * kBK > sq.len) {
-      io.clean(sq.len - qb * kBK, qd);
-      io.clean(sq.len - qb * kBK, dd);
+    if ((blk + 1) * kBK > sq.len) {
+      io.clean(sq.len - blk * kBK, qd);
+      io.clean(sq.len - blk * kBK, dd);
     }
   };
-  const int qb0 = from / kBK, qb1 = from < to ? (to - 1) / kBK + 1 : qb0;
-  int g = 0, qb = qb0;  // the block being used
+  const int qb0 = from / kBK, nqb = from < to ? (to - 1) / kBK + 1 - qb0 : 0;
+  int g = 0, qb = team;  // the team's block: head of the group, block from qb0
+  auto place = [&] {
+    while (qb >= nqb && g < rep) qb -= nqb, ++g;
+  };
   auto step = [&](const bf16* qc, const bf16* dc, const float* lc, bf16* qn, bf16* dn, float* ln) {
-    const int gn = qb + 1 < qb1 ? g : g + 1, qn_b = qb + 1 < qb1 ? qb + 1 : qb0;
-    if (gn < rep) fetch(gn, qn_b, qn, dn, ln);
-    const int q0 = qb * kBK, q1 = q0 + kBK - 1;
-    if (wave_live && !none_sees(q0, q1, wk0, wk0 + 31, p.window, p.sinks))
+    const int g0 = g, q0 = (qb0 + qb) * kBK, q1 = q0 + kBK - 1;
+    qb += 2;
+    place();
+    if (g < rep) fetch(g, qb0 + qb, qn, dn, ln);
+    if (g0 < rep && wave_live && !none_sees(q0, q1, wk0, wk0 + 31, p.window, p.sinks))
       block(q0 < from || q1 >= to || !all_see(q0, q1, wk0, wk0 + 31, p.window, p.sinks), qc, dc, lc, q0);
-    if (gn < rep) arrive(qn_b, qn, dn);
-    g = gn;
-    qb = qn_b;
+    if (g < rep) arrive(qb0 + qb, qn, dn);
     __syncthreads();
   };
-  if (qb0 < qb1) {
-    fetch(0, qb0, Qs0, Ds0, Ls0);
-    arrive(qb0, Qs0, Ds0);
+  bf16 *const q0p = Qs0 + team * kBK * D, *const q1p = Qs1 + team * kBK * D, *const d0p = Ds0 + team * kBK * D, *const d1p = Ds1 + team * kBK * D;
+  if (nqb) {
+    place();
+    if (g < rep) {
+      fetch(g, qb0 + qb, q0p, d0p, Ls0[team]);
+      arrive(qb0 + qb, q0p, d0p);
+    }
     __syncthreads();
-    while (g < rep) {
-      step(Qs0, Ds0, Ls0, Qs1, Ds1, Ls1);
-      if (g < rep) step(Qs1, Ds1, Ls1, Qs0, Ds0, Ls0);
+    const int turns = (rep * nqb + 1) / 2;  // the same for both teams
+    for (int n = 0; n < turns; n += 2) {
+      step(q0p, d0p, Ls0[team], q1p, d1p, Ls1[team]);
+      if (n + 1 < turns) step(q1p, d1p, Ls1[team], q0p, d0p, Ls0[team]);
+    }
+    // the second team's sums, a wave's 32 KB (16 KB) in a tile array
+    f32x4* const sums = reinterpret_cast<f32x4*>(w == 0 ? Qs0 : w == 1 ? Qs1 : w == 2 ? Ds0 : Ds1) + lane;
+    if (team) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sums[(4 * d + j) * kWave] = f32x4{dk[d][4 * j], dk[d][4 * j + 1], dk[d][4 * j + 2], dk[d][4 * j + 3]};
+          sums[(4 * (DT + d) + j) * kWave] = f32x4{dv[d][4 * j], dv[d][4 * j + 1], dv[d][4 * j + 2], dv[d][4 * j + 3]};
+        }
+    }
+    __syncthreads();
+    if (!team) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 a = sums[(4 * d + j) * kWave], b = sums[(4 * (DT + d) + j) * kWave];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dk[d][4 * j + e] += a[e], dv[d][4 * j + e] += b[e];
+        }
     }
   }
+  if (team) return;
   bool fine = finite_all(dk) && finite_all(dv);
   fine = __shfl_xor((int)fine, 32, kWave) && fine;
   const int64_t out = ((tok + kc) * p.HKV + job.hkv) * D;
@@ -499,18 +545,20 @@ static int far_window(int64_t window) { return window <= 0 || window > kFar ? kF
 // without a window sinks say nothing; sinks as far as the first window reaches neither change who sees what, nor are they cut
 static int far_sinks(int64_t window, int64_t sinks) { return window <= 0 ? 0 : sinks > kFar ? kFar : (int)sinks; }
 
-// A piece of the far queries: as many as a tile's near ones, so that the jobs are of one length, and 512 at least.
-static int far_piece(int window) { return window >= kFar / 2 ? kFar : (window + kBQ > 512 ? window + kBQ : 512) / kBK * kBK; }
+
+// Far queries a job, with one tile of sinks: short jobs, which fill up the CUs behind the near ones.
+constexpr int kFarPiece = 256;
 
 struct FarPlan {
   int far, sink_tiles, sink_rows;
   int64_t pieces;
 };
 static FarPlan far_plan(int64_t B, int64_t T, int64_t N, bool varlen, int window, int sinks) {
-  FarPlan f{far_piece(window), 0, 0, 0};
+  FarPlan f{kFarPiece, 0, 0, 0};
   if (!sinks || (int64_t)window + 1 >= T) return f;  // every query is a near one
   const int64_t some = sinks < T ? sinks : T;
   f.sink_tiles = (int)((some + kBQ - 1) / kBQ);
+  f.far = (int)(kFarPiece * f.sink_tiles < kFar ? kFarPiece * f.sink_tiles : kFar);  // with more tiles longer pieces: the partial sums stay as large
   f.sink_rows = f.sink_tiles > 1 ? kBQ : (int)((some + 31) / 32 * 32);
   f.pieces = varlen ? packed_tiles(T, N, 1, f.far) : B * ((T + f.far - 1) / f.far);
   return f;
@@ -624,8 +672,8 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<128>, dim3((unsigned)q_groups), block, 0, s, p);
   else hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<64>, dim3((unsigned)q_groups), block, 0, s, p);
   if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dq_kernel")) return rc;
-  if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<128>, dim3((unsigned)k_groups), block, 0, s, p);
-  else hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<64>, dim3((unsigned)k_groups), block, 0, s, p);
+  if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<128>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
+  else hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<64>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
   if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dkv_kernel")) return rc;
   if (f.sink_tiles) {
     hipLaunchKernelGGL(gated_delta_window_attn_sinks_kernel, dim3((unsigned)s_groups), block, 0, s, p, (int)D);

@@ -159,8 +159,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
     o = torch.empty(b, t, hq, d, device=q.device, dtype=q.dtype)
     width = table.shape[1]
-    nbytes = int(_lib.load().gdn_paged_attn_workspace_size(b, t, hq, hkv, d, n, size, width, window, sinks, int(cu is not None),
-                                                           int(tree is not None)))
+    nbytes = int(_lib.load().gdn_paged_attn_workspace_size(b, t, hq, hkv, d, n, size, width, window, sinks, int(cu is not None)))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     kc, vc, ptr = k_cache.stride(), v_cache.stride(), _lib.ptr
     ts = (0, 0) if tree is None else tree.stride()
