@@ -17,8 +17,8 @@ namespace gdn {
 
 // ------------------------------------------------------------------------------------------------ append
 // k' = rotate(norm(k)) and v into their places, q' = rotate(norm(q)) beside them, fp32 with one rounding. Bound by the rows'
-// bytes, or by the launch where tokens are few. A wave takes a token (with few tokens four share one) and its heads D / 8 lanes
-// each; a lane holds two pieces of 4 elements that turn with one another. Angles are taken in turns in 64 bits,
+// bytes, or by the launch where tokens are few. A wave takes a token (with few tokens four share one) and its heads D / 16 lanes
+// each; a lane holds two pieces of 8 elements that turn with one another. Angles are taken in turns in 64 bits,
 // position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.
 struct AppendParams {
   const void* x[3];                // q (or null), k, v [B, T, heads, D] by strides (elements)
@@ -44,20 +44,20 @@ constexpr int64_t kAppendShared = 256;
 
 template <int D, typename E>
 __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendParams p) {
-  constexpr int LPR = D / 8, RPW = kWave / LPR, U = 4;  // lanes a row, rows a pass, passes in flight
-  using X4 = typename Pack<E>::x4;
+  constexpr int LPR = D / 16, RPW = kWave / LPR, U = 2;  // lanes a row, rows a pass, passes in flight
+  using X8 = typename Pack<E>::x8;
   __shared__ __align__(16) float tab[4][2][D / 2];
   const int lane = threadIdx.x % kWave, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int li = lane % LPR, sub = lane / LPR, half = p.rot >> 1, np = half >> 2;
+  const int li = lane % LPR, sub = lane / LPR, half = p.rot >> 1, np = half >> 3;
   const bool in_rot = li < np;
-  const int d0 = in_rot ? 4 * li : p.rot + 8 * (li - np), d1 = in_rot ? d0 + half : d0 + 4;  // the lane's two pieces
+  const int d0 = in_rot ? 8 * li : p.rot + 16 * (li - np), d1 = in_rot ? d0 + half : d0 + 8;  // the lane's two pieces
   const int rows = p.HQ + 2 * p.HKV, r_first = (w % p.wpt) * RPW + sub, r_step = p.wpt * RPW;
   const int64_t stride = (int64_t)gridDim.x * 4 / p.wpt;
   for (int64_t bt = ((int64_t)blockIdx.x * 4 + w) / p.wpt; bt < p.tokens; bt += stride) {
     const int64_t bi = bt / p.T, ti = bt - bi * p.T;
     auto kind = [&](int r) { return r < p.HQ ? 0 : r < p.HQ + p.HKV ? 1 : 2; };
     auto head = [&](int r, int m) { return r - (m == 0 ? 0 : m == 1 ? p.HQ : p.HQ + p.HKV); };
-    X4 xv[U][2];
+    X8 xv[U][2];
     auto load = [&](int r0) {  // U passes' rows; past the last the last again
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
         const int64_t sb = m == 0 ? p.sb[0] : m == 1 ? p.sb[1] : p.sb[2], st = m == 0 ? p.st[0] : m == 1 ? p.st[1] : p.st[2];
         const E* base = static_cast<const E*>(m == 0 ? p.x[0] : m == 1 ? p.x[1] : p.x[2]);
         const E* src = base + bi * sb + ti * st + head(r, m) * (m == 0 ? p.sh[0] : m == 1 ? p.sh[1] : p.sh[2]);
-        xv[u][0] = *reinterpret_cast<const X4*>(src + d0);
-        xv[u][1] = *reinterpret_cast<const X4*>(src + d1);
+        xv[u][0] = *reinterpret_cast<const X8*>(src + d0);
+        xv[u][1] = *reinterpret_cast<const X8*>(src + d1);
       }
     };
     load(r_first);
@@ -108,9 +108,9 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // the table is the wave's own
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    float c[4], s[4];
+    float c[8], s[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
       c[e] = in_rot ? tab[w][0][d0 + e] : 1.f;
       s[e] = in_rot ? tab[w][1][d0 + e] : 0.f;
     }
@@ -121,23 +121,25 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
         const int r = r0 + u * r_step;
         if (r >= rows) break;
         const int m = kind(r), h = head(r, m);
-        X4 o0 = xv[u][0], o1 = xv[u][1];
+        X8 o0 = xv[u][0], o1 = xv[u][1];
         if (m < 2) {
           const float* wt = m ? p.w[1] : p.w[0];
-          float x[8], ss = 0.f;
+          float x[16], ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = (float)xv[u][e >> 2][e & 3];
+          for (int e = 0; e < 16; ++e) {
+            x[e] = (float)xv[u][e >> 3][e & 7];
             ss += x[e] * x[e];
           }
           if (wt) {
-            const float rr = 1.f / sqrtf(group_sum<LPR>(ss) / (float)D + p.eps);
+            ss = dpp_add<0x4e, 0xf>(dpp_add<0xb1, 0xf>(ss));  // over quads, then over the halves of a row of 16 lanes
+            if (LPR == 8) ss = dpp_add<0x141, 0xf>(ss);
+            const float rr = 1.f / sqrtf(ss / (float)D + p.eps);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * rr * wt[(e < 4 ? d0 : d1) + (e & 3)];
+            for (int e = 0; e < 16; ++e) x[e] = x[e] * rr * wt[(e < 8 ? d0 : d1) + (e & 7)];
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = x[e], b = x[4 + e];
+          for (int e = 0; e < 8; ++e) {
+            const float a = x[e], b = x[8 + e];
             o0[e] = (E)(a * c[e] - b * s[e]);
             o1[e] = (E)(b * c[e] + a * s[e]);
           }
@@ -145,15 +147,15 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
         E* dst;
         if (m == 0) {
           dst = static_cast<E*>(p.q_out) + (bt * p.HQ + h) * D;
-          if (!member) o0 = X4{}, o1 = X4{};
+          if (!member) o0 = X8{}, o1 = X8{};
         } else {
           if (page < 0) continue;
           const int i = m - 1;
           dst = static_cast<E*>(i ? p.cache[1] : p.cache[0]) + page * (i ? p.cp[1] : p.cp[0]) + h * (i ? p.ch[1] : p.ch[0]) +
                 in * (i ? p.ct[1] : p.ct[0]);
         }
-        *reinterpret_cast<X4*>(dst + d0) = o0;
-        *reinterpret_cast<X4*>(dst + d1) = o1;
+        *reinterpret_cast<X8*>(dst + d0) = o0;
+        *reinterpret_cast<X8*>(dst + d1) = o1;
       }
     }
     __builtin_amdgcn_wave_barrier();  // the table is read before the next token's is written
@@ -482,7 +484,7 @@ struct PagedCut {
 // that share what they load.
 constexpr int64_t kFewMost = 64;
 // Workgroups that the runs are to make, in all; a run has 4 blocks at least.
-constexpr int64_t kFewGroups = 1024, kManyGroups = 1024;
+constexpr int64_t kFewGroups = 256, kManyGroups = 512;
 static PagedCut paged_cut(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t N, bool varlen, int64_t page_size, int64_t width,
                           int64_t window, int64_t sinks) {
   const int64_t rep = HQ / HKV, tokens = varlen ? (T + N - 1) / N : T;
