@@ -228,6 +228,13 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) acc[d] = mma32(tr_frag(vb + (2 * kt + h) * 16 * D, rd, d), pb[h], acc[d]);
   }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * KT * (D / 32) - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 }
 
 // ------------------------------------------------------------------------------------------------ rows one by one
@@ -535,6 +542,14 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
       for (int st = 0; st < DS; ++st) s[kt] = mma32(row_frag(kb + 32 * kt * D, rd, st), qf[st], s[kt]);
     }
+    // the fragments' reads two products ahead
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * DS - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
     if (masked) {  // selects throughout: branches a lane apart cost more than the comparisons
       const int hi = view.place - k0, lo = hi - p.window, sk = p.sinks - k0;  // seen: <= hi and (> lo or < sk)
 #pragma unroll

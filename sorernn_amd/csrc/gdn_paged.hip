@@ -627,9 +627,11 @@ extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t
   }
   const bool few = cut.rows == kFewRows;
   const int64_t jobs = cut.tiles * HKV, groups = (few ? jobs : job_groups(HKV, 1, cut.tiles)) * cut.splits;
-  // the merge: a row's threads in 8 groups where there are many runs
-  const int merge_groups = cut.splits > 8 ? 8 : 1, merge_rows = (int)(256 / (D / 4) / merge_groups);
+  // the merge: a row's threads in up to 8 groups, two runs for each at least, while that makes no more than 2,048 workgroups
   const int64_t tile_rows = cu_seqlens || T * (HQ / HKV) > cut.rows ? cut.rows : T * (HQ / HKV);
+  int merge_groups = 1;
+  while (merge_groups < 8 && merge_groups * 4 <= cut.splits && jobs * tile_rows * (D / 4) * merge_groups * 2 <= 2048 * 256) merge_groups *= 2;
+  const int merge_rows = (int)(256 / (D / 4) / merge_groups);
   const int merge_passes = (int)((tile_rows + merge_rows - 1) / merge_rows);
   if (groups > kMaxGroups256 || (cut.splits > 1 && jobs * merge_passes > kMaxGroups256)) {
     gdn_internal_set_error("%s: grid too large", name);
