@@ -207,9 +207,6 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
   }
 }
 
-// The queries of a key tile end here: near ones, which see keys through the window. Those behind see sinks only.
-__device__ __forceinline__ int near_end(int tile, int window, int len) { return imin(len, tile * kBQ + kBQ - 1 + window); }
-
 // dk and dv: 128 keys of one kv head a workgroup, 32 a wave in registers; blocks of 64 queries with their do pass through LDS,
 // head after head. Two teams of four waves take every other block and add their sums at the end: two waves a SIMD also where a
 // layer has no more key tiles than there are CUs. Sinks are seen by far queries too: the first k_tiles jobs are every tile's

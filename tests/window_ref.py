@@ -71,6 +71,8 @@ def window_attention(q, k, v, window, sinks, scale, cu=None, do=None):
     names = ("o", "o_tol") + (("dq", "dq_tol", "dk", "dk_tol", "dv", "dv_tol") if do is not None else ())
     out = {m: torch.zeros((k if m[:2] in ("dk", "dv") else q).shape, dtype=F64, device=q.device) for m in names}
     for bi, s, e in spans:
+        if s == e:
+            continue
         at = torch.arange(e - s, device=q.device)
         mask = seen(at, at, window, sinks)
         for i in range(hq):
