@@ -101,18 +101,19 @@ def paged_kv_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page
                              f"{tuple(positions.shape)}")
         if positions.dim() == 1:
             positions = positions.expand(b, t)
-    ptr = _lib.ptr
     (ks, kst), (vs, vst) = _strided(k), _strided(v)
-    qs, qst = (None, (0, 0, 0)) if q is None else _strided(q)
     qw, kw = _weight(q_weight), _weight(k_weight)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    out = None if q is None else torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    ps = (None, 0, 0, 0) if positions is None else (ptr(positions), *positions.stride(), positions.dtype == torch.int32)
-    kc, vc = k_cache.stride(), v_cache.stride()
-    _launch("gdn_paged_append", k, ptr(qs), *qst[:3], ptr(ks), *kst[:3], ptr(vs), *vst[:3], ptr(qw), ptr(kw), ptr(out),
-            ptr(k_cache), *kc[:3], ptr(v_cache), *vc[:3], ptr(table), table.stride(0), ptr(lens), lens.dtype == torch.int32,
-            *ps, ptr(cu), b, t, 0 if q is None else q.shape[2], hkv, d, n, pages, size, table.shape[1], _CODES[k.dtype], rot_dim,
-            float(theta), float(eps), flags)
+    out, hq, qa = None, 0, (None, 0, 0, 0)
+    if q is not None:
+        qs, qst = _strided(q)
+        out, hq, qa = torch.empty(q.shape, device=q.device, dtype=q.dtype), q.shape[2], (qs.data_ptr(), *qst[:3])
+    ps = (None, 0, 0, 0) if positions is None else (positions.data_ptr(), *positions.stride(), positions.dtype == torch.int32)
+    _launch("gdn_paged_append", k, *qa, ks.data_ptr(), *kst[:3], vs.data_ptr(), *vst[:3], None if qw is None else qw.data_ptr(),
+            None if kw is None else kw.data_ptr(), None if out is None else out.data_ptr(), k_cache.data_ptr(),
+            *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], table.data_ptr(), table.stride(0), lens.data_ptr(),
+            lens.dtype == torch.int32, *ps, None if cu is None else cu.data_ptr(), b, t, hq, hkv, d, n, pages, size,
+            table.shape[1], _CODES[k.dtype], rot_dim, float(theta), float(eps), flags)
     torch.autograd.graph.increment_version((k_cache, v_cache))  # a graph that saved them must not use what they hold now
     return out
 
@@ -161,9 +162,9 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
     width = table.shape[1]
     nbytes = int(_lib.load().gdn_paged_attn_workspace_size(b, t, hq, hkv, d, n, size, width, window, sinks, int(cu is not None)))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
-    kc, vc, ptr = k_cache.stride(), v_cache.stride(), _lib.ptr
-    ts = (0, 0) if tree is None else tree.stride()
-    _launch("gdn_paged_attn_fwd", q, ptr(qs), *qst[:3], ptr(k_cache), *kc[:3], ptr(v_cache), *vc[:3], ptr(table), table.stride(0),
-            ptr(lens), lens.dtype == torch.int32, ptr(tree), *ts, ptr(o), ptr(cu), b, t, hq, hkv, d, n, pages, size, width,
-            _CODES[q.dtype], window, sinks, float(d**-0.5 if scale is None else scale), flags, ptr(ws), nbytes)
+    words = (None, 0, 0) if tree is None else (tree.data_ptr(), *tree.stride())
+    _launch("gdn_paged_attn_fwd", q, qs.data_ptr(), *qst[:3], k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
+            *v_cache.stride()[:3], table.data_ptr(), table.stride(0), lens.data_ptr(), lens.dtype == torch.int32, *words,
+            o.data_ptr(), None if cu is None else cu.data_ptr(), b, t, hq, hkv, d, n, pages, size, width, _CODES[q.dtype],
+            window, sinks, float(d**-0.5 if scale is None else scale), flags, None if ws is None else ws.data_ptr(), nbytes)
     return o
