@@ -276,6 +276,9 @@ __device__ __forceinline__ bool paged_plan(const FlashParams& p, int64_t t, int 
   return true;
 }
 
+// bits 0 .. n - 1
+__device__ __forceinline__ uint64_t bits_below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
+
 // What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
 struct RowView {
   int place, base;  // base: the first drafted token's place; without a tree behind every place
@@ -284,6 +287,13 @@ struct RowView {
     const int n = j - base;
     const bool by_place = (j <= place) & ((place - j < window) | (j < sinks));
     return ((n < 0) & by_place) | ((n >= 0) & (n < 64) & ((bits >> (n & 63) & 1) != 0));
+  }
+  // bit x: whether key k0 + x is seen, x = 0 .. 63
+  __device__ __forceinline__ uint64_t block(int k0, int window, int sinks) const {
+    const int n = k0 - base, at = place - k0;
+    const uint64_t by_place = bits_below(at + 1) & (~bits_below(at - window + 1) | bits_below(sinks - k0)) & bits_below(-n);
+    const uint64_t drafted = n >= 64 || n <= -64 ? 0 : n >= 0 ? bits >> n : bits << -n;
+    return by_place | drafted;
   }
 };
 __device__ __forceinline__ RowView row_view(const FlashParams& p, const PagedPlan& f, int row) {
@@ -321,7 +331,6 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   const int* table = nullptr;
   RowView view;
   int wq0, wq1;  // places of the wave's first and last row
-  bool tree = false;
   if constexpr (PAGED) {
     const int64_t jobs = gridDim.x / p.splits;
     split = (int)(blockIdx.x / jobs);
@@ -335,10 +344,9 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     n0 = split * f.per;
     n1 = imin(n0 + f.per, bl.count);
     if (sq.num >= 0) table = p.table + sq.num * p.table_stride;
-    tree = p.tree != nullptr;
     view = row_view(p, f, row0 + imin(32 * w + li, rows - 1));
-    wq0 = tree ? f.first : f.base + (row0 + 32 * w) / rep;
-    wq1 = tree ? f.last : f.base + (row0 + imin(32 * w + 31, rows - 1)) / rep;
+    wq0 = p.tree ? f.first : f.base + (row0 + 32 * w) / rep;
+    wq1 = p.tree ? f.last : f.base + (row0 + imin(32 * w + 31, rows - 1)) / rep;
   } else {
     if (!job_of(blockIdx.x, p.HKV, rep, p.parts, p.tiles, job)) return;
     if (p.seqs.cu) {
@@ -462,20 +470,19 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-    if (masked) {  // selects throughout: branches a lane apart cost more than the comparisons
-      const int hi = view.place - k0, lo = hi - p.window, sk = p.sinks - k0;  // seen: <= hi and (> lo or < sk)
+    if (masked) {  // selects, from one word of bits a lane: branches a lane apart cost more
+      uint64_t seen = view.block(k0, p.window, p.sinks);
+      if (PAGED) {
+        seen &= bits_below(klen - k0);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) seen &= ok >> g & 1 ? ~0ull : ~(0xffffull << 16 * g);
+      }
+      seen >>= 4 * hh;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          bool seen = (ko <= hi) & ((ko > lo) | (ko < sk));
-          if (PAGED) {
-            if (tree) seen = view(k0 + ko, p.window, p.sinks);
-            seen &= (k0 + ko < klen) & ((ok >> (2 * kt + (e >> 3)) & 1) != 0);
-          }
-          s[kt][e] = seen ? s[kt][e] : -INFINITY;
-        }
+        for (int e = 0; e < 16; ++e)
+          s[kt][e] = (uint32_t)(seen >> 32 * kt) >> (8 * (e >> 2) + (e & 3)) & 1 ? s[kt][e] : -INFINITY;
     }
     softmax_step<2, D, E>(s, acc, m, l, c, slack, vb, rd);
   };

@@ -272,12 +272,11 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
 #pragma unroll
     for (int st = 0; st < DS; ++st) s[0] = mma32(row_frag(kc, rd, st), qf[st], s[0]);
     if (partial || (p.tree && k1 >= f.base) || !all_see(f.first, f.last, k0, k1, p.window, p.sinks)) {
+      uint32_t seen = (uint32_t)(view.block(k0, p.window, p.sinks) & bits_below(f.klen - k0));
+      seen &= (ok & 1 ? 0xffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
+      seen >>= 4 * hh;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int j = k0 + 8 * (e >> 2) + 4 * hh + (e & 3);
-        const bool seen = view(j, p.window, p.sinks) & (j < f.klen) & ((ok >> (e >> 3) & 1) != 0);
-        s[0][e] = seen ? s[0][e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) s[0][e] = seen >> (8 * (e >> 2) + (e & 3)) & 1 ? s[0][e] : -INFINITY;
     }
     softmax_step<1, D, E>(s, acc, m, l, c, slack, vc, rd);
     ok = ok_next;

@@ -89,6 +89,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
   if (q0 >= sq.len) return;
   const int q1 = imin(q0 + kBQ, sq.len) - 1, qi = q0 + 32 * w + li, wq0 = q0 + 32 * w, wq1 = imin(wq0 + 31, q1);
   const bool wave_live = wq0 <= wq1, row_ok = wave_live && qi < sq.len;
+  const RowView view{qi, kFar, 0};
   Blocks bl = blocks_of<kBK>(q0, q1, p.window, p.sinks);
   if (sq.num < 0) bl.count = 0;
   const int64_t tok = sq.row * p.seqs.T + sq.start, all = p.B * p.seqs.T;
@@ -132,12 +133,9 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - delta);
       if (masked) {
-        const int hi = qi - k0, lo = qi - p.window - k0, sk = p.sinks - k0;
+        const uint32_t seen = (uint32_t)(view.block(k0 + 32 * kt, p.window, p.sinks) >> 4 * hh);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int ko = 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          s[e] = ((ko <= hi) & ((ko > lo) | (ko < sk))) ? s[e] : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = seen >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : 0.f;
       }
       bf16x8 pb[2];
       pack16<bf16>(s, pb);
@@ -290,9 +288,12 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   const float c = p.scale_log2;
   auto block = [&](bool masked, const bf16* qb, const bf16* db, const float* lb, int q0) {
     const bf16* const vh = vl + opaque_int(0);
-    // the lane's key is seen by the block's queries lo .. hi - 1 (made here: registers are short)
-    const int kk = wk0 + (opaque_int(lane) & 31);
-    const int lo = imax(kk, from) - q0, hi = (kk < p.sinks ? to : imin(to, kk + p.window)) - q0;
+    // the block's queries that see the lane's key (made here: registers are short)
+    uint64_t seen = ~0ull;
+    if (masked) {
+      const int kk = wk0 + (opaque_int(lane) & 31), hi = kk < p.sinks ? to : imin(to, kk + p.window);
+      seen = (bits_below(hi - q0) & ~bits_below(imax(kk, from) - q0)) >> 4 * hh;
+    }
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       f32x16 s{}, dp{};
@@ -309,10 +310,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       }
       if (masked) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          s[e] = ((qo >= lo) & (qo < hi)) ? s[e] : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = (uint32_t)(seen >> 32 * qt) >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : 0.f;
       }
       bf16x8 pb[2];
       pack16<bf16>(s, pb);
@@ -335,10 +333,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       }
       if (masked) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int qo = 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3);
-          s[e] = ((qo >= lo) & (qo < hi)) ? s[e] : 0.f;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = (uint32_t)(seen >> 32 * qt) >> (8 * (e >> 2) + (e & 3)) & 1 ? s[e] : 0.f;
       }
       pack16<bf16>(s, pb);
       rd = reads.here();
