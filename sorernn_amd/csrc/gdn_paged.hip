@@ -474,32 +474,40 @@ static bool rows_ok(const int64_t* st, int n, uintptr_t all) {
   return !(all & 15);
 }
 
-// How a call is cut: tiles of `rows` rows, blocks of `keys` keys, `splits` runs of them a tile.
+// How a call is cut: tiles of `rows` rows, blocks of `keys` keys, `splits` runs of them a tile. bf16, 16 / 4 heads of 128, us:
+//   rows a sequence (new tokens times heads of a group): tiles of 32 with a run of keys a wave, or of 128 that share what they
+//   load. Up to 64 rows the former; up to 256 while the tiles make no more than 4,400 blocks of keys in all:
+//     tokens, cached   1 sequence      2               4
+//       61,  1,000     14.7, 18.9      16.1, 20.2      18.9, 22.0
+//       61,  4,000     20.5, 23.9      25.7, 27.0      36.5, 31.2
+//       64, 16,000     37.6, 34.9      58.9, 42.1       102, 60.9
+//   runs: as many as make about kFewGroups or kManyGroups workgroups (256 and 512: one token over 32,768 keys 20.8 and 26.2,
+//   1,024 workgroups 36.9; 8 trees of 61 tokens 48.3 and 41.0, 59.5), of 4 blocks at least (one token over 1,024 keys with 4, 8
+//   and 16: 10.6, 11.6, 14.1). Up to 256 keys one run without a merge (8.1, with two runs 9.8).
 struct PagedCut {
   int rows, keys, splits;
   int64_t tiles;
 };
-// Up to this many rows (new tokens times heads of a group) a sequence, tiles of 32 with a run of keys a wave; else tiles of 128
-// that share what they load.
-constexpr int64_t kFewMost = 64;
-// Workgroups that the runs are to make, in all; a run has 4 blocks at least.
-constexpr int64_t kFewGroups = 256, kManyGroups = 512;
+constexpr int64_t kFewMost = 64, kFewMostShort = 256, kFewBlocks = 4400, kFewGroups = 256, kManyGroups = 512;
 static PagedCut paged_cut(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t N, bool varlen, int64_t page_size, int64_t width,
                           int64_t window, int64_t sinks) {
   const int64_t rep = HQ / HKV, tokens = varlen ? (T + N - 1) / N : T;
-  PagedCut c{};
-  const bool few = tokens * rep <= kFewMost;
-  c.rows = few ? kFewRows : kBQ;
-  c.keys = few ? kFewKeys : kBK;
-  c.tiles = varlen ? packed_tiles(T, N, (int)rep, c.rows) : B * ((T * rep + c.rows - 1) / c.rows);
+  auto tiles_of = [&](int rows) { return varlen ? packed_tiles(T, N, (int)rep, rows) : B * ((T * rep + rows - 1) / rows); };
+  auto blocks_seen = [&](int rows, int keys) {  // by a tile, at most
+    int64_t most = width * page_size;
+    if (window > 0 && window < most) {
+      const int64_t some = window + rows / rep + 1 + (sinks < most ? sinks : most);
+      if (some < most) most = some;
+    }
+    return (most + keys - 1) / keys + 1;
+  };
+  const bool few = tokens * rep <= kFewMost ||
+                   (tokens * rep <= kFewMostShort && tiles_of(kFewRows) * HKV * blocks_seen(kFewRows, kFewKeys) <= kFewBlocks);
+  PagedCut c{few ? kFewRows : kBQ, few ? kFewKeys : kBK, 1, 0};
+  c.tiles = tiles_of(c.rows);
   const int64_t busy = (varlen ? (T * rep + c.rows - 1) / c.rows + N : c.tiles) * HKV;  // about as many do anything
-  int64_t keys = width * page_size;  // that a tile sees at most
-  if (window > 0 && window < keys) {
-    const int64_t some = window + c.rows / rep + 1 + (sinks < keys ? sinks : keys);
-    if (some < keys) keys = some;
-  }
-  const int64_t blocks = (keys + c.keys - 1) / c.keys + 1, most = (blocks + 3) / 4;
-  int64_t splits = ((few ? kFewGroups : kManyGroups) + busy - 1) / busy;
+  const int64_t blocks = blocks_seen(c.rows, c.keys), most = blocks * c.keys <= 256 + c.keys ? 1 : (blocks + 3) / 4;
+  const int64_t splits = ((few ? kFewGroups : kManyGroups) + busy - 1) / busy;
   c.splits = (int)(splits > most ? most : splits);
   return c;
 }

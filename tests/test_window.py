@@ -191,9 +191,13 @@ def test_sizes_of_the_workspaces():
     assert size(1, 1, 16, 4, 128, 1, 64, 512, 0, 0, 0) == 4 * 64 * 32 * 130 * 4
     # as many tiles as there are CUs: one run
     assert size(64, 1, 16, 4, 128, 64, 16, 512, 0, 0, 0) == 0
-    # a short cache makes no more runs than it has fours of blocks
-    assert size(1, 1, 16, 4, 128, 1, 64, 4, 0, 0, 0) == 4 * 3 * 32 * 130 * 4
-    assert size(1, 1, 16, 4, 128, 1, 64, 1024, 100, 0, 0) == 4 * 2 * 32 * 130 * 4
+    # a short cache makes no more runs than it has fours of blocks, one of 256 keys a single one
+    assert size(1, 1, 16, 4, 128, 1, 64, 8, 0, 0, 0) == 4 * 5 * 32 * 130 * 4
+    assert size(1, 1, 16, 4, 128, 1, 64, 4, 0, 0, 0) == 0
+    # 244 rows a sequence: tiles of 32 while there is little to do, else of 128
+    assert size(1, 61, 16, 4, 128, 1, 64, 16, 0, 0, 0) == 8 * 4 * 8 * 32 * 130 * 4
+    assert size(8, 61, 16, 4, 128, 8, 64, 64, 0, 0, 0) == 16 * 4 * 8 * 128 * 130 * 4
+    assert size(1, 1, 16, 4, 128, 1, 64, 1024, 300, 0, 0) == 4 * 3 * 32 * 130 * 4
     assert size(0, 1, 16, 4, 128, 1, 64, 512, 0, 0, 0) == size(1, 1, 15, 4, 128, 1, 64, 512, 0, 0, 0) == 0
 
 
