@@ -152,7 +152,8 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 // ------------------------------------------------------------------------------------------------ rows one by one
 // The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
 // reach rows that do not see it. Such a row's result is not finite, so rows with finite results are right, and the others
-// are computed again here, key by key, over the keys that they see. A wave a row; lane l holds columns l and l + 64.
+// are computed again here, key by key, over the keys that they see. (Masked scores take part in nothing: a row whose sum is NaN
+// sees a NaN, all of it is NaN, and it stays as it is.) A wave a row; lane l holds columns l and l + 64.
 template <int D, typename E>
 __device__ __forceinline__ float dot_row(const E* a, const E* b) {
   float x = 0.f;
@@ -181,11 +182,16 @@ __device__ __forceinline__ void slow_row(const E* q, int key0, int key1, Key key
     const float p = kr ? __builtin_amdgcn_exp2f(s * c - (m == -INFINITY ? 0.f : m * c)) : 0.f;
     l = l * alpha + wave_xor_sum(p, 1);
     for (int i = 0; i < D / 64; ++i) acc[i] *= alpha;
+    const int some = __ffsll((unsigned long long)live) - 1;  // read in place of keys that are not seen
+#pragma unroll 8
     for (int n = 0; n < kWave; ++n) {
-      if (!(live >> n & 1)) continue;
+      const bool on = live >> n & 1;
       const float pn = __shfl(p, n, kWave);
-      const E* vr = val(base + n);
-      for (int i = 0; i < D / 64; ++i) acc[i] += pn * (float)vr[lane + 64 * i];
+      const E* vr = val(base + (on ? n : some));
+      for (int i = 0; i < D / 64; ++i) {
+        const float x = (float)vr[lane + 64 * i];
+        acc[i] += on ? pn * x : 0.f;
+      }
     }
   }
 }
@@ -528,13 +534,13 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     pml = p.part + p.tiles * p.HKV * p.splits * kBQ * D + (f.job * p.splits + split) * 2 * kBQ;
   }
   l += __shfl_xor(l, 32, kWave);
-  bool fine = finite_all(acc) && finite_f(l);
-  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  bool fine = finite_all(acc);
+  fine = l != l || (__shfl_xor((int)fine, 32, kWave) && fine);
   const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;
   const int r = 32 * w + li;
   if (row_ok && fine) {
     if (whole) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       E* const to = o_at(r);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -545,7 +551,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
           for (int e = 0; e < 4; ++e) x[e] = (E)(acc[d][4 * j + e] * inv);
           *reinterpret_cast<X4*>(to + 32 * d + 8 * j + 4 * hh) = x;
         }
-      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l > 0.f ? m * c + __builtin_amdgcn_logf(l) : INFINITY;
+      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + __builtin_amdgcn_logf(l);
     } else {
 #pragma unroll
       for (int d = 0; d < DT; ++d)

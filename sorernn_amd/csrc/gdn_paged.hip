@@ -333,12 +333,12 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
                                            4 * (piece ^ (r & (CH - 1))));
     }
-    if (!finite_f(sum) || !finite_f(x[0]) || !finite_f(x[1]) || !finite_f(x[2]) || !finite_f(x[3])) {
+    if (sum == sum && !(finite_f(x[0]) && finite_f(x[1]) && finite_f(x[2]) && finite_f(x[3]))) {
       atomicOr(&redo_rows, 1u << r);
       continue;
     }
     if (f.used == 1) {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       typename Pack<E>::x4 y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);

@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
     }
   }
   bool fine = finite_all(acc);
-  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  fine = lse != lse || !finite_f(delta) || (__shfl_xor((int)fine, 32, kWave) && fine);  // of those no ds that is seen is finite
   if (row_ok && fine) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -189,16 +189,22 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
       const int j = base + lane;
       const bool see = j <= r && sees(r, j, p.window, p.sinks);
       const uint64_t live = __ballot(see);
+      if (!live) continue;
       float ds = 0.f;
       if (see) {
         const float s = dot_row<D>(qp, reinterpret_cast<const bf16*>(kbase + (int64_t)j * kst));
         ds = __builtin_amdgcn_exp2f(fmaf(s, c, -lr)) * (dot_row<D>(p.d_o + at, reinterpret_cast<const bf16*>(vbase + (int64_t)j * vst)) - dr);
       }
+      const int some = __ffsll((unsigned long long)live) - 1;
+#pragma unroll 8
       for (int i = 0; i < kWave; ++i) {
-        if (!(live >> i & 1)) continue;
+        const bool on = live >> i & 1;
         const float x = __shfl(ds, i, kWave);
-        const bf16* kr = reinterpret_cast<const bf16*>(kbase + (int64_t)(base + i) * kst);
-        for (int e = 0; e < D / 64; ++e) a[e] += x * (float)kr[lane + 64 * e];
+        const bf16* kr = reinterpret_cast<const bf16*>(kbase + (int64_t)(base + (on ? i : some)) * kst);
+        for (int e = 0; e < D / 64; ++e) {
+          const float y = (float)kr[lane + 64 * e];
+          a[e] += on ? x * y : 0.f;
+        }
       }
     }
     for (int e = 0; e < D / 64; ++e) p.dq[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
@@ -431,8 +437,9 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     const bf16* kr = p.k + sq.row * p.ksb + (sq.start + j) * p.kst + job.hkv * p.ksh;
     const bf16* vr = p.v + sq.row * p.vsb + (sq.start + j) * p.vst + job.hkv * p.vsh;
     float a[D / 64] = {}, b[D / 64] = {};
-    for (int h = 0; h < rep; ++h)
-      for (int base = from; base < to; base += kWave) {
+    bool over = false;  // a weight is NaN: all of the row's dk and dv are
+    for (int h = 0; h < rep && !over; ++h)
+      for (int base = from; base < to && !over; base += kWave) {
         const int i = base + lane;
         const bool see = i < to && sees(i, j, p.window, p.sinks);
         const uint64_t live = __ballot(see);
@@ -445,12 +452,16 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
           pr = __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q_at(i), kr), c, -p.lse[at]));
           ds = pr * (dot_row<D>(d_at(i), vr) - p.delta[at]);
         }
+        over = __any(pr != pr);
+        const int some = __ffsll((unsigned long long)live) - 1;
+#pragma unroll 8
         for (int x = 0; x < kWave; ++x) {
-          if (!(live >> x & 1)) continue;
+          const bool on = live >> x & 1;
           const float px = __shfl(pr, x, kWave), dx = __shfl(ds, x, kWave);
           for (int e = 0; e < D / 64; ++e) {
-            a[e] += dx * (float)q_at(base + x)[lane + 64 * e];
-            b[e] += px * (float)d_at(base + x)[lane + 64 * e];
+            const float qx = (float)q_at(base + (on ? x : some))[lane + 64 * e], ox = (float)d_at(base + (on ? x : some))[lane + 64 * e];
+            a[e] += on ? dx * qx : 0.f;
+            b[e] += on ? px * ox : 0.f;
           }
         }
       }
@@ -654,7 +665,7 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   p.far = f.far, p.sink_tiles = f.sink_tiles, p.sink_rows = f.sink_rows, p.pieces = f.pieces;
   const int64_t q_groups = job_groups(HKV, HQ / HKV, p.q_tiles);
   const int64_t k_groups = job_groups(HKV, 1, p.k_tiles + p.pieces * p.sink_tiles), s_groups = N * HKV * p.sink_tiles;
-  if (q_groups > kMaxGroups256 || k_groups > kMaxGroups256 || s_groups > kMaxGroups256) {
+  if (q_groups > kMaxGroups256 || k_groups > kMaxGroups256 / 2 || s_groups > kMaxGroups256) {  // k_groups: of 512 threads
     gdn_internal_set_error("gdn_window_attn_bwd: grid too large");
     return GDN_ERR_UNSUPPORTED;
   }

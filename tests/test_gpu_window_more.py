@@ -260,3 +260,36 @@ def test_no_tokens_and_unused_outputs():
     (g,) = torch.autograd.grad(o.float().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         g.float().sum().backward()
+
+
+def test_int32_bounds_and_their_check_without_a_host_copy():
+    *x, do = _inputs(1, 300, 2, 1, 64, seed=16)
+    bounds = [0, 5, 170, 300]
+    want = _grads(x, do, window=40, sinks=1, cu_seqlens=torch.tensor(bounds, device=DEV))
+    got = _grads(x, do, window=40, sinks=1, cu_seqlens=torch.tensor(bounds, device=DEV, dtype=torch.int32))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_nothing_but_nan():
+    """A diverged step ends as soon as another: rows that see a NaN are not computed again."""
+    x = [torch.full_like(y, torch.nan) for y in _inputs(1, 3000, 4, 2, 128)]
+    out = _grads(x[:3], x[3])
+    torch.cuda.synchronize()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    a.record()
+    out = _grads(x[:3], x[3])
+    b.record()
+    torch.cuda.synchronize()
+    assert all(y.isnan().all() for y in out)
+    assert a.elapsed_time(b) < 50
+
+
+def test_batched_gradients():
+    *x, do = _inputs(1, 90, 2, 1, 64, seed=17)
+    leaves = [y.requires_grad_(True) for y in x]
+    o = window_attention(*leaves, window=20)
+    ups = torch.stack([do, 2 * do])
+    got = torch.autograd.grad(o, leaves, ups, is_grads_batched=True, retain_graph=True)
+    for i in range(2):
+        want = torch.autograd.grad(o, leaves, ups[i], retain_graph=True)
+        assert all(torch.equal(a[i], b) for a, b in zip(got, want))
