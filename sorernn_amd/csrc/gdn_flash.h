@@ -151,9 +151,11 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 
 // ------------------------------------------------------------------------------------------------ rows one by one
 // The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
-// reach rows that do not see it. Such a row's result is not finite, so rows with finite results are right, and the others
-// are computed again here, key by key, over the keys that they see. (Masked scores take part in nothing: a row whose sum is NaN
-// sees a NaN, all of it is NaN, and it stays as it is.) A wave a row; lane l holds columns l and l + 64.
+// reach rows that do not see it. Finite columns of a row are right all the same, and the others are summed again here, key by
+// key, over the keys that the row sees, until they are what they are: not finite, or done. (Masked scores take part in
+// nothing: the row's maximum and sum are right, and where the sum is NaN the row is.) A wave a row; lane l holds columns l and
+// l + 64.
+__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 template <int D, typename E>
 __device__ __forceinline__ float dot_row(const E* a, const E* b) {
   float x = 0.f;
@@ -165,23 +167,18 @@ __device__ __forceinline__ float dot_row(const E* a, const E* b) {
   return x;
 }
 
-// Adds keys [key0, key1) to a row's running maximum, sum and output. key(j): K row j or null (not to be seen); val(j): V row j.
+// Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c. key(j): K row j or null (not to
+// be seen); val(j): V row j. False once none of the columns can become finite.
 template <int D, typename E, typename Key, typename Val, typename Seen>
-__device__ __forceinline__ void slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float& m, float& l,
-                                      float (&acc)[D / 64]) {
+__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, int again,
+                                         float (&acc)[D / 64]) {
   const int lane = threadIdx.x % kWave;
   for (int base = key0; base < key1; base += kWave) {
     const int j = base + lane;
     const E* kr = j < key1 && seen(j) ? key(j) : nullptr;
     const uint64_t live = __ballot(kr != nullptr);
     if (!live) continue;
-    const float s = kr ? dot_row<D>(q, kr) : -INFINITY;
-    const float top = fmaxf(m, wave_max(s));
-    const float alpha = top == m ? 1.f : __builtin_amdgcn_exp2f((m - top) * c);
-    m = top;
-    const float p = kr ? __builtin_amdgcn_exp2f(s * c - (m == -INFINITY ? 0.f : m * c)) : 0.f;
-    l = l * alpha + wave_xor_sum(p, 1);
-    for (int i = 0; i < D / 64; ++i) acc[i] *= alpha;
+    const float p = kr ? __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q, kr), c, nmc)) : 0.f;
     const int some = __ffsll((unsigned long long)live) - 1;  // read in place of keys that are not seen
 #pragma unroll 8
     for (int n = 0; n < kWave; ++n) {
@@ -193,10 +190,13 @@ __device__ __forceinline__ void slow_row(const E* q, int key0, int key1, Key key
         acc[i] += on ? pn * x : 0.f;
       }
     }
+    bool open = false;
+    for (int i = 0; i < D / 64; ++i) open |= (again >> i & 1) && finite_f(acc[i]);
+    if (!__any(open)) return false;
   }
+  return true;
 }
 
-__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // whether a lane's accumulators are all finite: 0 x stays 0 unless x is not
 template <int N>
 __device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
@@ -206,6 +206,24 @@ __device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) z = fmaf(a[n][e], 0.f, z);
   return z == 0.f;
+}
+
+// Of row n of the wave's (in lanes n and n + 32): which of lane l's columns l and l + 64 are not finite.
+template <int D>
+__device__ __forceinline__ int not_finite(const f32x16 (&a)[D / 32], int n) {
+  uint64_t mine = 0;  // bit 16 d + e: column 32 d + 8 (e / 4) + 4 hh + e % 4
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mine |= finite_f(a[d][e]) ? 0ull : 1ull << (16 * d + e);
+  const int lane = threadIdx.x % kWave;
+  int bits = 0;
+  for (int i = 0; i < D / 64; ++i) {
+    const int col = lane + 64 * i, from = n + (col >> 2 & 1) * 32, e = (col >> 3 & 3) * 4 + (col & 3);
+    const uint32_t lo = __shfl((uint32_t)mine, from, kWave), hi = __shfl((uint32_t)(mine >> 32), from, kWave);
+    bits |= (int)(((uint64_t)hi << 32 | lo) >> (16 * (col >> 5) + e) & 1) << i;
+  }
+  return bits;
 }
 
 // ------------------------------------------------------------------------------------------------ parameters and plans
@@ -538,7 +556,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   fine = l != l || (__shfl_xor((int)fine, 32, kWave) && fine);
   const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;
   const int r = 32 * w + li;
-  if (row_ok && fine) {
+  if (row_ok) {
     if (whole) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       E* const to = o_at(r);
@@ -566,6 +584,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     }
   }
   uint64_t redo = __ballot(row_ok && !fine && hh == 0);
+  if (redo) wait_loads();  // what was written above is there before parts of it are written again
   while (redo) {
     const int n = __ffsll((unsigned long long)redo) - 1, rr = 32 * w + n;
     redo &= redo - 1;
@@ -577,23 +596,20 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
                                      : reinterpret_cast<const E*>(base + id * page_bytes + (j & ((1 << p.shift) - 1)) * row_bytes);
     };
-    float mr = -INFINITY, lr = 0.f, a[D / 64] = {};
+    const float mr = __shfl(m, n, kWave), lr = __shfl(l, n, kWave), nmc = mr == -INFINITY ? 0.f : -mr * c;
+    const int again = not_finite<D>(acc, n);
+    float a[D / 64] = {};
     for (int b = n0; b < n1; ++b) {
       const int k0 = bl.at(b) * kBK;
-      slow_row<D, E>(q_at(rr), k0, imin(k0 + kBK, klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
-                     [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); }, c,
-                     mr, lr, a);
+      if (!slow_row<D, E>(q_at(rr), k0, imin(k0 + kBK, klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
+                          [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
+                          c, nmc, again, a))
+        break;
     }
-    if (whole) {
-      for (int i = 0; i < D / 64; ++i) o_at(rr)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
-      if (!PAGED && p.lse && lane == 0)
-        p.lse[head_of(rr) * all + tok + token_of(rr)] = lr == 0.f ? INFINITY : mr * c + __builtin_amdgcn_logf(lr);
-    } else {
-      for (int i = 0; i < D / 64; ++i) po[rr * D + lane + 64 * i] = a[i];
-      if (lane == 0) {
-        pml[rr] = mr;
-        pml[kBQ + rr] = lr;
-      }
+    for (int i = 0; i < D / 64; ++i) {
+      if (!(again >> i & 1)) continue;
+      if (whole) o_at(rr)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+      else po[rr * D + lane + 64 * i] = a[i];
     }
   }
 }

@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
   __shared__ __align__(16) E V0[4 * TILE];
   __shared__ __align__(16) E V1[4 * TILE];
   __shared__ float ml[4][2][kFewRows];
-  __shared__ uint32_t redo_rows;
+  __shared__ uint32_t redo_cols[kFewRows][D / 32];  // columns of rows that are summed again
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
   const int rep = p.HQ / p.HKV;
   PagedPlan f;
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
     ml[w][0][li] = m;
     ml[w][1][li] = l;
   }
-  if (t == 0) redo_rows = 0;
+  if (t < kFewRows * (D / 32)) redo_cols[t / (D / 32)][t % (D / 32)] = 0;
   __syncthreads();  // every wave is done with its tiles, which take the sums
   const float top = fmaxf(fmaxf(ml[0][0][li], ml[1][0][li]), fmaxf(ml[2][0][li], ml[3][0][li]));
   const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
@@ -329,13 +329,15 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float mv = ml[v][0][r];
-      if (mv != -INFINITY) sum += ml[v][1][r] * __builtin_amdgcn_exp2f((mv - tm) * c);
+      sum += mv == -INFINITY ? ml[v][1][r] : ml[v][1][r] * __builtin_amdgcn_exp2f((mv - tm) * c);  // of the former 0, or NaN
       x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
                                            4 * (piece ^ (r & (CH - 1))));
     }
-    if (sum == sum && !(finite_f(x[0]) && finite_f(x[1]) && finite_f(x[2]) && finite_f(x[3]))) {
-      atomicOr(&redo_rows, 1u << r);
-      continue;
+    if (sum == sum) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= finite_f(x[e]) ? 0u : 1u << e;
+      if (bad) atomicOr(&redo_cols[r][piece / 8], bad << piece % 8 * 4);
     }
     if (f.used == 1) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -351,31 +353,33 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       }
     }
   }
+  wait_loads();  // what was written above is there before parts of it are written again
   __syncthreads();
-  for (uint32_t redo = redo_rows; redo; redo &= redo - 1) {  // over the keys that the row sees only
-    const int r = __ffs(redo) - 1;
-    if (r % 4 != w) continue;
+  for (int r = w; r < f.rows; r += 4) {
+    int again = 0;
+    for (int i = 0; i < D / 64; ++i) again |= (int)(redo_cols[r][(lane + 64 * i) / 32] >> (lane % 32) & 1) << i;
+    if (!__any(again)) continue;
     const RowView v = row_view(p, f, f.row0 + r);
     auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
       const int id = table[j >> p.shift];
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
                                      : reinterpret_cast<const E*>(base + id * page_bytes + (j & in_page) * row_bytes);
     };
-    float mr = -INFINITY, lr = 0.f, a[D / 64] = {};
+    const float tm = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
+    float lr = 0.f, a[D / 64] = {};
+    for (int u = 0; u < 4; ++u)
+      if (ml[u][0][r] != -INFINITY) lr += ml[u][1][r] * __builtin_amdgcn_exp2f((ml[u][0][r] - tm) * c);
     for (int n = n0; n < n1; ++n) {
       const int k0 = f.bl.at(n) * kFewKeys;
-      slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
-                     [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); }, c,
-                     mr, lr, a);
+      if (!slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
+                          [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
+                          c, tm == -INFINITY ? 0.f : -tm * c, again, a))
+        break;
     }
-    if (f.used == 1) {
-      for (int i = 0; i < D / 64; ++i) out_row(f.row0 + r)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
-    } else {
-      for (int i = 0; i < D / 64; ++i) po[r * D + lane + 64 * i] = a[i];
-      if (lane == 0) {
-        pml[r] = mr;
-        pml[kFewRows + r] = lr;
-      }
+    for (int i = 0; i < D / 64; ++i) {
+      if (!(again >> i & 1)) continue;
+      if (f.used == 1) out_row(f.row0 + r)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+      else po[r * D + lane + 64 * i] = a[i];
     }
   }
 }

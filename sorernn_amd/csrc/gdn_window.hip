@@ -408,12 +408,13 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     }
   }
   if (team) return;
-  bool fine = finite_all(dk) && finite_all(dv);
-  fine = __shfl_xor((int)fine, 32, kWave) && fine;
+  bool fine_k = finite_all(dk), fine_v = finite_all(dv);
+  fine_k = __shfl_xor((int)fine_k, 32, kWave) && fine_k;
+  fine_v = __shfl_xor((int)fine_v, 32, kWave) && fine_v;
   const int64_t out = ((tok + kc) * p.HKV + job.hkv) * D;
   const bool to_part = slot >= 0 && key < p.sinks;
   float* const part = p.part + (((slot >= 0 ? slot : 0) * p.HKV + job.hkv) * p.sink_tiles + tile) * 2 * p.sink_rows * D;
-  if (row_ok && fine) {
+  if (row_ok) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -430,14 +431,17 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
         }
       }
   }
-  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
+  const uint64_t redo_v = __ballot(row_ok && !fine_v && hh == 0);
+  uint64_t redo = __ballot(row_ok && !(fine_k && fine_v) && hh == 0);
+  if (redo) wait_loads();  // what was written above is there before parts of it are written again
   while (redo) {  // over the queries that see the key only
     const int n = __ffsll((unsigned long long)redo) - 1, j = wk0 + n;
+    const bool want_v = redo_v >> n & 1;
     redo &= redo - 1;
     const bf16* kr = p.k + sq.row * p.ksb + (sq.start + j) * p.kst + job.hkv * p.ksh;
     const bf16* vr = p.v + sq.row * p.vsb + (sq.start + j) * p.vst + job.hkv * p.vsh;
     float a[D / 64] = {}, b[D / 64] = {};
-    bool over = false;  // a weight is NaN: all of the row's dk and dv are
+    bool over = false;  // a weight is NaN: all of dk and dv are; a ds is not finite: no entry of dk is
     for (int h = 0; h < rep && !over; ++h)
       for (int base = from; base < to && !over; base += kWave) {
         const int i = base + lane;
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
           pr = __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q_at(i), kr), c, -p.lse[at]));
           ds = pr * (dot_row<D>(d_at(i), vr) - p.delta[at]);
         }
-        over = __any(pr != pr);
+        over = __any(pr != pr) || (!want_v && __any(!finite_f(ds)));
         const int some = __ffsll((unsigned long long)live) - 1;
 #pragma unroll 8
         for (int x = 0; x < kWave; ++x) {
@@ -469,10 +473,10 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     for (int e = 0; e < D / 64; ++e) {
       if (slot >= 0 && j < p.sinks) {
         part[(32 * w + n) * D + lane + 64 * e] = a[e];
-        part[(p.sink_rows + 32 * w + n) * D + lane + 64 * e] = b[e];
+        if (want_v) part[(p.sink_rows + 32 * w + n) * D + lane + 64 * e] = b[e];
       } else {
         p.dk[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
-        p.dv[at + lane + 64 * e] = (bf16)b[e];
+        if (want_v) p.dv[at + lane + 64 * e] = (bf16)b[e];
       }
     }
   }
