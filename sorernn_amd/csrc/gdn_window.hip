@@ -36,6 +36,10 @@ struct WindowBwdParams {
   // of 128 sinks: [slots][HKV][sink tiles][2][sink rows][D]
   float* part;
   int far, sink_tiles, sink_rows;
+  // few key tiles: the near queries of one are dealt out to `shares` workgroups, whose sums meet in another kernel:
+  // [shares][B T][HKV][2][D]
+  float* near;
+  int shares;
 };
 
 // Loads of 64 rows of `stride` bytes from `base` (the block's first row) into a tile, `rows` of them there.
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 
 // dk and dv: 128 keys of one kv head a workgroup, 32 a wave in registers; blocks of 64 queries with their do pass through LDS,
 // head after head. Two teams of four waves take every other block and add their sums at the end: two waves a SIMD also where a
-// layer has no more key tiles than there are CUs. Sinks are seen by far queries too: the first k_tiles jobs are every tile's
+// layer has no more key tiles than there are CUs. Where it has fewer, several workgroups share a tile's blocks. Sinks are seen by far queries too: the first k_tiles jobs are every tile's
 // near queries, the others a piece of the far queries for one tile of sinks. A tile's sums over those meet in
 // gated_delta_window_attn_sinks_kernel.
 template <int D>
@@ -232,20 +236,23 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   const int w = w8 & 3, team = w8 >> 2;
   const int rep = p.HQ / p.HKV;
   Job job;
-  if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles + p.pieces * p.sink_tiles, job)) return;
+  if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles * p.shares + p.pieces * p.sink_tiles, job)) return;
+  const bool far_job = job.tile >= p.k_tiles * p.shares;
   Seq sq;
-  int tile, from, to;
+  int tile, from, to, share = 0;
   int64_t slot;  // where sums over part of a sink's queries go
-  if (job.tile < p.k_tiles) {
-    if (p.seqs.cu) sq = packed_tile(p.seqs, job.tile, 1, kBQ);
-    else sq = Seq{job.tile % p.B, 0, (int)p.seqs.T, (int)(job.tile % p.B), (int)(job.tile / p.B)};  // those that most see first
+  if (!far_job) {
+    const int64_t kt = job.tile / p.shares;
+    share = (int)(job.tile - kt * p.shares);
+    if (p.seqs.cu) sq = packed_tile(p.seqs, kt, 1, kBQ);
+    else sq = Seq{kt % p.B, 0, (int)p.seqs.T, (int)(kt % p.B), (int)(kt / p.B)};  // those that most see first
     tile = sq.tile;
     if (tile * kBQ >= sq.len) return;
     from = tile * kBQ;
     to = sq.num < 0 ? from : near_end(tile, p.window, sq.len);
-    slot = to < sq.len && sq.num >= 0 ? p.pieces + sq.num : -1;
+    slot = to < sq.len && sq.num >= 0 && p.shares == 1 ? p.pieces + sq.num : -1;
   } else {
-    const int64_t f = job.tile - p.k_tiles;
+    const int64_t f = job.tile - p.k_tiles * p.shares;
     slot = f / p.sink_tiles;
     tile = (int)(f - slot * p.sink_tiles);
     if (p.seqs.cu) sq = packed_tile(p.seqs, slot, 1, p.far);
@@ -255,7 +262,6 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     to = imin(sq.len, (sq.tile + 1) * p.far);
     if (from >= to) return;
   }
-  const bool far_job = job.tile >= p.k_tiles;
   const int wk0 = tile * kBQ + 32 * w, key = wk0 + li, kc = imin(key, sq.len - 1);
   const bool wave_live = wk0 < sq.len && !(far_job && wk0 >= p.sinks);
   const bool row_ok = key < sq.len && !(far_job && key >= p.sinks);
@@ -357,13 +363,14 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     }
   };
   const int qb0 = from / kBK, nqb = from < to ? (to - 1) / kBK + 1 - qb0 : 0;
-  int g = 0, qb = team;  // the team's block: head of the group, block from qb0
+  const int step_by = far_job ? 2 : 2 * p.shares;  // blocks between two of a team's
+  int g = 0, qb = 2 * share + team;  // the team's block: head of the group, block from qb0
   auto place = [&] {
     while (qb >= nqb && g < rep) qb -= nqb, ++g;
   };
   auto step = [&](const bf16* qc, const bf16* dc, const float* lc, bf16* qn, bf16* dn, float* ln) {
     const int g0 = g, q0 = (qb0 + qb) * kBK, q1 = q0 + kBK - 1;
-    qb += 2;
+    qb += step_by;
     place();
     if (g < rep) fetch(g, qb0 + qb, qn, dn, ln);
     if (g0 < rep && wave_live && !none_sees(q0, q1, wk0, wk0 + 31, p.window, p.sinks))
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       arrive(qb0 + qb, q0p, d0p);
     }
     __syncthreads();
-    const int turns = (rep * nqb + 1) / 2;  // the same for both teams
+    const int turns = (rep * nqb + step_by - 1) / step_by;  // the same for both teams
     for (int n = 0; n < turns; n += 2) {
       step(q0p, d0p, Ls0[team], q1p, d1p, Ls1[team]);
       if (n + 1 < turns) step(q1p, d1p, Ls1[team], q0p, d0p, Ls0[team]);
@@ -412,8 +419,16 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   fine_k = __shfl_xor((int)fine_k, 32, kWave) && fine_k;
   fine_v = __shfl_xor((int)fine_v, 32, kWave) && fine_v;
   const int64_t out = ((tok + kc) * p.HKV + job.hkv) * D;
-  const bool to_part = slot >= 0 && key < p.sinks;
-  float* const part = p.part + (((slot >= 0 ? slot : 0) * p.HKV + job.hkv) * p.sink_tiles + tile) * 2 * p.sink_rows * D;
+  // sums that meet others': where those of key j go (dk; dv `dv_at` behind them), null: the result
+  const bool alone = far_job || p.shares == 1;
+  const int dv_at = alone ? p.sink_rows * D : D;
+  auto part_at = [&](int j) -> float* {
+    if (!alone) return p.near + ((share * all + tok + j) * p.HKV + job.hkv) * 2 * D;
+    return slot >= 0 && j < p.sinks
+               ? p.part + ((slot * p.HKV + job.hkv) * p.sink_tiles + tile) * 2 * p.sink_rows * D + (j - tile * kBQ) * D
+               : nullptr;
+  };
+  float* const part = part_at(kc);
   if (row_ok) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -422,9 +437,9 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
         const int at = 32 * d + 8 * j + 4 * hh;
         const f32x4 a = {dk[d][4 * j], dk[d][4 * j + 1], dk[d][4 * j + 2], dk[d][4 * j + 3]};
         const f32x4 b = {dv[d][4 * j], dv[d][4 * j + 1], dv[d][4 * j + 2], dv[d][4 * j + 3]};
-        if (to_part) {
-          *reinterpret_cast<f32x4*>(part + (32 * w + li) * D + at) = a;
-          *reinterpret_cast<f32x4*>(part + (p.sink_rows + 32 * w + li) * D + at) = b;
+        if (part) {
+          *reinterpret_cast<f32x4*>(part + at) = a;
+          *reinterpret_cast<f32x4*>(part + dv_at + at) = b;
         } else {
           *reinterpret_cast<bf16x4*>(p.dk + out + at) = to_bf16x4(a[0] * p.scale, a[1] * p.scale, a[2] * p.scale, a[3] * p.scale);
           *reinterpret_cast<bf16x4*>(p.dv + out + at) = to_bf16x4(b[0], b[1], b[2], b[3]);
@@ -444,8 +459,9 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     bool over = false;  // a weight is NaN: all of dk and dv are; a ds is not finite: no entry of dk is
     for (int h = 0; h < rep && !over; ++h)
       for (int base = from; base < to && !over; base += kWave) {
-        const int i = base + lane;
-        const bool see = i < to && sees(i, j, p.window, p.sinks);
+        const int i = base + lane;  // of a shared tile the blocks of this workgroup only
+        const bool mine = far_job || (h * nqb + i / kBK - qb0) / 2 % p.shares == share;
+        const bool see = i < to && mine && sees(i, j, p.window, p.sinks);
         const uint64_t live = __ballot(see);
         if (!live) continue;
         auto q_at = [&](int x) { return reinterpret_cast<const bf16*>(qbase + h * p.qsh * 2 + (int64_t)x * qst); };
@@ -471,9 +487,9 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       }
     const int64_t at = ((tok + j) * p.HKV + job.hkv) * D;
     for (int e = 0; e < D / 64; ++e) {
-      if (slot >= 0 && j < p.sinks) {
-        part[(32 * w + n) * D + lane + 64 * e] = a[e];
-        if (want_v) part[(p.sink_rows + 32 * w + n) * D + lane + 64 * e] = b[e];
+      if (float* const to_part = part_at(j)) {
+        to_part[lane + 64 * e] = a[e];
+        if (want_v) to_part[dv_at + lane + 64 * e] = b[e];
       } else {
         p.dk[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
         if (want_v) p.dv[at + lane + 64 * e] = (bf16)b[e];
@@ -505,11 +521,30 @@ __global__ __launch_bounds__(256) void gated_delta_window_attn_sinks_kernel(Wind
   for (int i = threadIdx.x; i < 2 * rows * quads; i += 256) {
     const int which = i / (rows * quads), r = i / quads % rows, d = i % quads * 4;
     const int64_t at = here + (which * p.sink_rows + r) * D + d;
-    f32x4 x = *reinterpret_cast<const f32x4*>(p.part + (p.pieces + num) * per + at);
+    const int64_t token = row * p.seqs.T + start + tile * kBQ + r;
+    f32x4 x{};
+    if (p.shares == 1) x = *reinterpret_cast<const f32x4*>(p.part + (p.pieces + num) * per + at);
+    else
+      for (int n = 0; n < p.shares; ++n)
+        x += *reinterpret_cast<const f32x4*>(p.near + (((n * p.B * p.seqs.T + token) * p.HKV + hkv) * 2 + which) * D + d);
     for (int n = near / p.far; n <= (len - 1) / p.far; ++n) x += *reinterpret_cast<const f32x4*>(p.part + (first + n * step) * per + at);
     if (!which) x *= p.scale;
-    bf16* to = (which ? p.dv : p.dk) + ((row * p.seqs.T + start + tile * kBQ + r) * p.HKV + hkv) * D + d;
+    bf16* to = (which ? p.dv : p.dk) + (token * p.HKV + hkv) * D + d;
     *reinterpret_cast<bf16x4*>(to) = to_bf16x4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// dk and dv of shared key tiles: the workgroups' sums, in order. Four columns a thread. Rows of sinks that far queries see are
+// written again by the kernel above.
+__global__ __launch_bounds__(256) void gated_delta_window_attn_join_kernel(WindowBwdParams p, int D) {
+  const int64_t rows = p.B * p.seqs.T * p.HKV, quads = rows * 2 * D / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (int64_t)gridDim.x * 256) {
+    f32x4 x{};
+    for (int n = 0; n < p.shares; ++n) x += *reinterpret_cast<const f32x4*>(p.near + (n * quads + i) * 4);
+    const int64_t row = i / (D / 2);
+    const int at = (int)(i - row * (D / 2)) * 4;
+    if (at < D) x *= p.scale;
+    *reinterpret_cast<bf16x4*>((at < D ? p.dk : p.dv) + row * D + at % D) = to_bf16x4(x[0], x[1], x[2], x[3]);
   }
 }
 
@@ -571,6 +606,38 @@ static FarPlan far_plan(int64_t B, int64_t T, int64_t N, bool varlen, int window
   return f;
 }
 
+// Workgroups that share a key tile's queries: as many as there are idle CUs for, with 8 blocks of queries each at least; and
+// where the first tiles have twice the average to do (no window), two waves of workgroups, with 24 blocks each at least.
+// Measured, training step of 16 query heads and D = 128 in us, one workgroup a tile -> this rule: 1,024 tokens of 1 kv head
+// 611 -> 123; 4,096 of 4 without a window 762 -> 418, window 512 182 -> 152; 8,192 of 4 1,792 -> 1,283. The other side: three
+// waves and 8 blocks cost 4,096 tokens of 16 kv heads 414 -> 447, sharing where far pieces of sinks fill the card
+// (4,096 tokens, 4 kv heads, window 300) 158 -> 182. Each share costs 8 D bytes a key and kv head, written and read.
+static int dkv_shares(int64_t T, int64_t HQ, int64_t HKV, int64_t k_tiles, int64_t far_tiles, int window) {
+  const int64_t jobs = k_tiles * HKV, blocks = HQ / HKV * ((T < window + kBQ ? T : window + kBQ) / kBK + 1);
+  const int64_t idle = (256 - far_tiles * HKV) / jobs;
+  int64_t n = idle < blocks / 8 ? idle : blocks / 8;
+  if (window > T / 2) {
+    const int64_t even = (512 + jobs - 1) / jobs, m = even < blocks / 24 ? even : blocks / 24;
+    n = n > m ? n : m;
+  }
+  return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+}
+
+struct BwdSizes {
+  FarPlan far;
+  int64_t tiles;
+  int shares;
+  size_t delta, part, near;  // bytes
+};
+static BwdSizes bwd_sizes(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, bool varlen, int window, int sinks) {
+  BwdSizes b{far_plan(B, T, N, varlen, window, sinks), varlen ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ), 1, 0, 0, 0};
+  b.shares = dkv_shares(T, HQ, HKV, b.tiles, b.far.pieces * b.far.sink_tiles, window);
+  b.delta = ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256;
+  b.part = (size_t)(b.far.sink_tiles ? b.far.pieces + N : 0) * HKV * b.far.sink_tiles * 2 * b.far.sink_rows * D * 4;
+  b.near = b.shares > 1 ? (size_t)b.shares * B * T * HKV * 2 * D * 4 : 0;
+  return b;
+}
+
 }  // namespace gdn
 
 using namespace gdn;
@@ -622,10 +689,9 @@ extern "C" int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_
 
 extern "C" size_t gdn_window_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N,
                                                      int64_t window, int64_t sinks, int varlen) {
-  if (B <= 0 || T <= 0 || HQ <= 0 || HKV <= 0 || D <= 0 || N <= 0 || window < 0 || sinks < 0) return 0;
-  const FarPlan f = far_plan(B, T, N, varlen != 0, far_window(window), far_sinks(window, sinks));
-  const size_t delta = ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256;
-  return delta + (size_t)(f.sink_tiles ? f.pieces + N : 0) * HKV * f.sink_tiles * 2 * f.sink_rows * D * 4;
+  if (B <= 0 || T <= 0 || HQ <= 0 || HKV <= 0 || HQ % HKV || D <= 0 || N <= 0 || window < 0 || sinks < 0) return 0;
+  const BwdSizes b = bwd_sizes(B, T, HQ, HKV, D, N, varlen != 0, far_window(window), far_sinks(window, sinks));
+  return b.delta + b.part + b.near;
 }
 
 extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
@@ -658,17 +724,20 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   p.qsb = st[0], p.qst = st[1], p.qsh = st[2], p.ksb = st[3], p.kst = st[4], p.ksh = st[5], p.vsb = st[6], p.vst = st[7], p.vsh = st[8];
   p.dq = static_cast<bf16*>(dq), p.dk = static_cast<bf16*>(dk), p.dv = static_cast<bf16*>(dv);
   p.delta = static_cast<float*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256);
   p.seqs = Packed{cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, N, T};
   p.B = B;
-  p.q_tiles = p.k_tiles = cu_seqlens ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ);
   p.HQ = (int)HQ, p.HKV = (int)HKV, p.parts = job_parts(HKV);
   p.window = far_window(window), p.sinks = far_sinks(window, sinks);
   p.scale = scale, p.scale_log2 = scale * 1.4426950408889634f;
-  const FarPlan f = far_plan(B, T, N, cu_seqlens != nullptr, p.window, p.sinks);
+  const BwdSizes sizes = bwd_sizes(B, T, HQ, HKV, D, N, cu_seqlens != nullptr, p.window, p.sinks);
+  const FarPlan& f = sizes.far;
+  p.q_tiles = p.k_tiles = sizes.tiles;
+  p.shares = sizes.shares;
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizes.delta);
+  p.near = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizes.delta + sizes.part);
   p.far = f.far, p.sink_tiles = f.sink_tiles, p.sink_rows = f.sink_rows, p.pieces = f.pieces;
   const int64_t q_groups = job_groups(HKV, HQ / HKV, p.q_tiles);
-  const int64_t k_groups = job_groups(HKV, 1, p.k_tiles + p.pieces * p.sink_tiles), s_groups = N * HKV * p.sink_tiles;
+  const int64_t k_groups = job_groups(HKV, 1, p.k_tiles * p.shares + p.pieces * p.sink_tiles), s_groups = N * HKV * p.sink_tiles;
   if (q_groups > kMaxGroups256 || k_groups > kMaxGroups256 / 2 || s_groups > kMaxGroups256) {  // k_groups: of 512 threads
     gdn_internal_set_error("gdn_window_attn_bwd: grid too large");
     return GDN_ERR_UNSUPPORTED;
@@ -682,6 +751,11 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<128>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
   else hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<64>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
   if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dkv_kernel")) return rc;
+  if (p.shares > 1) {
+    const int64_t quads = B * T * HKV * 2 * D / 4, groups = (quads + 255) / 256;
+    hipLaunchKernelGGL(gated_delta_window_attn_join_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), block, 0, s, p, (int)D);
+    if (int rc = gdn_internal_check_launch("gated_delta_window_attn_join_kernel")) return rc;
+  }
   if (f.sink_tiles) {
     hipLaunchKernelGGL(gated_delta_window_attn_sinks_kernel, dim3((unsigned)s_groups), block, 0, s, p, (int)D);
     return gdn_internal_check_launch("gated_delta_window_attn_sinks_kernel");
