@@ -20,6 +20,7 @@ namespace gdn {
 // bytes, or by the launch where tokens are few. A wave takes a token (with few tokens four share one) and its heads D / 16 lanes
 // each; a lane holds two pieces of 8 elements that turn with one another. Angles are taken in turns in 64 bits,
 // position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.
+// Measured, 16 query and 4 kv heads of 128: 16,384 tokens 44 us, 4.6 TB/s (a large copy: 5.1); one token 4.1 us, 64 tokens 5.1.
 struct AppendParams {
   const void* x[3];                // q (or null), k, v [B, T, heads, D] by strides (elements)
   int64_t sb[3], st[3], sh[3];
@@ -164,6 +165,9 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
 
 // ------------------------------------------------------------------------------------------------ attention, many rows
 // Tiles of 128 rows (token, q head of the group) of a kv head; where they are few their keys are cut into `splits` runs.
+// Measured, 16 heads on 4 of 128: 512 new tokens of 4 sequences over up to 8,192 162 us, 552 TFLOP/s, bound as the forward over whole
+// sequences, and 14 us for the join of two runs (without runs 241 us); trees of 61 tokens of 8 sequences over up to 4,096 33 us
+// and 9, bound by start and end of runs of 5 to 8 blocks.
 template <int D, typename E>
 __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashParams p) {
   __shared__ __align__(16) E Ks0[kBK * D];
@@ -176,7 +180,10 @@ __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashPar
 // ------------------------------------------------------------------------------------------------ attention, few new tokens
 // A kv head's new rows (token, q head of the group) in tiles of 32; the keys that they see in blocks of 32, cut into `splits`
 // runs, a workgroup each. Every wave takes blocks of its own, loaded straight into its own LDS one ahead: no barrier until the
-// four waves' sums meet, 128 KB a CU under way. Bound by the cache's bytes.
+// four waves' sums meet, 128 KB a CU under way. Bound by the cache's bytes: 64 sequences of up to 8,192 tokens, 4 kv heads of 128,
+// 144-152 us, 4.6-4.9 TB/s (a large copy: 5.1); with a window of 1,024, 8 kv heads of 64, 31 us, 4.3 TB/s. One token of one
+// sequence over 32,768 takes 17 us, 4.0 TB/s, and 4.5 for the join: the start of a run (length, table, first loads, one after
+// the other) is as long as its work.
 constexpr int kFewRows = 32, kFewKeys = 32;
 
 template <int D, typename E>
