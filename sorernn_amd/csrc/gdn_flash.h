@@ -483,7 +483,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float m = -INFINITY, l = 0.f;
-  const float c = p.scale_log2, slack = 8.f / c;
+  const float c = p.scale_log2, slack = fminf(8.f / c, 3e38f);  // finite: a first maximum is always taken
 
   auto block = [&](bool masked, int ok, const E* kb, const E* vb, int k0) {
     f32x16 s[2];

@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
   float m = -INFINITY, l = 0.f;
-  const float c = p.scale_log2, slack = 8.f / c;
+  const float c = p.scale_log2, slack = fminf(8.f / c, 3e38f);
   int ok = 3, ok_next = 3;
   auto step = [&](int n, const E* kc, E* vc, E* kn, E* vn) {
     const int k0 = f.bl.at(n) * kFewKeys, k1 = k0 + kFewKeys - 1;
@@ -601,7 +601,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t
                            (long long)HQ, (long long)HKV, (long long)window, (long long)sinks);
     return GDN_ERR_INVALID;
   }
-  if (!(scale > 0.f) || scale > 3.0e38f) {
+  if (!(scale > 0.f) || scale > 2.0e38f) {
     gdn_internal_set_error("%s: scale %g unsupported (a positive finite softmax scale)", name, (double)scale);
     return GDN_ERR_INVALID;
   }

@@ -566,7 +566,7 @@ static int window_check(const char* name, int64_t B, int64_t T, int64_t HQ, int6
     gdn_internal_set_error("%s: head dim %lld unsupported (64 or 128)", name, (long long)D);
     return GDN_ERR_UNSUPPORTED;
   }
-  if (!(scale > 0.f) || scale > 3.0e38f) {
+  if (!(scale > 0.f) || scale > 2.0e38f) {
     gdn_internal_set_error("%s: scale %g unsupported (a positive finite softmax scale)", name, (double)scale);
     return GDN_ERR_INVALID;
   }
