@@ -133,7 +133,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
     from the place behind as many as the token's ancestors, ``lengths[n] - T_n + (bits set) - 1``.
 
     Rows that see nothing are zero: tokens at a place below 0, of no sequence, without a length. A length above what its row of
-    the table can hold counts as that. Keys on pages that the cache does not have are not seen. An infinity or NaN in the cache reaches the tokens that see it, not the others.
+    the table can hold counts as that. Keys on pages that the cache does not have are not seen. An infinity or NaN in the cache
+    reaches the tokens that see it, not the others.
     """
     name = "paged_attention"
     _check_cuda(name, q, k_cache, v_cache, page_table, lengths, tree, cu_seqlens)
