@@ -436,26 +436,27 @@ GDN_API size_t gdn_qk_norm_rope_bwd_workspace_size(int64_t B, int64_t T, int64_t
  * Causal attention with a sliding window and sinks over whole sequences: token i of a sequence sees token j <= i if
  * i - j < window or j < sinks; o = softmax(scale q k^T) v, q head i reading kv head i / (HQ / HKV). q [B, T, HQ, D],
  * k, v [B, T, HKV, D] in dtype (bf16 or fp16) by element strides (the last axis contiguous; multiples of 8 elements, tensors
- * 16-byte aligned, at most 2^23 elements between tokens); o [B, T, HQ, D] contiguous; lse [HQ, B T] fp32 or NULL (log2 of a
- * row's sum of 2^(scale log2(e) q.k); infinity for a row that sees nothing), which the backward reads. window 0: none.
+ * 16-byte aligned, at most 2^23 elements between tokens); o [B, T, HQ, D] contiguous; kept NULL or, for the backward,
+ * B T HQ (D / 2 + 1) floats, 16-byte aligned: [B, T, HQ, D] in dtype, what the rounding of o left, then [HQ, B T] fp32, log2
+ * of a row's sum of 2^(scale log2(e) q.k), infinity for a row that sees nothing. window 0: none.
  * cu_seqlens ascends (empty sequences allowed); rows of tokens in no sequence are zero. D = 64 or 128, T < 2^28.
  */
 GDN_API int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
                                 const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                                 const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
-                                void* o, float* lse, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
+                                void* o, float* kept, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
                                 int64_t D, int64_t N, int dtype, int64_t window, int64_t sinks, float scale, unsigned flags,
                                 void* stream);
 
 /*
- * Backward of gdn_window_attn_fwd in bf16: its inputs, o and lse, and d_o [B, T, HQ, D] contiguous, into contiguous dq
+ * Backward of gdn_window_attn_fwd in bf16: its inputs, o and kept, and d_o [B, T, HQ, D] contiguous, into contiguous dq
  * [B, T, HQ, D], dk, dv [B, T, HKV, D]. Rows of tokens in no sequence are zero. workspace:
  * gdn_window_attn_bwd_workspace_size bytes, 16-byte aligned.
  */
 GDN_API int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
                                 const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                                 const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
-                                const void* o, const float* lse, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
+                                const void* o, const float* kept, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
                                 int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t window, int64_t sinks, float scale,
                                 unsigned flags, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                 void* stream);

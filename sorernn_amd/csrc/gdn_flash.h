@@ -232,6 +232,7 @@ struct FlashParams {
   const void *q, *k, *v;
   int64_t qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh;
   void* o;       // [B, T, HQ, D]
+  void* o_rest;  // like o, or null: what o's rounding left, rounded in its turn
   float* lse;    // [HQ, B T] or null: log2 of the sum of 2^(c s)
   Packed seqs;   // cu null: batch rows of T tokens
   int64_t B, tiles;
@@ -302,6 +303,13 @@ __device__ __forceinline__ bool paged_plan(const FlashParams& p, int64_t t, int 
 
 // bits 0 .. n - 1
 __device__ __forceinline__ uint64_t bits_below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
+
+// what the rounding of x to E left
+template <typename E>
+__device__ __forceinline__ E rest_of(float x) {
+  const float r = x - (float)(E)x;
+  return (E)(finite_f(r) ? r : 0.f);
+}
 
 // What one row sees: a place in the sequence and, for a tree, the drafted tokens' bits.
 struct RowView {
@@ -572,6 +580,11 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = (E)(acc[d][4 * j + e] * inv);
           *reinterpret_cast<X4*>(to + 32 * d + 8 * j + 4 * hh) = x;
+          if (!PAGED && p.o_rest) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = rest_of<E>(acc[d][4 * j + e] * inv);
+            *reinterpret_cast<X4*>(static_cast<E*>(p.o_rest) + (to - static_cast<E*>(p.o)) + 32 * d + 8 * j + 4 * hh) = x;
+          }
         }
       if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + __builtin_amdgcn_logf(l);
     } else {
@@ -612,8 +625,10 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     }
     for (int i = 0; i < D / 64; ++i) {
       if (!(again >> i & 1)) continue;
-      if (whole) o_at(rr)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+      const float x = lr == 0.f ? 0.f : a[i] / lr;
+      if (whole) o_at(rr)[lane + 64 * i] = (E)x;
       else po[rr * D + lane + 64 * i] = a[i];
+      if (!PAGED && p.o_rest) static_cast<E*>(p.o_rest)[o_at(rr) - static_cast<E*>(p.o) + lane + 64 * i] = rest_of<E>(x);
     }
   }
 }

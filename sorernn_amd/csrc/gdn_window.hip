@@ -29,6 +29,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_fwd_kernel(Fla
 struct WindowBwdParams {
   const bf16 *q, *k, *v, *o, *d_o;  // o, d_o [B, T, HQ, D]
   int64_t qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh;
+  const bf16* o_rest;               // [B, T, HQ, D]
   const float* lse;                 // [HQ, B T]
   float* delta;                     // [HQ, B T]
   bf16 *dq, *dk, *dv;               // contiguous
@@ -74,7 +75,9 @@ __device__ __forceinline__ float dot8(bf16x8 a, bf16x8 b) {
   return x;
 }
 
-// dq and delta: 128 queries of one head a workgroup, as the forward's.
+// dq and delta: 128 queries of one head a workgroup, as the forward's. delta takes o with what its rounding left (kept by a forward
+// that a backward follows): where few keys are seen dp - delta is small against o, and o's half step would come out larger in
+// dq and dk than the roundings of ds and of the results together.
 template <int D>
 __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(WindowBwdParams p) {
   constexpr int DS = D / 16, DT = D / 32;
@@ -111,6 +114,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
     qf[s] = *reinterpret_cast<const bf16x8*>(qrow + 16 * s + 8 * hh);
     df[s] = *reinterpret_cast<const bf16x8*>(p.d_o + orow + 16 * s + 8 * hh);
     delta += dot8<D>(df[s], *reinterpret_cast<const bf16x8*>(p.o + orow + 16 * s + 8 * hh));
+    delta += dot8<D>(df[s], *reinterpret_cast<const bf16x8*>(p.o_rest + orow + 16 * s + 8 * hh));
   }
   delta += __shfl_xor(delta, 32, kWave);
   const float lse = p.lse[hq * all + tok + qc];
@@ -650,7 +654,7 @@ using namespace gdn;
 extern "C" int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
                                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                                    const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
-                                   void* o, float* lse, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
+                                   void* o, float* kept, const void* cu_seqlens, int64_t B, int64_t T, int64_t HQ, int64_t HKV,
                                    int64_t D, int64_t N, int dtype, int64_t window, int64_t sinks, float scale, unsigned flags,
                                    void* stream) {
   const int64_t st[9] = {q_batch_stride, q_token_stride, q_head_stride, k_batch_stride, k_token_stride, k_head_stride,
@@ -662,12 +666,13 @@ extern "C" int gdn_window_attn_fwd(const void* q, int64_t q_batch_stride, int64_
   }
   if (T == 0) return GDN_OK;
   if (!q || !k || !v || !o || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-                                reinterpret_cast<uintptr_t>(o)) & 15)) {
+                                reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(kept)) & 15)) {
     gdn_internal_set_error("gdn_window_attn_fwd: null or misaligned (16 bytes) tensor pointer");
     return GDN_ERR_INVALID;
   }
   FlashParams p{};
-  p.q = q, p.k = k, p.v = v, p.o = o, p.lse = lse;
+  p.q = q, p.k = k, p.v = v, p.o = o;
+  p.o_rest = kept, p.lse = kept ? kept + B * T * HQ * D / 2 : nullptr;
   p.qsb = st[0], p.qst = st[1], p.qsh = st[2], p.ksb = st[3], p.kst = st[4], p.ksh = st[5], p.vsb = st[6], p.vst = st[7], p.vsh = st[8];
   p.seqs = Packed{cu_seqlens, (flags & GDN_FLAG_CU_INT32) ? 1 : 0, N, T};
   p.B = B;
@@ -702,7 +707,7 @@ extern "C" size_t gdn_window_attn_bwd_workspace_size(int64_t B, int64_t T, int64
 extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
                                    const void* k, int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
                                    const void* v, int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride,
-                                   const void* o, const float* lse, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
+                                   const void* o, const float* kept, const void* d_o, const void* cu_seqlens, int64_t B, int64_t T,
                                    int64_t HQ, int64_t HKV, int64_t D, int64_t N, int64_t window, int64_t sinks, float scale,
                                    unsigned flags, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                                    void* stream) {
@@ -711,8 +716,8 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   if (int rc = window_check("gdn_window_attn_bwd", B, T, HQ, HKV, D, N, cu_seqlens, st, window, sinks, scale)) return rc;
   if (T == 0) return GDN_OK;
   uintptr_t every = 0;
-  bool null = !lse;
-  const void* const all[] = {q, k, v, o, d_o, dq, dk, dv, workspace};
+  bool null = false;
+  const void* const all[] = {q, k, v, o, kept, d_o, dq, dk, dv, workspace};
   for (const void* x : all) every |= reinterpret_cast<uintptr_t>(x), null |= !x;
   if (null || (every & 15)) {
     gdn_internal_set_error("gdn_window_attn_bwd: null or misaligned (16 bytes) tensor pointer");
@@ -725,7 +730,8 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   }
   WindowBwdParams p{};
   p.q = static_cast<const bf16*>(q), p.k = static_cast<const bf16*>(k), p.v = static_cast<const bf16*>(v);
-  p.o = static_cast<const bf16*>(o), p.d_o = static_cast<const bf16*>(d_o), p.lse = lse;
+  p.o = static_cast<const bf16*>(o), p.d_o = static_cast<const bf16*>(d_o);
+  p.o_rest = reinterpret_cast<const bf16*>(kept), p.lse = kept + B * T * HQ * D / 2;
   p.qsb = st[0], p.qst = st[1], p.qsh = st[2], p.ksb = st[3], p.kst = st[4], p.ksh = st[5], p.vsb = st[6], p.vst = st[7], p.vsh = st[8];
   p.dq = static_cast<bf16*>(dq), p.dk = static_cast<bf16*>(dk), p.dv = static_cast<bf16*>(dv);
   p.delta = static_cast<float*>(workspace);

@@ -38,18 +38,24 @@ def _heads(x: Tensor):
     return x, st
 
 
+def _kept_size(q: Tensor):
+    """Floats that a forward keeps for its backward: what o's rounding left, in 16 bits, and a logarithm a row."""
+    b, t, hq, d = q.shape
+    return b * t * hq * (d // 2 + 1)
+
+
 def fwd_impl(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Optional[Tensor], window: int, sinks: int, scale: float,
              flags: int, num_seqs: int, save: bool) -> tuple[Tensor, Tensor]:
     b, t, hq, d = q.shape
     (qs, qst), (ks, kst), (vs, vst) = _heads(q), _heads(k), _heads(v)
     cu = None if cu_seqlens is None else cu_seqlens.contiguous()
     o = torch.empty(b, t, hq, d, device=q.device, dtype=q.dtype)
-    lse = torch.empty((hq, b * t) if save else (0,), device=q.device, dtype=torch.float32)
+    kept = torch.empty(_kept_size(q) if save else 0, device=q.device, dtype=torch.float32)
     ptr = _lib.ptr
     _launch("gdn_window_attn_fwd", q, ptr(qs), *qst[:3], ptr(ks), *kst[:3], ptr(vs), *vst[:3], ptr(o),
-            ptr(lse if save else None), ptr(cu), b, t, hq, k.shape[2], d, num_seqs, _CODES[q.dtype], window, sinks, scale,
+            ptr(kept if save else None), ptr(cu), b, t, hq, k.shape[2], d, num_seqs, _CODES[q.dtype], window, sinks, scale,
             flags)
-    return o, lse
+    return o, kept
 
 
 fwd = torch.library.custom_op("sorernn::window_attention_fwd", mutates_args=())(fwd_impl)
@@ -58,10 +64,10 @@ fwd = torch.library.custom_op("sorernn::window_attention_fwd", mutates_args=())(
 @fwd.register_fake
 def _fwd_fake(q, k, v, cu_seqlens, window, sinks, scale, flags, num_seqs, save):
     b, t, hq, d = q.shape
-    return q.new_empty(b, t, hq, d), q.new_empty((hq, b * t) if save else (0,), dtype=torch.float32)
+    return q.new_empty(b, t, hq, d), q.new_empty((_kept_size(q) if save else 0,), dtype=torch.float32)
 
 
-def bwd_impl(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, d_o: Tensor, cu_seqlens: Optional[Tensor], window: int,
+def bwd_impl(q: Tensor, k: Tensor, v: Tensor, o: Tensor, kept: Tensor, d_o: Tensor, cu_seqlens: Optional[Tensor], window: int,
              sinks: int, scale: float, flags: int, num_seqs: int) -> tuple[Tensor, Tensor, Tensor]:
     b, t, hq, d = q.shape
     hkv = k.shape[2]
@@ -71,7 +77,7 @@ def bwd_impl(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, d_o: Tenso
     nbytes = int(_lib.load().gdn_window_attn_bwd_workspace_size(b, t, hq, hkv, d, num_seqs, window, sinks, int(cu is not None)))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
     ptr = _lib.ptr
-    _launch("gdn_window_attn_bwd", q, ptr(qs), *qst[:3], ptr(ks), *kst[:3], ptr(vs), *vst[:3], ptr(oc), ptr(lse), ptr(do),
+    _launch("gdn_window_attn_bwd", q, ptr(qs), *qst[:3], ptr(ks), *kst[:3], ptr(vs), *vst[:3], ptr(oc), ptr(kept), ptr(do),
             ptr(cu), b, t, hq, hkv, d, num_seqs, window, sinks, scale, flags, ptr(dq), ptr(dk), ptr(dv), ptr(ws), nbytes)
     return dq, dk, dv
 
@@ -80,7 +86,7 @@ bwd = torch.library.custom_op("sorernn::window_attention_bwd", mutates_args=())(
 
 
 @bwd.register_fake
-def _bwd_fake(q, k, v, o, lse, d_o, cu_seqlens, window, sinks, scale, flags, num_seqs):
+def _bwd_fake(q, k, v, o, kept, d_o, cu_seqlens, window, sinks, scale, flags, num_seqs):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
@@ -93,11 +99,11 @@ def _setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, d_o, _d_lse):
-    q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+def _backward(ctx, d_o, _d_kept):
+    q, k, v, o, kept, cu_seqlens = ctx.saved_tensors
     if d_o is None:
         d_o = torch.zeros_like(o)
-    return *_library._run_bwd(bwd, bwd_impl, q, k, v, o, lse, d_o, cu_seqlens, *ctx.meta), *(None,) * 7
+    return *_library._run_bwd(bwd, bwd_impl, q, k, v, o, kept, d_o, cu_seqlens, *ctx.meta), *(None,) * 7
 
 
 fwd.register_autograd(_backward, setup_context=_setup)
