@@ -10,8 +10,9 @@
 // way), the other holds 32 keys and walks their queries (dk, dv, summed over the q heads of the kv head in fp32). No atomics.
 //
 // Measured on 2 x 4,096 tokens, 16 heads on 4 of 128, window 1,024, 4 sinks, operations of visible pairs only (a large bf16
-// product reaches 1,228 TFLOP/s): forward 93 us, 647 TFLOP/s; dq 128 us, 707; dk and dv 218 us, 545; sinks 6 us. A prompt of
-// 8,192 tokens 85-97 us. 5,003 tokens in 7 documents, 8 heads on 2 of 64, window 200: 19, 23, 32 us, join 5, sinks 4.
+// product reaches 1,228 TFLOP/s): forward 102 us, 591 TFLOP/s (93 where nothing is kept for a backward); dq 137 us, 660; dk
+// and dv 218 us, 545; sinks 6 us. A prompt of 8,192 tokens 85-97 us. 5,003 tokens in 7 documents, 8 heads on 2 of 64, window
+// 200: 21, 25, 32 us, join 5, sinks 4.
 
 #include "gdn_flash.h"
 
