@@ -102,7 +102,8 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70
 // p = 2^(s c - m c), c = scale log2(e) > 0. The row's m moves only when a block's maximum exceeds it by more than `slack` =
 // 8 / c: p <= 2^8 meanwhile, which costs no precision, and O^T is rescaled rarely. A row that saw no key yet keeps m = -inf and
 // uses 0. P is rounded to the inputs' type for the product (off by half a step of it a term, as the output itself is); the
-// row sum adds p in fp32, so that the backward's logarithm of it is exact to fp32.
+// row sum adds p in fp32, so that the backward's logarithm of it is exact to fp32. The sum of a row that saw a key whose score
+// is above -inf is 1 at least.
 template <int KT, int D, typename E>
 __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 32], float& m, float& l, float c, float slack,
                                              const E* vb, const TileReads<D>& rd) {
@@ -340,6 +341,24 @@ __device__ __forceinline__ RowView row_view(const FlashParams& p, const PagedPla
   return v;
 }
 
+// Whether a row sees any key of the cache. Asked of rows whose sum is 0: with a key all their scores are -inf, and their softmax
+// is 0 / 0.
+template <int BK>
+__device__ __forceinline__ bool sees_any(const FlashParams& p, const PagedPlan& f, const RowView& v) {
+  if (f.sq.num < 0) return false;
+  const int* const table = p.table + f.sq.num * p.table_stride;
+  for (int n = 0; n < f.bl.count; ++n) {
+    const int k0 = f.bl.at(n) * BK;
+    const uint64_t seen = v.block(k0, p.window, p.sinks) & bits_below(f.klen - k0);
+    for (int g = 0; g < BK / 16; ++g) {
+      if (!(seen >> 16 * g & 0xffff)) continue;
+      const int id = table[(k0 + 16 * g) >> p.shift];
+      if (id >= 0 && id < p.pages) return true;
+    }
+  }
+  return false;
+}
+
 // ------------------------------------------------------------------------------------------------ forward over whole tiles
 constexpr int kBQ = 128;  // rows a workgroup: 32 a wave
 constexpr int kBK = 64;   // keys a block
@@ -564,6 +583,10 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
     pml = p.part + p.tiles * p.HKV * p.splits * kBQ * D + (f.job * p.splits + split) * 2 * kBQ;
   }
   l += __shfl_xor(l, 32, kWave);
+  if (whole && row_ok && l == 0.f) {  // NaN where keys were seen, all with scores of -inf
+    if constexpr (PAGED) l = sees_any<kBK>(p, f, view) ? NAN : 0.f;
+    else l = sq.num >= 0 ? NAN : 0.f;
+  }
   bool fine = finite_all(acc);
   fine = l != l || (__shfl_xor((int)fine, 32, kWave) && fine);
   const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;

@@ -340,6 +340,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
                                            4 * (piece ^ (r & (CH - 1))));
     }
+    if (f.used == 1 && sum == 0.f && sees_any<kFewKeys>(p, f, row_view(p, f, f.row0 + r))) sum = NAN;
     if (sum == sum) {
       uint32_t bad = 0;
 #pragma unroll
@@ -432,11 +433,12 @@ __global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(Flash
     x = x * a + *reinterpret_cast<const f32x4*>(xs + 4 * o) * b;
     top = now;
   }
+  const int row = f.row0 + r;
+  if (sum == 0.f && sees_any<BK>(p, f, row_view(p, f, row))) sum = NAN;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   typename Pack<E>::x4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
-  const int row = f.row0 + r;
   *reinterpret_cast<typename Pack<E>::x4*>(static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + row / rep) * p.HQ) +
                                                                    f.hkv * rep + row % rep) * D + 4 * piece) = y;
 }
