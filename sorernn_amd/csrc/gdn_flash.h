@@ -168,6 +168,30 @@ __device__ __forceinline__ float dot_row(const E* a, const E* b) {
   return x;
 }
 
+// Whether any of a row's columns `again` (bit i: l + 64 i) is finite so far: a sum that is not stays so.
+template <int D>
+__device__ __forceinline__ bool open_columns(int again, const float (&acc)[D / 64]) {
+  bool open = false;
+  for (int i = 0; i < D / 64; ++i) open |= (again >> i & 1) && finite_f(acc[i]);
+  return __any(open);
+}
+
+// acc += the sum over lanes z of `live` of lane z's w times row(z); others' rows are not read, and have no part in it.
+template <int D, typename Row>
+__device__ __forceinline__ void add_rows(uint64_t live, float w, Row row, float (&acc)[D / 64]) {
+  const int lane = threadIdx.x % kWave, some = __ffsll((unsigned long long)live) - 1;  // read in place of the others
+#pragma unroll 8
+  for (int z = 0; z < kWave; ++z) {
+    const bool on = live >> z & 1;
+    const float wz = __shfl(w, z, kWave);
+    const auto* r = row(on ? z : some);
+    for (int i = 0; i < D / 64; ++i) {
+      const float x = (float)r[lane + 64 * i];
+      acc[i] += on ? wz * x : 0.f;
+    }
+  }
+}
+
 // Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c. key(j): K row j or null (not to
 // be seen); val(j): V row j. False once none of the columns can become finite.
 template <int D, typename E, typename Key, typename Val, typename Seen>
@@ -180,20 +204,8 @@ __device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key
     const uint64_t live = __ballot(kr != nullptr);
     if (!live) continue;
     const float p = kr ? __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q, kr), c, nmc)) : 0.f;
-    const int some = __ffsll((unsigned long long)live) - 1;  // read in place of keys that are not seen
-#pragma unroll 8
-    for (int n = 0; n < kWave; ++n) {
-      const bool on = live >> n & 1;
-      const float pn = __shfl(p, n, kWave);
-      const E* vr = val(base + (on ? n : some));
-      for (int i = 0; i < D / 64; ++i) {
-        const float x = (float)vr[lane + 64 * i];
-        acc[i] += on ? pn * x : 0.f;
-      }
-    }
-    bool open = false;
-    for (int i = 0; i < D / 64; ++i) open |= (again >> i & 1) && finite_f(acc[i]);
-    if (!__any(open)) return false;
+    add_rows<D>(live, p, [&](int n) { return val(base + n); }, acc);
+    if (!open_columns<D>(again, acc)) return false;
   }
   return true;
 }

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
   }
   delta += __shfl_xor(delta, 32, kWave);
   const float lse = p.lse[hq * all + tok + qc];
-  if (row_ok && hh == 0) p.delta[hq * all + tok + qi] = delta;
+  if (row_ok && hh == 0) p.delta[hq * all + tok + qi] = finite_f(lse) ? delta : NAN;  // of those no ds is finite
 
   const char* const kbase = reinterpret_cast<const char*>(p.k + sq.row * p.ksb + sq.start * p.kst + job.hkv * p.ksh);
   const char* const vbase = reinterpret_cast<const char*>(p.v + sq.row * p.vsb + sq.start * p.vst + job.hkv * p.vsh);
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
   }
   bool fine = finite_all(acc);
   fine = lse != lse || !finite_f(delta) || (__shfl_xor((int)fine, 32, kWave) && fine);  // of those no ds that is seen is finite
-  if (row_ok && fine) {
+  if (row_ok) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -191,12 +191,14 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
             to_bf16x4(acc[d][4 * j] * p.scale, acc[d][4 * j + 1] * p.scale, acc[d][4 * j + 2] * p.scale, acc[d][4 * j + 3] * p.scale);
   }
   uint64_t redo = __ballot(row_ok && !fine && hh == 0);
-  while (redo) {  // over the keys that the row sees only
+  if (redo) wait_loads();  // what was written above is there before parts of it are written again
+  while (redo) {  // columns that are not finite, over the keys that the row sees only, until none of them can be
     const int n = __ffsll((unsigned long long)redo) - 1, r = wq0 + n;
     redo &= redo - 1;
     const bf16* qp = p.q + sq.row * p.qsb + (sq.start + r) * p.qst + hq * p.qsh;
     const int64_t at = ((tok + r) * p.HQ + hq) * D;
     const float lr = __shfl(lse, n, kWave), dr = __shfl(delta, n, kWave);
+    const int again = not_finite<D>(acc, n);
     float a[D / 64] = {};
     for (int base = 0; base <= r; base += kWave) {
       const int j = base + lane;
@@ -208,19 +210,11 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
         const float s = dot_row<D>(qp, reinterpret_cast<const bf16*>(kbase + (int64_t)j * kst));
         ds = __builtin_amdgcn_exp2f(fmaf(s, c, -lr)) * (dot_row<D>(p.d_o + at, reinterpret_cast<const bf16*>(vbase + (int64_t)j * vst)) - dr);
       }
-      const int some = __ffsll((unsigned long long)live) - 1;
-#pragma unroll 8
-      for (int i = 0; i < kWave; ++i) {
-        const bool on = live >> i & 1;
-        const float x = __shfl(ds, i, kWave);
-        const bf16* kr = reinterpret_cast<const bf16*>(kbase + (int64_t)(base + (on ? i : some)) * kst);
-        for (int e = 0; e < D / 64; ++e) {
-          const float y = (float)kr[lane + 64 * e];
-          a[e] += on ? x * y : 0.f;
-        }
-      }
+      add_rows<D>(live, ds, [&](int z) { return reinterpret_cast<const bf16*>(kbase + (int64_t)(base + z) * kst); }, a);
+      if (!open_columns<D>(again, a)) break;
     }
-    for (int e = 0; e < D / 64; ++e) p.dq[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
+    for (int e = 0; e < D / 64; ++e)
+      if (again >> e & 1) p.dq[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
   }
 }
 
@@ -230,7 +224,12 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
 // workgroups share a tile's blocks. Sinks are seen by far queries too: the first k_tiles * shares jobs are every tile's near
 // queries, the others a piece of the far queries for one tile of sinks. A tile's sums over those meet in
 // gated_delta_window_attn_sinks_kernel.
-template <int D>
+//
+// BAD: a launch behind the one that computes everything, which takes a tile again if masked blocks of it hold queries whose
+// logarithm or delta is not finite, and ends at once if none does. There a masked weight, 0, met an infinity or NaN of do or q, and
+// keys that do not see it became NaN too. (As a second path of one kernel it cost the ordinary one registers, and the training
+// step 420 -> 433 to 449 us; summing such keys again row by row took 95 ms for 6,000 tokens of 16:4 heads under a NaN loss.)
+template <int D, bool BAD>
 __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(WindowBwdParams p) {
   // of D = 128 half of each wave's V fragments lie in LDS (VL k-steps): with all of them in registers the loop reloads spilled
   // ones, and waits for the tiles under way with them
@@ -242,6 +241,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   __shared__ __align__(16) float Ls0[2][2 * kBK];  // lse, delta
   __shared__ __align__(16) float Ls1[2][2 * kBK];
   __shared__ __align__(16) bf16 Vs[VL ? 4 * VL * kWave * 8 : 8];
+  __shared__ int bads[8];
   const int t = threadIdx.x, lane = t & 63, w8 = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
   const int w = w8 & 3, team = w8 >> 2;
   const int rep = p.HQ / p.HKV;
@@ -278,6 +278,21 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   const int64_t tok = sq.row * p.seqs.T + sq.start, all = p.B * p.seqs.T;
   const bf16* const krow = p.k + sq.row * p.ksb + (sq.start + kc) * p.kst + job.hkv * p.ksh;
   const bf16* const vrow = p.v + sq.row * p.vsb + (sq.start + kc) * p.vst + job.hkv * p.vsh;
+  if constexpr (BAD) {
+    // masked blocks are those of a near tile's first and last queries, and of far pieces all
+    bool bad = false;
+    const int some = imin(to - from, far_job ? to - from : 192), each = far_job ? some : 2 * some;
+    for (int x = t; x < rep * each; x += 512) {
+      const int h = x / each, r = x - h * each, i = r < some ? from + r : to - 2 * some + r;
+      bad |= !finite_f(p.delta[(job.hkv * rep + h) * all + tok + i]);
+    }
+    const bool any = __any(bad);
+    if (lane == 0) bads[w8] = any;
+    __syncthreads();
+    int count = 0;
+    for (int x = 0; x < 8; ++x) count += bads[x];
+    if (!count) return;
+  }
   bf16x8 kf[DS], vf[VR];
 #pragma unroll
   for (int s = 0; s < DS; ++s) kf[s] = *reinterpret_cast<const bf16x8*>(krow + 16 * s + 8 * hh);
@@ -365,6 +380,68 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
         for (int d = 0; d < DT; ++d) dk[d] = mma32(tr_frag(qb + (2 * qt + h) * 16 * D, rd, d), pb[h], dk[d]);
     }
   };
+  // The same with queries whose logarithm (`lbad`: all their weights are NaN) or delta (`dbad`: none of their ds is finite) is not
+  // finite: their entries that are not are left out of the products, and the keys that see them become NaN.
+  auto block_bad = [&](const bf16* qb, const bf16* db, const float* lb, int q0) {
+    const uint64_t there = bits_below(to - q0), lbad = __ballot(!finite_f(lb[lane])) & there, dbad = __ballot(!finite_f(lb[kBK + lane])) & there;
+    const int kk = wk0 + li, hi = kk < p.sinks ? to : imin(to, kk + p.window);
+    const uint64_t seen = bits_below(hi - q0) & ~bits_below(imax(kk, from) - q0);
+    const uint64_t seen_v = (seen & ~lbad) >> 4 * hh, seen_k = (seen & ~(lbad | dbad)) >> 4 * hh;
+    const float to_k = seen & (lbad | dbad) ? NAN : 0.f, to_v = seen & lbad ? NAN : 0.f;
+    auto finite = [](bf16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7f80) != 0x7f80; };
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dk[d] += to_k, dv[d] += to_v;
+#pragma nounroll
+    for (int qt = 0; qt < 2; ++qt) {
+      TileReads<D> rd = reads.here();
+      f32x16 s{}, dp{}, one;
+#pragma unroll
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(qb + 32 * qt * D, rd, st), kf[st], s);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool see = (uint32_t)(seen_v >> 32 * qt) >> (8 * (e >> 2) + (e & 3)) & 1;
+        s[e] = see ? __builtin_amdgcn_exp2f(fmaf(s[e], c, -lb[32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3)])) : 0.f;
+        one[e] = see ? 1.f : 0.f;
+      }
+      bf16x8 pb[2], ones[2];
+      pack16<bf16>(s, pb);
+      pack16<bf16>(one, ones);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          bf16x8 x = tr_frag(db + (2 * qt + h) * 16 * D, rd, d), odd;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool fine = finite(x[e]);
+            odd[e] = (bf16)(fine ? 0.f : 1.f);
+            x[e] = fine ? x[e] : (bf16)0.f;
+          }
+          dv[d] = mma32(x, pb[h], dv[d]);
+          const f32x16 n = mma32(odd, ones[h], f32x16{});  // entries that the key sees and that are not finite
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dv[d][e] = n[e] > 0.f ? NAN : dv[d][e];
+        }
+#pragma unroll
+      for (int st = 0; st < DS; ++st)
+        dp = mma32(row_frag(db + 32 * qt * D, rd, st), st < VR ? vf[st < VR ? st : 0] : ld8(vl + (st - VR) * kWave * 8), dp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool see = (uint32_t)(seen_k >> 32 * qt) >> (8 * (e >> 2) + (e & 3)) & 1;
+        s[e] = see ? s[e] * (dp[e] - lb[kBK + 32 * qt + 8 * (e >> 2) + 4 * hh + (e & 3)]) : 0.f;
+      }
+      pack16<bf16>(s, pb);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          bf16x8 x = tr_frag(qb + (2 * qt + h) * 16 * D, rd, d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = finite(x[e]) ? x[e] : (bf16)0.f;
+          dk[d] = mma32(x, pb[h], dk[d]);
+        }
+    }
+  };
   auto arrive = [&](int blk, bf16* qd, bf16* dd) {
     wait_loads();
     if ((blk + 1) * kBK > sq.len) {
@@ -397,9 +474,24 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     }
     __syncthreads();
     const int turns = (rep * nqb + step_by - 1) / step_by;  // the same for both teams
-    for (int n = 0; n < turns; n += 2) {
-      step(q0p, d0p, Ls0[team], q1p, d1p, Ls1[team]);
-      if (n + 1 < turns) step(q1p, d1p, Ls1[team], q0p, d0p, Ls0[team]);
+    if constexpr (!BAD) {
+      for (int n = 0; n < turns; n += 2) {
+        step(q0p, d0p, Ls0[team], q1p, d1p, Ls1[team]);
+        if (n + 1 < turns) step(q1p, d1p, Ls1[team], q0p, d0p, Ls0[team]);
+      }
+    } else {
+      for (int n = 0; n < turns; ++n) {
+        const int q0 = (qb0 + qb) * kBK, q1 = q0 + kBK - 1;
+        if (g < rep && wave_live && !none_sees(q0, q1, wk0, wk0 + 31, p.window, p.sinks)) block_bad(q0p, d0p, Ls0[team], q0);
+        qb += step_by;
+        place();
+        __syncthreads();
+        if (g < rep) {
+          fetch(g, qb0 + qb, q0p, d0p, Ls0[team]);
+          arrive(qb0 + qb, q0p, d0p);
+        }
+        __syncthreads();
+      }
     }
     // the second team's sums, a wave's 32 KB (16 KB) in a tile array
     f32x4* const sums = reinterpret_cast<f32x4*>(w == 0 ? Qs0 : w == 1 ? Qs1 : w == 2 ? Ds0 : Ds1) + lane;
@@ -425,9 +517,6 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     }
   }
   if (team) return;
-  bool fine_k = finite_all(dk), fine_v = finite_all(dv);
-  fine_k = __shfl_xor((int)fine_k, 32, kWave) && fine_k;
-  fine_v = __shfl_xor((int)fine_v, 32, kWave) && fine_v;
   const int64_t out = ((tok + kc) * p.HKV + job.hkv) * D;
   // sums that meet others': where those of key j go (dk; dv `dv_at` behind them), null: the result
   const bool alone = far_job || p.shares == 1;
@@ -455,56 +544,6 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
           *reinterpret_cast<bf16x4*>(p.dv + out + at) = to_bf16x4(b[0], b[1], b[2], b[3]);
         }
       }
-  }
-  const uint64_t redo_v = __ballot(row_ok && !fine_v && hh == 0);
-  uint64_t redo = __ballot(row_ok && !(fine_k && fine_v) && hh == 0);
-  if (redo) wait_loads();  // what was written above is there before parts of it are written again
-  while (redo) {  // over the queries that see the key only
-    const int n = __ffsll((unsigned long long)redo) - 1, j = wk0 + n;
-    const bool want_v = redo_v >> n & 1;
-    redo &= redo - 1;
-    const bf16* kr = p.k + sq.row * p.ksb + (sq.start + j) * p.kst + job.hkv * p.ksh;
-    const bf16* vr = p.v + sq.row * p.vsb + (sq.start + j) * p.vst + job.hkv * p.vsh;
-    float a[D / 64] = {}, b[D / 64] = {};
-    bool over = false;  // a weight is NaN: all of dk and dv are; a ds is not finite: no entry of dk is
-    for (int h = 0; h < rep && !over; ++h)
-      for (int base = from; base < to && !over; base += kWave) {
-        const int i = base + lane;  // of a shared tile the blocks of this workgroup only
-        const bool mine = far_job || (h * nqb + i / kBK - qb0) / 2 % p.shares == share;
-        const bool see = i < to && mine && sees(i, j, p.window, p.sinks);
-        const uint64_t live = __ballot(see);
-        if (!live) continue;
-        auto q_at = [&](int x) { return reinterpret_cast<const bf16*>(qbase + h * p.qsh * 2 + (int64_t)x * qst); };
-        auto d_at = [&](int x) { return reinterpret_cast<const bf16*>(dbase + (int64_t)h * D * 2 + (int64_t)x * dst); };
-        const int64_t at = (job.hkv * rep + h) * all + tok + i;
-        float pr = 0.f, ds = 0.f;
-        if (see) {
-          pr = __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q_at(i), kr), c, -p.lse[at]));
-          ds = pr * (dot_row<D>(d_at(i), vr) - p.delta[at]);
-        }
-        over = __any(pr != pr) || (!want_v && __any(!finite_f(ds)));
-        const int some = __ffsll((unsigned long long)live) - 1;
-#pragma unroll 8
-        for (int x = 0; x < kWave; ++x) {
-          const bool on = live >> x & 1;
-          const float px = __shfl(pr, x, kWave), dx = __shfl(ds, x, kWave);
-          for (int e = 0; e < D / 64; ++e) {
-            const float qx = (float)q_at(base + (on ? x : some))[lane + 64 * e], ox = (float)d_at(base + (on ? x : some))[lane + 64 * e];
-            a[e] += on ? dx * qx : 0.f;
-            b[e] += on ? px * ox : 0.f;
-          }
-        }
-      }
-    const int64_t at = ((tok + j) * p.HKV + job.hkv) * D;
-    for (int e = 0; e < D / 64; ++e) {
-      if (float* const to_part = part_at(j)) {
-        to_part[lane + 64 * e] = a[e];
-        if (want_v) to_part[dv_at + lane + 64 * e] = b[e];
-      } else {
-        p.dk[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
-        if (want_v) p.dv[at + lane + 64 * e] = (bf16)b[e];
-      }
-    }
   }
 }
 
@@ -760,8 +799,11 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<128>, dim3((unsigned)q_groups), block, 0, s, p);
   else hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<64>, dim3((unsigned)q_groups), block, 0, s, p);
   if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dq_kernel")) return rc;
-  if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<128>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
-  else hipLaunchKernelGGL(gated_delta_window_attn_dkv_kernel<64>, dim3((unsigned)k_groups), dim3(512), 0, s, p);
+  if (D == 128) hipLaunchKernelGGL((gated_delta_window_attn_dkv_kernel<128, false>), dim3((unsigned)k_groups), dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((gated_delta_window_attn_dkv_kernel<64, false>), dim3((unsigned)k_groups), dim3(512), 0, s, p);
+  if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dkv_kernel")) return rc;
+  if (D == 128) hipLaunchKernelGGL((gated_delta_window_attn_dkv_kernel<128, true>), dim3((unsigned)k_groups), dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((gated_delta_window_attn_dkv_kernel<64, true>), dim3((unsigned)k_groups), dim3(512), 0, s, p);
   if (int rc = gdn_internal_check_launch("gated_delta_window_attn_dkv_kernel")) return rc;
   if (p.shares > 1) {
     const int64_t quads = B * T * HKV * 2 * D / 4, groups = (quads + 255) / 256;
