@@ -35,13 +35,15 @@ struct WindowBwdParams {
   float* delta;                     // [HQ, B T]
   bf16 *dq, *dk, *dv;               // contiguous
   Packed seqs;
-  int64_t B, q_tiles, k_tiles, pieces;
+  int64_t B, q_tiles, k_tiles;
   int HQ, HKV, parts, window, sinks;
   float scale, scale_log2;
-  // far queries of the sinks: a slot for each piece of `far` queries and one a sequence for the near ones, per kv head and tile
-  // of 128 sinks: [slots][HKV][sink tiles][2][sink rows][D]
+  // far queries of the sinks: slots for pieces of them and, behind those, for the near ones, per kv head and tile of 128 sinks:
+  // [far_jobs + near slots][HKV][2][sink rows][D]
   float* part;
-  int far, sink_tiles, sink_rows;
+  FarList far;
+  int64_t far_jobs;
+  int sink_rows;
   // few key tiles: the near queries of one are dealt out to `shares` workgroups, whose sums meet in another kernel:
   // [shares][B T][HKV][2][D]
   float* near;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   const int w = w8 & 3, team = w8 >> 2;
   const int rep = p.HQ / p.HKV;
   Job job;
-  if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles * p.shares + p.pieces * p.sink_tiles, job)) return;
+  if (!job_of(blockIdx.x, p.HKV, 1, p.parts, p.k_tiles * p.shares + p.far_jobs, job)) return;
   const bool far_job = job.tile >= p.k_tiles * p.shares;
   Seq sq;
   int tile, from, to, share = 0;
@@ -260,16 +262,15 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     if (tile * kBQ >= sq.len) return;
     from = tile * kBQ;
     to = sq.num < 0 ? from : near_end(tile, p.window, sq.len);
-    slot = to < sq.len && sq.num >= 0 && p.shares == 1 ? p.pieces + sq.num : -1;
+    slot = to < sq.len && sq.num >= 0 && p.shares == 1 ? p.far_jobs + near_slot(p.far, sq, tile) : -1;
   } else {
-    const int64_t f = job.tile - p.k_tiles * p.shares;
-    slot = f / p.sink_tiles;
-    tile = (int)(f - slot * p.sink_tiles);
-    if (p.seqs.cu) sq = packed_tile(p.seqs, slot, 1, p.far);
-    else sq = Seq{slot % p.B, 0, (int)p.seqs.T, 0, (int)(slot / p.B)};
-    if (sq.num < 0 || tile * kBQ >= sq.len || sq.tile > sq.len / p.far) return;
-    from = imax(near_end(tile, p.window, sq.len), sq.tile * p.far);
-    to = imin(sq.len, (sq.tile + 1) * p.far);
+    slot = job.tile - p.k_tiles * p.shares;
+    const FarWork f = far_work(p.seqs, p.far, p.B, slot);
+    sq = f.sq;
+    tile = f.sink_tile;
+    if (tile < 0 || tile * kBQ >= sq.len) return;
+    from = imax(near_end(tile, p.window, sq.len), p.far.first_query() + sq.tile * p.far.far);
+    to = imin(sq.len, p.far.first_query() + (sq.tile + 1) * p.far.far);
     if (from >= to) return;
   }
   const int wk0 = tile * kBQ + 32 * w, key = wk0 + li, kc = imin(key, sq.len - 1);
@@ -524,7 +525,7 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   auto part_at = [&](int j) -> float* {
     if (!alone) return p.near + ((share * all + tok + j) * p.HKV + job.hkv) * 2 * D;
     return slot >= 0 && j < p.sinks
-               ? p.part + ((slot * p.HKV + job.hkv) * p.sink_tiles + tile) * 2 * p.sink_rows * D + (j - tile * kBQ) * D
+               ? p.part + (slot * p.HKV + job.hkv) * 2 * p.sink_rows * D + (j - tile * kBQ) * D
                : nullptr;
   };
   float* const part = part_at(kc);
@@ -547,36 +548,29 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   }
 }
 
-// dk and dv of sinks that far queries see: the near queries' sums and each piece's, in order. A workgroup a sequence, kv head
-// and tile of sinks.
+// dk and dv of sinks that far queries see: the near queries' sums and each piece's, in order. A workgroup a near slot and kv head.
 __global__ __launch_bounds__(256) void gated_delta_window_attn_sinks_kernel(WindowBwdParams p, int D) {
-  const int tile = blockIdx.x % p.sink_tiles, hkv = blockIdx.x / p.sink_tiles % p.HKV;
-  const int64_t num = blockIdx.x / p.sink_tiles / p.HKV;
-  int64_t row = 0, start = 0, first = num, step = p.B;  // slots of the sequence's pieces
-  int len = (int)p.seqs.T;
-  if (p.seqs.cu) {
-    const int64_t b0 = p.seqs.bound(num + 1), b1 = p.seqs.bound(num + 2);
-    start = b0;
-    len = (int)(b1 > b0 ? b1 - b0 : 0);
-    first = b0 / p.far + num + 1;
-    step = 1;
-  } else {
-    row = num;
-  }
+  const int hkv = blockIdx.x % p.HKV;
+  const FarWork f = near_work(p.seqs, p.far, blockIdx.x / p.HKV);
+  const Seq sq = f.sq;
+  const int tile = f.sink_tile, len = sq.len;
+  if (tile < 0) return;
   const int near = near_end(tile, p.window, len), rows = imin(imin(p.sinks, len) - tile * kBQ, kBQ);
   if (near >= len || rows <= 0) return;  // written where it was computed
+  const int64_t first = far_slot(p.seqs, p.far, sq, tile), step = far_step(p.seqs, p.far, sq, p.B);
+  const int q0 = p.far.first_query(), n0 = (near - q0) / p.far.far, n1 = (len - 1 - q0) / p.far.far;
   const int quads = D / 4;
-  const int64_t one = (int64_t)2 * p.sink_rows * D, per = p.HKV * p.sink_tiles * one, here = (hkv * p.sink_tiles + tile) * one;
+  const int64_t one = (int64_t)2 * p.sink_rows * D, per = p.HKV * one;
   for (int i = threadIdx.x; i < 2 * rows * quads; i += 256) {
     const int which = i / (rows * quads), r = i / quads % rows, d = i % quads * 4;
-    const int64_t at = here + (which * p.sink_rows + r) * D + d;
-    const int64_t token = row * p.seqs.T + start + tile * kBQ + r;
+    const int64_t at = hkv * one + (which * p.sink_rows + r) * D + d;
+    const int64_t token = sq.row * p.seqs.T + sq.start + tile * kBQ + r;
     f32x4 x{};
-    if (p.shares == 1) x = *reinterpret_cast<const f32x4*>(p.part + (p.pieces + num) * per + at);
+    if (p.shares == 1) x = *reinterpret_cast<const f32x4*>(p.part + (p.far_jobs + near_slot(p.far, sq, tile)) * per + at);
     else
       for (int n = 0; n < p.shares; ++n)
         x += *reinterpret_cast<const f32x4*>(p.near + (((n * p.B * p.seqs.T + token) * p.HKV + hkv) * 2 + which) * D + d);
-    for (int n = near / p.far; n <= (len - 1) / p.far; ++n) x += *reinterpret_cast<const f32x4*>(p.part + (first + n * step) * per + at);
+    for (int n = n0; n <= n1; ++n) x += *reinterpret_cast<const f32x4*>(p.part + (first + n * step) * per + at);
     if (!which) x *= p.scale;
     bf16* to = (which ? p.dv : p.dk) + (token * p.HKV + hkv) * D + d;
     *reinterpret_cast<bf16x4*>(to) = to_bf16x4(x[0], x[1], x[2], x[3]);
@@ -641,17 +635,29 @@ static int far_sinks(int64_t window, int64_t sinks) { return window <= 0 ? 0 : s
 constexpr int kFarPiece = 256;
 
 struct FarPlan {
-  int far, sink_tiles, sink_rows;
-  int64_t pieces;
+  FarList list;
+  int sink_rows;
+  int64_t jobs, near;  // slots of far pieces and of near queries, both times tiles of sinks
 };
+// Slots by number where all sequences together have no more tiles of sinks than there is room for by start (batch rows always);
+// else by start: 65,536 tokens in 2,000 documents, 8 kv heads of 128, window 256, 4 sinks take 138 MB, by number 1.1 GB.
 static FarPlan far_plan(int64_t B, int64_t T, int64_t N, bool varlen, int window, int sinks) {
-  FarPlan f{kFarPiece, 0, 0, 0};
-  if (!sinks || (int64_t)window + 1 >= T) return f;  // every query is a near one
+  FarPlan f{FarList{kFarPiece, 0, 0, 0}, 0, 0, 0};
+  if (!sinks || (int64_t)window + kBQ > T) return f;  // every query is a near one
+  FarList& l = f.list;
   const int64_t some = sinks < T ? sinks : T;
-  f.sink_tiles = (int)((some + kBQ - 1) / kBQ);
-  f.far = (int)(kFarPiece * f.sink_tiles < kFar ? kFarPiece * f.sink_tiles : kFar);  // with more tiles longer pieces: the partial sums stay as large
-  f.sink_rows = f.sink_tiles > 1 ? kBQ : (int)((some + 31) / 32 * 32);
-  f.pieces = varlen ? packed_tiles(T, N, 1, f.far) : B * ((T + f.far - 1) / f.far);
+  l.tiles = (int)((some + kBQ - 1) / kBQ);
+  l.far = kFarPiece * l.tiles;  // with more tiles longer pieces: the partial sums stay as large
+  l.reach = window + kBQ;
+  const int by_start = far_by_start(l.reach, l.tiles);
+  if (varlen && N * l.tiles > T / by_start) {
+    l.by_start = by_start;
+    f.jobs = f.near = T / by_start;
+  } else {
+    f.jobs = (varlen ? packed_tiles(T, N, 1, l.far) : B * ((T + l.far - 1) / l.far)) * l.tiles;
+    f.near = N * l.tiles;
+  }
+  f.sink_rows = l.tiles > 1 ? kBQ : (int)((some + 31) / 32 * 32);
   return f;
 }
 
@@ -680,9 +686,9 @@ struct BwdSizes {
 };
 static BwdSizes bwd_sizes(int64_t B, int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t N, bool varlen, int window, int sinks) {
   BwdSizes b{far_plan(B, T, N, varlen, window, sinks), varlen ? packed_tiles(T, N, 1, kBQ) : B * ((T + kBQ - 1) / kBQ), 1, 0, 0, 0};
-  b.shares = dkv_shares(T, HQ, HKV, b.tiles, b.far.pieces * b.far.sink_tiles, window);
+  b.shares = dkv_shares(T, HQ, HKV, b.tiles, b.far.jobs, window);
   b.delta = ((size_t)(B * T * HQ) * 4 + 255) / 256 * 256;
-  b.part = (size_t)(b.far.sink_tiles ? b.far.pieces + N : 0) * HKV * b.far.sink_tiles * 2 * b.far.sink_rows * D * 4;
+  b.part = (size_t)(b.far.jobs + b.far.near) * HKV * 2 * b.far.sink_rows * D * 4;
   b.near = b.shares > 1 ? (size_t)b.shares * B * T * HKV * 2 * D * 4 : 0;
   return b;
 }
@@ -786,14 +792,13 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
   p.shares = sizes.shares;
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizes.delta);
   p.near = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizes.delta + sizes.part);
-  p.far = f.far, p.sink_tiles = f.sink_tiles, p.sink_rows = f.sink_rows, p.pieces = f.pieces;
+  p.far = f.list, p.far_jobs = f.jobs, p.sink_rows = f.sink_rows;
   const int64_t q_groups = job_groups(HKV, HQ / HKV, p.q_tiles);
-  const int64_t k_groups = job_groups(HKV, 1, p.k_tiles * p.shares + p.pieces * p.sink_tiles), s_groups = N * HKV * p.sink_tiles;
+  const int64_t k_groups = job_groups(HKV, 1, p.k_tiles * p.shares + p.far_jobs), s_groups = f.near * HKV;
   if (q_groups > kMaxGroups256 || k_groups > kMaxGroups256 / 2 || s_groups > kMaxGroups256) {  // k_groups: of 512 threads
     gdn_internal_set_error("gdn_window_attn_bwd: grid too large");
     return GDN_ERR_UNSUPPORTED;
   }
-  if (!f.sink_tiles) p.sink_tiles = 1, p.pieces = 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 block(256);
   if (D == 128) hipLaunchKernelGGL(gated_delta_window_attn_dq_kernel<128>, dim3((unsigned)q_groups), block, 0, s, p);
@@ -810,7 +815,7 @@ extern "C" int gdn_window_attn_bwd(const void* q, int64_t q_batch_stride, int64_
     hipLaunchKernelGGL(gated_delta_window_attn_join_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), block, 0, s, p, (int)D);
     if (int rc = gdn_internal_check_launch("gated_delta_window_attn_join_kernel")) return rc;
   }
-  if (f.sink_tiles) {
+  if (f.near) {
     hipLaunchKernelGGL(gated_delta_window_attn_sinks_kernel, dim3((unsigned)s_groups), block, 0, s, p, (int)D);
     return gdn_internal_check_launch("gated_delta_window_attn_sinks_kernel");
   }
