@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
     float c[8], s[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      c[e] = in_rot ? tab[w][0][d0 + e] : 1.f;
+      c[e] = in_rot ? tab[w][0][d0 + e] : 1.f;  // of others unused
       s[e] = in_rot ? tab[w][1][d0 + e] : 0.f;
     }
     for (int r0 = r_first; r0 < rows; r0 += U * r_step) {  // uniform inside a row's lanes
@@ -138,11 +138,17 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = x[e] * rr * wt[(e < 8 ? d0 : d1) + (e & 7)];
           }
+          // what does not turn stays by itself: times 1 and 0 an infinity would reach the entry beside it
+          if (in_rot) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = x[e], b = x[8 + e];
-            o0[e] = (E)(a * c[e] - b * s[e]);
-            o1[e] = (E)(b * c[e] + a * s[e]);
+            for (int e = 0; e < 8; ++e) {
+              const float a = x[e], b = x[8 + e];
+              o0[e] = (E)(a * c[e] - b * s[e]);
+              o1[e] = (E)(b * c[e] + a * s[e]);
+            }
+          } else if (wt) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o0[e] = (E)x[e], o1[e] = (E)x[8 + e];
           }
         }
         E* dst;
