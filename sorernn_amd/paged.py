@@ -23,10 +23,20 @@ from sorernn_amd.window import _CODES, _whole
 __all__ = ["paged_kv_append", "paged_attention"]
 
 
+def _cache_strides(name: str, c: Tensor):
+    """Strides between pages, heads and tokens; of a dimension of one, which may have any, 0."""
+    st = c.stride()
+    if c.shape[0] == 1 or c.shape[1] == 1:
+        st = tuple(0 if n == 1 else s for n, s in zip(c.shape, st))
+    if st[3] != 1 or c.data_ptr() & 15 or (st[0] | st[1] | st[2]) & 7 or st[2] > 1 << 23:
+        raise ValueError(f"{name}: rows of the caches must be contiguous and 16-byte aligned, strides {c.stride()}")
+    return st[:3]
+
+
 def _cache_args(name: str, x: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor,
                 cu_seqlens: Tensor | None, cu_seqlens_cpu: Tensor | None):
-    """Checks of what both calls take, ``x [B,T,heads,D]`` among it. Returns the table with contiguous rows, the lengths, the
-    number of sequences and the flags."""
+    """Checks of what both calls take, ``x [B,T,heads,D]`` among it. Returns the caches' strides, the table with contiguous rows, the
+    lengths, the number of sequences and the flags."""
     b, t, _, d = x.shape
     if d not in (64, 128):
         raise NotImplementedError(f"{name}: head dim {d} unsupported (64 or 128)")
@@ -41,10 +51,7 @@ def _cache_args(name: str, x: Tensor, k_cache: Tensor, v_cache: Tensor, page_tab
         raise ValueError(f"{name}: no batch, no heads or no pages in {tuple(x.shape)}, {tuple(k_cache.shape)}")
     if size < 16 or size > 65536 or size & (size - 1):
         raise NotImplementedError(f"{name}: page size {size} unsupported (a power of two from 16 to 65536)")
-    for c in (k_cache, v_cache):
-        st = c.stride()
-        if st[3] != 1 or c.data_ptr() & 15 or (st[0] | st[1] | st[2]) & 7 or st[2] > 1 << 23:
-            raise ValueError(f"{name}: rows of the caches must be contiguous and 16-byte aligned, strides {st}")
+    kst, vst = _cache_strides(name, k_cache), _cache_strides(name, v_cache)
     n, flags = _cu_info(name, cu_seqlens, cu_seqlens_cpu, b, t)
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n or not page_table.shape[1]:
         raise ValueError(f"{name}: page_table must be int32 [{n}, width], got {page_table.dtype} {tuple(page_table.shape)}")
@@ -52,7 +59,7 @@ def _cache_args(name: str, x: Tensor, k_cache: Tensor, v_cache: Tensor, page_tab
         raise ValueError(f"{name}: lengths must be int32 or int64 [{n}], got {lengths.dtype} {tuple(lengths.shape)}")
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
-    return page_table, lengths.contiguous(), n, flags
+    return kst, vst, page_table, lengths.contiguous(), n, flags
 
 
 def paged_kv_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor,
@@ -82,7 +89,7 @@ def paged_kv_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page
                          f"{None if q is None else tuple(q.shape)}")
     if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         raise ValueError(f"{name}: q, k, v must share a dtype")
-    table, lens, n, flags = _cache_args(name, k, k_cache, v_cache, page_table, lengths, cu_seqlens, cu_seqlens_cpu)
+    kcs, vcs, table, lens, n, flags = _cache_args(name, k, k_cache, v_cache, page_table, lengths, cu_seqlens, cu_seqlens_cpu)
     b, t, hkv, d = k.shape
     pages, _, size, _ = k_cache.shape
     if k_cache.shape[1] != hkv:
@@ -111,7 +118,7 @@ def paged_kv_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, page
     ps = (None, 0, 0, 0) if positions is None else (positions.data_ptr(), *positions.stride(), positions.dtype == torch.int32)
     _launch("gdn_paged_append", k, *qa, ks.data_ptr(), *kst[:3], vs.data_ptr(), *vst[:3], None if qw is None else qw.data_ptr(),
             None if kw is None else kw.data_ptr(), None if out is None else out.data_ptr(), k_cache.data_ptr(),
-            *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], table.data_ptr(), table.stride(0), lens.data_ptr(),
+            *kcs, v_cache.data_ptr(), *vcs, table.data_ptr(), table.stride(0), lens.data_ptr(),
             lens.dtype == torch.int32, *ps, None if cu is None else cu.data_ptr(), b, t, hq, hkv, d, n, pages, size,
             table.shape[1], _CODES[k.dtype], rot_dim, float(theta), float(eps), flags)
     torch.autograd.graph.increment_version((k_cache, v_cache))  # a graph that saved them must not use what they hold now
@@ -147,7 +154,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
             raise ValueError(f"{name}: tree must be int64 {(b, t)}, got {tree.dtype} {tuple(tree.shape)}")
         if cu_seqlens is not None and cu_seqlens_cpu is None and not torch.compiler.is_compiling():
             cu_seqlens_cpu = cu_seqlens.detach().cpu()
-    table, lens, n, flags = _cache_args(name, q, k_cache, v_cache, page_table, lengths, cu_seqlens, cu_seqlens_cpu)
+    kcs, vcs, table, lens, n, flags = _cache_args(name, q, k_cache, v_cache, page_table, lengths, cu_seqlens, cu_seqlens_cpu)
     if tree is not None:
         longest = t if cu_seqlens is None else 0 if cu_seqlens_cpu is None else int(cu_seqlens_cpu.diff().max())
         if longest > 64:
@@ -164,8 +171,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
     nbytes = int(_lib.load().gdn_paged_attn_workspace_size(b, t, hq, hkv, d, n, size, width, window, sinks, int(cu is not None)))
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     words = (None, 0, 0) if tree is None else (tree.data_ptr(), *tree.stride())
-    _launch("gdn_paged_attn_fwd", q, qs.data_ptr(), *qst[:3], k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(),
-            *v_cache.stride()[:3], table.data_ptr(), table.stride(0), lens.data_ptr(), lens.dtype == torch.int32, *words,
+    _launch("gdn_paged_attn_fwd", q, qs.data_ptr(), *qst[:3], k_cache.data_ptr(), *kcs, v_cache.data_ptr(),
+            *vcs, table.data_ptr(), table.stride(0), lens.data_ptr(), lens.dtype == torch.int32, *words,
             o.data_ptr(), None if cu is None else cu.data_ptr(), b, t, hq, hkv, d, n, pages, size, width, _CODES[q.dtype],
             window, sinks, float(d**-0.5 if scale is None else scale), flags, None if ws is None else ws.data_ptr(), nbytes)
     return o
