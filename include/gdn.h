@@ -495,7 +495,7 @@ GDN_API int gdn_paged_append(const void* q, int64_t q_batch_stride, int64_t q_to
  * Attention of the call's new tokens over the cache that holds their keys and values too: q [B, T, HQ, D] by strides, o
  * contiguous. A token at place i sees place j <= i if i - j < window (0: none) or j < sinks. tree: [B, T] by strides, T_n at
  * most 64, or NULL: bit t of a token's word says that it sees the sequence's new token t; the tokens before the new ones are
- * then seen from place lengths[n] - T_n + (bits set) - 1. Rows that see nothing are zero. workspace:
+ * then seen from place lengths[n] - T_n + (bits set) - 1. Rows that see nothing are zero. T HQ / HKV < 2^29. workspace:
  * gdn_paged_attn_workspace_size bytes, 16-byte aligned (0: may be NULL), contents irrelevant; calls that share it must not
  * overlap.
  */

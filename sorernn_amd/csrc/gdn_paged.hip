@@ -609,6 +609,10 @@ extern "C" int gdn_paged_attn_fwd(const void* q, int64_t q_batch_stride, int64_t
                            (long long)HQ, (long long)HKV, (long long)window, (long long)sinks);
     return GDN_ERR_INVALID;
   }
+  if (T * (HQ / HKV) >= kFar) {  // row numbers inside a sequence are 32 bits, tiles from here on are none
+    gdn_internal_set_error("%s: too many rows (T=%lld times HQ / HKV=%lld)", name, (long long)T, (long long)(HQ / HKV));
+    return GDN_ERR_UNSUPPORTED;
+  }
   if (!(scale > 0.f) || scale > 2.0e38f) {
     gdn_internal_set_error("%s: scale %g unsupported (a positive finite softmax scale)", name, (double)scale);
     return GDN_ERR_INVALID;
