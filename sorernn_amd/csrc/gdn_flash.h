@@ -152,10 +152,11 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 
 // ------------------------------------------------------------------------------------------------ rows one by one
 // The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
-// reach rows that do not see it. Finite columns of a row are right all the same, and the others are summed again here, key by
-// key, over the keys that the row sees, until they are what they are: not finite, or done. (Masked scores take part in
-// nothing: the row's maximum and sum are right, and where the sum is NaN the row is.) A wave a row; lane l holds columns l and
-// l + 64.
+// reach rows that do not see it. And weights of up to 2^8, of any number of keys, times finite values may pass fp32's range before
+// they are divided by the row's sum. Finite columns of a row are right all the same, and the others are summed again here, key by
+// key, over the keys that the row sees, with weights that are divided first, until they are what they are: not finite, or done.
+// (Masked scores take part in nothing: the row's maximum and sum are right, and where the sum is NaN the row is.) A wave a row;
+// lane l holds columns l and l + 64.
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 template <int D, typename E>
 __device__ __forceinline__ float dot_row(const E* a, const E* b) {
@@ -192,10 +193,10 @@ __device__ __forceinline__ void add_rows(uint64_t live, float w, Row row, float 
   }
 }
 
-// Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c. key(j): K row j or null (not to
-// be seen); val(j): V row j. False once none of the columns can become finite.
+// Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c, with weights times `by`, one by
+// the row's sum. key(j): K row j or null (not to be seen); val(j): V row j. False once none of the columns can become finite.
 template <int D, typename E, typename Key, typename Val, typename Seen>
-__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, int again,
+__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, float by, int again,
                                          float (&acc)[D / 64]) {
   const int lane = threadIdx.x % kWave;
   for (int base = key0; base < key1; base += kWave) {
@@ -203,7 +204,7 @@ __device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key
     const E* kr = j < key1 && seen(j) ? key(j) : nullptr;
     const uint64_t live = __ballot(kr != nullptr);
     if (!live) continue;
-    const float p = kr ? __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q, kr), c, nmc)) : 0.f;
+    const float p = kr ? __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q, kr), c, nmc)) * by : 0.f;
     add_rows<D>(live, p, [&](int n) { return val(base + n); }, acc);
     if (!open_columns<D>(again, acc)) return false;
   }
@@ -259,7 +260,7 @@ struct FlashParams {
   const int64_t* tree;  // [B, T] bits of the sequence's drafted tokens that each sees, or null
   int64_t tb, tt;
   int splits;
-  float* part;          // [tiles HKV][splits][rows a tile][D], then [tiles HKV][splits][2][rows a tile]: O, maximum and sum
+  float* part;          // [tiles HKV][splits][rows a tile][D], then [tiles HKV][splits][2][rows a tile]: O (divided), maximum, sum
 };
 
 // Entry `at` of a row of a page table, `at` the same in every lane: through the scalar cache, apart from the vector loads that
@@ -604,8 +605,8 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;
   const int r = 32 * w + li;
   if (row_ok) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     if (whole) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
       E* const to = o_at(r);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -628,7 +629,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<f32x4*>(po + r * D + 32 * d + 8 * j + 4 * hh) =
-              f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+              f32x4{acc[d][4 * j] * inv, acc[d][4 * j + 1] * inv, acc[d][4 * j + 2] * inv, acc[d][4 * j + 3] * inv};
       if (hh == 0) {
         pml[r] = m;
         pml[kBQ + r] = l;
@@ -655,15 +656,14 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
       const int k0 = bl.at(b) * kBK;
       if (!slow_row<D, E>(q_at(rr), k0, imin(k0 + kBK, klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
                           [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
-                          c, nmc, again, a))
+                          c, nmc, lr == 0.f ? 0.f : 1.f / lr, again, a))
         break;
     }
     for (int i = 0; i < D / 64; ++i) {
       if (!(again >> i & 1)) continue;
-      const float x = lr == 0.f ? 0.f : a[i] / lr;
-      if (whole) o_at(rr)[lane + 64 * i] = (E)x;
+      if (whole) o_at(rr)[lane + 64 * i] = (E)a[i];
       else po[rr * D + lane + 64 * i] = a[i];
-      if (!PAGED && p.o_rest) static_cast<E*>(p.o_rest)[o_at(rr) - static_cast<E*>(p.o) + lane + 64 * i] = rest_of<E>(x);
+      if (!PAGED && p.o_rest) static_cast<E*>(p.o_rest)[o_at(rr) - static_cast<E*>(p.o) + lane + 64 * i] = rest_of<E>(a[i]);
     }
   }
 }

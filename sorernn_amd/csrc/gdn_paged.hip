@@ -353,14 +353,14 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       for (int e = 0; e < 4; ++e) bad |= finite_f(x[e]) ? 0u : 1u << e;
       if (bad) atomicOr(&redo_cols[r][piece / 8], bad << piece % 8 * 4);
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (f.used == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       typename Pack<E>::x4 y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
       *reinterpret_cast<typename Pack<E>::x4*>(out_row(f.row0 + r) + 4 * piece) = y;
     } else {
-      *reinterpret_cast<f32x4*>(po + r * D + 4 * piece) = x;
+      *reinterpret_cast<f32x4*>(po + r * D + 4 * piece) = x * inv;
       if (piece == 0) {
         pml[r] = tm;
         pml[kFewRows + r] = sum;
@@ -387,19 +387,30 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       const int k0 = f.bl.at(n) * kFewKeys;
       if (!slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
                           [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
-                          c, tm == -INFINITY ? 0.f : -tm * c, again, a))
+                          c, tm == -INFINITY ? 0.f : -tm * c, lr == 0.f ? 0.f : 1.f / lr, again, a))
         break;
     }
     for (int i = 0; i < D / 64; ++i) {
       if (!(again >> i & 1)) continue;
-      if (f.used == 1) out_row(f.row0 + r)[lane + 64 * i] = (E)(lr == 0.f ? 0.f : a[i] / lr);
+      if (f.used == 1) out_row(f.row0 + r)[lane + 64 * i] = (E)a[i];
       else po[r * D + lane + 64 * i] = a[i];
     }
   }
 }
 
-// The runs' sums of each row at one maximum: D / 4 threads a row, each in `groups` groups that take every groups-th run, so that
-// many runs' loads are under way at once. In a fixed order.
+// A run's result (maximum, sum, O divided by the sum) joins what others left: O as an average by the sums at the larger maximum, so
+// that no more than fp32 holds is ever added up.
+__device__ __forceinline__ void join_run(float& top, float& sum, f32x4& x, float m, float l, f32x4 y, float c) {
+  const float now = fmaxf(top, m), a = sum * (now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * c));
+  const float b = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * c));
+  sum = a + b;
+  const float by = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);  // 2^-23 a run; a division costs one token over 32,768 keys 0.5 us
+  x = x * (a * by) + y * (b * by);
+  top = now;
+}
+
+// The runs' results of each row joined: D / 4 threads a row, each in `groups` groups that take every groups-th run, so that many
+// runs' loads are under way at once. In a fixed order.
 template <int D, typename E, int ROWS, int BK>
 __global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(FlashParams p, int groups, int passes) {
   constexpr int CH = D / 4;
@@ -419,11 +430,7 @@ __global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(Flash
     for (int s = g; s < f.used; s += groups) {
       const float m = pml[s * 2 * ROWS + r], l = pml[(s * 2 + 1) * ROWS + r];
       const f32x4 y = *reinterpret_cast<const f32x4*>(po + (int64_t)(s * ROWS + r) * D + 4 * piece);
-      const float now = fmaxf(top, m), a = now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2);
-      const float b = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
-      sum = sum * a + l * b;
-      x = x * a + y * b;
-      top = now;
+      join_run(top, sum, x, m, l, y, p.scale_log2);
     }
   }
   ms[t] = top;
@@ -433,18 +440,13 @@ __global__ __launch_bounds__(256) void gated_delta_paged_attn_merge_kernel(Flash
   if (g || r >= f.rows) return;
   for (int i = 1; i < groups; ++i) {
     const int o = t + i * CH;
-    const float m = ms[o], now = fmaxf(top, m), a = now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * p.scale_log2);
-    const float b = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * p.scale_log2);
-    sum = sum * a + ls[o] * b;
-    x = x * a + *reinterpret_cast<const f32x4*>(xs + 4 * o) * b;
-    top = now;
+    join_run(top, sum, x, ms[o], ls[o], *reinterpret_cast<const f32x4*>(xs + 4 * o), p.scale_log2);
   }
   const int row = f.row0 + r;
-  if (sum == 0.f && sees_any<BK>(p, f, row_view(p, f, row))) sum = NAN;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const bool lost = sum == 0.f && sees_any<BK>(p, f, row_view(p, f, row));
   typename Pack<E>::x4 y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
+  for (int e = 0; e < 4; ++e) y[e] = (E)(lost ? NAN : x[e]);
   *reinterpret_cast<typename Pack<E>::x4*>(static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + row / rep) * p.HQ) +
                                                                    f.hkv * rep + row % rep) * D + 4 * piece) = y;
 }
