@@ -12,9 +12,11 @@
 
 namespace gdn {
 
+// lift: the weights' exponent at the running maximum. fp16's lie 2^7 higher, so that those as far as 2^8 above the maximum still fit:
+// below 2^-14 a weight keeps fewer bits, and a row that gives most of its sum to one key has many small ones.
 template <typename E> struct Pack;
-template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; };
-template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; };
+template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; static constexpr float lift = 0.f; };
+template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; static constexpr float lift = 7.f; };
 
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -99,11 +101,11 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70
 
 // ------------------------------------------------------------------------------------------------ softmax
 // Online softmax of KT x 32 keys of the wave's 32 queries (raw scores s, masked ones -inf) and O^T += V^T P^T.
-// p = 2^(s c - m c), c = scale log2(e) > 0. The row's m moves only when a block's maximum exceeds it by more than `slack` =
-// 8 / c: p <= 2^8 meanwhile, which costs no precision, and O^T is rescaled rarely. A row that saw no key yet keeps m = -inf and
-// uses 0. P is rounded to the inputs' type for the product (off by half a step of it a term, as the output itself is); the
-// row sum adds p in fp32, so that the backward's logarithm of it is exact to fp32. The sum of a row that saw a key whose score
-// is above -inf is 1 at least.
+// p = 2^(s c - m c + lift), c = scale log2(e) > 0. The row's m moves only when a block's maximum exceeds it by more than `slack` =
+// 8 / c: p <= 2^(8 + lift) meanwhile, which costs no precision, and O^T is rescaled rarely. A row that saw no key yet keeps
+// m = -inf and uses 0. P is rounded to the inputs' type for the product: off by half a step of it a term, as the output itself is,
+// or in fp16 by 2^-32 of the row's sum. The row sum adds p in fp32, so that the backward's logarithm of it is exact to fp32. The
+// sum of a row that saw a key whose score is above -inf is 2^lift at least.
 template <int KT, int D, typename E>
 __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 32], float& m, float& l, float c, float slack,
                                              const E* vb, const TileReads<D>& rd) {
@@ -121,7 +123,7 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) acc[d] *= alpha;
   }
-  const float nmc = m == -INFINITY ? 0.f : -m * c;
+  const float nmc = m == -INFINITY ? 0.f : Pack<E>::lift - m * c;
   float sum = 0.f;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) {
@@ -622,7 +624,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
             *reinterpret_cast<X4*>(static_cast<E*>(p.o_rest) + (to - static_cast<E*>(p.o)) + 32 * d + 8 * j + 4 * hh) = x;
           }
         }
-      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + __builtin_amdgcn_logf(l);
+      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + (__builtin_amdgcn_logf(l) - Pack<E>::lift);
     } else {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -649,7 +651,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
                                      : reinterpret_cast<const E*>(base + id * page_bytes + (j & ((1 << p.shift) - 1)) * row_bytes);
     };
-    const float mr = __shfl(m, n, kWave), lr = __shfl(l, n, kWave), nmc = mr == -INFINITY ? 0.f : -mr * c;
+    const float mr = __shfl(m, n, kWave), lr = __shfl(l, n, kWave), nmc = mr == -INFINITY ? 0.f : Pack<E>::lift - mr * c;
     const int again = not_finite<D>(acc, n);
     float a[D / 64] = {};
     for (int b = n0; b < n1; ++b) {

@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
       const int k0 = f.bl.at(n) * kFewKeys;
       if (!slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
                           [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
-                          c, tm == -INFINITY ? 0.f : -tm * c, lr == 0.f ? 0.f : 1.f / lr, again, a))
+                          c, tm == -INFINITY ? 0.f : Pack<E>::lift - tm * c, lr == 0.f ? 0.f : 1.f / lr, again, a))
         break;
     }
     for (int i = 0; i < D / 64; ++i) {
