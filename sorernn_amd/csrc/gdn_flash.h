@@ -12,8 +12,8 @@
 
 namespace gdn {
 
-// lift: the weights' exponent at the running maximum. fp16's lie 2^7 higher, so that those as far as 2^8 above the maximum still fit:
-// below 2^-14 a weight keeps fewer bits, and a row that gives most of its sum to one key has many small ones.
+// lift: the weights' exponent at the running maximum. fp16's lie 2^7 higher, so that those as far as 2^8 above the maximum still
+// fit: below 2^-14 a weight keeps fewer bits, and a row that gives most of its sum to one key has many small ones.
 template <typename E> struct Pack;
 template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; static constexpr float lift = 0.f; };
 template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; static constexpr float lift = 7.f; };
@@ -41,11 +41,6 @@ __device__ __forceinline__ int lanes_of(F yes) {
 namespace gdn {
 
 constexpr int64_t kMaxRowBytes = 1 << 24;  // bytes between two tokens of an operand read through 32-bit offsets inside a block
-
-__device__ __forceinline__ float wave_max(float x) {
-  for (int s = 1; s < kWave; s <<= 1) x = fmaxf(x, __shfl_xor(x, s, kWave));
-  return x;
-}
 
 // ------------------------------------------------------------------------------------------------ tiles in LDS
 // Rows of D elements lie unpadded (a load straight into LDS fills 1 KB contiguously); the 16-byte chunk c of row r is stored
@@ -143,13 +138,13 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) acc[d] = mma32(tr_frag(vb + (2 * kt + h) * 16 * D, rd, d), pb[h], acc[d]);
   }
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+  __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // the fragments' reads two products ahead
 #pragma unroll
-    for (int i = 0; i < 2 * KT * (D / 32) - 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+  for (int i = 0; i < 2 * KT * (D / 32) - 2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 }
 
 // ------------------------------------------------------------------------------------------------ rows one by one
@@ -198,8 +193,8 @@ __device__ __forceinline__ void add_rows(uint64_t live, float w, Row row, float 
 // Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c, with weights times `by`, one by
 // the row's sum. key(j): K row j or null (not to be seen); val(j): V row j. False once none of the columns can become finite.
 template <int D, typename E, typename Key, typename Val, typename Seen>
-__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, float by, int again,
-                                         float (&acc)[D / 64]) {
+__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, float by,
+                                         int again, float (&acc)[D / 64]) {
   const int lane = threadIdx.x % kWave;
   for (int base = key0; base < key1; base += kWave) {
     const int j = base + lane;
@@ -624,7 +619,8 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
             *reinterpret_cast<X4*>(static_cast<E*>(p.o_rest) + (to - static_cast<E*>(p.o)) + 32 * d + 8 * j + 4 * hh) = x;
           }
         }
-      if (!PAGED && p.lse && hh == 0) p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + (__builtin_amdgcn_logf(l) - Pack<E>::lift);
+      if (!PAGED && p.lse && hh == 0)
+        p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + (__builtin_amdgcn_logf(l) - Pack<E>::lift);
     } else {
 #pragma unroll
       for (int d = 0; d < DT; ++d)

@@ -398,13 +398,13 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
   }
 }
 
-// A run's result (maximum, sum, O divided by the sum) joins what others left: O as an average by the sums at the larger maximum, so
-// that no more than fp32 holds is ever added up.
+// A run's result (maximum, sum, O divided by the sum) joins what others left: O as an average by the sums at the larger maximum,
+// so that no more than fp32 holds is ever added up.
 __device__ __forceinline__ void join_run(float& top, float& sum, f32x4& x, float m, float l, f32x4 y, float c) {
   const float now = fmaxf(top, m), a = sum * (now == top ? 1.f : __builtin_amdgcn_exp2f((top - now) * c));
   const float b = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * c));
   sum = a + b;
-  const float by = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);  // 2^-23 a run; a division costs one token over 32,768 keys 0.5 us
+  const float by = sum == 0.f ? 0.f : __builtin_amdgcn_rcpf(sum);  // off by 2^-23; divisions cost one token over 32,768 keys 0.3 us
   x = x * (a * by) + y * (b * by);
   top = now;
 }

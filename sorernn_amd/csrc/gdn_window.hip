@@ -384,7 +384,8 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   // The same with queries whose logarithm (`lbad`: all their weights are NaN) or delta (`dbad`: none of their ds is finite) is not
   // finite: their entries that are not are left out of the products, and the keys that see them become NaN.
   auto block_bad = [&](const bf16* qb, const bf16* db, const float* lb, int q0) {
-    const uint64_t there = bits_below(to - q0), lbad = __ballot(!finite_f(lb[lane])) & there, dbad = __ballot(!finite_f(lb[kBK + lane])) & there;
+    const uint64_t there = bits_below(to - q0), lbad = __ballot(!finite_f(lb[lane])) & there;
+    const uint64_t dbad = __ballot(!finite_f(lb[kBK + lane])) & there;
     const int kk = wk0 + li, hi = kk < p.sinks ? to : imin(to, kk + p.window);
     const uint64_t seen = bits_below(hi - q0) & ~bits_below(imax(kk, from) - q0);
     const uint64_t seen_v = (seen & ~lbad) >> 4 * hh, seen_k = (seen & ~(lbad | dbad)) >> 4 * hh;
@@ -629,7 +630,6 @@ static int window_check(const char* name, int64_t B, int64_t T, int64_t HQ, int6
 static int far_window(int64_t window) { return window <= 0 || window > kFar ? kFar : (int)window; }
 // without a window sinks say nothing; sinks as far as the first window reaches neither change who sees what, nor are they cut
 static int far_sinks(int64_t window, int64_t sinks) { return window <= 0 ? 0 : sinks > kFar ? kFar : (int)sinks; }
-
 
 // Far queries a job, with one tile of sinks: short jobs, which fill up the CUs behind the near ones.
 constexpr int kFarPiece = 256;

@@ -35,8 +35,8 @@ def _cache_strides(name: str, c: Tensor):
 
 def _cache_args(name: str, x: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor,
                 cu_seqlens: Tensor | None, cu_seqlens_cpu: Tensor | None):
-    """Checks of what both calls take, ``x [B,T,heads,D]`` among it. Returns the caches' strides, the table with contiguous rows, the
-    lengths, the number of sequences and the flags."""
+    """Checks of what both calls take, ``x [B,T,heads,D]`` among it. Returns the caches' strides, the table with contiguous rows,
+    the lengths, the number of sequences and the flags."""
     b, t, _, d = x.shape
     if d not in (64, 128):
         raise NotImplementedError(f"{name}: head dim {d} unsupported (64 or 128)")

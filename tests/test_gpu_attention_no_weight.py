@@ -21,8 +21,8 @@ def _against(q):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("t, d, win, sinks, lens, at", [
-    (1, 64, None, 0, None, [0]), (200, 128, None, 0, None, [0]), (200, 64, 1, 0, None, [0, 77, 199]), (300, 128, 2, 0, None, [70, 71]),
-    (300, 64, 40, 3, [100, 1, 199], [0, 100, 101]), (150, 128, 1, 1, None, [0, 90]),
+    (1, 64, None, 0, None, [0]), (200, 128, None, 0, None, [0]), (200, 64, 1, 0, None, [0, 77, 199]),
+    (300, 128, 2, 0, None, [70, 71]), (300, 64, 40, 3, [100, 1, 199], [0, 100, 101]), (150, 128, 1, 1, None, [0, 90]),
 ])
 def test_window_forward(t, d, win, sinks, lens, at, dtype):
     q, k, v, _ = _inputs(1, t, 2, 1, d, dtype, seed=1)
