@@ -315,7 +315,7 @@ __device__ __forceinline__ bool paged_plan(const FlashParams& p, int64_t t, int 
 // bits 0 .. n - 1
 __device__ __forceinline__ uint64_t bits_below(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1; }
 
-// what the rounding of x to E left
+// What the rounding of x to E left, in 16 bits: with o it is x to 16 bits and more, a 2^-8th of the step that delta is to be free of.
 template <typename E>
 __device__ __forceinline__ E rest_of(float x) {
   const float r = x - (float)(E)x;

@@ -20,7 +20,8 @@ namespace gdn {
 // bytes, or by the launch where tokens are few. A wave takes a token (with few tokens four share one) and its heads D / 16 lanes
 // each; a lane holds two pieces of 8 elements that turn with one another. Angles are taken in turns in 64 bits,
 // position * (theta^(-2f / rot) / 2 pi) less its whole part: at position 1,000,000 a 32-bit angle is off by 0.06 rad.
-// Measured, 16 query and 4 kv heads of 128: 16,384 tokens 44 us, 4.6 TB/s (a large copy: 5.1); one token 4.1 us, 64 tokens 5.1.
+// Measured, 16 query and 4 kv heads of 128: 16,384 tokens 47 us a call, 4.3 TB/s (a large copy: 5.1); one token 4.4 us, 64 tokens
+// 5.4 in the kernel.
 struct AppendParams {
   const void* x[3];                // q (or null), k, v [B, T, heads, D] by strides (elements)
   int64_t sb[3], st[3], sh[3];
@@ -502,9 +503,13 @@ static bool rows_ok(const int64_t* st, int n, uintptr_t all) {
 //       61,  1,000     14.7, 18.9      16.1, 20.2      18.9, 22.0
 //       61,  4,000     20.5, 23.9      25.7, 27.0      36.5, 31.2
 //       64, 16,000     37.6, 34.9      58.9, 42.1       102, 60.9
+//     Two sequences of 61 tokens over 4,000 keys (8,100 blocks) are 5% slower in tiles of 128, which they take; four (16,200) faster.
+//     With bounds the mean number of new tokens counts: 512 of one sequence beside single ones of 63 others over 4,000 keys take
+//     157 us in tiles of 32; each part alone 50 and 103.
 //   runs: as many as make about kFewGroups or kManyGroups workgroups (256 and 512: one token over 32,768 keys 20.8 and 26.2,
 //   1,024 workgroups 36.9; 8 trees of 61 tokens 48.3 and 41.0, 59.5), of 4 blocks at least (one token over 1,024 keys with 4, 8
-//   and 16: 10.6, 11.6, 14.1). Up to 256 keys one run without a merge (8.1, with two runs 9.8).
+//   and 16: 10.6, 11.6, 14.1). Up to 256 keys one run without a merge (8.1, with two runs 9.8). The lengths are on the device and
+//   have no part in this: one sequence of 32,768 in a batch of 64 with 256 tokens else is read by 4 workgroups, 415 us (by itself 26).
 struct PagedCut {
   int rows, keys, splits;
   int64_t tiles;

@@ -7,8 +7,10 @@
 
 The cache is a pair of tensors ``[pages, HKV, page_size, D]`` that the caller owns; any strides with a contiguous last axis do
 (``[pages, page_size, HKV, D]`` transposed is one). ``page_table [N, width]`` (int32) names each sequence's pages in order,
-``lengths [N]`` its tokens in the cache with the new ones counted, in both calls. Nothing is read on the host: both calls can be
-captured and replayed with new tables and lengths. The reference has no cache and no decoding (``sore/model/lm.py:206-208``).
+``lengths [N]`` its tokens in the cache with the new ones counted, in both calls. Tables and lengths are not read on the host, and
+``cu_seqlens`` only where ``cu_seqlens_cpu`` is missing: with it both calls can be captured, and replayed with new tables, lengths
+and bounds. Replayed and compiled calls take ``cu_seqlens`` unchecked, in ascending order; a sequence may then be without new
+tokens. The reference has no cache and no decoding (``sore/model/lm.py:206-208``).
 """
 from __future__ import annotations
 
@@ -141,7 +143,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_table: Ten
 
     Rows that see nothing are zero: tokens at a place below 0, of no sequence, without a length. A length above what its row of
     the table can hold counts as that. Keys on pages that the cache does not have are not seen. An infinity or NaN in the cache
-    reaches the tokens that see it, not the others.
+    reaches the tokens that see it, not the others; where all scores that a token sees are -inf, its row is NaN.
     """
     name = "paged_attention"
     _check_cuda(name, q, k_cache, v_cache, page_table, lengths, tree, cu_seqlens)

@@ -126,7 +126,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int | None = None,
     row, or in every document of ``cu_seqlens`` (``[N+1]``, needs ``B == 1``); ``cu_seqlens_cpu`` lets the bounds be checked
     without a device sync. ``scale`` (positive) defaults to ``D**-0.5``; scaled scores have to fit fp32. Returns
     ``o [B,T,HQ,D]``; differentiable in q, k and v in bf16. An infinity or NaN in a token reaches the tokens that see it, not
-    the others.
+    the others; where all scores that a token sees are -inf, its row is NaN.
 
     Replayed and compiled calls take ``cu_seqlens`` unchecked, in ascending order: a document may be empty, and tokens before
     the first or behind the last have zeros in ``o`` and in the gradients.
