@@ -280,11 +280,12 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
   const bf16* const krow = p.k + sq.row * p.ksb + (sq.start + kc) * p.kst + job.hkv * p.ksh;
   const bf16* const vrow = p.v + sq.row * p.vsb + (sq.start + kc) * p.vst + job.hkv * p.vsh;
   if constexpr (BAD) {
-    // masked blocks are those of a near tile's first and last queries, and of far pieces all
+    // masked blocks are those with a near tile's first and last queries, and of far pieces all; as whole blocks, which reach past them
+    const int lo = from / kBK * kBK, hi = imin((to + kBK - 1) / kBK * kBK, sq.len), most = from < to ? hi - lo : 0;
+    const int some = imin(most, far_job ? most : 256), each = far_job ? some : 2 * some;
     bool bad = false;
-    const int some = imin(to - from, far_job ? to - from : 192), each = far_job ? some : 2 * some;
     for (int x = t; x < rep * each; x += 512) {
-      const int h = x / each, r = x - h * each, i = r < some ? from + r : to - 2 * some + r;
+      const int h = x / each, r = x - h * each, i = r < some ? lo + r : hi - 2 * some + r;
       bad |= !finite_f(p.delta[(job.hkv * rep + h) * all + tok + i]);
     }
     const bool any = __any(bad);

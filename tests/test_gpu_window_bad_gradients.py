@@ -118,3 +118,14 @@ def test_columns(t, heads, d, win, sinks, spoiled):
         g, fine = got[name][0, :, 0], wanted[name].isfinite()
         assert torch.equal(g.isfinite(), fine), (name, (g.isfinite() != fine).nonzero()[:4].tolist())
         check(torch.where(fine, g, 0), {m: torch.where(fine, keys[m], 0) for m in (name, name + "_tol")}, name)
+
+
+@pytest.mark.parametrize("t, heads, d, win, sinks, spoiled", [
+    (300, 1, 64, 2, 5, [("do", 186, 0, 7, torch.inf)]),       # behind the last query that sees the tile, in its block
+    (300, 2, 64, 2, 0, [("do", 130, 1, 7, torch.nan), ("q", 131, 0, 3, torch.inf)]),
+    (500, 16, 64, 100, 0, [("do", 255, 3, 1, torch.inf)]),
+    (700, 2, 128, 60, 130, [("do", 190, 0, 1, torch.nan), ("do", 320, 1, 2, torch.inf), ("do", 577, 1, 2, -torch.inf)]),
+    (1000, 2, 64, 70, 4, [("do", 197, 0, 1, torch.nan), ("do", 256, 1, 2, torch.inf), ("q", 511, 1, 2, -torch.inf)]),
+])
+def test_blocks_that_reach_past_a_tile_s_queries(t, heads, d, win, sinks, spoiled):
+    test_columns(t, heads, d, win, sinks, spoiled)
