@@ -15,8 +15,8 @@ namespace gdn {
 // lift: the weights' exponent at the running maximum. fp16's lie 2^7 higher, so that those as far as 2^8 above the maximum still
 // fit: below 2^-14 a weight keeps fewer bits, and a row that gives most of its sum to one key has many small ones.
 template <typename E> struct Pack;
-template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; static constexpr float lift = 0.f; };
-template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; static constexpr float lift = 7.f; };
+template <> struct Pack<bf16> { using x8 = bf16x8; using x4 = bf16x4; static constexpr float lift = 0.f; static constexpr uint16_t infinity = 0x7f80; };
+template <> struct Pack<f16> { using x8 = f16x8; using x4 = f16x4; static constexpr float lift = 7.f; static constexpr uint16_t infinity = 0x7c00; };
 
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -147,13 +147,13 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
   __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 }
 
-// ------------------------------------------------------------------------------------------------ rows one by one
+// ------------------------------------------------------------------------------------------------ sums that are not finite
 // The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
 // reach rows that do not see it. And weights of up to 2^8, of any number of keys, times finite values may pass fp32's range before
-// they are divided by the row's sum. Finite columns of a row are right all the same, and the others are summed again here, key by
-// key, over the keys that the row sees, with weights that are divided first, until they are what they are: not finite, or done.
-// (Masked scores take part in nothing: the row's maximum and sum are right, and where the sum is NaN the row is.) A wave a row;
-// lane l holds columns l and l + 64.
+// they are divided by the row's sum. (Masked scores take part in nothing: the row's maximum and sum are right, and where the sum
+// is NaN the row is.) The forwards take rows whose sums are not finite again, with again_block. The backward's dq sums their
+// columns that are not finite again key by key, over the keys that the row sees, until they are what they are: not finite, or
+// done. A wave a row; lane l holds columns l and l + 64.
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 template <int D, typename E>
 __device__ __forceinline__ float dot_row(const E* a, const E* b) {
@@ -190,24 +190,6 @@ __device__ __forceinline__ void add_rows(uint64_t live, float w, Row row, float 
   }
 }
 
-// Adds keys [key0, key1) to columns `again` (bit i: l + 64 i) of a row, at reference nmc = -m c, with weights times `by`, one by
-// the row's sum. key(j): K row j or null (not to be seen); val(j): V row j. False once none of the columns can become finite.
-template <int D, typename E, typename Key, typename Val, typename Seen>
-__device__ __forceinline__ bool slow_row(const E* q, int key0, int key1, Key key, Val val, Seen seen, float c, float nmc, float by,
-                                         int again, float (&acc)[D / 64]) {
-  const int lane = threadIdx.x % kWave;
-  for (int base = key0; base < key1; base += kWave) {
-    const int j = base + lane;
-    const E* kr = j < key1 && seen(j) ? key(j) : nullptr;
-    const uint64_t live = __ballot(kr != nullptr);
-    if (!live) continue;
-    const float p = kr ? __builtin_amdgcn_exp2f(fmaf(dot_row<D>(q, kr), c, nmc)) * by : 0.f;
-    add_rows<D>(live, p, [&](int n) { return val(base + n); }, acc);
-    if (!open_columns<D>(again, acc)) return false;
-  }
-  return true;
-}
-
 // whether a lane's accumulators are all finite: 0 x stays 0 unless x is not
 template <int N>
 __device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
@@ -235,6 +217,69 @@ __device__ __forceinline__ int not_finite(const f32x16 (&a)[D / 32], int n) {
     bits |= (int)(((uint64_t)hi << 32 | lo) >> (16 * (col >> 5) + e) & 1) << i;
   }
   return bits;
+}
+
+// The product with the values again for the wave's rows whose sums are not finite, a block of KT x 32 keys at a time: weights are
+// divided by the row's sum first (`by`; the maximum is the final one), and infinities and NaN among the values are left out of the
+// product and reach the rows that see them. `seen`: the block's keys that the lane's row sees. key(j), val(j): rows of key j of the
+// block, null: none. `tile`: LDS of the wave's own for the values. acc: O^T times 2^raise<E>.
+template <typename E>
+constexpr float raise = Pack<E>::lift > 0.f ? 14.f : 0.f;  // weights of 1 at most: fp16's are raised as far as they fit
+template <int KT, int D, typename E, typename Key, typename Val>
+__device__ __forceinline__ void again_block(f32x16 (&acc)[D / 32], const typename Pack<E>::x8 (&qf)[D / 16], uint64_t seen, Key key, Val val,
+                                            E* tile, float c, float nmc, float by, const TileReads<D>& rd) {
+  using X8 = typename Pack<E>::x8;
+  constexpr int CPR = D / 8, RPL = 512 / D;
+  const int lane = threadIdx.x % kWave, hh = lane >> 5, li = lane & 31;
+  auto fine = [](E x) { return (__builtin_bit_cast(uint16_t, x) & Pack<E>::infinity) != Pack<E>::infinity; };
+#pragma unroll 4
+  for (int u = 0; u < KT * 32 / RPL; ++u) {
+    const int r = u * RPL + lane / CPR, ch = lane % CPR;
+    const E* const v = val(r);
+    *reinterpret_cast<X8*>(tile + r * D + ((ch ^ swz<D>(r)) << 3)) = v ? *reinterpret_cast<const X8*>(v + 8 * ch) : X8{};
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) {
+    f32x16 s{}, one;
+    const E* const k = key(32 * kt + li);
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) s = mma32(k ? *reinterpret_cast<const X8*>(k + 16 * st + 8 * hh) : X8{}, qf[st], s);
+    const uint32_t bits = (uint32_t)(seen >> 32 * kt) >> 4 * hh;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const bool see = bits >> (8 * (e >> 2) + (e & 3)) & 1;
+      s[e] = see ? __builtin_amdgcn_exp2f(fmaf(s[e], c, nmc)) * by : 0.f;
+      one[e] = see ? 1.f : 0.f;
+    }
+    X8 pb[2], ones[2];
+    pack16<E>(s, pb);
+    pack16<E>(one, ones);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {
+        X8 x = tr_frag(tile + (2 * kt + h) * 16 * D, rd, d), up, down;
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool ok = fine(x[e]), more = !(x[e] < (E)0.f), less = !(x[e] > (E)0.f);  // NaN: both
+          any |= !ok;
+          up[e] = (E)(!ok && more ? 1.f : 0.f);
+          down[e] = (E)(!ok && less ? 1.f : 0.f);
+          x[e] = ok ? x[e] : (E)0.f;
+        }
+        acc[d] = mma32(x, pb[h], acc[d]);
+        if (__any(any)) {
+          const f32x16 n = mma32(up, ones[h], f32x16{}), m = mma32(down, ones[h], f32x16{});
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[d][e] += (n[e] > 0.f ? INFINITY : 0.f) - (m[e] > 0.f ? INFINITY : 0.f);
+        }
+      }
+  }
+  __builtin_amdgcn_wave_barrier();  // the tile is read before the next block's is written
 }
 
 // ------------------------------------------------------------------------------------------------ parameters and plans
@@ -601,8 +646,7 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
   fine = l != l || (__shfl_xor((int)fine, 32, kWave) && fine);
   const int64_t all = p.B * p.seqs.T, tok = sq.row * p.seqs.T + sq.start;
   const int r = 32 * w + li;
-  if (row_ok) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+  auto write = [&](float inv) {
     if (whole) {
       E* const to = o_at(r);
 #pragma unroll
@@ -619,8 +663,6 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
             *reinterpret_cast<X4*>(static_cast<E*>(p.o_rest) + (to - static_cast<E*>(p.o)) + 32 * d + 8 * j + 4 * hh) = x;
           }
         }
-      if (!PAGED && p.lse && hh == 0)
-        p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + (__builtin_amdgcn_logf(l) - Pack<E>::lift);
     } else {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -628,42 +670,45 @@ __device__ __forceinline__ void flash_forward(const FlashParams& p, E* Ks0, E* K
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<f32x4*>(po + r * D + 32 * d + 8 * j + 4 * hh) =
               f32x4{acc[d][4 * j] * inv, acc[d][4 * j + 1] * inv, acc[d][4 * j + 2] * inv, acc[d][4 * j + 3] * inv};
-      if (hh == 0) {
-        pml[r] = m;
-        pml[kBQ + r] = l;
-      }
+    }
+  };
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (row_ok) {
+    write(inv);
+    if (whole) {
+      if (!PAGED && p.lse && hh == 0)
+        p.lse[head_of(r) * all + tok + token_of(r)] = l == 0.f ? INFINITY : m * c + (__builtin_amdgcn_logf(l) - Pack<E>::lift);
+    } else if (hh == 0) {
+      pml[r] = m;
+      pml[kBQ + r] = l;
     }
   }
-  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
-  if (redo) wait_loads();  // what was written above is there before parts of it are written again
-  while (redo) {
-    const int n = __ffsll((unsigned long long)redo) - 1, rr = 32 * w + n;
-    redo &= redo - 1;
-    RowView v{row0 + rr, kFar, 0};
-    if constexpr (PAGED) v = row_view(p, f, row0 + rr);
+  if (!__any(row_ok && !fine)) return;
+  wait_loads();  // what was written above is there before rows are written again
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  E* const tile = w == 0 ? Ks0 : w == 1 ? Ks1 : w == 2 ? Vs0 : Vs1;  // all waves are behind their last block
+  const float nmc = m == -INFINITY ? 0.f : Pack<E>::lift - m * c, by = exp2f(raise<E>) * inv;
+  for (int n = n0; n < n1; ++n) {
+    const int k0 = bl.at(n) * kBK;
+    if (none_sees(wq0, wq1, k0, k0 + kBK - 1, p.window, p.sinks)) continue;
     auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
-      if (!PAGED) return reinterpret_cast<const E*>(base + j * row_bytes);
-      const int id = table[j >> p.shift];
+      if (k0 + j >= klen) return static_cast<const E*>(nullptr);
+      if (!PAGED) return reinterpret_cast<const E*>(base + (k0 + j) * row_bytes);
+      const int id = table[(k0 + j) >> p.shift];
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
-                                     : reinterpret_cast<const E*>(base + id * page_bytes + (j & ((1 << p.shift) - 1)) * row_bytes);
+                                     : reinterpret_cast<const E*>(base + id * page_bytes + ((k0 + j) & ((1 << p.shift) - 1)) * row_bytes);
     };
-    const float mr = __shfl(m, n, kWave), lr = __shfl(l, n, kWave), nmc = mr == -INFINITY ? 0.f : Pack<E>::lift - mr * c;
-    const int again = not_finite<D>(acc, n);
-    float a[D / 64] = {};
-    for (int b = n0; b < n1; ++b) {
-      const int k0 = bl.at(b) * kBK;
-      if (!slow_row<D, E>(q_at(rr), k0, imin(k0 + kBK, klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
-                          [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
-                          c, nmc, lr == 0.f ? 0.f : 1.f / lr, again, a))
-        break;
+    auto key = [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); };
+    uint64_t seen = view.block(k0, p.window, p.sinks) & bits_below(klen - k0);
+    if (PAGED) {
+      look_up(bl.at(n));
+#pragma unroll
+      for (int g = 0; g < 4; ++g) seen &= pid[g] >= 0 ? ~0ull : ~(0xffffull << 16 * g);
     }
-    for (int i = 0; i < D / 64; ++i) {
-      if (!(again >> i & 1)) continue;
-      if (whole) o_at(rr)[lane + 64 * i] = (E)a[i];
-      else po[rr * D + lane + 64 * i] = a[i];
-      if (!PAGED && p.o_rest) static_cast<E*>(p.o_rest)[o_at(rr) - static_cast<E*>(p.o) + lane + 64 * i] = rest_of<E>(a[i]);
-    }
+    again_block<2, D, E>(acc, qf, seen, key, [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, tile, c, nmc, by, rd);
   }
+  if (row_ok && !fine) write(exp2f(-raise<E>));
 }
 
 }  // namespace gdn

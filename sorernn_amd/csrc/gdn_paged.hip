@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
   __shared__ __align__(16) E V0[4 * TILE];
   __shared__ __align__(16) E V1[4 * TILE];
   __shared__ float ml[4][2][kFewRows];
-  __shared__ uint32_t redo_cols[kFewRows][D / 32];  // columns of rows that are summed again
+  __shared__ uint32_t redo_rows;  // rows whose sums are not finite
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), hh = lane >> 5, li = lane & 31;
   const int rep = p.HQ / p.HKV;
   PagedPlan f;
@@ -315,19 +315,30 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
     ml[w][0][li] = m;
     ml[w][1][li] = l;
   }
-  if (t < kFewRows * (D / 32)) redo_cols[t / (D / 32)][t % (D / 32)] = 0;
+  if (t == 0) redo_rows = 0;
   __syncthreads();  // every wave is done with its tiles, which take the sums
   const float top = fmaxf(fmaxf(ml[0][0][li], ml[1][0][li]), fmaxf(ml[2][0][li], ml[3][0][li]));
   const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
   float* const red = reinterpret_cast<float*>(w < 2 ? K0 : K1) + (w & 1) * kFewRows * D;
+  auto put = [&](float by) {
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int piece = (8 * d + 2 * j + hh) ^ (li & (CH - 1));
-      *reinterpret_cast<f32x4*>(red + li * D + 4 * piece) =
-          f32x4{acc[d][4 * j] * mine, acc[d][4 * j + 1] * mine, acc[d][4 * j + 2] * mine, acc[d][4 * j + 3] * mine};
-    }
+      for (int j = 0; j < 4; ++j) {
+        const int piece = (8 * d + 2 * j + hh) ^ (li & (CH - 1));
+        *reinterpret_cast<f32x4*>(red + li * D + 4 * piece) =
+            f32x4{acc[d][4 * j] * by, acc[d][4 * j + 1] * by, acc[d][4 * j + 2] * by, acc[d][4 * j + 3] * by};
+      }
+  };
+  auto take = [&](int r, int piece) {
+    f32x4 x{};
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
+                                           4 * (piece ^ (r & (CH - 1))));
+    return x;
+  };
+  put(mine);
   __syncthreads();
   const int64_t place = f.job * p.splits + split;
   float* const po = p.part + place * kFewRows * D;
@@ -335,68 +346,63 @@ __global__ __launch_bounds__(256, 1) void gated_delta_paged_attn_few_kernel(Flas
   auto out_row = [&](int r) {
     return static_cast<E*>(p.o) + (((f.sq.row * p.seqs.T + f.sq.start + r / rep) * p.HQ) + f.hkv * rep + r % rep) * D;
   };
-  for (int i = t; i < f.rows * CH; i += 256) {
-    const int r = i / CH, piece = i % CH;
+  auto sum_of = [&](int r) {  // of the row's weights, at the four waves' maximum
     const float tm = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
     float sum = 0.f;
-    f32x4 x{};
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
       const float mv = ml[v][0][r];
       sum += mv == -INFINITY ? ml[v][1][r] : ml[v][1][r] * __builtin_amdgcn_exp2f((mv - tm) * c);  // of the former 0, or NaN
-      x += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(v < 2 ? K0 : K1) + (v & 1) * kFewRows * D + r * D +
-                                           4 * (piece ^ (r & (CH - 1))));
     }
-    if (f.used == 1 && sum == 0.f && sees_any<kFewKeys>(p, f, row_view(p, f, f.row0 + r))) sum = NAN;
-    if (sum == sum) {
-      uint32_t bad = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bad |= finite_f(x[e]) ? 0u : 1u << e;
-      if (bad) atomicOr(&redo_cols[r][piece / 8], bad << piece % 8 * 4);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    return sum;
+  };
+  auto write = [&](int r, int piece, f32x4 x) {
     if (f.used == 1) {
       typename Pack<E>::x4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (E)(x[e] * inv);
+      for (int e = 0; e < 4; ++e) y[e] = (E)x[e];
       *reinterpret_cast<typename Pack<E>::x4*>(out_row(f.row0 + r) + 4 * piece) = y;
     } else {
-      *reinterpret_cast<f32x4*>(po + r * D + 4 * piece) = x * inv;
-      if (piece == 0) {
-        pml[r] = tm;
-        pml[kFewRows + r] = sum;
-      }
+      *reinterpret_cast<f32x4*>(po + r * D + 4 * piece) = x;
+    }
+  };
+  for (int i = t; i < f.rows * CH; i += 256) {
+    const int r = i / CH, piece = i % CH;
+    float sum = sum_of(r);
+    const f32x4 x = take(r, piece);
+    if (f.used == 1 && sum == 0.f && sees_any<kFewKeys>(p, f, row_view(p, f, f.row0 + r))) sum = NAN;
+    if (sum == sum && !(finite_f(x[0]) && finite_f(x[1]) && finite_f(x[2]) && finite_f(x[3]))) atomicOr(&redo_rows, 1u << r);
+    write(r, piece, x * (sum == 0.f ? 0.f : 1.f / sum));
+    if (f.used > 1 && piece == 0) {
+      pml[r] = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
+      pml[kFewRows + r] = sum;
     }
   }
-  wait_loads();  // what was written above is there before parts of it are written again
+  wait_loads();  // what was written above is there before rows are written again
   __syncthreads();
-  for (int r = w; r < f.rows; r += 4) {
-    int again = 0;
-    for (int i = 0; i < D / 64; ++i) again |= (int)(redo_cols[r][(lane + 64 * i) / 32] >> (lane % 32) & 1) << i;
-    if (!__any(again)) continue;
-    const RowView v = row_view(p, f, f.row0 + r);
+  const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_rows);
+  if (!redo) return;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  const float all = sum_of(li), by = all == 0.f ? 0.f : exp2f(raise<E>) / all;
+  for (int n = n0 + w; n < n1; n += 4) {
+    const int k0 = f.bl.at(n) * kFewKeys;
     auto row_of = [&](const char* base, int64_t page_bytes, int64_t row_bytes, int j) {
-      const int id = table[j >> p.shift];
+      if (k0 + j >= f.klen) return static_cast<const E*>(nullptr);
+      const int id = table[(k0 + j) >> p.shift];
       return id < 0 || id >= p.pages ? static_cast<const E*>(nullptr)
-                                     : reinterpret_cast<const E*>(base + id * page_bytes + (j & in_page) * row_bytes);
+                                     : reinterpret_cast<const E*>(base + id * page_bytes + ((k0 + j) & in_page) * row_bytes);
     };
-    const float tm = fmaxf(fmaxf(ml[0][0][r], ml[1][0][r]), fmaxf(ml[2][0][r], ml[3][0][r]));
-    float lr = 0.f, a[D / 64] = {};
-    for (int u = 0; u < 4; ++u)
-      if (ml[u][0][r] != -INFINITY) lr += ml[u][1][r] * __builtin_amdgcn_exp2f((ml[u][0][r] - tm) * c);
-    for (int n = n0; n < n1; ++n) {
-      const int k0 = f.bl.at(n) * kFewKeys;
-      if (!slow_row<D, E>(q_at(f.row0 + r), k0, imin(k0 + kFewKeys, f.klen), [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); },
-                          [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); }, [&](int j) { return v(j, p.window, p.sinks); },
-                          c, tm == -INFINITY ? 0.f : Pack<E>::lift - tm * c, lr == 0.f ? 0.f : 1.f / lr, again, a))
-        break;
-    }
-    for (int i = 0; i < D / 64; ++i) {
-      if (!(again >> i & 1)) continue;
-      if (f.used == 1) out_row(f.row0 + r)[lane + 64 * i] = (E)a[i];
-      else po[r * D + lane + 64 * i] = a[i];
-    }
+    look_up(n);
+    const uint64_t there = (pid[0] >= 0 ? 0xffffu : 0u) | (pid[1] >= 0 ? 0xffff0000u : 0u);
+    again_block<1, D, E>(acc, qf, view.block(k0, p.window, p.sinks) & bits_below(f.klen - k0) & there,
+                         [&](int j) { return row_of(kbase, p.ksb * 2, kst, j); }, [&](int j) { return row_of(vbase, p.vsb * 2, vst, j); },
+                         V0 + w * TILE, c, top == -INFINITY ? 0.f : Pack<E>::lift - top * c, by, rd);
   }
+  put(exp2f(-raise<E>));
+  __syncthreads();
+  for (int i = t; i < f.rows * CH; i += 256)
+    if (redo >> i / CH & 1) write(i / CH, i % CH, take(i / CH, i % CH));
 }
 
 // A run's result (maximum, sum, O divided by the sum) joins what others left: O as an average by the sums at the larger maximum,
