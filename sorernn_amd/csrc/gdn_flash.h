@@ -219,6 +219,30 @@ __device__ __forceinline__ int not_finite(const f32x16 (&a)[D / 32], int n) {
   return bits;
 }
 
+// Entries of an A operand that are not finite: x keeps 0 in their place, `up` and `down` hold a 1 where +inf and -inf were, and both
+// where NaN was.
+template <typename E>
+__device__ __forceinline__ void split_infinite(typename Pack<E>::x8& x, typename Pack<E>::x8& up, typename Pack<E>::x8& down) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool fine = (__builtin_bit_cast(uint16_t, (E)x[e]) & Pack<E>::infinity) != Pack<E>::infinity;
+    up[e] = (E)(fine || x[e] < (E)0.f ? 0.f : 1.f);
+    down[e] = (E)(fine || x[e] > (E)0.f ? 0.f : 1.f);
+    x[e] = fine ? x[e] : (E)0.f;
+  }
+}
+// They reach the columns of acc that see their rows (`ones`: 1 where seen, a B operand).
+template <typename E>
+__device__ __forceinline__ void add_infinite(f32x16& acc, typename Pack<E>::x8 up, typename Pack<E>::x8 down, typename Pack<E>::x8 ones) {
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) any |= up[e] != (E)0.f || down[e] != (E)0.f;
+  if (!__any(any)) return;
+  const f32x16 n = mma32(up, ones, f32x16{}), m = mma32(down, ones, f32x16{});
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] += (n[e] > 0.f ? INFINITY : 0.f) - (m[e] > 0.f ? INFINITY : 0.f);
+}
+
 // The product with the values again for the wave's rows whose sums are not finite, a block of KT x 32 keys at a time: weights are
 // divided by the row's sum first (`by`; the maximum is the final one), and infinities and NaN among the values are left out of the
 // product and reach the rows that see them. `seen`: the block's keys that the lane's row sees. key(j), val(j): rows of key j of the
@@ -231,7 +255,6 @@ __device__ __forceinline__ void again_block(f32x16 (&acc)[D / 32], const typenam
   using X8 = typename Pack<E>::x8;
   constexpr int CPR = D / 8, RPL = 512 / D;
   const int lane = threadIdx.x % kWave, hh = lane >> 5, li = lane & 31;
-  auto fine = [](E x) { return (__builtin_bit_cast(uint16_t, x) & Pack<E>::infinity) != Pack<E>::infinity; };
 #pragma unroll 4
   for (int u = 0; u < KT * 32 / RPL; ++u) {
     const int r = u * RPL + lane / CPR, ch = lane % CPR;
@@ -262,21 +285,9 @@ __device__ __forceinline__ void again_block(f32x16 (&acc)[D / 32], const typenam
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) {
         X8 x = tr_frag(tile + (2 * kt + h) * 16 * D, rd, d), up, down;
-        bool any = false;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool ok = fine(x[e]), more = !(x[e] < (E)0.f), less = !(x[e] > (E)0.f);  // NaN: both
-          any |= !ok;
-          up[e] = (E)(!ok && more ? 1.f : 0.f);
-          down[e] = (E)(!ok && less ? 1.f : 0.f);
-          x[e] = ok ? x[e] : (E)0.f;
-        }
+        split_infinite<E>(x, up, down);
         acc[d] = mma32(x, pb[h], acc[d]);
-        if (__any(any)) {
-          const f32x16 n = mma32(up, ones[h], f32x16{}), m = mma32(down, ones[h], f32x16{});
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[d][e] += (n[e] > 0.f ? INFINITY : 0.f) - (m[e] > 0.f ? INFINITY : 0.f);
-        }
+        add_infinite<E>(acc[d], up, down, ones[h]);
       }
   }
   __builtin_amdgcn_wave_barrier();  // the tile is read before the next block's is written

@@ -383,7 +383,8 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     }
   };
   // The same with queries whose logarithm (`lbad`: all their weights are NaN) or delta (`dbad`: none of their ds is finite) is not
-  // finite: their entries that are not are left out of the products, and the keys that see them become NaN.
+  // finite: their entries that are not are left out of the products, and the keys that see them become NaN, or of do's infinities
+  // those, by sign.
   auto block_bad = [&](const bf16* qb, const bf16* db, const float* lb, int q0) {
     const uint64_t there = bits_below(to - q0), lbad = __ballot(!finite_f(lb[lane])) & there;
     const uint64_t dbad = __ballot(!finite_f(lb[kBK + lane])) & there;
@@ -391,7 +392,6 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
     const uint64_t seen = bits_below(hi - q0) & ~bits_below(imax(kk, from) - q0);
     const uint64_t seen_v = (seen & ~lbad) >> 4 * hh, seen_k = (seen & ~(lbad | dbad)) >> 4 * hh;
     const float to_k = seen & (lbad | dbad) ? NAN : 0.f, to_v = seen & lbad ? NAN : 0.f;
-    auto finite = [](bf16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7f80) != 0x7f80; };
 #pragma unroll
     for (int d = 0; d < DT; ++d) dk[d] += to_k, dv[d] += to_v;
 #pragma nounroll
@@ -413,17 +413,10 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          bf16x8 x = tr_frag(db + (2 * qt + h) * 16 * D, rd, d), odd;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool fine = finite(x[e]);
-            odd[e] = (bf16)(fine ? 0.f : 1.f);
-            x[e] = fine ? x[e] : (bf16)0.f;
-          }
+          bf16x8 x = tr_frag(db + (2 * qt + h) * 16 * D, rd, d), up, down;
+          split_infinite<bf16>(x, up, down);
           dv[d] = mma32(x, pb[h], dv[d]);
-          const f32x16 n = mma32(odd, ones[h], f32x16{});  // entries that the key sees and that are not finite
-#pragma unroll
-          for (int e = 0; e < 16; ++e) dv[d][e] = n[e] > 0.f ? NAN : dv[d][e];
+          add_infinite<bf16>(dv[d], up, down, ones[h]);
         }
 #pragma unroll
       for (int st = 0; st < DS; ++st)
@@ -438,9 +431,8 @@ __global__ __launch_bounds__(512, 2) void gated_delta_window_attn_dkv_kernel(Win
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          bf16x8 x = tr_frag(qb + (2 * qt + h) * 16 * D, rd, d);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = finite(x[e]) ? x[e] : (bf16)0.f;
+          bf16x8 x = tr_frag(qb + (2 * qt + h) * 16 * D, rd, d), up, down;
+          split_infinite<bf16>(x, up, down);
           dk[d] = mma32(x, pb[h], dk[d]);
         }
     }

@@ -129,3 +129,23 @@ def test_columns(t, heads, d, win, sinks, spoiled):
 ])
 def test_blocks_that_reach_past_a_tile_s_queries(t, heads, d, win, sinks, spoiled):
     test_columns(t, heads, d, win, sinks, spoiled)
+
+
+@pytest.mark.parametrize("t, win, heads", [(300, None, 2), (500, 200, 1), (900, 150, 16)])
+def test_signs_of_values_gradients(t, win, heads):
+    """An infinity of do reaches dv of every key that its query sees, with its sign; both signs make NaN."""
+    *x, do = _inputs(1, t, heads, 1, 64, seed=4)
+    up, down, both = t - 140, t - 70, t - 20
+    do[0, up, 0, 3], do[0, down, heads - 1, 9] = torch.inf, -torch.inf
+    do[0, up, 0, 20], do[0, both, 0, 20] = torch.inf, -torch.inf
+    dv = _grads(x, do, window=win)[3][0, :, 0]
+    at = torch.arange(t, device=DEV)
+    by = {q: (at <= q) & ((at > q - win) if win else (at >= 0)) for q in (up, down, both)}
+    want = torch.zeros(t, 3, device=DEV)
+    want[by[up], 0] = torch.inf
+    want[by[down], 1] = -torch.inf
+    want[by[up], 2] = torch.inf
+    want[by[both], 2] -= torch.inf
+    for i, c in enumerate((3, 9, 20)):
+        got = torch.where(dv[:, c].isfinite(), 0, dv[:, c].float())
+        assert torch.equal(got.nan_to_num(7, 8, 9), want[:, i].nan_to_num(7, 8, 9)), c
