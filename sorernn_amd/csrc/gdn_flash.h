@@ -151,44 +151,9 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KT], f32x16 (&acc)[D / 
 // The matrix products multiply a masked place's weight, 0, with what lies there: an infinity or NaN among the values would
 // reach rows that do not see it. And weights of up to 2^8, of any number of keys, times finite values may pass fp32's range before
 // they are divided by the row's sum. (Masked scores take part in nothing: the row's maximum and sum are right, and where the sum
-// is NaN the row is.) The forwards take rows whose sums are not finite again, with again_block. The backward's dq sums their
-// columns that are not finite again key by key, over the keys that the row sees, until they are what they are: not finite, or
-// done. A wave a row; lane l holds columns l and l + 64.
+// is NaN the row is.) Rows whose sums are not finite are taken again, without the infinities and NaN, which are then added to the
+// rows that see them.
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
-template <int D, typename E>
-__device__ __forceinline__ float dot_row(const E* a, const E* b) {
-  float x = 0.f;
-  for (int d = 0; d < D; d += 8) {
-    const auto u = *reinterpret_cast<const typename Pack<E>::x8*>(a + d), w = *reinterpret_cast<const typename Pack<E>::x8*>(b + d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x += (float)u[e] * (float)w[e];
-  }
-  return x;
-}
-
-// Whether any of a row's columns `again` (bit i: l + 64 i) is finite so far: a sum that is not stays so.
-template <int D>
-__device__ __forceinline__ bool open_columns(int again, const float (&acc)[D / 64]) {
-  bool open = false;
-  for (int i = 0; i < D / 64; ++i) open |= (again >> i & 1) && finite_f(acc[i]);
-  return __any(open);
-}
-
-// acc += the sum over lanes z of `live` of lane z's w times row(z); others' rows are not read, and have no part in it.
-template <int D, typename Row>
-__device__ __forceinline__ void add_rows(uint64_t live, float w, Row row, float (&acc)[D / 64]) {
-  const int lane = threadIdx.x % kWave, some = __ffsll((unsigned long long)live) - 1;  // read in place of the others
-#pragma unroll 8
-  for (int z = 0; z < kWave; ++z) {
-    const bool on = live >> z & 1;
-    const float wz = __shfl(w, z, kWave);
-    const auto* r = row(on ? z : some);
-    for (int i = 0; i < D / 64; ++i) {
-      const float x = (float)r[lane + 64 * i];
-      acc[i] += on ? wz * x : 0.f;
-    }
-  }
-}
 
 // whether a lane's accumulators are all finite: 0 x stays 0 unless x is not
 template <int N>
@@ -199,24 +164,6 @@ __device__ __forceinline__ bool finite_all(const f32x16 (&a)[N]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) z = fmaf(a[n][e], 0.f, z);
   return z == 0.f;
-}
-
-// Of row n of the wave's (in lanes n and n + 32): which of lane l's columns l and l + 64 are not finite.
-template <int D>
-__device__ __forceinline__ int not_finite(const f32x16 (&a)[D / 32], int n) {
-  uint64_t mine = 0;  // bit 16 d + e: column 32 d + 8 (e / 4) + 4 hh + e % 4
-#pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mine |= finite_f(a[d][e]) ? 0ull : 1ull << (16 * d + e);
-  const int lane = threadIdx.x % kWave;
-  int bits = 0;
-  for (int i = 0; i < D / 64; ++i) {
-    const int col = lane + 64 * i, from = n + (col >> 2 & 1) * 32, e = (col >> 3 & 3) * 4 + (col & 3);
-    const uint32_t lo = __shfl((uint32_t)mine, from, kWave), hi = __shfl((uint32_t)(mine >> 32), from, kWave);
-    bits |= (int)(((uint64_t)hi << 32 | lo) >> (16 * (col >> 5) + e) & 1) << i;
-  }
-  return bits;
 }
 
 // Entries of an A operand that are not finite: x keeps 0 in their place, `up` and `down` hold a 1 where +inf and -inf were, and both
@@ -243,15 +190,14 @@ __device__ __forceinline__ void add_infinite(f32x16& acc, typename Pack<E>::x8 u
   for (int e = 0; e < 16; ++e) acc[e] += (n[e] > 0.f ? INFINITY : 0.f) - (m[e] > 0.f ? INFINITY : 0.f);
 }
 
-// The product with the values again for the wave's rows whose sums are not finite, a block of KT x 32 keys at a time: weights are
-// divided by the row's sum first (`by`; the maximum is the final one), and infinities and NaN among the values are left out of the
-// product and reach the rows that see them. `seen`: the block's keys that the lane's row sees. key(j), val(j): rows of key j of the
-// block, null: none. `tile`: LDS of the wave's own for the values. acc: O^T times 2^raise<E>.
+// The product with the values again for the wave's rows whose sums are not finite, a block of KT x 32 keys at a time, with weights
+// that are divided by the row's sum first (`by`; the maximum is the final one). `seen`: the block's keys that the lane's row sees.
+// key(j), val(j): rows of key j of the block, null: none. `tile`: LDS of the wave's own for the values. acc: O^T times 2^raise<E>.
 template <typename E>
 constexpr float raise = Pack<E>::lift > 0.f ? 14.f : 0.f;  // weights of 1 at most: fp16's are raised as far as they fit
 template <int KT, int D, typename E, typename Key, typename Val>
-__device__ __forceinline__ void again_block(f32x16 (&acc)[D / 32], const typename Pack<E>::x8 (&qf)[D / 16], uint64_t seen, Key key, Val val,
-                                            E* tile, float c, float nmc, float by, const TileReads<D>& rd) {
+__device__ __forceinline__ void again_block(f32x16 (&acc)[D / 32], const typename Pack<E>::x8 (&qf)[D / 16], uint64_t seen, Key key,
+                                            Val val, E* tile, float c, float nmc, float by, const TileReads<D>& rd) {
   using X8 = typename Pack<E>::x8;
   constexpr int CPR = D / 8, RPL = 512 / D;
   const int lane = threadIdx.x % kWave, hh = lane >> 5, li = lane & 31;

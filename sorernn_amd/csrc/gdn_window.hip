@@ -184,40 +184,66 @@ __global__ __launch_bounds__(256, 2) void gated_delta_window_attn_dq_kernel(Wind
   }
   bool fine = finite_all(acc);
   fine = lse != lse || !finite_f(delta) || (__shfl_xor((int)fine, 32, kWave) && fine);  // of those no ds that is seen is finite
-  if (row_ok) {
+  auto write = [&]() {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<bf16x4*>(p.dq + orow + 32 * d + 8 * j + 4 * hh) =
             to_bf16x4(acc[d][4 * j] * p.scale, acc[d][4 * j + 1] * p.scale, acc[d][4 * j + 2] * p.scale, acc[d][4 * j + 3] * p.scale);
-  }
-  uint64_t redo = __ballot(row_ok && !fine && hh == 0);
-  if (redo) wait_loads();  // what was written above is there before parts of it are written again
-  while (redo) {  // columns that are not finite, over the keys that the row sees only, until none of them can be
-    const int n = __ffsll((unsigned long long)redo) - 1, r = wq0 + n;
-    redo &= redo - 1;
-    const bf16* qp = p.q + sq.row * p.qsb + (sq.start + r) * p.qst + hq * p.qsh;
-    const int64_t at = ((tok + r) * p.HQ + hq) * D;
-    const float lr = __shfl(lse, n, kWave), dr = __shfl(delta, n, kWave);
-    const int again = not_finite<D>(acc, n);
-    float a[D / 64] = {};
-    for (int base = 0; base <= r; base += kWave) {
-      const int j = base + lane;
-      const bool see = j <= r && sees(r, j, p.window, p.sinks);
-      const uint64_t live = __ballot(see);
-      if (!live) continue;
-      float ds = 0.f;
-      if (see) {
-        const float s = dot_row<D>(qp, reinterpret_cast<const bf16*>(kbase + (int64_t)j * kst));
-        ds = __builtin_amdgcn_exp2f(fmaf(s, c, -lr)) * (dot_row<D>(p.d_o + at, reinterpret_cast<const bf16*>(vbase + (int64_t)j * vst)) - dr);
-      }
-      add_rows<D>(live, ds, [&](int z) { return reinterpret_cast<const bf16*>(kbase + (int64_t)(base + z) * kst); }, a);
-      if (!open_columns<D>(again, a)) break;
+  };
+  if (row_ok) write();
+  if (!__any(row_ok && !fine)) return;
+  // Rows whose sums are not finite, over the wave's blocks once more: infinities and NaN among the keys are left out of the products,
+  // and the rows that see them become NaN there (the score is -inf, and 0 times them is none).
+  wait_loads();  // what was written above is there before rows are written again
+#pragma unroll
+  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  bf16* const tile = w == 0 ? Ks0 : w == 1 ? Ks1 : w == 2 ? Vs0 : Vs1;  // all waves are behind their last block
+  constexpr int CPR = D / 8, RPL = 512 / D;
+  for (int n = 0; n < bl.count; ++n) {
+    const int k0 = bl.at(n) * kBK;
+    if (none_sees(wq0, wq1, k0, k0 + kBK - 1, p.window, p.sinks)) continue;
+#pragma unroll 4
+    for (int u = 0; u < kBK / RPL; ++u) {
+      const int r = u * RPL + lane / CPR, ch = lane % CPR;
+      *reinterpret_cast<bf16x8*>(tile + r * D + ((ch ^ swz<D>(r)) << 3)) =
+          k0 + r < sq.len ? *reinterpret_cast<const bf16x8*>(kbase + (int64_t)(k0 + r) * kst + 16 * ch) : bf16x8{};
     }
-    for (int e = 0; e < D / 64; ++e)
-      if (again >> e & 1) p.dq[at + lane + 64 * e] = (bf16)(a[e] * p.scale);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma nounroll
+    for (int kt = 0; kt < 2; ++kt) {
+      f32x16 s{}, dp{}, one;
+      const bf16* const v = reinterpret_cast<const bf16*>(vbase + (int64_t)imin(k0 + 32 * kt + li, sq.len - 1) * vst);
+#pragma unroll
+      for (int st = 0; st < DS; ++st) s = mma32(row_frag(tile + 32 * kt * D, rd, st), qf[st], s);
+#pragma unroll
+      for (int st = 0; st < DS; ++st) dp = mma32(ld8(v + 16 * st + 8 * hh), df[st], dp);
+      const uint32_t seen = (uint32_t)(view.block(k0 + 32 * kt, p.window, p.sinks) >> 4 * hh);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool see = seen >> (8 * (e >> 2) + (e & 3)) & 1;
+        s[e] = see ? __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse)) * (dp[e] - delta) : 0.f;
+        one[e] = see ? 1.f : 0.f;
+      }
+      bf16x8 pb[2], ones[2];
+      pack16<bf16>(s, pb);
+      pack16<bf16>(one, ones);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          bf16x8 x = tr_frag(tile + (2 * kt + h) * 16 * D, rd, d), up, down;
+          split_infinite<bf16>(x, up, down);
+          acc[d] = mma32(x, pb[h], acc[d]);
+          add_infinite<bf16>(acc[d], up + down, up + down, ones[h]);
+        }
+    }
+    __builtin_amdgcn_wave_barrier();  // the tile is read before the next block's is written
   }
+  if (row_ok && !fine) write();
 }
 
 // dk and dv: 128 keys of one kv head a workgroup, 32 a wave in registers; blocks of 64 queries with their do pass through LDS,

@@ -64,15 +64,14 @@ def test_a_bad_incoming_gradient_takes_no_longer(t, hq, hkv, win, sinks, spoil):
 @pytest.mark.parametrize("win, sinks", [(None, 0), (1024, 4)])
 def test_an_infinite_key_takes_no_longer(win, sinks):
     """Queries of one sign there: the rows lose that key's weight and stay finite, with NaN (0 times infinity) in one column of
-    their dq. Rows that share a block with it and do not see it are summed again: behind a window's end up to 32 a wave, one after
-    the other, over 18 times 64 keys of 25 us at most, 14.4 ms. Without a window no row is, and 29 ms were all rows' walks."""
+    their dq. Rows that share a block with it and do not see it are taken again (key by key, one row after the other, 12 to 29 ms)."""
     *x, do = _inputs(1, 6000, 16, 4, 128, seed=2)
     healthy = _ms(lambda: _grads(x, do, window=win, sinks=sinks))
     x[0][..., 5] = -x[0][..., 5].abs() - 1
     x[1][:, 40, :, 5] = torch.inf
     bad = _ms(lambda: _grads(x, do, window=win, sinks=sinks))
     print(f"{healthy:.2f} ms, {bad:.2f} ms")
-    assert bad < 5 * healthy + 2 + (14.4 if win else 0), (healthy, bad)
+    assert bad < 5 * healthy + 2, (healthy, bad)
 
 
 CASES = [
