@@ -172,8 +172,8 @@ __global__ __launch_bounds__(256) void gated_delta_paged_append_kernel(AppendPar
 
 // ------------------------------------------------------------------------------------------------ attention, many rows
 // Tiles of 128 rows (token, q head of the group) of a kv head; where they are few their keys are cut into `splits` runs.
-// Measured, 16 heads on 4 of 128: 512 new tokens of 4 sequences over up to 8,192 162 us, 552 TFLOP/s, bound as the forward over whole
-// sequences, and 14 us for the join of two runs (without runs 241 us); trees of 61 tokens of 8 sequences over up to 4,096 33 us
+// Measured, 16 heads on 4 of 128: 512 new tokens of 4 sequences over up to 8,192 160 us, 562 TFLOP/s, bound as the forward over whole
+// sequences, and 15 us for the join of two runs (without runs 241 us); trees of 61 tokens of 8 sequences over up to 4,096 31 us
 // and 9, bound by start and end of runs of 5 to 8 blocks.
 template <int D, typename E>
 __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashParams p) {
@@ -188,8 +188,8 @@ __global__ __launch_bounds__(256, 2) void gated_delta_paged_attn_kernel(FlashPar
 // A kv head's new rows (token, q head of the group) in tiles of 32; the keys that they see in blocks of 32, cut into `splits`
 // runs, a workgroup each. Every wave takes blocks of its own, loaded straight into its own LDS one ahead: no barrier until the
 // four waves' sums meet, 128 KB a CU under way. Bound by the cache's bytes: 64 sequences of up to 8,192 tokens, 4 kv heads of 128,
-// 144-152 us, 4.6-4.9 TB/s (a large copy: 5.1); with a window of 1,024, 8 kv heads of 64, 31 us, 4.3 TB/s. One token of one
-// sequence over 32,768 takes 17 us, 4.0 TB/s, and 4.5 for the join: the start of a run (length, table, first loads, one after
+// 147-153 us, 4.6-4.8 TB/s (a large copy: 5.1); with a window of 1,024, 8 kv heads of 64, 31 us, 4.3 TB/s. One token of one
+// sequence over 32,768 takes 16.4 us, 4.1 TB/s, and 4.7 for the join: the start of a run (length, table, first loads, one after
 // the other) is as long as its work.
 constexpr int kFewRows = 32, kFewKeys = 32;
 

@@ -10,9 +10,9 @@
 // way), the other holds 32 keys and walks their queries (dk, dv, summed over the q heads of the kv head in fp32). No atomics.
 //
 // Measured on 2 x 4,096 tokens, 16 heads on 4 of 128, window 1,024, 4 sinks, each kernel by itself in a trace, operations of
-// visible pairs only (a large bf16 product reaches 1,228 TFLOP/s): forward 99 us, 607 TFLOP/s; dq 134 us, 673; dk and dv 213 us,
-// 566, and 7 for the launch behind it; sinks 7 us; the step as a whole 420-432. A prompt of 8,192 tokens 102 us by itself, 86-88
-// among others of its kind. 5,003 tokens in 7 documents, 8 heads on 2 of 64, window 200: 20, 25, 30 and 5 us, join 5, sinks 4.
+// visible pairs only (a large bf16 product reaches 1,228 TFLOP/s): forward 100 us, 601 TFLOP/s; dq 135 us, 672; dk and dv 216 us,
+// 560, and 7 for the launch behind it; sinks 7 us; the step as a whole 425-431. A prompt of 8,192 tokens 100 us by itself, 87-88
+// among others of its kind. 5,003 tokens in 7 documents, 8 heads on 2 of 64, window 200: 20, 25, 31 and 5 us, join 5, sinks 4.
 
 #include "gdn_flash.h"
 
