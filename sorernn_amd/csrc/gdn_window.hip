@@ -652,6 +652,7 @@ static int far_sinks(int64_t window, int64_t sinks) { return window <= 0 ? 0 : s
 
 // Far queries a job, with one tile of sinks: short jobs, which fill up the CUs behind the near ones.
 constexpr int kFarPiece = 256;
+constexpr int64_t kCus = 256;
 
 struct FarPlan {
   FarList list;
@@ -688,10 +689,10 @@ static FarPlan far_plan(int64_t B, int64_t T, int64_t N, bool varlen, int window
 // (4,096 tokens, 4 kv heads, window 300) 158 -> 182. Each share costs 8 D bytes a key and kv head, written and read.
 static int dkv_shares(int64_t T, int64_t HQ, int64_t HKV, int64_t k_tiles, int64_t far_tiles, int window) {
   const int64_t jobs = k_tiles * HKV, blocks = HQ / HKV * ((T < window + kBQ ? T : window + kBQ) / kBK + 1);
-  const int64_t idle = (256 - far_tiles * HKV) / jobs;
+  const int64_t idle = (kCus - far_tiles * HKV) / jobs;
   int64_t n = idle < blocks / 8 ? idle : blocks / 8;
   if (window > T / 2) {
-    const int64_t even = (512 + jobs - 1) / jobs, m = even < blocks / 24 ? even : blocks / 24;
+    const int64_t even = (2 * kCus + jobs - 1) / jobs, m = even < blocks / 24 ? even : blocks / 24;
     n = n > m ? n : m;
   }
   return (int)(n < 1 ? 1 : n > 16 ? 16 : n);
